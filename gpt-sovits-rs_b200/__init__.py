@@ -18,7 +18,8 @@ from typing import Mapping, Optional, Sequence
 
 import numpy as np
 
-from . import shard, synth  # noqa: F401  (multi-GPU plumbing, seeded weights / inputs)
+from . import ops, shard, synth  # noqa: F401  (device operators, multi-GPU plumbing, seeded weights / inputs)
+from .ops import add_norm, add_norm_backward, attention, attention_backward  # noqa: F401
 
 PKG_DIR = Path(__file__).resolve().parent
 LIB_PATH = PKG_DIR / "_build" / "libgsvdec.so"
@@ -43,6 +44,8 @@ EXPORTS = (
     "gsvdec_encp_speed_len", "gsvdec_encp_interpolate", "gsvdec_encp_project",
     "gsvdec_forward_multi", "gsvdec_plan_multi", "gsvdec_sync_status", "gsvdec_selftest_wait",
     "gsvdec_set_alloc_fail_after", "gsvdec_workspace_bytes",
+    "gsvdec_attention_workspace", "gsvdec_attention_forward", "gsvdec_attention_backward",
+    "gsvdec_norm_workspace", "gsvdec_norm_forward", "gsvdec_norm_backward",
 )
 
 # EncP encoder stacks (GSV_ENCP_SSL / _TEXT / _2), by their enc_p.* names.
@@ -125,6 +128,7 @@ def library(path: Optional[Path] = None) -> ctypes.CDLL:
     lib.gsvdec_selftest_wait.argtypes = [vp, ctypes.c_int64, vp]
     lib.gsvdec_set_alloc_fail_after.argtypes = [i]
     lib.gsvdec_workspace_bytes.argtypes = [vp, ctypes.POINTER(ctypes.c_int64)]
+    ops.declare(lib)
     _lib = lib
     return lib
 

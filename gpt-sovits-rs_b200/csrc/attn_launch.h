@@ -1,0 +1,47 @@
+// attn_launch.h -- the attention kernels' launchers and the backward's workspace.
+#pragma once
+#include "attn.h"
+
+namespace gsv {
+
+constexpr int kRelBlocks = 296;  // partial sums of the relative gradients (two blocks per SM)
+
+// Backward workspace, all fp32: per query row (b, h, i) delta = do . o and
+// lse * log2(e); per row and offset the products q . relk_r, do . relv_r (read
+// by the score tiles) and the near values of p and ds (written by the dq
+// tiles); partial sums of the relative gradients.
+struct BwdWs {
+  float *delta, *lse2, *qrel, *grel, *pband, *sband, *part;
+  size_t bytes;
+};
+
+inline BwdWs carve_bwd(const AttnArgs& a) {
+  BwdWs w{};
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    float* p = reinterpret_cast<float*>(a.ws + at);
+    at += (n * sizeof(float) + 255) / 256 * 256;
+    return p;
+  };
+  const size_t rows = (size_t)a.B * a.H * a.Tq;
+  w.delta = take(rows);
+  w.lse2 = take(rows);
+  if (a.nrel) {
+    w.qrel = take(rows * a.nrel);
+    w.grel = take(rows * a.nrel);
+    w.pband = take(rows * a.nrel);
+    w.sband = take(rows * a.nrel);
+    w.part = take((size_t)kRelBlocks * 2 * a.nrel * a.D);
+  }
+  w.bytes = at;
+  return w;
+}
+
+cudaError_t attn_fwd_cores(const AttnArgs& a, cudaStream_t st);
+cudaError_t attn_bwd_cores(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
+// delta, lse2 and the relative products of every query row.
+cudaError_t attn_bwd_rows(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
+// drelk, drelv from the near values.
+cudaError_t attn_bwd_rel(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
+
+}  // namespace gsv

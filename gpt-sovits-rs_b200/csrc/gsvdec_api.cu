@@ -31,6 +31,8 @@ namespace {
 
 thread_local std::string g_last_error;
 
+}  // namespace
+
 int set_err(int code, const char* fmt, ...) {
   char buf[1024];
   va_list ap;
@@ -40,6 +42,8 @@ int set_err(int code, const char* fmt, ...) {
   g_last_error = buf;
   return code;
 }
+
+namespace {
 
 #define CUDA_TRY(expr)                                                                 \
   do {                                                                                 \

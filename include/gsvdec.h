@@ -382,6 +382,99 @@ int gsvdec_set_alloc_fail_after(int n);
  * layer, flow, EncP), i.e. everything but its packed weights. */
 int gsvdec_workspace_bytes(const gsvdec_t* h, int64_t* bytes);
 
+/* ---- Attention and residual norm with their gradients ----------------------
+ * The text encoder's attention and post-norm as stand-alone operators on
+ * device memory, forward and backward, for training the encoder (the
+ * reference only runs it forward: MultiHeadAttention::forward and
+ * LayerNorm::forward, src/models/sovits_encp.rs:98-110).  No handle: every
+ * call takes its tensors, a workspace and a stream, keeps nothing, allocates
+ * nothing and is stream-async, so it can be captured in a CUDA graph; calls
+ * overlap freely as long as their outputs and workspaces differ.  Outputs and
+ * workspace must not overlap inputs or one another.
+ *
+ * Attention, for utterance b with ql = q_lengths[b] queries and kl =
+ * k_lengths[b] keys (clamped to [0, Tq] / [0, Tk]; NULL: all): the sequences
+ * are aligned at their ends, so query i stands at key position pos = i + kl -
+ * ql.  It may attend to keys j < kl and, with causal, j <= pos.  With window w
+ * >= 0 the learned relative keys and values of the offsets r = j - pos in
+ * [-w, w] are added (emb_rel_k / emb_rel_v of the checkpoint, shared by the
+ * heads):
+ *   s_ij = scale q_i . (k_j + rel_k[r + w]),   p = softmax over the allowed j
+ *   o_i = sum_j p_ij (v_j + rel_v[r + w]),      lse_i = log sum_j exp(s_ij)
+ * Query head h reads key head h / (H / Hkv).  A query without an allowed key,
+ * and every i >= ql, gives o = 0, lse = -inf and dq = 0; keys j >= kl are not
+ * read and give dk = dv = 0.  All tensors are [B, heads, T, D] by element
+ * strides (batch, head, time); the D channels of a row are contiguous.  All
+ * arithmetic accumulates in fp32 and each output is rounded once to dtype. */
+typedef struct gsvdec_attention {
+  int dtype;      /* GSV_DTYPE_* of every tensor but lse */
+  int B, H, Hkv;  /* H a multiple of Hkv */
+  int Tq, Tk;     /* may be 0 */
+  int D;          /* channels per head, 1 .. 128 */
+  int window;     /* w in 0 .. 15, or -1: no relative terms */
+  int causal;     /* 0 or 1 */
+  float scale;    /* finite and positive; usually 1 / sqrt(D) */
+  const int32_t* q_lengths; /* [B] or NULL */
+  const int32_t* k_lengths; /* [B] or NULL */
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+  const void *rel_k, *rel_v; /* [2 w + 1, D] contiguous; NULL without a window */
+  void* o;                   /* forward: written; backward: read */
+  int64_t o_stride[3];
+  float* lse;                /* [B, H, Tq]; forward: written (or NULL); backward: read */
+  /* Backward only. */
+  const void* d_o;           /* gradient of o */
+  int64_t d_o_stride[3];
+  void *dq, *dk, *dv;
+  int64_t dq_stride[3], dk_stride[3], dv_stride[3];
+  void *drel_k, *drel_v;     /* [2 w + 1, D]; NULL without a window */
+  /* gsvdec_attention_workspace bytes, 16-byte aligned; its contents need no
+   * initialisation and are left behind. */
+  void* workspace;
+  size_t workspace_bytes;
+} gsvdec_attention;
+
+/* Workspace of a forward (backward = 0) or backward call; only the sizes,
+ * dtype, window, causal and strides of *a are read.  May be 0 bytes. */
+int gsvdec_attention_workspace(const gsvdec_attention* a, int backward, size_t* bytes);
+int gsvdec_attention_forward(const gsvdec_attention* a, int device, void* stream);
+/* Every gradient element is summed by one thread in a fixed order: equal
+ * inputs give equal bits. */
+int gsvdec_attention_backward(const gsvdec_attention* a, int device, void* stream);
+
+/* out = LayerNorm over channels of x + y (norm1(x + attn(x)) of
+ * EncoderLayer::forward, src/models/sovits_encp.rs:102), keeping what the
+ * backward needs:  mean, rstd = 1 / sqrt(biased variance + eps) per frame,
+ * xh = (x + y - mean) rstd, out = xh gamma + beta.  Backward, with a = d_out
+ * gamma:  dx = rstd (a - mean(a) - xh mean(a xh)), the gradient of x and of y
+ * alike; dgamma = sum over frames of d_out xh, dbeta = sum of d_out.  Frames
+ * t >= lengths[b] give out = 0, mean = rstd = 0, dx = 0 and add nothing.
+ * x, y, out, d_out, dx have dtype and element strides (batch, outer axis). */
+#define GSV_LAYOUT_BCT 0 /* [B, C, T], time contiguous (the reference's); C <= 2048 */
+#define GSV_LAYOUT_BTC 1 /* [B, T, C], channels contiguous; C <= 8192 */
+typedef struct gsvdec_norm {
+  int dtype, layout;
+  int B, C, T;              /* T may be 0 */
+  float eps;
+  const int32_t* lengths;   /* [B] or NULL */
+  const void *x, *y;        /* y may be NULL */
+  int64_t x_stride[2], y_stride[2];
+  const float *gamma, *beta; /* [C]; beta is not read by the backward */
+  float *mean, *rstd;       /* [B, T]; forward: written; backward: read */
+  void* out;                /* forward only */
+  int64_t out_stride[2];
+  /* Backward only. */
+  const void* d_out;
+  void* dx;
+  int64_t d_out_stride[2], dx_stride[2];
+  float *dgamma, *dbeta;    /* [C] */
+  void* workspace;          /* gsvdec_norm_workspace bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} gsvdec_norm;
+int gsvdec_norm_workspace(const gsvdec_norm* a, size_t* bytes);
+int gsvdec_norm_forward(const gsvdec_norm* a, int device, void* stream);
+int gsvdec_norm_backward(const gsvdec_norm* a, int device, void* stream);
+
 /* Thread-local message describing the last error on this thread. */
 const char* gsvdec_last_error(void);
 
