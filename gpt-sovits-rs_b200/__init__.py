@@ -19,7 +19,7 @@ from typing import Mapping, Optional, Sequence
 import numpy as np
 
 from . import ops, shard, synth  # noqa: F401  (device operators, multi-GPU plumbing, seeded weights / inputs)
-from .ops import add_norm, add_norm_backward, attention, attention_backward  # noqa: F401
+from .ops import add_norm, add_norm_backward, attention, attention_backward, ops_status  # noqa: F401
 
 PKG_DIR = Path(__file__).resolve().parent
 LIB_PATH = PKG_DIR / "_build" / "libgsvdec.so"
@@ -44,7 +44,7 @@ EXPORTS = (
     "gsvdec_encp_speed_len", "gsvdec_encp_interpolate", "gsvdec_encp_project",
     "gsvdec_forward_multi", "gsvdec_plan_multi", "gsvdec_sync_status", "gsvdec_selftest_wait",
     "gsvdec_set_alloc_fail_after", "gsvdec_workspace_bytes",
-    "gsvdec_attention_workspace", "gsvdec_attention_forward", "gsvdec_attention_backward",
+    "gsvdec_attention_workspace", "gsvdec_attention_forward", "gsvdec_attention_backward", "gsvdec_ops_status",
     "gsvdec_norm_workspace", "gsvdec_norm_forward", "gsvdec_norm_backward",
 )
 

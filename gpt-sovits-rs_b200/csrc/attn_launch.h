@@ -37,6 +37,7 @@ inline BwdWs carve_bwd(const AttnArgs& a) {
   return w;
 }
 
+cudaError_t attn_fwd_tensor(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_fwd_cores(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_bwd_cores(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
 // delta, lse2 and the relative products of every query row.

@@ -146,7 +146,8 @@ size_t attn_fwd_workspace(const AttnArgs&) { return 0; }
 size_t attn_bwd_workspace(const AttnArgs& a) { return carve_bwd(a).bytes; }
 
 cudaError_t attn_forward(const AttnArgs& a, cudaStream_t st) {
-  return a.Tq ? attn_fwd_cores(a, st) : cudaSuccess;
+  if (!a.Tq) return cudaSuccess;
+  return a.ty == Ty::F32 ? attn_fwd_cores(a, st) : attn_fwd_tensor(a, st);
 }
 
 cudaError_t attn_backward(const AttnArgs& a, cudaStream_t st) {

@@ -1,0 +1,249 @@
+// attn_tc.cuh -- shared pieces of the tcgen05 attention kernels: TMEM loads and
+// stores, descriptors, and the tile loader.
+//
+// Operand tiles live in shared memory as 64-channel chunks of 128-byte rows
+// with the 128-byte swizzle (16-byte unit u of row r sits at unit u ^ (r & 7)).
+// One such tile serves as a K-major operand (contraction over channels: q k^T)
+// and as an MN-major one (contraction over rows: p v), so nothing is
+// transposed or stored twice.
+#pragma once
+#include "attn_common.cuh"
+#include "tc_common.cuh"
+
+namespace gsv {
+namespace {
+
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, float* v) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_load64(uint32_t taddr, float* v) {
+  uint32_t r[64];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, "
+      "%36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, "
+      "%57, %58, %59, %60, %61, %62, %63}, [%64];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               :
+               : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16};"
+               :
+               : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+        "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+      "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+               :
+               : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+        "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// MN-major operand tile, 128-byte swizzle: 8-row groups 1024 bytes apart,
+// 64-channel chunks `chunk` bytes apart.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t chunk) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(chunk >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+// Instruction descriptor: fp32 accumulator, M = 128, operands of type T, B
+// K-major or MN-major.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_attn(int n, bool b_mn) {
+  constexpr uint32_t f = std::is_same<T, __half>::value ? 0u : 1u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kM >> 4) << 24);
+}
+
+// D (+)= A . B with A in TMEM (lane = row, two 16-bit values per column).
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Rows [0, rows) x DP channels of a tile, from `valid` global rows of D
+// channels; everything else is zero (rows behind a length may hold NaN, and
+// 0 . NaN would reach the accumulators).  `vec`: rows are whole aligned
+// 16-byte vectors and move by cp.async; else by single elements.
+template <typename T, int DP>
+__device__ __forceinline__ void load_tile(uint32_t dst, uint32_t chunk, const T* g, int64_t stride, int rows,
+                                          int valid, int D, bool vec, int tid, int nthreads) {
+  constexpr int U = DP / 8;  // 16-byte units per row
+  for (int e = tid; e < rows * U; e += nthreads) {
+    const int r = e / U, u = e - r * U;
+    const uint32_t a = dst + (u >> 3) * chunk + r * 128 + ((u ^ r) & 7) * 16;
+    const bool in = r < valid && u * 8 < D;
+    if (vec) {
+      cp_async16(a, in ? (const void*)(g + (int64_t)r * stride + u * 8) : (const void*)g, in ? 16 : 0);
+    } else {
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+      if (in) {
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(g + (int64_t)r * stride + u * 8);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (u * 8 + i < D) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+      }
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                   : "memory");
+    }
+  }
+}
+
+// The loader warps' side of a full barrier: a tile's copies are handed over
+// (completed, made visible to the tensor core, signalled) when the next tile's
+// copies are under way, or before the loader has to block.
+struct Handover {
+  uint32_t bar = 0;
+  __device__ __forceinline__ void flush() {
+    if (!bar) return;
+    cp_wait<0>();
+    fence_async_smem();
+    mbar_arrive(bar);
+    bar = 0;
+  }
+  __device__ __forceinline__ void next(uint32_t full) {
+    cp_commit();
+    if (bar) {
+      cp_wait<1>();
+      fence_async_smem();
+      mbar_arrive(bar);
+    }
+    bar = full;
+  }
+  __device__ __forceinline__ bool wait_free(uint32_t empty, uint32_t parity, volatile int* abort) {
+    if (mbar_try_nohint(empty, parity)) return true;
+    flush();
+    return mbar_wait_fast(empty, parity, abort);
+  }
+};
+
+// A bounded wait of a whole warp, with one answer for all its lanes (the TMEM
+// accesses after it need the warp together).
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait_fast(bar, parity, abort));
+}
+
+// Waits for the stream, then reads and clears a give-up word.
+cudaError_t take_gave_up(int& word, int* out, cudaStream_t st) {
+  void* p = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&p, word);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(out, p, sizeof(int), cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && *out) e = cudaMemsetAsync(p, 0, sizeof(int), st);
+  return e;
+}
+
+template <int N>
+__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// One row of 32 output channels starting at channel c.
+template <typename T>
+__device__ __forceinline__ void store_row32(T* row, int c, int D, bool vec, const float* v, float f) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 8) {
+    if (vec) {
+      if (c + k < D) {
+        uint4 u;
+        u.x = pack2<T>(v[k] * f, v[k + 1] * f);
+        u.y = pack2<T>(v[k + 2] * f, v[k + 3] * f);
+        u.z = pack2<T>(v[k + 4] * f, v[k + 5] * f);
+        u.w = pack2<T>(v[k + 6] * f, v[k + 7] * f);
+        *reinterpret_cast<uint4*>(row + c + k) = u;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + k + i < D) row[c + k + i] = from_f<T>(v[k + i] * f);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace gsv

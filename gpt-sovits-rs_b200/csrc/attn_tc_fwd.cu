@@ -1,0 +1,357 @@
+// attn_tc_fwd.cu -- attention forward on the tensor cores for fp16 and bf16
+// (formulas in attn.h).
+//
+// A block of 8 warps takes 128 queries of one head and walks its key tiles of
+// 128 with a running maximum and sum.  S = q k^T goes to TMEM (128 columns);
+// warps 0-3 hold one query row per thread, turn S into P = exp2(s - m) and put
+// it back over S in 16 bits, from where it is the A operand of O += P v (also
+// in TMEM).  Warp 4 issues the MMAs, warps 5-7 load tiles.  TMEM (256 columns)
+// and shared memory are sized for two blocks per SM, so one block's softmax
+// runs beside the other's MMAs.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the
+// scale in use was taken: P then stays below 2^8, which fp16 and bf16 hold
+// with the same relative rounding, and most tiles skip the pass over O.
+// P is rounded to the operands' type (the MMA takes no other); its row sum is
+// taken in fp32 before that, so the rounding is unbiased noise of 2^-9 (bf16)
+// or 2^-12 (fp16) of each term against one rounding of the same size at the
+// output.
+//
+// Relative keys: q relk^T is one more small MMA ahead of the key tiles, kept as
+// a table of 2 w + 1 values per row; the near scores replace their table entry
+// when their tile comes by, and after the last tile their probabilities are
+// one more P operand against the relative values' tile.
+#include "attn_launch.h"
+#include "attn_tc.cuh"
+
+namespace gsv {
+namespace {
+
+__device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out
+
+constexpr int kBM = 128, kBN = 128;
+constexpr int kFwdThreads = 256;
+constexpr int kLoaders = 96;
+constexpr int kSoftRegs = 192, kRestRegs = 64;  // 128 x 192 + 128 x 64 = 256 x 128
+
+template <int DP>
+struct FwdCfg {
+  static constexpr int NC = (DP + 63) / 64;
+  static constexpr uint32_t chunk = kBN * 128;     // bytes of a 64-channel chunk
+  static constexpr uint32_t tile = NC * chunk;
+  static constexpr int ST = NC == 1 ? 2 : 1;       // stages of the K and V rings
+  static constexpr uint32_t smem = tile * (1 + 2 * ST);
+};
+
+struct FwdBars {
+  uint64_t q_full, k_full[2], k_free[2], v_full[2], v_free[2], s_full, p_full, o_full;
+};
+
+template <typename T, int DP, bool REL>
+__global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, const bool vec, const bool ovec) {
+  using C = FwdCfg<DP>;
+  constexpr int ST = C::ST;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ FwdBars bars;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort;
+  const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
+  const uint32_t sQ = base, sK = sQ + C::tile, sV = sK + ST * C::tile;
+  float* tab = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + C::smem);  // [nrel][128]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Long rows of a causal mask first, so that the last blocks are short ones.
+  const int i0 = (int)(gridDim.x - 1 - blockIdx.x) * kBM, h = blockIdx.y, b = blockIdx.z;
+  const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk), off = kl - ql;
+  const int last = min(i0 + kBM, ql) - 1;
+  const int kend = last < i0 ? 0 : allowed_keys(last, ql, kl, a.causal);
+  const int nt = (kend + kBN - 1) / kBN;
+  const int hk = h / (a.H / a.Hkv), D = a.D;
+  volatile int* abort = &s_abort;
+  auto bar = [&](const uint64_t& m) { return smem_u32(&m); };
+
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    mbar_init(bar(bars.q_full), kLoaders);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar(bars.k_full[s]), kLoaders);
+      mbar_init(bar(bars.v_full[s]), kLoaders);
+      mbar_init(bar(bars.k_free[s]), 1);
+      mbar_init(bar(bars.v_free[s]), 1);
+    }
+    mbar_init(bar(bars.s_full), 1);
+    mbar_init(bar(bars.p_full), kBM);
+    mbar_init(bar(bars.o_full), 1);
+    fence_async_smem();
+  }
+  if (warp == 4) tmem_alloc(smem_u32(&s_tmem), 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tS = s_tmem, tO = tS + kBN;
+  const int nrp = REL ? (a.nrel + 15) / 16 * 16 : 0;
+
+  if (warp >= 4) {
+    reg_dec<kRestRegs>();
+    if (nt > 0 && warp == 4) {
+      if (lane == 0) {
+        constexpr uint32_t id_s = idesc_attn<T>(kBN, false), id_o = idesc_attn<T>(DP, true);
+        bool ok = mbar_wait_fast(bar(bars.q_full), 0, abort);
+        int kt = 0, vt = 0, pp = 0;
+        auto scores = [&](uint32_t id) {  // S = q . (tile kt)^T
+          const int s = kt % ST;
+          ok = ok && mbar_wait_fast(bar(bars.k_full[s]), (kt / ST) & 1, abort);
+          if (!ok) return;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < DP / 16; ++c) {
+            const uint32_t o = (c >> 2) * C::chunk + (c & 3) * 32;
+            mma_bf16(tS, sdesc<64>(sQ + o), sdesc<64>(sK + s * C::tile + o), id, c > 0);
+          }
+          mma_commit(bar(bars.k_free[s]));
+          mma_commit(bar(bars.s_full));
+          ++kt;
+        };
+        auto values = [&](int rows, uint32_t acc) {  // O += P . (tile vt)
+          const int s = vt % ST;
+          ok = ok && mbar_wait_fast(bar(bars.v_full[s]), (vt / ST) & 1, abort);
+          ok = ok && mbar_wait_fast(bar(bars.p_full), pp & 1, abort);
+          ++pp;
+          if (!ok) return;
+          tc_fence_after();
+          for (int c = 0; c < rows / 16; ++c)
+            mma_ts(tO, tS + c * 8, desc_mn(sV + s * C::tile + c * 2048, C::chunk), id_o, acc | (c > 0));
+          mma_commit(bar(bars.v_free[s]));
+          ++vt;
+        };
+        if (REL) {
+          scores(idesc_attn<T>(nrp, false));
+          ok = ok && mbar_wait_fast(bar(bars.p_full), pp & 1, abort);
+          ++pp;
+          tc_fence_after();
+        }
+        for (int t = 0; t < nt && ok; ++t) {
+          scores(id_s);
+          values(kBN, t > 0);
+        }
+        mma_commit(bar(bars.o_full));
+        if (REL && ok) {
+          values(nrp, 1);
+          mma_commit(bar(bars.o_full));
+        }
+        if (!ok) raise_err(&g_gave_up, abort, 1);
+        // Nothing of this block is in flight when its memory is given back.
+        mbar_wait_fast(bar(bars.o_full), REL && ok ? 1 : 0, abort);
+      }
+      __syncwarp();
+    } else if (nt > 0) {
+      const int tid = threadIdx.x - (kFwdThreads - kLoaders);
+      const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + (int64_t)i0 * a.sq.t;
+      const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
+      const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
+      Handover ho;
+      int kt = 0, vt = 0;
+      bool ok = true;
+      auto put = [&](bool is_k, const T* g, int64_t stride, int rows, int valid, bool al) {
+        int& n = is_k ? kt : vt;
+        const int s = n % ST;
+        const uint32_t dst = (is_k ? sK : sV) + s * C::tile;
+        if (n >= ST)
+          ok = ok && ho.wait_free(bar(is_k ? bars.k_free[s] : bars.v_free[s]), (n / ST - 1) & 1, abort);
+        if (!ok) return;
+        load_tile<T, DP>(dst, C::chunk, g, stride, rows, valid, D, al, tid, kLoaders);
+        ho.next(bar(is_k ? bars.k_full[s] : bars.v_full[s]));
+        ++n;
+      };
+      load_tile<T, DP>(sQ, C::chunk, q, a.sq.t, kBM, ql - i0, D, vec, tid, kLoaders);
+      ho.next(bar(bars.q_full));
+      if (REL) put(true, static_cast<const T*>(a.relk), D, nrp, a.nrel, D % 8 == 0 && vec);
+      for (int t = 0; t < nt && ok; ++t) {
+        put(true, k + (int64_t)t * kBN * a.sk.t, a.sk.t, kBN, kl - t * kBN, vec);
+        put(false, v + (int64_t)t * kBN * a.sv.t, a.sv.t, kBN, kl - t * kBN, vec);
+      }
+      if (REL && ok) put(false, static_cast<const T*>(a.relv), D, nrp, a.nrel, D % 8 == 0 && vec);
+      ho.flush();
+      cp_wait<0>();
+      if (!ok) raise_err(&g_gave_up, abort, 1);
+    }
+  } else {
+    reg_inc<kSoftRegs>();
+    const int row = threadIdx.x, i = i0 + row;
+    const int n = allowed_keys(i, ql, kl, a.causal);
+    const uint32_t lanes = (uint32_t)warp << 21;
+    const float sl2 = a.scale * kLog2e;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    int sp = 0;
+    if (nt > 0) {
+      if (REL) {
+        ok = warp_wait(bar(bars.s_full), sp++ & 1, abort);
+        tc_fence_after();
+        if (ok)
+          for (int r0 = 0; r0 < nrp; r0 += 16) {
+            float v[16];
+            tmem_load16(tS + lanes + r0, v);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (r0 + r < a.nrel) tab[(r0 + r) * kBM + row] = v[r];
+          }
+        tc_fence_before();
+        mbar_arrive(bar(bars.p_full));
+      }
+      for (int t = 0; t < nt && ok; ++t) {
+        ok = warp_wait(bar(bars.s_full), sp++ & 1, abort);
+        if (!ok) break;
+        tc_fence_after();
+        const int j0 = t * kBN;
+        float s[kBN];
+        tmem_load64(tS + lanes, s);
+        tmem_load64(tS + lanes + 64, s + 64);
+        if (REL) {
+          // Offsets of the warp's rows in this tile: j - pos + w for its first and last row.
+          const int d0 = j0 - (i + off) + a.window;
+          if (__any_sync(0xffffffffu, d0 < a.nrel && d0 + kBN > 0)) {
+#pragma unroll
+            for (int c = 0; c < kBN; ++c) {
+              const unsigned r = (unsigned)(d0 + c);
+              if (r < (unsigned)a.nrel) {
+                s[c] += tab[r * kBM + row];
+                tab[r * kBM + row] = s[c];
+              }
+            }
+          }
+        }
+        const int lim = n - j0;
+        if (__any_sync(0xffffffffu, lim < kBN)) {
+#pragma unroll
+          for (int c = 0; c < kBN; ++c)
+            if (c >= lim) s[c] = -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int c = 1; c < kBN; ++c) mx = fmaxf(mx, s[c]);
+        // m is the maximum the scale in use was taken from; see the note on rescaling above.
+        const bool grow = mx > m && (m == -INFINITY || (mx - m) * sl2 > 8.f);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float mn = fmaxf(m, mx);
+          const float alpha = m == -INFINITY ? 0.f : ex2((m - mn) * sl2);
+          m = mn;
+          l *= alpha;
+          if (t > 0) {
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+              float o[32];
+              tmem_load32(tO + lanes + c, o);
+              uint32_t u[32];
+#pragma unroll
+              for (int x = 0; x < 32; ++x) u[x] = __float_as_uint(o[x] * alpha);
+              tmem_store32(tO + lanes + c, u);
+            }
+          }
+        }
+        const float mu = m == -INFINITY ? 0.f : m * sl2;
+        uint32_t p[kBN / 2];
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int c = 0; c < kBN; c += 2) {
+          const float x = ex2(fmaf(s[c], sl2, -mu)), y = ex2(fmaf(s[c + 1], sl2, -mu));
+          l0 += x;
+          l1 += y;
+          p[c / 2] = pack2<T>(x, y);
+        }
+        l += l0 + l1;
+        tmem_store32(tS + lanes, p);
+        tmem_store32(tS + lanes + 32, p + 32);
+        tmem_store_wait();
+        tc_fence_before();
+        mbar_arrive(bar(bars.p_full));
+      }
+      ok = ok && warp_wait(bar(bars.o_full), 0, abort);
+      if (REL && ok) {
+        tc_fence_after();
+        const float mu = m == -INFINITY ? 0.f : m * sl2;
+        const int base_j = i + off - a.window;
+        for (int r0 = 0; r0 < nrp; r0 += 16) {
+          float pr[16];
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const int r = r0 + x, j = base_j + r;
+            pr[x] = r < a.nrel && j >= 0 && j < n ? ex2(fmaf(tab[r * kBM + row], sl2, -mu)) : 0.f;
+          }
+          uint32_t u[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) u[x] = pack2<T>(pr[2 * x], pr[2 * x + 1]);
+          tmem_store8(tS + lanes + r0 / 2, u);
+        }
+        tmem_store_wait();
+        tc_fence_before();
+        mbar_arrive(bar(bars.p_full));
+        ok = warp_wait(bar(bars.o_full), 1, abort);
+      }
+      if (!ok) raise_err(&g_gave_up, abort, 1);
+      tc_fence_after();
+    }
+    if (ok && i < a.Tq) {
+      const bool some = nt > 0 && l != 0.f;
+      T* out = static_cast<T*>(a.o) + b * a.so.b + h * a.so.h + (int64_t)i * a.so.t;
+      if (a.lse)
+        a.lse[((int64_t)b * a.H + h) * a.Tq + i] =
+            some ? ((m == -INFINITY ? 0.f : m * sl2) + log2f(l)) * kLn2 : -INFINITY;
+      if (!some) {
+        float z[32] = {};
+        for (int c = 0; c < DP; c += 32) store_row32<T>(out, c, D, ovec, z, 0.f);
+      }
+    }
+    if (nt > 0 && ok) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* out = static_cast<T*>(a.o) + b * a.so.b + h * a.so.h + (int64_t)i * a.so.t;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        tmem_load32(tO + lanes + c, o);
+        if (i < a.Tq && l != 0.f) store_row32<T>(out, c, D, ovec, o, inv);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(s_tmem, 256);
+  }
+}
+
+template <typename T, int DP, bool REL>
+cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
+  const size_t smem = FwdCfg<DP>::smem + 1024 + (size_t)a.nrel * kBM * sizeof(float);
+  int regs;
+  cudaError_t e = kernel_setup(attn_fwd_tc<T, DP, REL>, smem, &regs);
+  if (e != cudaSuccess) return e;
+  const bool vec = attn_rows_aligned(a.q, a.sq, a.D, 2) && attn_rows_aligned(a.k, a.sk, a.D, 2) &&
+                   attn_rows_aligned(a.v, a.sv, a.D, 2) && reinterpret_cast<uintptr_t>(a.relk) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(a.relv) % 16 == 0;
+  const bool ovec = attn_rows_aligned(a.o, a.so, a.D, 2);
+  attn_fwd_tc<T, DP, REL><<<dim3(cdiv(a.Tq, kBM), a.H, a.B), kFwdThreads, smem, st>>>(a, vec, ovec);
+  return cudaGetLastError();
+}
+
+template <typename T, int DP>
+cudaError_t rel(const AttnArgs& a, cudaStream_t st) {
+  return a.nrel ? launch<T, DP, true>(a, st) : launch<T, DP, false>(a, st);
+}
+
+template <typename T>
+cudaError_t width(const AttnArgs& a, cudaStream_t st) {
+  if (a.D <= 32) return rel<T, 32>(a, st);
+  if (a.D <= 64) return rel<T, 64>(a, st);
+  return a.D <= 96 ? rel<T, 96>(a, st) : rel<T, 128>(a, st);
+}
+
+}  // namespace
+
+cudaError_t attn_fwd_tensor(const AttnArgs& a, cudaStream_t st) {
+  return a.ty == Ty::F16 ? width<__half>(a, st) : width<__nv_bfloat16>(a, st);
+}
+
+cudaError_t attn_fwd_gave_up(int* out, cudaStream_t st) { return take_gave_up(g_gave_up, out, st); }
+
+}  // namespace gsv

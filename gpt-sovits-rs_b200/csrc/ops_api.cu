@@ -248,6 +248,16 @@ int gsvdec_attention_backward(const gsvdec_attention* a, int device, void* strea
   return gsv::attn_call(a, true, device, stream);
 }
 
+int gsvdec_ops_status(int device, void* stream) {
+  gsv::OnDevice dev(device);
+  if (dev.rc != GSV_OK) return dev.rc;
+  int gave_up = 0;
+  const cudaError_t e = gsv::attn_fwd_gave_up(&gave_up, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return gsv::finish(e, "operator status");
+  return gave_up ? gsv::set_err(GSV_E_TIMEOUT, "a bounded device wait of an attention call on device %d gave up", device)
+                 : GSV_OK;
+}
+
 int gsvdec_norm_workspace(const gsvdec_norm* a, size_t* bytes) {
   if (!bytes) return gsv::set_err(GSV_E_INVALID_ARG, "norm: NULL argument");
   gsv::NormArgs o{};

@@ -45,6 +45,7 @@ def declare(lib) -> None:
     lib.gsvdec_attention_workspace.argtypes = [at, ctypes.c_int, sz]
     lib.gsvdec_attention_forward.argtypes = [at, ctypes.c_int, _vp]
     lib.gsvdec_attention_backward.argtypes = [at, ctypes.c_int, _vp]
+    lib.gsvdec_ops_status.argtypes = [ctypes.c_int, _vp]
     lib.gsvdec_norm_workspace.argtypes = [nt, sz]
     lib.gsvdec_norm_forward.argtypes = [nt, ctypes.c_int, _vp]
     lib.gsvdec_norm_backward.argtypes = [nt, ctypes.c_int, _vp]
@@ -197,6 +198,15 @@ def attention_backward(do, q, k, v, o, lse, *, scale: Optional[float] = None, ca
     ws = _workspace(a, 1, dev)  # noqa: F841
     _run(_lib().gsvdec_attention_backward, a, dev)
     return dq, dk, dv, drk, drv
+
+
+def ops_status(device=None) -> None:
+    """Waits for the current stream of ``device`` (default: the current one) and
+    raises GsvDecError(GSV_E_TIMEOUT) if a bounded device wait of an attention
+    call there gave up (gsvdec_ops_status)."""
+    import torch
+    index = torch.cuda.current_device() if device is None else torch.device(device).index
+    _check(_lib().gsvdec_ops_status(index, torch.cuda.current_stream(index).cuda_stream))
 
 
 def _norm_args(x, y, gamma, beta, lengths, layout, eps):

@@ -442,6 +442,11 @@ int gsvdec_attention_forward(const gsvdec_attention* a, int device, void* stream
  * inputs give equal bits. */
 int gsvdec_attention_backward(const gsvdec_attention* a, int device, void* stream);
 
+/* Waits for `stream`, then reports whether a bounded device wait of an
+ * attention call on `device` gave up since the last such call (GSV_E_TIMEOUT;
+ * the results of the call concerned are undefined). */
+int gsvdec_ops_status(int device, void* stream);
+
 /* out = LayerNorm over channels of x + y (norm1(x + attn(x)) of
  * EncoderLayer::forward, src/models/sovits_encp.rs:102), keeping what the
  * backward needs:  mean, rstd = 1 / sqrt(biased variance + eps) per frame,

@@ -44,6 +44,7 @@ def run_and_check(gsv, x, **kw):
             continue
         assert got.dtype == t
         check(name, got, ref, t)
+    gsv.ops_status()
     return o, lse, grads
 
 
