@@ -61,7 +61,8 @@ size_t attn_bwd_workspace(const AttnArgs& a);
 cudaError_t attn_forward(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_backward(const AttnArgs& a, cudaStream_t st);
 // Waits for the stream; *out != 0 when a bounded device wait of the forward's
-// kernels gave up since the last call on this device.
+// (backward's) kernels gave up since the last such call on this device.
 cudaError_t attn_fwd_gave_up(int* out, cudaStream_t st);
+cudaError_t attn_bwd_gave_up(int* out, cudaStream_t st);
 
 }  // namespace gsv

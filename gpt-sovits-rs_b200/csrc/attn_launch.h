@@ -7,11 +7,12 @@ namespace gsv {
 constexpr int kRelBlocks = 296;  // partial sums of the relative gradients (two blocks per SM)
 
 // Backward workspace, all fp32: per query row (b, h, i) delta = do . o and
-// lse * log2(e); per row and offset the products q . relk_r, do . relv_r (read
+// lse * log2(e) (+inf for a row without keys, so that every exp2(s - lse2) of
+// it is 0); for fp16 the norms |do_i| and |v_j| + max |relv|; per row and offset the products q . relk_r, do . relv_r (read
 // by the score tiles) and the near values of p and ds (written by the dq
 // tiles); partial sums of the relative gradients.
 struct BwdWs {
-  float *delta, *lse2, *qrel, *grel, *pband, *sband, *part;
+  float *delta, *lse2, *ndo, *nv, *qrel, *grel, *pband, *sband, *part;
   size_t bytes;
 };
 
@@ -26,6 +27,10 @@ inline BwdWs carve_bwd(const AttnArgs& a) {
   const size_t rows = (size_t)a.B * a.H * a.Tq;
   w.delta = take(rows);
   w.lse2 = take(rows);
+  if (a.ty == Ty::F16) {
+    w.ndo = take(rows);
+    w.nv = take((size_t)a.B * a.Hkv * a.Tk);
+  }
   if (a.nrel) {
     w.qrel = take(rows * a.nrel);
     w.grel = take(rows * a.nrel);
@@ -39,8 +44,9 @@ inline BwdWs carve_bwd(const AttnArgs& a) {
 
 cudaError_t attn_fwd_tensor(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_fwd_cores(const AttnArgs& a, cudaStream_t st);
+cudaError_t attn_bwd_tensor(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
 cudaError_t attn_bwd_cores(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
-// delta, lse2 and the relative products of every query row.
+// delta, lse2, the norms and the relative products of every row.
 cudaError_t attn_bwd_rows(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
 // drelk, drelv from the near values.
 cudaError_t attn_bwd_rel(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);

@@ -10,9 +10,21 @@ namespace {
 
 constexpr int kRowWarps = 8;
 
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
 // One warp per query row.  delta = do . o in fp32; lane r then holds offset r's
 // products with the row, read from shared memory, against relk / relv rows of
-// odd pitch (no bank conflicts between lanes).
+// odd pitch (no bank conflicts between lanes).  fp16 (F16) adds the norms of
+// the rows of do and v.
 template <typename T>
 __global__ void __launch_bounds__(kRowWarps * 32) bwd_rows_kernel(const AttnArgs a, const BwdWs ws) {
   extern __shared__ float sm[];
@@ -27,28 +39,55 @@ __global__ void __launch_bounds__(kRowWarps * 32) bwd_rows_kernel(const AttnArgs
     srv[r * L + d] = to_f(static_cast<const T*>(a.relv)[e]);
   }
   __syncthreads();
+  constexpr bool F16 = std::is_same<T, __half>::value;
   const int64_t rows = (int64_t)a.B * a.H * a.Tq;
+  if (F16) {
+    float ev = 0.f;  // largest |relv|^2
+    if (lane < a.nrel)
+      for (int d = 0; d < D; ++d) ev = fmaf(srv[lane * L + d], srv[lane * L + d], ev);
+    ev = sqrtf(warp_max(ev));
+    const int64_t keys = (int64_t)a.B * a.Hkv * a.Tk;
+    for (int64_t row = (int64_t)blockIdx.x * kRowWarps + w; row < keys; row += (int64_t)gridDim.x * kRowWarps) {
+      const int j = (int)(row % a.Tk), h = (int)(row / a.Tk % a.Hkv), b = (int)(row / a.Tk / a.Hkv);
+      if (j >= clamp_len(a.klen, b, a.Tk)) continue;
+      const T* v = static_cast<const T*>(a.v) + b * a.sv.b + h * a.sv.h + j * a.sv.t;
+      float s = 0.f;
+      for (int d = lane; d < D; d += 32) s = fmaf(to_f(v[d]), to_f(v[d]), s);
+      s = warp_sum(s);
+      if (lane == 0) ws.nv[row] = sqrtf(s) + ev;
+    }
+  }
   for (int64_t row = (int64_t)blockIdx.x * kRowWarps + w; row < rows; row += (int64_t)gridDim.x * kRowWarps) {
     const int i = (int)(row % a.Tq), h = (int)(row / a.Tq % a.H), b = (int)(row / a.Tq / a.H);
     const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk);
-    if (allowed_keys(i, ql, kl, a.causal) == 0) continue;  // the row is read nowhere
+    if (allowed_keys(i, ql, kl, a.causal) == 0) {
+      if (lane == 0) {
+        ws.delta[row] = 0.f;
+        ws.lse2[row] = INFINITY;
+        if (F16) ws.ndo[row] = 0.f;
+      }
+      if (lane < a.nrel) ws.qrel[row * a.nrel + lane] = ws.grel[row * a.nrel + lane] = 0.f;
+      continue;
+    }
     const T* g = static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + i * a.sdo.t;
     const T* o = static_cast<const T*>(a.o) + b * a.so.b + h * a.so.h + i * a.so.t;
     const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + i * a.sq.t;
-    float s = 0.f;
+    float s = 0.f, gg = 0.f;
     for (int d = lane; d < D; d += 32) {
       const float gv = to_f(g[d]);
       s = fmaf(gv, to_f(o[d]), s);
+      if (F16) gg = fmaf(gv, gv, gg);
       if (a.nrel) {
         sg[d] = gv;
         sq[d] = to_f(q[d]);
       }
     }
-#pragma unroll
-    for (int k = 16; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+    s = warp_sum(s);
+    if (F16) gg = warp_sum(gg);
     if (lane == 0) {
       ws.delta[row] = s;
       ws.lse2[row] = a.lse[row] * kLog2e;
+      if (F16) ws.ndo[row] = sqrtf(gg);
     }
     __syncwarp();
     if (lane < a.nrel) {
@@ -153,7 +192,7 @@ cudaError_t attn_forward(const AttnArgs& a, cudaStream_t st) {
 cudaError_t attn_backward(const AttnArgs& a, cudaStream_t st) {
   const BwdWs ws = carve_bwd(a);
   cudaError_t e = a.Tq ? attn_bwd_rows(a, ws, st) : cudaSuccess;
-  if (e == cudaSuccess && (a.Tq || a.Tk)) e = attn_bwd_cores(a, ws, st);
+  if (e == cudaSuccess && (a.Tq || a.Tk)) e = a.ty == Ty::F32 ? attn_bwd_cores(a, ws, st) : attn_bwd_tensor(a, ws, st);
   if (e == cudaSuccess && a.nrel) e = attn_bwd_rel(a, ws, st);
   return e;
 }

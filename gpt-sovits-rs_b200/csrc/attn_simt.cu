@@ -404,19 +404,11 @@ cudaError_t bwd_d(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
 }  // namespace
 
 cudaError_t attn_fwd_cores(const AttnArgs& a, cudaStream_t st) {
-  switch (a.ty) {
-    case Ty::F32: return fwd_d<float>(a, st);
-    case Ty::F16: return fwd_d<__half>(a, st);
-    default: return fwd_d<__nv_bfloat16>(a, st);
-  }
+  return fwd_d<float>(a, st);
 }
 
 cudaError_t attn_bwd_cores(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
-  switch (a.ty) {
-    case Ty::F32: return bwd_d<float>(a, ws, st);
-    case Ty::F16: return bwd_d<__half>(a, ws, st);
-    default: return bwd_d<__nv_bfloat16>(a, ws, st);
-  }
+  return bwd_d<float>(a, ws, st);
 }
 
 }  // namespace gsv

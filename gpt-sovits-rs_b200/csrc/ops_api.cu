@@ -251,10 +251,11 @@ int gsvdec_attention_backward(const gsvdec_attention* a, int device, void* strea
 int gsvdec_ops_status(int device, void* stream) {
   gsv::OnDevice dev(device);
   if (dev.rc != GSV_OK) return dev.rc;
-  int gave_up = 0;
-  const cudaError_t e = gsv::attn_fwd_gave_up(&gave_up, static_cast<cudaStream_t>(stream));
+  int fwd = 0, bwd = 0;
+  cudaError_t e = gsv::attn_fwd_gave_up(&fwd, static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) e = gsv::attn_bwd_gave_up(&bwd, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return gsv::finish(e, "operator status");
-  return gave_up ? gsv::set_err(GSV_E_TIMEOUT, "a bounded device wait of an attention call on device %d gave up", device)
+  return fwd || bwd ? gsv::set_err(GSV_E_TIMEOUT, "a bounded device wait of an attention call on device %d gave up", device)
                  : GSV_OK;
 }
 
