@@ -126,6 +126,33 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Two fp32 lanes per instruction.
+struct F2 {
+  unsigned long long v;
+  __device__ __forceinline__ F2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ void get(float& lo, float& hi) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+  }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(a.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return a;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(a.v) : "l"(a.v), "l"(b.v));
+  return a;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(a.v) : "l"(a.v), "l"(b.v));
+  return a;
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (std::is_same<T, __half>::value) {
@@ -146,30 +173,45 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Rows [0, rows) x DP channels of a tile, from `valid` global rows of D
-// channels; everything else is zero (rows behind a length may hold NaN, and
-// 0 . NaN would reach the accumulators).  `vec`: rows are whole aligned
-// 16-byte vectors and move by cp.async; else by single elements.
-template <typename T, int DP>
-__device__ __forceinline__ void load_tile(uint32_t dst, uint32_t chunk, const T* g, int64_t stride, int rows,
-                                          int valid, int D, bool vec, int tid, int nthreads) {
-  constexpr int U = DP / 8;  // 16-byte units per row
-  for (int e = tid; e < rows * U; e += nthreads) {
-    const int r = e / U, u = e - r * U;
-    const uint32_t a = dst + (u >> 3) * chunk + r * 128 + ((u ^ r) & 7) * 16;
-    const bool in = r < valid && u * 8 < D;
-    if (vec) {
-      cp_async16(a, in ? (const void*)(g + (int64_t)r * stride + u * 8) : (const void*)g, in ? 16 : 0);
-    } else {
-      uint32_t w[4] = {0u, 0u, 0u, 0u};
-      if (in) {
-        const uint16_t* p = reinterpret_cast<const uint16_t*>(g + (int64_t)r * stride + u * 8);
+constexpr int kLoaders = 64;  // threads that load tiles
+
+// ROWS x DP channels of a tile, from `valid` global rows of D channels;
+// everything else is zero (rows behind a length may hold NaN, and 0 . NaN would
+// reach the accumulators).  `vec`: rows are whole aligned 16-byte vectors and
+// move by cp.async; else by single elements.  A chunk's 8 (or 4) units per row
+// divide the 64 threads, so a thread keeps its unit and its swizzle and steps
+// down the rows by one constant: three instructions per copy.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void load_tile(uint32_t dst, uint32_t chunk, const T* g, int64_t stride, int valid, int D,
+                                          bool vec, int tid) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (u * 8 + i < D) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+  for (int c = 0; c < (DP + 63) / 64; ++c) {
+    constexpr int kFull = 8;
+    const int units = DP - c * 64 >= 64 ? kFull : (DP - c * 64) / 8;
+    const int step = kLoaders / units, u = tid % units, r0 = tid / units, col = c * 64 + u * 8;
+    uint32_t a = dst + c * chunk + r0 * 128 + ((u ^ r0) & 7) * 16;
+    const T* p = g + (int64_t)r0 * stride + col;
+    const int64_t ps = (int64_t)step * stride;
+    if (vec && valid >= ROWS && DP == D) {
+#pragma unroll 4
+      for (int i = 0; i < ROWS / step; ++i, a += step * 128, p += ps) cp_async16(a, p, 16);
+    } else if (vec) {
+      for (int r = r0; r < ROWS; r += step, a += step * 128, p += ps) {
+        const bool in = r < valid && col < D;
+        cp_async16(a, in ? (const void*)p : (const void*)g, in ? 16 : 0);
       }
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                   : "memory");
+    } else {
+      for (int r = r0; r < ROWS; r += step, a += step * 128, p += ps) {
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (r < valid) {
+          const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col + i < D) w[i >> 1] |= (uint32_t)e[i] << (16 * (i & 1));
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                     : "memory");
+      }
     }
   }
 }

@@ -14,7 +14,7 @@
 //
 // S and dP have two buffers: warps 0-3 and 4-7 take alternate tiles (one row
 // per thread), while warp 8 issues the next tile's score products before it
-// waits for this tile's operands.  Warps 9-11 load tiles.
+// waits for this tile's operands.  Warps 9 and 10 load tiles.
 //
 // Rounding: P and dS are rounded to the operands' type.  fp16 holds 2^-24 to
 // 2^15 only, so P is carried as 2^15 P and dS with a power of two per head,
@@ -30,7 +30,6 @@ __device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out
 
 constexpr int kBA = 128, kBB = 64;  // rows of the resident and of the streamed tiles
 constexpr int kThreads = 384;
-constexpr int kLoaders = 96;
 
 template <int DP, bool REL>
 struct BwdCfg {
@@ -189,8 +188,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const AttnArgs a, con
         mbar_wait_fast(bar(bars.acc_full), 0, abort);  // nothing in flight when memory is given back
       }
       __syncwarp();
-    } else if (nt > 0) {
-      const int tid = threadIdx.x - (kThreads - kLoaders);
+    } else if (nt > 0 && warp < 11) {
+      const int tid = threadIdx.x - 9 * 32;
       Handover ho;
       bool ok = true;
       const T* q = static_cast<const T*>(a.q) + b * a.sq.b;
@@ -198,16 +197,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const AttnArgs a, con
       const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
       const T* dout = static_cast<const T*>(a.dout) + b * a.sdo.b;
       if (keys) {
-        load_tile<T, DP>(sA0, C::chunkA, k + (int64_t)r0 * a.sk.t, a.sk.t, kBA, kl - r0, D, vec, tid, kLoaders);
-        load_tile<T, DP>(sA1, C::chunkA, v + (int64_t)r0 * a.sv.t, a.sv.t, kBA, kl - r0, D, vec, tid, kLoaders);
+        load_tile<T, DP, kBA>(sA0, C::chunkA, k + (int64_t)r0 * a.sk.t, a.sk.t, kl - r0, D, vec, tid);
+        load_tile<T, DP, kBA>(sA1, C::chunkA, v + (int64_t)r0 * a.sv.t, a.sv.t, kl - r0, D, vec, tid);
       } else {
         const int h = blockIdx.y;
-        load_tile<T, DP>(sA0, C::chunkA, q + h * a.sq.h + (int64_t)r0 * a.sq.t, a.sq.t, kBA, ql - r0, D, vec, tid,
-                         kLoaders);
-        load_tile<T, DP>(sA1, C::chunkA, dout + h * a.sdo.h + (int64_t)r0 * a.sdo.t, a.sdo.t, kBA, ql - r0, D, vec,
-                         tid, kLoaders);
+        load_tile<T, DP, kBA>(sA0, C::chunkA, q + h * a.sq.h + (int64_t)r0 * a.sq.t, a.sq.t, ql - r0, D, vec, tid);
+        load_tile<T, DP, kBA>(sA1, C::chunkA, dout + h * a.sdo.h + (int64_t)r0 * a.sdo.t, a.sdo.t, ql - r0, D, vec, tid);
         if (REL)
-          load_tile<T, DP>(sR, C::chunkR, static_cast<const T*>(a.relk), D, 32, a.nrel, D, vec, tid, kLoaders);
+          load_tile<T, DP, 32>(sR, C::chunkR, static_cast<const T*>(a.relk), D, a.nrel, D, vec, tid);
       }
       ho.next(bar(bars.a_full));
       int hh = 0, x = first;
@@ -218,10 +215,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const AttnArgs a, con
         if (!ok) break;
         if (keys) {
           const int h = hk * g + hh;
-          load_tile<T, DP>(b0, C::chunkB, q + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t, kBB, ql - i0, D, vec, tid,
-                           kLoaders);
-          load_tile<T, DP>(b1, C::chunkB, dout + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t, kBB, ql - i0, D, vec,
-                           tid, kLoaders);
+          load_tile<T, DP, kBB>(b0, C::chunkB, q + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t, ql - i0, D, vec, tid);
+          load_tile<T, DP, kBB>(b1, C::chunkB, dout + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t, ql - i0, D, vec, tid);
           const int64_t row = row_h0 + (int64_t)hh * a.Tq + i0;
           const uint32_t tab = sTab + s * (C::rows + C::rel);
           for (int e = tid; e < 2 * kBB; e += kLoaders) {
@@ -241,8 +236,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const AttnArgs a, con
               }
           }
         } else {
-          load_tile<T, DP>(b0, C::chunkB, k + (int64_t)i0 * a.sk.t, a.sk.t, kBB, kl - i0, D, vec, tid, kLoaders);
-          load_tile<T, DP>(b1, C::chunkB, v + (int64_t)i0 * a.sv.t, a.sv.t, kBB, kl - i0, D, vec, tid, kLoaders);
+          load_tile<T, DP, kBB>(b0, C::chunkB, k + (int64_t)i0 * a.sk.t, a.sk.t, kl - i0, D, vec, tid);
+          load_tile<T, DP, kBB>(b1, C::chunkB, v + (int64_t)i0 * a.sv.t, a.sv.t, kl - i0, D, vec, tid);
         }
         ho.next(bar(bars.b_full[s]));
         if (++x == first + per) {

@@ -4,10 +4,12 @@
 // A block of 8 warps takes 128 queries of one head and walks its key tiles of
 // 128 with a running maximum and sum.  S = q k^T goes to TMEM (128 columns);
 // warps 0-3 hold one query row per thread, turn S into P = exp2(s - m) and put
-// it back over S in 16 bits, from where it is the A operand of O += P v (also
-// in TMEM).  Warp 4 issues the MMAs, warps 5-7 load tiles.  TMEM (256 columns)
-// and shared memory are sized for two blocks per SM, so one block's softmax
-// runs beside the other's MMAs.
+// it back in 16 bits, from where it is the A operand of O += P v (also
+// in TMEM).  Warp 4 issues the MMAs, warps 5 and 6 load tiles.  TMEM (256
+// columns) and shared memory are sized for two blocks per SM, so one block's
+// softmax runs beside the other's MMAs.  Up to D = 64 the columns also hold P
+// beside S: the next tile's scores are then computed while this tile's are
+// being exponentiated.
 //
 // O is rescaled only when a row's maximum has grown by more than 2^8 since the
 // scale in use was taken: P then stays below 2^8, which fp16 and bf16 hold
@@ -31,8 +33,7 @@ __device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out
 
 constexpr int kBM = 128, kBN = 128;
 constexpr int kFwdThreads = 256;
-constexpr int kLoaders = 96;
-constexpr int kSoftRegs = 192, kRestRegs = 64;  // 128 x 192 + 128 x 64 = 256 x 128
+constexpr int kSoftRegs = 176, kRestRegs = 80;  // 128 x 176 + 128 x 80 = 256 x 128
 
 template <int DP>
 struct FwdCfg {
@@ -41,10 +42,11 @@ struct FwdCfg {
   static constexpr uint32_t tile = NC * chunk;
   static constexpr int ST = NC == 1 ? 2 : 1;       // stages of the K and V rings
   static constexpr uint32_t smem = tile * (1 + 2 * ST);
+  static constexpr bool own_p = DP <= 64;          // P beside S instead of over it
 };
 
 struct FwdBars {
-  uint64_t q_full, k_full[2], k_free[2], v_full[2], v_free[2], s_full, p_full, o_full;
+  uint64_t q_full, k_full[2], k_free[2], v_full[2], v_free[2], s_full, s_free, p_full, o_full, pv_done;
 };
 
 template <typename T, int DP, bool REL>
@@ -80,14 +82,16 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
     }
     mbar_init(bar(bars.s_full), 1);
     mbar_init(bar(bars.p_full), kBM);
+    mbar_init(bar(bars.s_free), kBM);
     mbar_init(bar(bars.o_full), 1);
+    mbar_init(bar(bars.pv_done), 1);
     fence_async_smem();
   }
   if (warp == 4) tmem_alloc(smem_u32(&s_tmem), 256);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tS = s_tmem, tO = tS + kBN;
+  const uint32_t tS = s_tmem, tO = tS + kBN, tP = C::own_p ? tO + 64 : tS;
   const int nrp = REL ? (a.nrel + 15) / 16 * 16 : 0;
 
   if (warp >= 4) {
@@ -96,7 +100,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
       if (lane == 0) {
         constexpr uint32_t id_s = idesc_attn<T>(kBN, false), id_o = idesc_attn<T>(DP, true);
         bool ok = mbar_wait_fast(bar(bars.q_full), 0, abort);
-        int kt = 0, vt = 0, pp = 0;
+        int kt = 0, vt = 0, pp = 0, sf = 0;
         auto scores = [&](uint32_t id) {  // S = q . (tile kt)^T
           const int s = kt % ST;
           ok = ok && mbar_wait_fast(bar(bars.k_full[s]), (kt / ST) & 1, abort);
@@ -111,6 +115,11 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
           mma_commit(bar(bars.s_full));
           ++kt;
         };
+        auto scores_read = [&] {  // the softmax warps hold S in registers
+          ok = ok && mbar_wait_fast(bar(bars.s_free), sf & 1, abort);
+          ++sf;
+          tc_fence_after();
+        };
         auto values = [&](int rows, uint32_t acc) {  // O += P . (tile vt)
           const int s = vt % ST;
           ok = ok && mbar_wait_fast(bar(bars.v_full[s]), (vt / ST) & 1, abort);
@@ -119,18 +128,23 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
           if (!ok) return;
           tc_fence_after();
           for (int c = 0; c < rows / 16; ++c)
-            mma_ts(tO, tS + c * 8, desc_mn(sV + s * C::tile + c * 2048, C::chunk), id_o, acc | (c > 0));
+            mma_ts(tO, tP + c * 8, desc_mn(sV + s * C::tile + c * 2048, C::chunk), id_o, acc | (c > 0));
           mma_commit(bar(bars.v_free[s]));
+          if (C::own_p) mma_commit(bar(bars.pv_done));
           ++vt;
         };
         if (REL) {
           scores(idesc_attn<T>(nrp, false));
-          ok = ok && mbar_wait_fast(bar(bars.p_full), pp & 1, abort);
-          ++pp;
-          tc_fence_after();
+          scores_read();
         }
+        if (C::own_p) scores(id_s);
         for (int t = 0; t < nt && ok; ++t) {
-          scores(id_s);
+          if (C::own_p) {
+            scores_read();
+            if (t + 1 < nt) scores(id_s);
+          } else {
+            scores(id_s);
+          }
           values(kBN, t > 0);
         }
         mma_commit(bar(bars.o_full));
@@ -143,33 +157,43 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
         mbar_wait_fast(bar(bars.o_full), REL && ok ? 1 : 0, abort);
       }
       __syncwarp();
-    } else if (nt > 0) {
-      const int tid = threadIdx.x - (kFwdThreads - kLoaders);
+    } else if (nt > 0 && warp < 7) {
+      const int tid = threadIdx.x - 5 * 32;
       const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + (int64_t)i0 * a.sq.t;
       const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
       const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
       Handover ho;
       int kt = 0, vt = 0;
       bool ok = true;
-      auto put = [&](bool is_k, const T* g, int64_t stride, int rows, int valid, bool al) {
-        int& n = is_k ? kt : vt;
+      // Free stage of the K or V ring, or 0 when a wait gave up.
+      auto stage = [&](bool is_k, int n) -> uint32_t {
         const int s = n % ST;
-        const uint32_t dst = (is_k ? sK : sV) + s * C::tile;
-        if (n >= ST)
-          ok = ok && ho.wait_free(bar(is_k ? bars.k_free[s] : bars.v_free[s]), (n / ST - 1) & 1, abort);
-        if (!ok) return;
-        load_tile<T, DP>(dst, C::chunk, g, stride, rows, valid, D, al, tid, kLoaders);
-        ho.next(bar(is_k ? bars.k_full[s] : bars.v_full[s]));
-        ++n;
+        if (n >= ST) ok = ho.wait_free(bar(is_k ? bars.k_free[s] : bars.v_free[s]), (n / ST - 1) & 1, abort);
+        return ok ? (is_k ? sK : sV) + s * C::tile : 0;
       };
-      load_tile<T, DP>(sQ, C::chunk, q, a.sq.t, kBM, ql - i0, D, vec, tid, kLoaders);
+      load_tile<T, DP, kBM>(sQ, C::chunk, q, a.sq.t, ql - i0, D, vec, tid);
       ho.next(bar(bars.q_full));
-      if (REL) put(true, static_cast<const T*>(a.relk), D, nrp, a.nrel, D % 8 == 0 && vec);
-      for (int t = 0; t < nt && ok; ++t) {
-        put(true, k + (int64_t)t * kBN * a.sk.t, a.sk.t, kBN, kl - t * kBN, vec);
-        put(false, v + (int64_t)t * kBN * a.sv.t, a.sv.t, kBN, kl - t * kBN, vec);
+      if (REL) {
+        load_tile<T, DP, 32>(sK, C::chunk, static_cast<const T*>(a.relk), D, a.nrel, D, vec, tid);
+        ho.next(bar(bars.k_full[kt++]));
       }
-      if (REL && ok) put(false, static_cast<const T*>(a.relv), D, nrp, a.nrel, D % 8 == 0 && vec);
+      for (int t = 0; t < nt && ok; ++t) {
+        uint32_t dst = stage(true, kt);
+        if (!dst) break;
+        load_tile<T, DP, kBN>(dst, C::chunk, k + (int64_t)t * kBN * a.sk.t, a.sk.t, kl - t * kBN, D, vec, tid);
+        ho.next(bar(bars.k_full[kt++ % ST]));
+        dst = stage(false, vt);
+        if (!dst) break;
+        load_tile<T, DP, kBN>(dst, C::chunk, v + (int64_t)t * kBN * a.sv.t, a.sv.t, kl - t * kBN, D, vec, tid);
+        ho.next(bar(bars.v_full[vt++ % ST]));
+      }
+      if (REL && ok) {
+        const uint32_t dst = stage(false, vt);
+        if (dst) {
+          load_tile<T, DP, 32>(dst, C::chunk, static_cast<const T*>(a.relv), D, a.nrel, D, vec, tid);
+          ho.next(bar(bars.v_full[vt % ST]));
+        }
+      }
       ho.flush();
       cp_wait<0>();
       if (!ok) raise_err(&g_gave_up, abort, 1);
@@ -196,7 +220,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
               if (r0 + r < a.nrel) tab[(r0 + r) * kBM + row] = v[r];
           }
         tc_fence_before();
-        mbar_arrive(bar(bars.p_full));
+        mbar_arrive(bar(bars.s_free));
       }
       for (int t = 0; t < nt && ok; ++t) {
         ok = warp_wait(bar(bars.s_full), sp++ & 1, abort);
@@ -206,6 +230,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
         float s[kBN];
         tmem_load64(tS + lanes, s);
         tmem_load64(tS + lanes + 64, s + 64);
+        if (C::own_p) {
+          tc_fence_before();
+          mbar_arrive(bar(bars.s_free));
+        }
         if (REL) {
           // Offsets of the warp's rows in this tile: j - pos + w for its first and last row.
           const int d0 = j0 - (i + off) + a.window;
@@ -226,9 +254,20 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
           for (int c = 0; c < kBN; ++c)
             if (c >= lim) s[c] = -INFINITY;
         }
-        float mx = s[0];
+        float m4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int c = 1; c < kBN; ++c) mx = fmaxf(mx, s[c]);
+        for (int c = 4; c < kBN - 4; c += 8)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) m4[x] = max3(m4[x], s[c + x], s[c + 4 + x]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) m4[x] = fmaxf(m4[x], s[kBN - 4 + x]);
+        const float mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
+        // The MMAs of the tile before have read P and added to O.
+        if (C::own_p && t > 0) {
+          ok = warp_wait(bar(bars.pv_done), (t - 1) & 1, abort);
+          if (!ok) break;
+          tc_fence_after();
+        }
         // m is the maximum the scale in use was taken from; see the note on rescaling above.
         const bool grow = mx > m && (m == -INFINITY || (mx - m) * sl2 > 8.f);
         if (__any_sync(0xffffffffu, grow)) {
@@ -250,17 +289,23 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
         }
         const float mu = m == -INFINITY ? 0.f : m * sl2;
         uint32_t p[kBN / 2];
-        float l0 = 0.f, l1 = 0.f;
+        const F2 sl(sl2, sl2), nm(-mu, -mu);
+        F2 la(0.f, 0.f), lb(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < kBN; c += 2) {
-          const float x = ex2(fmaf(s[c], sl2, -mu)), y = ex2(fmaf(s[c + 1], sl2, -mu));
-          l0 += x;
-          l1 += y;
+          float x, y;
+          fma2(F2(s[c], s[c + 1]), sl, nm).get(x, y);
+          x = ex2(x);
+          y = ex2(y);
+          if (c & 2) lb = add2(lb, F2(x, y));
+          else la = add2(la, F2(x, y));
           p[c / 2] = pack2<T>(x, y);
         }
+        float l0, l1;
+        add2(la, lb).get(l0, l1);
         l += l0 + l1;
-        tmem_store32(tS + lanes, p);
-        tmem_store32(tS + lanes + 32, p + 32);
+        tmem_store32(tP + lanes, p);
+        tmem_store32(tP + lanes + 32, p + 32);
         tmem_store_wait();
         tc_fence_before();
         mbar_arrive(bar(bars.p_full));
@@ -280,7 +325,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
           uint32_t u[8];
 #pragma unroll
           for (int x = 0; x < 8; ++x) u[x] = pack2<T>(pr[2 * x], pr[2 * x + 1]);
-          tmem_store8(tS + lanes + r0 / 2, u);
+          tmem_store8(tP + lanes + r0 / 2, u);
         }
         tmem_store_wait();
         tc_fence_before();
