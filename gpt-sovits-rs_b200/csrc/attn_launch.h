@@ -4,15 +4,19 @@
 
 namespace gsv {
 
-constexpr int kRelBlocks = 296;  // partial sums of the relative gradients (two blocks per SM)
+constexpr int kRelRows = 64;  // query rows of one head whose relative gradients one block sums
+inline int64_t rel_blocks(const AttnArgs& a) { return (int64_t)a.B * a.H * cdiv(a.Tq, kRelRows); }
 
-// Backward workspace, all fp32: per query row (b, h, i) delta = do . o and
-// lse * log2(e) (+inf for a row without keys, so that every exp2(s - lse2) of
-// it is 0); for fp16 the norms |do_i| and |v_j| + max |relv|; per row and offset the products q . relk_r, do . relv_r (read
-// by the score tiles) and the near values of p and ds (written by the dq
-// tiles); partial sums of the relative gradients.
+constexpr float kHalfShift = 15.f;  // fp16 probabilities are carried as 2^15 p
+
+// Backward workspace, all fp32: per query row (b, h, i) ndelta = -do . o and
+// nlse2 = -lse log2(e), plus kHalfShift for fp16 (-inf for a row without keys,
+// so that every exp2 of it is 0); for fp16 the norms |do_i| and |v_j| + max
+// |relv|; per row and offset the products q . relk_r, do . relv_r (read by the
+// score tiles) and the near values of p and ds (written by the dq tiles);
+// partial sums of the relative gradients.
 struct BwdWs {
-  float *delta, *lse2, *ndo, *nv, *qrel, *grel, *pband, *sband, *part;
+  float *ndelta, *nlse2, *ndo, *nv, *qrel, *grel, *pband, *sband, *part;
   size_t bytes;
 };
 
@@ -25,8 +29,8 @@ inline BwdWs carve_bwd(const AttnArgs& a) {
     return p;
   };
   const size_t rows = (size_t)a.B * a.H * a.Tq;
-  w.delta = take(rows);
-  w.lse2 = take(rows);
+  w.ndelta = take(rows);
+  w.nlse2 = take(rows);
   if (a.ty == Ty::F16) {
     w.ndo = take(rows);
     w.nv = take((size_t)a.B * a.Hkv * a.Tk);
@@ -36,7 +40,7 @@ inline BwdWs carve_bwd(const AttnArgs& a) {
     w.grel = take(rows * a.nrel);
     w.pband = take(rows * a.nrel);
     w.sband = take(rows * a.nrel);
-    w.part = take((size_t)kRelBlocks * 2 * a.nrel * a.D);
+    w.part = take((size_t)rel_blocks(a) * 2 * a.nrel * a.D);
   }
   w.bytes = at;
   return w;
@@ -46,7 +50,7 @@ cudaError_t attn_fwd_tensor(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_fwd_cores(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_bwd_tensor(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
 cudaError_t attn_bwd_cores(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
-// delta, lse2, the norms and the relative products of every row.
+// ndelta, nlse2, the norms and the relative products of every row.
 cudaError_t attn_bwd_rows(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
 // drelk, drelv from the near values.
 cudaError_t attn_bwd_rel(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);

@@ -8,11 +8,13 @@
 namespace gsv {
 namespace {
 
-constexpr int kRowWarps = 8;
+constexpr int kRowThreads = 256;
+constexpr int kFewKeys = 32;
 
-__device__ __forceinline__ float warp_sum(float v) {
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {  // over aligned groups of G lanes
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 __device__ __forceinline__ float warp_max(float v) {
@@ -21,151 +23,230 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// One warp per query row.  delta = do . o in fp32; lane r then holds offset r's
-// products with the row, read from shared memory, against relk / relv rows of
-// odd pitch (no bank conflicts between lanes).  fp16 (F16) adds the norms of
-// the rows of do and v.
+// Channels d0 .. d0 + 7 of a row, zeros from D on.
 template <typename T>
-__global__ void __launch_bounds__(kRowWarps * 32) bwd_rows_kernel(const AttnArgs a, const BwdWs ws) {
-  extern __shared__ float sm[];
-  const int D = a.D, L = D | 1, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  float* srk = sm;
-  float* srv = srk + a.nrel * L;
-  float* sq = srv + a.nrel * L + w * 2 * D;
-  float* sg = sq + D;
-  for (int e = threadIdx.x; e < a.nrel * D; e += blockDim.x) {
-    const int r = e / D, d = e - r * D;
-    srk[r * L + d] = to_f(static_cast<const T*>(a.relk)[e]);
-    srv[r * L + d] = to_f(static_cast<const T*>(a.relv)[e]);
-  }
-  __syncthreads();
-  constexpr bool F16 = std::is_same<T, __half>::value;
-  const int64_t rows = (int64_t)a.B * a.H * a.Tq;
-  if (F16) {
-    float ev = 0.f;  // largest |relv|^2
-    if (lane < a.nrel)
-      for (int d = 0; d < D; ++d) ev = fmaf(srv[lane * L + d], srv[lane * L + d], ev);
-    ev = sqrtf(warp_max(ev));
-    const int64_t keys = (int64_t)a.B * a.Hkv * a.Tk;
-    for (int64_t row = (int64_t)blockIdx.x * kRowWarps + w; row < keys; row += (int64_t)gridDim.x * kRowWarps) {
-      const int j = (int)(row % a.Tk), h = (int)(row / a.Tk % a.Hkv), b = (int)(row / a.Tk / a.Hkv);
-      if (j >= clamp_len(a.klen, b, a.Tk)) continue;
-      const T* v = static_cast<const T*>(a.v) + b * a.sv.b + h * a.sv.h + j * a.sv.t;
-      float s = 0.f;
-      for (int d = lane; d < D; d += 32) s = fmaf(to_f(v[d]), to_f(v[d]), s);
-      s = warp_sum(s);
-      if (lane == 0) ws.nv[row] = sqrtf(s) + ev;
+__device__ __forceinline__ void load8(const T* row, int d0, int D, bool vec, float* f) {
+  if (vec && d0 < D) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int k = 0; k < 8; k += V) {
+      const uint4 u = *reinterpret_cast<const uint4*>(row + d0 + k);
+      const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[k + i] = to_f(e[i]);
     }
-  }
-  for (int64_t row = (int64_t)blockIdx.x * kRowWarps + w; row < rows; row += (int64_t)gridDim.x * kRowWarps) {
-    const int i = (int)(row % a.Tq), h = (int)(row / a.Tq % a.H), b = (int)(row / a.Tq / a.H);
-    const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk);
-    if (allowed_keys(i, ql, kl, a.causal) == 0) {
-      if (lane == 0) {
-        ws.delta[row] = 0.f;
-        ws.lse2[row] = INFINITY;
-        if (F16) ws.ndo[row] = 0.f;
-      }
-      if (lane < a.nrel) ws.qrel[row * a.nrel + lane] = ws.grel[row * a.nrel + lane] = 0.f;
-      continue;
-    }
-    const T* g = static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + i * a.sdo.t;
-    const T* o = static_cast<const T*>(a.o) + b * a.so.b + h * a.so.h + i * a.so.t;
-    const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + i * a.sq.t;
-    float s = 0.f, gg = 0.f;
-    for (int d = lane; d < D; d += 32) {
-      const float gv = to_f(g[d]);
-      s = fmaf(gv, to_f(o[d]), s);
-      if (F16) gg = fmaf(gv, gv, gg);
-      if (a.nrel) {
-        sg[d] = gv;
-        sq[d] = to_f(q[d]);
-      }
-    }
-    s = warp_sum(s);
-    if (F16) gg = warp_sum(gg);
-    if (lane == 0) {
-      ws.delta[row] = s;
-      ws.lse2[row] = a.lse[row] * kLog2e;
-      if (F16) ws.ndo[row] = sqrtf(gg);
-    }
-    __syncwarp();
-    if (lane < a.nrel) {
-      float x = 0.f, y = 0.f;
-      for (int d = 0; d < D; ++d) {
-        x = fmaf(sq[d], srk[lane * L + d], x);
-        y = fmaf(sg[d], srv[lane * L + d], y);
-      }
-      ws.qrel[row * a.nrel + lane] = x;
-      ws.grel[row * a.nrel + lane] = y;
-    }
-    __syncwarp();
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = d0 + i < D ? to_f(row[d0 + i]) : 0.f;
   }
 }
 
-// Partial sums over a block's run of rows: thread d holds channel d of every
-// offset (NR of them).  Fixed row order, so the result does not depend on
-// scheduling.
-template <typename T, int NR>
-__global__ void __launch_bounds__(kAttnMaxD) bwd_rel_kernel(const AttnArgs a, const BwdWs ws, const int64_t per) {
-  const int d = threadIdx.x, D = a.D;
-  const int64_t rows = (int64_t)a.B * a.H * a.Tq;
-  const int64_t r0 = blockIdx.x * per, r1 = min(rows, r0 + per);
-  float ak[NR] = {}, av[NR] = {};
-  for (int64_t row = r0; row < r1; ++row) {
-    const int i = (int)(row % a.Tq), h = (int)(row / a.Tq % a.H), b = (int)(row / a.Tq / a.H);
-    const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk);
-    const int n = allowed_keys(i, ql, kl, a.causal);
-    if (n == 0) continue;
-    const int base = i + kl - ql - a.window;  // key of offset 0
-    float q = 0.f, g = 0.f;
-    if (d < D) {
-      q = to_f(static_cast<const T*>(a.q)[b * a.sq.b + h * a.sq.h + i * a.sq.t + d]);
-      g = to_f(static_cast<const T*>(a.dout)[b * a.sdo.b + h * a.sdo.h + i * a.sdo.t + d]);
-    }
+__device__ __forceinline__ float dot8(const float* a, const float* b) {
+  float s = 0.f;
 #pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      if (r >= a.nrel || base + r < 0 || base + r >= n) continue;
-      ak[r] = fmaf(ws.sband[row * a.nrel + r], q, ak[r]);
-      av[r] = fmaf(ws.pband[row * a.nrel + r], g, av[r]);
+  for (int i = 0; i < 8; ++i) s = fmaf(a[i], b[i], s);
+  return s;
+}
+
+// G lanes share one row, 8 channels each.  Query rows: delta = do . o in fp32
+// and the products with the relative rows; fp16 adds the norms of the rows of
+// do and v.
+//
+// The o given here carries its rounding to 16 bits, which reaches ds through
+// delta as p_ij (2^-9 |do| |o|).  Over many keys o shrinks against v and the
+// term disappears; rows of up to kFewKeys keys, where it would be as large as
+// the rounding of ds itself, take delta = sum_j p_ij dp_ij instead (fp32
+// inputs have no such rounding).
+template <typename T, int G>
+__global__ void __launch_bounds__(kRowThreads) bwd_rows_kernel(const AttnArgs a, const BwdWs ws, const bool vec) {
+  extern __shared__ float sm[];  // relk, relv as [nrel][8 G]
+  constexpr bool F16 = std::is_same<T, __half>::value, kExact = std::is_same<T, float>::value;
+  constexpr int L = 8 * G, R = kRowThreads / G;
+  const int D = a.D, lane = threadIdx.x % G, grp = threadIdx.x / G, d0 = lane * 8;
+  float* srk = sm;
+  float* srv = srk + a.nrel * L;
+  for (int e = threadIdx.x; e < a.nrel * L; e += kRowThreads) {
+    const int r = e / L, d = e - r * L;
+    srk[e] = d < D ? to_f(static_cast<const T*>(a.relk)[r * D + d]) : 0.f;
+    srv[e] = d < D ? to_f(static_cast<const T*>(a.relv)[r * D + d]) : 0.f;
+  }
+  __syncthreads();
+  if (F16) {
+    float ev = 0.f;  // largest |relv|^2
+    if ((threadIdx.x & 31) < a.nrel)
+      for (int d = 0; d < L; ++d) ev = fmaf(srv[(threadIdx.x & 31) * L + d], srv[(threadIdx.x & 31) * L + d], ev);
+    ev = sqrtf(warp_max(ev));
+    const int64_t keys = (int64_t)a.B * a.Hkv * a.Tk, steps = (keys + R - 1) / R;
+    for (int64_t x = blockIdx.x; x < steps; x += gridDim.x) {
+      const int64_t row = x * R + grp;
+      const int64_t bh = row / max(a.Tk, 1);
+      const int j = (int)(row - bh * a.Tk), b = (int)(bh / a.Hkv), h = (int)(bh - (int64_t)b * a.Hkv);
+      float s = 0.f;
+      const bool in = row < keys && j < clamp_len(a.klen, b, a.Tk);
+      if (in) {
+        float v[8];
+        load8(static_cast<const T*>(a.v) + b * a.sv.b + h * a.sv.h + j * a.sv.t, d0, D, vec, v);
+        s = dot8(v, v);
+      }
+      s = group_sum<G>(s);
+      if (in && lane == 0) ws.nv[row] = sqrtf(s) + ev;
     }
   }
-  if (d >= D) return;
+  const int64_t rows = (int64_t)a.B * a.H * a.Tq, steps = (rows + R - 1) / R;
+  const float sl2 = a.scale * kLog2e;
+  for (int64_t x = blockIdx.x; x < steps; x += gridDim.x) {
+    const int64_t row = x * R + grp;
+    const int64_t bh = row / a.Tq;
+    const int i = (int)(row - bh * a.Tq), b = (int)(bh / a.H), h = (int)(bh - (int64_t)b * a.H);
+    const bool in = row < rows;
+    const int ql = in ? clamp_len(a.qlen, b, a.Tq) : 0, kl = in ? clamp_len(a.klen, b, a.Tk) : 0;
+    const int n = in ? allowed_keys(i, ql, kl, a.causal) : 0;
+    float g[8] = {}, q[8] = {}, o[8] = {};
+    if (n > 0) {
+      load8(static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + i * a.sdo.t, d0, D, vec, g);
+      load8(static_cast<const T*>(a.o) + b * a.so.b + h * a.so.h + i * a.so.t, d0, D, vec, o);
+      if (a.nrel || !kExact) load8(static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + i * a.sq.t, d0, D, vec, q);
+    }
+    float s = group_sum<G>(dot8(g, o));
+    const float lse2 = n > 0 ? a.lse[row] * kLog2e : INFINITY;
+    for (int r = 0; r < a.nrel; ++r) {
+      const float u = group_sum<G>(dot8(q, srk + r * L + d0)), w = group_sum<G>(dot8(g, srv + r * L + d0));
+      if (in && lane == r % G) {
+        ws.qrel[row * a.nrel + r] = u;
+        ws.grel[row * a.nrel + r] = w;
+      }
+    }
+    if (!kExact) {
+      const bool few = n > 0 && n <= kFewKeys;
+      if (__any_sync(0xffffffffu, few)) {
+        const int hk = h / (a.H / a.Hkv);
+        const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
+        const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
+        float t = 0.f;
+        const int most = (int)warp_max(few ? (float)n : 0.f);
+#pragma unroll 4
+        for (int j = 0; j < most; ++j) {
+          const bool use = few && j < n;
+          float kk[8], vv[8];
+          load8(k + (use ? j : 0) * a.sk.t, use ? d0 : D, D, vec, kk);
+          load8(v + (use ? j : 0) * a.sv.t, use ? d0 : D, D, vec, vv);
+          const unsigned r = (unsigned)(j - (i + kl - ql) + a.window);
+          if (use && r < (unsigned)a.nrel)
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              kk[y] += srk[r * L + d0 + y];
+              vv[y] += srv[r * L + d0 + y];
+            }
+          const float sc = group_sum<G>(dot8(q, kk)), dp = group_sum<G>(dot8(g, vv));
+          if (use) t = fmaf(exp2f(fmaf(sc, sl2, -lse2)), dp, t);
+        }
+        if (few) s = t;
+      }
+    }
+    const float gg = F16 ? sqrtf(group_sum<G>(dot8(g, g))) : 0.f;
+    if (in && lane == 0) {
+      ws.ndelta[row] = n > 0 ? -s : 0.f;
+      ws.nlse2[row] = (F16 ? kHalfShift : 0.f) - lse2;
+      if (F16) ws.ndo[row] = n > 0 ? gg : 0.f;
+    }
+  }
+}
+
+// Partial sums over kRelRows query rows of one head: thread (d, half) holds
+// channel d of every offset over one half of the rows.  Fixed row order, so
+// the result does not depend on scheduling.
+template <typename T, int NR>
+__global__ void __launch_bounds__(2 * kAttnMaxD) bwd_rel_kernel(const AttnArgs a, const BwdWs ws) {
+  __shared__ float sp[kRelRows][NR], ss[kRelRows][NR];
+  __shared__ float red[2 * NR][kAttnMaxD];
+  const int tiles = cdiv(a.Tq, kRelRows), bh = blockIdx.x / tiles, i0 = (blockIdx.x - bh * tiles) * kRelRows;
+  const int b = bh / a.H, h = bh - b * a.H, D = a.D;
+  const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk);
+  for (int e = threadIdx.x; e < kRelRows * NR; e += 2 * kAttnMaxD) {
+    const int y = e / NR, r = e - y * NR, i = i0 + y, j = i + kl - ql - a.window + r;
+    const bool in = r < a.nrel && j >= 0 && j < allowed_keys(i, ql, kl, a.causal);
+    const int64_t at = ((int64_t)bh * a.Tq + i) * a.nrel + r;
+    ss[y][r] = in ? ws.sband[at] : 0.f;
+    sp[y][r] = in ? ws.pband[at] : 0.f;
+  }
+  __syncthreads();
+  const int d = threadIdx.x % kAttnMaxD, half = threadIdx.x / kAttnMaxD;
+  float ak[NR] = {}, av[NR] = {};
+  const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + d;
+  const T* g = static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + d;
+  const int y1 = min(half * (kRelRows / 2) + kRelRows / 2, ql - i0);
+#pragma unroll 4
+  for (int y = half * (kRelRows / 2); y < y1; ++y) {
+    const float qv = d < D ? to_f(q[(int64_t)(i0 + y) * a.sq.t]) : 0.f;
+    const float gv = d < D ? to_f(g[(int64_t)(i0 + y) * a.sdo.t]) : 0.f;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      ak[r] = fmaf(ss[y][r], qv, ak[r]);
+      av[r] = fmaf(sp[y][r], gv, av[r]);
+    }
+  }
+  if (half == 1)
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      red[r][d] = ak[r];
+      red[NR + r][d] = av[r];
+    }
+  __syncthreads();
+  if (half == 1 || d >= D) return;
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     if (r >= a.nrel) continue;
-    ws.part[((int64_t)blockIdx.x * 2 * a.nrel + r) * D + d] = ak[r] * a.scale;
-    ws.part[((int64_t)blockIdx.x * 2 * a.nrel + a.nrel + r) * D + d] = av[r];
+    ws.part[((int64_t)blockIdx.x * 2 * a.nrel + r) * D + d] = (ak[r] + red[r][d]) * a.scale;
+    ws.part[((int64_t)blockIdx.x * 2 * a.nrel + a.nrel + r) * D + d] = av[r] + red[NR + r][d];
   }
 }
 
+// 32 sums per block, its 16 warps taking every 16th partial sum.
 template <typename T>
-__global__ void bwd_rel_sum_kernel(const AttnArgs a, const BwdWs ws, const int blocks) {
-  const int n = a.nrel * a.D, e = blockIdx.x * blockDim.x + threadIdx.x;
-  if (e >= 2 * n) return;
-  float s = 0.f;
-  for (int x = 0; x < blocks; ++x) s += ws.part[(int64_t)x * 2 * n + e];
-  if (e < n) static_cast<T*>(a.drelk)[e] = from_f<T>(s);
-  else static_cast<T*>(a.drelv)[e - n] = from_f<T>(s);
+__global__ void __launch_bounds__(512) bwd_rel_sum_kernel(const AttnArgs a, const BwdWs ws, const int64_t blocks) {
+  __shared__ float s[16][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int n = a.nrel * a.D, e = blockIdx.x * 32 + lane;
+  float v = 0.f;
+  if (e < 2 * n) {
+#pragma unroll 4
+    for (int64_t x = w; x < blocks; x += 16) v += ws.part[x * 2 * n + e];
+  }
+  s[w][lane] = v;
+  __syncthreads();
+  if (w != 0 || e >= 2 * n) return;
+  for (int x = 1; x < 16; ++x) v += s[x][lane];
+  if (e < n) static_cast<T*>(a.drelk)[e] = from_f<T>(v);
+  else static_cast<T*>(a.drelv)[e - n] = from_f<T>(v);
 }
 
-template <typename T>
-cudaError_t rows_t(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.B * a.H * a.Tq;
-  const int grid = (int)std::min<int64_t>((rows + kRowWarps - 1) / kRowWarps, 148 * 8);
-  const size_t smem = sizeof(float) * (2 * a.nrel * (a.D | 1) + kRowWarps * 2 * a.D);
-  bwd_rows_kernel<T><<<grid, kRowWarps * 32, smem, st>>>(a, ws);
+template <typename T, int G>
+cudaError_t rows_g(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
+  const int64_t rows = std::max((int64_t)a.B * a.H * a.Tq, (int64_t)a.B * a.Hkv * a.Tk), R = kRowThreads / G;
+  const int grid = (int)std::min<int64_t>((rows + R - 1) / R, 148 * 4);
+  const size_t smem = sizeof(float) * 2 * a.nrel * 8 * G;
+  const int el = sizeof(T);
+  const bool vec = attn_rows_aligned(a.q, a.sq, a.D, el) && attn_rows_aligned(a.o, a.so, a.D, el) &&
+                   attn_rows_aligned(a.dout, a.sdo, a.D, el) && attn_rows_aligned(a.k, a.sk, a.D, el) &&
+                   attn_rows_aligned(a.v, a.sv, a.D, el) && a.D % 8 == 0;
+  bwd_rows_kernel<T, G><<<grid, kRowThreads, smem, st>>>(a, ws, vec);
   return cudaGetLastError();
 }
 
 template <typename T>
+cudaError_t rows_t(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
+  if (a.D <= 32) return rows_g<T, 4>(a, ws, st);
+  return a.D <= 64 ? rows_g<T, 8>(a, ws, st) : rows_g<T, 16>(a, ws, st);
+}
+
+template <typename T>
 cudaError_t rel_t(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.B * a.H * a.Tq;
-  const int64_t per = std::max<int64_t>(1, (rows + kRelBlocks - 1) / kRelBlocks);
-  const int blocks = (int)std::max<int64_t>(1, (rows + per - 1) / per);
-  if (a.nrel <= 9) bwd_rel_kernel<T, 9><<<blocks, kAttnMaxD, 0, st>>>(a, ws, per);
-  else bwd_rel_kernel<T, 2 * kAttnMaxWindow + 1><<<blocks, kAttnMaxD, 0, st>>>(a, ws, per);
-  bwd_rel_sum_kernel<T><<<cdiv(2 * a.nrel * a.D, 128), 128, 0, st>>>(a, ws, blocks);
+  const int64_t blocks = rel_blocks(a);
+  if (blocks > 0) {
+    if (a.nrel <= 9) bwd_rel_kernel<T, 9><<<(unsigned)blocks, 2 * kAttnMaxD, 0, st>>>(a, ws);
+    else bwd_rel_kernel<T, 2 * kAttnMaxWindow + 1><<<(unsigned)blocks, 2 * kAttnMaxD, 0, st>>>(a, ws);
+  }
+  bwd_rel_sum_kernel<T><<<cdiv(2 * a.nrel * a.D, 32), 512, 0, st>>>(a, ws, blocks);
   return cudaGetLastError();
 }
 

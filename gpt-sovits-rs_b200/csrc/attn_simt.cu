@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const AttnArgs a, cons
         for (int c = 0; c < 4; ++c) {
           const int i = i0 + tx + 16 * c;
           const int n = allowed_keys(i, ql, kl, a.causal);
-          const float lse2 = n > 0 ? ws.lse2[row + i] : 0.f, delta = n > 0 ? ws.delta[row + i] : 0.f;
+          const float nlse2 = n > 0 ? ws.nlse2[row + i] : 0.f, ndelta = n > 0 ? ws.ndelta[row + i] : 0.f;
           float p4[4], s4[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const AttnArgs a, cons
               s[x][c] += ws.qrel[(row + i) * a.nrel + r];
               dp[x][c] += ws.grel[(row + i) * a.nrel + r];
             }
-            p4[x] = ok ? exp2f(fmaf(s[x][c], sl2, -lse2)) : 0.f;
-            s4[x] = ok ? p4[x] * (dp[x][c] - delta) : 0.f;
+            p4[x] = ok ? exp2f(fmaf(s[x][c], sl2, nlse2)) : 0.f;
+            s4[x] = ok ? p4[x] * (dp[x][c] + ndelta) : 0.f;
           }
           *reinterpret_cast<float4*>(sP + (tx + 16 * c) * kLdP + 4 * ty) = make_float4(p4[0], p4[1], p4[2], p4[3]);
           *reinterpret_cast<float4*>(sS + (tx + 16 * c) * kLdP + 4 * ty) = make_float4(s4[0], s4[1], s4[2], s4[3]);
@@ -294,14 +294,14 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const AttnArgs a, cons
                    D, vec);
   load_rows<T, DP>(s1, static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t,
                    ql - i0, D, vec);
-  float dq[4][W] = {}, lse2[4], delta[4];
+  float dq[4][W] = {}, nlse2[4], ndelta[4];
   int n[4];
 #pragma unroll
   for (int x = 0; x < 4; ++x) {
     const int i = i0 + 4 * ty + x;
     n[x] = allowed_keys(i, ql, kl, a.causal);
-    lse2[x] = n[x] > 0 ? ws.lse2[row + i] : 0.f;
-    delta[x] = n[x] > 0 ? ws.delta[row + i] : 0.f;
+    nlse2[x] = n[x] > 0 ? ws.nlse2[row + i] : 0.f;
+    ndelta[x] = n[x] > 0 ? ws.ndelta[row + i] : 0.f;
   }
   const int last = min(i0 + kBT, ql) - 1;
   const int kend = last < i0 ? 0 : allowed_keys(last, ql, kl, a.causal);
@@ -328,8 +328,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const AttnArgs a, cons
           s[x][c] += ws.qrel[(row + i) * a.nrel + r];
           dp[x][c] += ws.grel[(row + i) * a.nrel + r];
         }
-        const float p = ok ? exp2f(fmaf(s[x][c], sl2, -lse2[x])) : 0.f;
-        s4[x] = ok ? p * (dp[x][c] - delta[x]) : 0.f;
+        const float p = ok ? exp2f(fmaf(s[x][c], sl2, nlse2[x])) : 0.f;
+        s4[x] = ok ? p * (dp[x][c] + ndelta[x]) : 0.f;
         if (near) {
           ws.pband[(row + i) * a.nrel + r] = p;
           ws.sband[(row + i) * a.nrel + r] = s4[x];

@@ -110,14 +110,30 @@ __host__ __device__ constexpr uint32_t idesc_attn(int n, bool b_mn) {
          ((uint32_t)(kM >> 4) << 24);
 }
 
-// D (+)= A . B with A in TMEM (lane = row, two 16-bit values per column).
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+// D = A . B and D += A . B with A in TMEM (lane = row, two 16-bit values per
+// column).  The accumulate flag is part of the instruction's form and the
+// descriptors advance by constants, so that the issuing thread spends little
+// between two MMAs.
+__device__ __forceinline__ void mma_ts_first(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, 0;" ::"r"(d), "r"(a), "l"(b), "r"(idesc)
+               : "memory");
+}
+__device__ __forceinline__ void mma_ts_acc(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  asm volatile("tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, 1;" ::"r"(d), "r"(a), "l"(b), "r"(idesc)
+               : "memory");
+}
+
+// D = A . B^T over DP channels of two K-major tiles (descriptors of their first
+// chunk; chunks of chA and chB bytes).
+template <int DP>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint64_t a, uint32_t chA, uint64_t b, uint32_t chB,
+                                         uint32_t idesc) {
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+    const uint64_t da = a + (c >> 2) * (chA >> 4) + (c & 3) * 2, db = b + (c >> 2) * (chB >> 4) + (c & 3) * 2;
+    if (c == 0) mma_bf16_first(d, da, db, idesc);
+    else mma_bf16_acc(d, da, db, idesc);
+  }
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -173,7 +189,7 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-constexpr int kLoaders = 64;  // threads that load tiles
+constexpr int kLoaders = 64;  // threads that load tiles (two warps)
 
 // ROWS x DP channels of a tile, from `valid` global rows of D channels;
 // everything else is zero (rows behind a length may hold NaN, and 0 . NaN would
@@ -216,6 +232,13 @@ __device__ __forceinline__ void load_tile(uint32_t dst, uint32_t chunk, const T*
   }
 }
 
+// One arrival for a warp, after what its lanes did before (32 lanes arriving on
+// one barrier are served one by one).
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 // The loader warps' side of a full barrier: a tile's copies are handed over
 // (completed, made visible to the tensor core, signalled) when the next tile's
 // copies are under way, or before the loader has to block.
@@ -225,7 +248,7 @@ struct Handover {
     if (!bar) return;
     cp_wait<0>();
     fence_async_smem();
-    mbar_arrive(bar);
+    warp_arrive(bar);
     bar = 0;
   }
   __device__ __forceinline__ void next(uint32_t full) {
@@ -233,14 +256,14 @@ struct Handover {
     if (bar) {
       cp_wait<1>();
       fence_async_smem();
-      mbar_arrive(bar);
+      warp_arrive(bar);
     }
     bar = full;
   }
   __device__ __forceinline__ bool wait_free(uint32_t empty, uint32_t parity, volatile int* abort) {
-    if (mbar_try_nohint(empty, parity)) return true;
+    if (__all_sync(0xffffffffu, mbar_try_nohint(empty, parity))) return true;
     flush();
-    return mbar_wait_fast(empty, parity, abort);
+    return __all_sync(0xffffffffu, mbar_wait_fast(empty, parity, abort));
   }
 };
 
@@ -258,6 +281,44 @@ cudaError_t take_gave_up(int& word, int* out, cudaStream_t st) {
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (e == cudaSuccess && *out) e = cudaMemsetAsync(p, 0, sizeof(int), st);
   return e;
+}
+
+// A [B][heads][T][D] tensor as a 4-D tensor map whose boxes are ROWS rows of a
+// 64-channel chunk.  Axes of one element, or shared by broadcasting (stride 0),
+// have extent 1 and coordinate 0.
+struct RowsMap {
+  CUtensorMap map;
+  int mh, mb;  // 1: the axis is there
+};
+
+// False when the tensor cannot be mapped; its tiles then move by cp.async.
+bool map_rows(RowsMap* m, const void* p, Ty ty, const Str3& s, int B, int heads, int T, int D, int rows) {
+  if (T < rows || s.t <= 0 || !encode_fn()) return false;
+  m->mh = heads > 1 && s.h != 0;
+  m->mb = B > 1 && s.b != 0;
+  const cuuint64_t pad = ((cuuint64_t)D * 2 + 15) / 16 * 16;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)(m->mh ? heads : 1),
+                              (cuuint64_t)(m->mb ? B : 1)};
+  const cuuint64_t strides[3] = {(cuuint64_t)s.t * 2, m->mh ? (cuuint64_t)s.h * 2 : pad,
+                                 m->mb ? (cuuint64_t)s.b * 2 : pad};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, es[4] = {1, 1, 1, 1};
+  return encode_fn()(&m->map, ty == Ty::F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                     const_cast<void*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// One tile of whole valid rows by TMA (one thread); its bytes count on `bar`.
+template <int DP>
+__device__ __forceinline__ void tma_tile(uint32_t dst, uint32_t chunk, const RowsMap& m, uint32_t bar, int row, int h,
+                                         int b) {
+#pragma unroll
+  for (int c = 0; c < (DP + 63) / 64; ++c)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst + c * chunk),
+        "l"(reinterpret_cast<uint64_t>(&m.map)), "r"(bar), "r"(c * 64), "r"(row), "r"(h * m.mh), "r"(b * m.mb)
+        : "memory");
 }
 
 template <int N>

@@ -12,9 +12,11 @@
 // That is 7 products for 5, the price of giving every gradient element one
 // owner: no atomics, no fp32 copy of dq in memory, and bits that repeat.
 //
-// S and dP have two buffers: warps 0-3 and 4-7 take alternate tiles (one row
-// per thread), while warp 8 issues the next tile's score products before it
-// waits for this tile's operands.  Warps 9 and 10 load tiles.
+// S and dP have two buffers: warp 8 issues the next tile's score products
+// before it waits for this tile's operands.  Warps 0-3 and 4-7 take one half of
+// a tile's columns each, one row per thread, which halves the time from scores
+// to operands (alternate tiles per group: 2870 cycles a tile on the long causal
+// case).  Warps 9 and 10 load tiles.
 //
 // Rounding: P and dS are rounded to the operands' type.  fp16 holds 2^-24 to
 // 2^15 only, so P is carried as 2^15 P and dS with a power of two per head,
@@ -29,6 +31,7 @@ namespace {
 __device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out
 
 constexpr int kBA = 128, kBB = 64;  // rows of the resident and of the streamed tiles
+constexpr int kHalfB = kBB / 2;
 constexpr int kThreads = 384;
 
 template <int DP, bool REL>
@@ -36,8 +39,8 @@ struct BwdCfg {
   static constexpr int NC = (DP + 63) / 64;
   static constexpr uint32_t chunkA = kBA * 128, chunkB = kBB * 128, chunkR = 32 * 128;
   static constexpr uint32_t tileA = NC * chunkA, tileB = NC * chunkB;
-  static constexpr int ST = 3;
-  static constexpr uint32_t rows = 2 * kBB * 4;  // lse2 and delta of a streamed query tile
+  static constexpr int ST = NC == 2 && REL ? 3 : 4;
+  static constexpr uint32_t rows = 2 * kBB * 4;  // nlse2 and ndelta of a streamed query tile
   static constexpr uint32_t rel = REL ? 2 * kBB * 32 * 4 : 0;  // its relative products (up to 32 offsets)
   static constexpr uint32_t stage = 2 * tileB;
   static constexpr uint32_t relk = REL ? NC * chunkR : 0;
@@ -48,15 +51,25 @@ struct BwdCfg {
 };
 
 struct BwdBars {
-  uint64_t a_full, b_full[3], b_free[3], s_full[2], p_full[2], acc_full;
+  uint64_t a_full, r_full, b_full[4], b_free[4], s_full[2], p_full[2], acc_full;
 };
 
 __device__ __forceinline__ void cp_async4(uint32_t dst, const float* src, bool in) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
 }
 
+// Tensor maps of the resident (128-row boxes) and the streamed tiles (64-row
+// boxes); `on`: full tiles come by TMA, the rest (tails, whose rows behind a
+// length must read as zeros) by cp.async.
+struct BwdMaps {
+  RowsMap qa, ka, va, ga, qb, kb, vb, gb;
+  bool a_on, b_on;
+};
+
 template <typename T, int DP, bool REL>
-__global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const AttnArgs a, const BwdWs ws, const int nk,
+__global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant__ AttnArgs a,
+                                                           const __grid_constant__ BwdWs ws,
+                                                           const __grid_constant__ BwdMaps maps, const int nk,
                                                            const bool vec, const bool ovec) {
   using C = BwdCfg<DP, REL>;
   constexpr int ST = C::ST;
@@ -95,14 +108,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const AttnArgs a, con
 
   if (threadIdx.x == 0) {
     s_abort = 0;
-    mbar_init(bar(bars.a_full), kLoaders);
+    mbar_init(bar(bars.a_full), 2);
+    mbar_init(bar(bars.r_full), 2);
     for (int s = 0; s < ST; ++s) {
-      mbar_init(bar(bars.b_full[s]), kLoaders);
+      mbar_init(bar(bars.b_full[s]), 2);
       mbar_init(bar(bars.b_free[s]), 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(bar(bars.s_full[s]), 1);
-      mbar_init(bar(bars.p_full[s]), 128);
+      mbar_init(bar(bars.p_full[s]), 8);
     }
     mbar_init(bar(bars.acc_full), 1);
     fence_async_smem();
@@ -143,45 +157,51 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const AttnArgs a, con
     if (nt > 0 && warp == 8) {
       if (lane == 0) {
         constexpr uint32_t id_s = idesc_attn<T>(kBB, false), id_a = idesc_attn<T>(DP, true);
+        const uint64_t dA0 = sdesc<64>(sA0), dA1 = sdesc<64>(sA1), dB = sdesc<64>(sB), mB = desc_mn(sB, C::chunkB);
         bool ok = mbar_wait_fast(bar(bars.a_full), 0, abort);
+        int fs = 0, fr = 0, us = 0;  // stage and round to fill from next, stage in use
         auto scores = [&](int t) {
-          const int s = t % ST;
-          ok = ok && mbar_wait_fast(bar(bars.b_full[s]), (t / ST) & 1, abort);
+          const int s = fs;
+          ok = ok && mbar_wait_fast(bar(bars.b_full[s]), fr & 1, abort);
           if (!ok) return;
+          if (++fs == ST) fs = 0, ++fr;
           tc_fence_after();
-          const uint32_t d = tS + (t & 1) * 2 * kBB, b0 = sB + s * C::stage, b1 = b0 + C::tileB;
-#pragma unroll
-          for (int c = 0; c < DP / 16; ++c)
-            mma_bf16(d, sdesc<64>(sA0 + (c >> 2) * C::chunkA + (c & 3) * 32),
-                     sdesc<64>(b0 + (c >> 2) * C::chunkB + (c & 3) * 32), id_s, c > 0);
-#pragma unroll
-          for (int c = 0; c < DP / 16; ++c)
-            mma_bf16(d + kBB, sdesc<64>(sA1 + (c >> 2) * C::chunkA + (c & 3) * 32),
-                     sdesc<64>(b1 + (c >> 2) * C::chunkB + (c & 3) * 32), id_s, c > 0);
+          const uint32_t d = tS + (t & 1) * 2 * kBB;
+          const uint64_t b0 = dB + s * (C::stage >> 4);
+          mma_rows<DP>(d, dA0, C::chunkA, b0, C::chunkB, id_s);
+          mma_rows<DP>(d + kBB, dA1, C::chunkA, b0 + (C::tileB >> 4), C::chunkB, id_s);
           mma_commit(bar(bars.s_full[t & 1]));
         };
         scores(0);
         for (int t = 0; t < nt && ok; ++t) {
           if (t + 1 < nt) scores(t + 1);
-          const int s = t % ST;
+          const int s = us;
+          if (++us == ST) us = 0;
           ok = ok && mbar_wait_fast(bar(bars.p_full[t & 1]), (t >> 1) & 1, abort);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t p = tS + (t & 1) * 2 * kBB, b0 = sB + s * C::stage, b1 = b0 + C::tileB;
-          if (keys)
-            for (int c = 0; c < kBB / 16; ++c)
-              mma_ts(tAcc0, p + c * 8, desc_mn(b1 + c * 2048, C::chunkB), id_a, t > 0 || c > 0);
-          for (int c = 0; c < kBB / 16; ++c)
-            mma_ts(tAcc1, p + kBB + c * 8, desc_mn(b0 + c * 2048, C::chunkB), id_a, t > 0 || c > 0);
+          const uint32_t p = tS + (t & 1) * 2 * kBB;
+          const uint64_t m0 = mB + s * (C::stage >> 4), m1 = m0 + (C::tileB >> 4);
+          // Each group's 32 operand columns lie over the first half of its own scores.
+          auto accumulate = [&](uint32_t acc, uint32_t op, uint64_t m) {
+            if (t == 0) mma_ts_first(acc, op, m, id_a);
+            else mma_ts_acc(acc, op, m, id_a);
+#pragma unroll
+            for (int c = 1; c < kBB / 16; ++c)
+              mma_ts_acc(acc, op + (c >> 1) * kHalfB + (c & 1) * 8, m + c * (2048 >> 4), id_a);
+          };
+          if (keys) accumulate(tAcc0, p, m1);
+          accumulate(tAcc1, p + kBB, m0);
           mma_commit(bar(bars.b_free[s]));
         }
         if (REL && !keys && ok) {
           // dq += (near ds) relk; the operand comes over the buffer of tile nt, in its order.
-          ok = mbar_wait_fast(bar(bars.p_full[nt & 1]), (nt >> 1) & 1, abort);
+          ok = mbar_wait_fast(bar(bars.r_full), 0, abort) &&
+               mbar_wait_fast(bar(bars.p_full[nt & 1]), (nt >> 1) & 1, abort);
           tc_fence_after();
           if (ok)
             for (int c = 0; c < (a.nrel + 15) / 16; ++c)
-              mma_ts(tAcc1, tS + (nt & 1) * 2 * kBB + c * 8, desc_mn(sR + c * 2048, C::chunkR), id_a, 1);
+              mma_ts_acc(tAcc1, tS + (nt & 1) * 2 * kBB + c * 8, desc_mn(sR + c * 2048, C::chunkR), id_a);
         }
         mma_commit(bar(bars.acc_full));
         if (!ok) raise_err(&g_gave_up, abort, 1);
@@ -196,50 +216,89 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const AttnArgs a, con
       const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
       const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
       const T* dout = static_cast<const T*>(a.dout) + b * a.sdo.b;
-      if (keys) {
-        load_tile<T, DP, kBA>(sA0, C::chunkA, k + (int64_t)r0 * a.sk.t, a.sk.t, kl - r0, D, vec, tid);
-        load_tile<T, DP, kBA>(sA1, C::chunkA, v + (int64_t)r0 * a.sv.t, a.sv.t, kl - r0, D, vec, tid);
-      } else {
-        const int h = blockIdx.y;
-        load_tile<T, DP, kBA>(sA0, C::chunkA, q + h * a.sq.h + (int64_t)r0 * a.sq.t, a.sq.t, ql - r0, D, vec, tid);
-        load_tile<T, DP, kBA>(sA1, C::chunkA, dout + h * a.sdo.h + (int64_t)r0 * a.sdo.t, a.sdo.t, ql - r0, D, vec, tid);
-        if (REL)
-          load_tile<T, DP, 32>(sR, C::chunkR, static_cast<const T*>(a.relk), D, a.nrel, D, vec, tid);
-      }
-      ho.next(bar(bars.a_full));
-      int hh = 0, x = first;
-      for (int t = 0; t < nt; ++t) {
-        const int s = t % ST, i0 = x * kBB;
-        const uint32_t b0 = sB + s * C::stage, b1 = b0 + C::tileB;
-        if (t >= ST) ok = ho.wait_free(bar(bars.b_free[s]), (t / ST - 1) & 1, abort);
-        if (!ok) break;
+      const bool tma_warp = warp == 9;
+      // A pair of full tiles: the first loader warp's lane 0 issues it.
+      auto pair = [&](uint32_t d0, uint32_t d1, uint32_t chunk, uint32_t bytes, const RowsMap& m0, const RowsMap& m1,
+                      uint32_t full, int row, int h) {
+        if (lane == 0) {
+          mbar_expect_tx(full, bytes);
+          tma_tile<DP>(d0, chunk, m0, full, row, h, b);
+          tma_tile<DP>(d1, chunk, m1, full, row, h, b);
+        }
+      };
+      const bool full_a = maps.a_on && r0 + kBA <= (keys ? kl : ql);
+      const uint32_t a_full = bar(bars.a_full);
+      if (full_a && tma_warp)
+        pair(sA0, sA1, C::chunkA, 2 * C::tileA, keys ? maps.ka : maps.qa, keys ? maps.va : maps.ga, a_full, r0,
+             keys ? hk : (int)blockIdx.y);
+      if (!full_a) {
         if (keys) {
-          const int h = hk * g + hh;
+          load_tile<T, DP, kBA>(sA0, C::chunkA, k + (int64_t)r0 * a.sk.t, a.sk.t, kl - r0, D, vec, tid);
+          load_tile<T, DP, kBA>(sA1, C::chunkA, v + (int64_t)r0 * a.sv.t, a.sv.t, kl - r0, D, vec, tid);
+        } else {
+          const int h = blockIdx.y;
+          load_tile<T, DP, kBA>(sA0, C::chunkA, q + h * a.sq.h + (int64_t)r0 * a.sq.t, a.sq.t, ql - r0, D, vec, tid);
+          load_tile<T, DP, kBA>(sA1, C::chunkA, dout + h * a.sdo.h + (int64_t)r0 * a.sdo.t, a.sdo.t, ql - r0, D, vec,
+                                tid);
+        }
+      }
+      if (!full_a || !tma_warp) ho.next(a_full);
+      if (REL && !keys) {  // needed last: a barrier of its own
+        load_tile<T, DP, 32>(sR, C::chunkR, static_cast<const T*>(a.relk), D, a.nrel, D, vec, tid);
+        ho.next(bar(bars.r_full));
+      }
+      int hh = 0, x = first, s = 0, round = 0;
+      for (int t = 0; t < nt; ++t) {
+        const int i0 = x * kBB;
+        const uint32_t b0 = sB + s * C::stage, b1 = b0 + C::tileB, full = bar(bars.b_full[s]);
+        if (round > 0) ok = ho.wait_free(bar(bars.b_free[s]), (round - 1) & 1, abort);
+        if (!ok) break;
+        const int h = keys ? hk * g + hh : hk;
+        const bool whole = maps.b_on && i0 + kBB <= (keys ? ql : kl);
+        if (whole) {
+          if (tma_warp)
+            pair(b0, b1, C::chunkB, 2 * C::tileB, keys ? maps.qb : maps.kb, keys ? maps.gb : maps.vb, full, i0, h);
+        } else if (keys) {
           load_tile<T, DP, kBB>(b0, C::chunkB, q + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t, ql - i0, D, vec, tid);
-          load_tile<T, DP, kBB>(b1, C::chunkB, dout + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t, ql - i0, D, vec, tid);
+          load_tile<T, DP, kBB>(b1, C::chunkB, dout + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t, ql - i0, D, vec,
+                                tid);
+        } else {
+          load_tile<T, DP, kBB>(b0, C::chunkB, k + (int64_t)i0 * a.sk.t, a.sk.t, kl - i0, D, vec, tid);
+          load_tile<T, DP, kBB>(b1, C::chunkB, v + (int64_t)i0 * a.sv.t, a.sv.t, kl - i0, D, vec, tid);
+        }
+        if (keys && !tma_warp) {
           const int64_t row = row_h0 + (int64_t)hh * a.Tq + i0;
           const uint32_t tab = sTab + s * (C::rows + C::rel);
-          for (int e = tid; e < 2 * kBB; e += kLoaders) {
+#pragma unroll
+          for (int e = lane; e < 2 * kBB; e += 32) {
             const int c = e & (kBB - 1);
             const bool in = i0 + c < a.Tq;
-            cp_async4(tab + e * 4, (e < kBB ? ws.lse2 : ws.delta) + (in ? row + c : 0), in);
+            cp_async4(tab + e * 4, (e < kBB ? ws.nlse2 : ws.ndelta) + (in ? row + c : 0), in);
           }
           if (REL) {
             // Offsets of this pair of tiles: from r0 - (i0 + 63 + off) to r0 + 127 - (i0 + off).
             const int lo = r0 - (i0 + kBB - 1 + off), hi = r0 + kBA - 1 - (i0 + off);
             if (lo <= a.window && hi >= -a.window)
-              for (int e = tid; e < kBB * a.nrel; e += kLoaders) {
+              for (int e = lane; e < kBB * a.nrel; e += 32) {
                 const bool in = i0 + e / a.nrel < a.Tq;
                 const int64_t at = in ? row * a.nrel + e : 0;
                 cp_async4(tab + C::rows + e * 4, ws.qrel + at, in);
                 cp_async4(tab + C::rows + (kBB * 32 + e) * 4, ws.grel + at, in);
               }
           }
-        } else {
-          load_tile<T, DP, kBB>(b0, C::chunkB, k + (int64_t)i0 * a.sk.t, a.sk.t, kl - i0, D, vec, tid);
-          load_tile<T, DP, kBB>(b1, C::chunkB, v + (int64_t)i0 * a.sv.t, a.sv.t, kl - i0, D, vec, tid);
         }
-        ho.next(bar(bars.b_full[s]));
+        if (whole && tma_warp) {
+          ho.flush();
+        } else if (whole && !keys) {
+          ho.flush();
+          warp_arrive(full);
+        } else {
+          ho.next(full);
+        }
+        if (++s == ST) {
+          s = 0;
+          ++round;
+        }
         if (++x == first + per) {
           x = first;
           ++hh;
@@ -250,75 +309,86 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const AttnArgs a, con
       if (!ok) raise_err(&g_gave_up, abort, 1);
     }
   } else {
-    const int wg = warp >> 2, row = threadIdx.x & 127, own = r0 + row;
+    const int wg = warp >> 2, row = threadIdx.x & 127, own = r0 + row, c0 = wg * kHalfB;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;
     const float sl2 = a.scale * kLog2e, gp = gs * exp2f(-kShift);
+    const F2 sl(sl2, sl2), gp2(gp, gp);
     bool ok = true;
     if (keys) {
-      int x = first + wg;  // streamed tile within its head
-      for (int t = wg; t < nt && ok; t += 2, x += 2) {
-        while (x >= first + per) x -= per;
-        ok = warp_wait(bar(bars.s_full[wg]), (t >> 1) & 1, abort);
+      int x = first, st = 0, round = 0;  // streamed tile within its head; its stage
+      for (int t = 0; t < nt; ++t) {
+        ok = warp_wait(bar(bars.s_full[t & 1]), (t >> 1) & 1, abort);
         // The tables of the stage: written by the loaders, who signalled b_full before the MMAs began.
-        ok = ok && warp_wait(bar(bars.b_full[t % ST]), (t / ST) & 1, abort);
+        ok = ok && warp_wait(bar(bars.b_full[st]), round & 1, abort);
         if (!ok) break;
         tc_fence_after();
-        const int i0 = x * kBB;
-        const float* lse2 = tables + (t % ST) * ((C::rows + C::rel) / 4);
-        const float* delta = lse2 + kBB;
-        const float* qrel = lse2 + 2 * kBB;
-        const float* grel = qrel + kBB * 32;
-        const int d0 = own - (i0 + off) + a.window;       // offset index of column 0; falls by one per column
-        const int skip = a.causal ? own - off - i0 : 0;   // columns before it do not see this key
-        const bool near = REL && __any_sync(0xffffffffu, d0 >= 0 && d0 - (kBB - 1) < a.nrel);
-        const bool cut = __any_sync(0xffffffffu, skip > 0);
-        const uint32_t tb = tS + wg * 2 * kBB + lanes;
-#pragma unroll 1
-        for (int c0 = 0; c0 < kBB; c0 += 32) {
-          float s[32], dp[32];
-          tmem_load32(tb + c0, s);
-          tmem_load32(tb + kBB + c0, dp);
-          if (near) {
+        const int i0 = x * kBB + c0;  // query of this group's column 0
+        if (++x == first + per) x = first;
+        const float* tab = tables + st * ((C::rows + C::rel) / 4);
+        if (++st == ST) st = 0, ++round;
+        const float* nlse2 = tab + c0;
+        const float* ndelta = tab + kBB + c0;
+        const uint32_t tb = tS + (t & 1) * 2 * kBB + lanes;
+        float s[kHalfB], dp[kHalfB];
+        tmem_load32(tb + c0, s);
+        tmem_load32(tb + kBB + c0, dp);
+        if (REL) {
+          const float* qrel = tab + 2 * kBB + c0 * a.nrel;
+          const float* grel = qrel + kBB * 32;
+          const int d0 = own - (i0 + off) + a.window;  // offset index of column 0; falls by one per column
+          if (__any_sync(0xffffffffu, d0 >= 0 && d0 - (kHalfB - 1) < a.nrel)) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const unsigned r = (unsigned)(d0 - c0 - c);
+            for (int c = 0; c < kHalfB; ++c) {
+              const unsigned r = (unsigned)(d0 - c);
               if (r < (unsigned)a.nrel) {
-                s[c] += qrel[(c0 + c) * a.nrel + r];
-                dp[c] += grel[(c0 + c) * a.nrel + r];
+                s[c] += qrel[c * a.nrel + r];
+                dp[c] += grel[c * a.nrel + r];
               }
             }
           }
-          uint32_t p2[16], d2[16];
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const float4 L = *reinterpret_cast<const float4*>(lse2 + c0 + c);
-            const float4 E = *reinterpret_cast<const float4*>(delta + c0 + c);
-            const float l4[4] = {L.x, L.y, L.z, L.w}, e4[4] = {E.x, E.y, E.z, E.w};
-            float p[4], d[4];
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              p[y] = ex2(fmaf(s[c + y], sl2, kShift - l4[y]));
-              if (cut && c0 + c + y < skip) p[y] = 0.f;
-              d[y] = kHalf ? p[y] * (gp * (dp[c + y] - e4[y])) : p[y] * (dp[c + y] - e4[y]);
-            }
-            p2[c / 2] = pack2<T>(p[0], p[1]);
-            p2[c / 2 + 1] = pack2<T>(p[2], p[3]);
-            d2[c / 2] = pack2<T>(d[0], d[1]);
-            d2[c / 2 + 1] = pack2<T>(d[2], d[3]);
-          }
-          tmem_store16(tb + c0 / 2, p2);
-          tmem_store16(tb + kBB + c0 / 2, d2);
         }
+        float p[kHalfB];
+#pragma unroll
+        for (int c = 0; c < kHalfB; c += 4) {
+          const float4 L = *reinterpret_cast<const float4*>(nlse2 + c);
+          fma2(F2(s[c], s[c + 1]), sl, F2(L.x, L.y)).get(p[c], p[c + 1]);
+          fma2(F2(s[c + 2], s[c + 3]), sl, F2(L.z, L.w)).get(p[c + 2], p[c + 3]);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) p[c + y] = ex2(p[c + y]);
+        }
+        const int skip = a.causal ? own - off - i0 : 0;  // columns before it do not see this key
+        if (__any_sync(0xffffffffu, skip > 0)) {
+#pragma unroll
+          for (int c = 0; c < kHalfB; ++c)
+            if (c < skip) p[c] = 0.f;
+        }
+        uint32_t p2[kHalfB / 2], d2[kHalfB / 2];
+#pragma unroll
+        for (int c = 0; c < kHalfB; c += 4) {
+          const float4 E = *reinterpret_cast<const float4*>(ndelta + c);
+          F2 u = add2(F2(dp[c], dp[c + 1]), F2(E.x, E.y)), w = add2(F2(dp[c + 2], dp[c + 3]), F2(E.z, E.w));
+          if (kHalf) u = mul2(u, gp2), w = mul2(w, gp2);
+          float d[4];
+          mul2(u, F2(p[c], p[c + 1])).get(d[0], d[1]);
+          mul2(w, F2(p[c + 2], p[c + 3])).get(d[2], d[3]);
+          p2[c / 2] = pack2<T>(p[c], p[c + 1]);
+          p2[c / 2 + 1] = pack2<T>(p[c + 2], p[c + 3]);
+          d2[c / 2] = pack2<T>(d[0], d[1]);
+          d2[c / 2 + 1] = pack2<T>(d[2], d[3]);
+        }
+        tmem_store16(tb + c0, p2);
+        tmem_store16(tb + kBB + c0, d2);
         tmem_store_wait();
         tc_fence_before();
-        mbar_arrive(bar(bars.p_full[wg]));
+        warp_arrive(bar(bars.p_full[t & 1]));
       }
     } else {
       const int n = allowed_keys(own, ql, kl, a.causal);
       const int64_t qrow = row_h0 + own;
-      const float lse2 = n > 0 ? ws.lse2[qrow] : INFINITY, delta = n > 0 ? ws.delta[qrow] : 0.f;
+      const float nlse2 = n > 0 ? ws.nlse2[qrow] : -INFINITY, ndelta = n > 0 ? ws.ndelta[qrow] : 0.f;
+      const F2 nl(nlse2, nlse2), nd(ndelta, ndelta);
       float* tq = tables;               // q . relk by offset, [nrel][128]
-      float* tg = tables + 32 * kBA;    // do . relv, then the near ds
+      float* tg = tables + 32 * kBA;    // do . relv, then the near ds as carried
       if (REL && nt > 0) {
         for (int r = wg; r < a.nrel; r += 2) {
           tq[r * kBA + row] = n > 0 ? ws.qrel[qrow * a.nrel + r] : 0.f;
@@ -326,75 +396,84 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const AttnArgs a, con
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
-      for (int t = wg; t < nt && ok; t += 2) {
-        ok = warp_wait(bar(bars.s_full[wg]), (t >> 1) & 1, abort);
+      for (int t = 0; t < nt; ++t) {
+        ok = warp_wait(bar(bars.s_full[t & 1]), (t >> 1) & 1, abort);
         if (!ok) break;
         tc_fence_after();
-        const int j0 = t * kBB, lim = n - j0;
+        const int j0 = t * kBB + c0, lim = n - j0;
         const int d0 = j0 - (own + off) + a.window;
-        const bool near = REL && __any_sync(0xffffffffu, d0 < a.nrel && d0 + kBB > 0);
-        const bool cut = __any_sync(0xffffffffu, lim < kBB);
-        const uint32_t tb = tS + wg * 2 * kBB + lanes;
-#pragma unroll 1
-        for (int c0 = 0; c0 < kBB; c0 += 32) {
-          float s[32], dp[32];
-          tmem_load32(tb + c0, s);
-          tmem_load32(tb + kBB + c0, dp);
-          uint32_t d2[16];
-          if (near) {
+        const bool near = REL && __any_sync(0xffffffffu, d0 < a.nrel && d0 + kHalfB > 0);
+        const uint32_t tb = tS + (t & 1) * 2 * kBB + lanes;
+        float s[kHalfB], dp[kHalfB];
+        tmem_load32(tb + c0, s);
+        tmem_load32(tb + kBB + c0, dp);
+        if (near) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const unsigned r = (unsigned)(d0 + c0 + c);
-              if (r < (unsigned)a.nrel) {
-                s[c] += tq[r * kBA + row];
-                dp[c] += tg[r * kBA + row];
-              }
+          for (int c = 0; c < kHalfB; ++c) {
+            const unsigned r = (unsigned)(d0 + c);
+            if (r < (unsigned)a.nrel) {
+              s[c] += tq[r * kBA + row];
+              dp[c] += tg[r * kBA + row];
             }
           }
-          float d[32];
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            float p = ex2(fmaf(s[c], sl2, -lse2));
-            if (cut && c0 + c >= lim) p = 0.f;
-            d[c] = p * (dp[c] - delta);
-            if (near) {
-              const unsigned r = (unsigned)(d0 + c0 + c);
-              if (r < (unsigned)a.nrel && c0 + c < lim) {
-                ws.pband[qrow * a.nrel + r] = p;
-                ws.sband[qrow * a.nrel + r] = d[c];
-                tg[r * kBA + row] = d[c];
-              }
-            }
-            if (kHalf) d[c] *= gs;
-          }
-#pragma unroll
-          for (int c = 0; c < 32; c += 2) d2[c / 2] = pack2<T>(d[c], d[c + 1]);
-          tmem_store16(tb + kBB + c0 / 2, d2);
         }
+        float d[kHalfB];
+#pragma unroll
+        for (int c = 0; c < kHalfB; c += 2) {
+          fma2(F2(s[c], s[c + 1]), sl, nl).get(s[c], s[c + 1]);
+          s[c] = ex2(s[c]);
+          s[c + 1] = ex2(s[c + 1]);
+        }
+        if (__any_sync(0xffffffffu, lim < kHalfB)) {
+#pragma unroll
+          for (int c = 0; c < kHalfB; ++c)
+            if (c >= lim) s[c] = 0.f;
+        }
+        uint32_t d2[kHalfB / 2];
+#pragma unroll
+        for (int c = 0; c < kHalfB; c += 2) {
+          F2 u = add2(F2(dp[c], dp[c + 1]), nd);
+          if (kHalf) u = mul2(u, gp2);
+          mul2(u, F2(s[c], s[c + 1])).get(d[c], d[c + 1]);
+          d2[c / 2] = pack2<T>(d[c], d[c + 1]);
+        }
+        if (near) {
+          const float up = exp2f(-kShift), ud = 1.f / gs;
+#pragma unroll
+          for (int c = 0; c < kHalfB; ++c) {
+            const unsigned r = (unsigned)(d0 + c);
+            if (r < (unsigned)a.nrel && c < lim) {
+              ws.pband[qrow * a.nrel + r] = s[c] * up;
+              ws.sband[qrow * a.nrel + r] = d[c] * ud;
+              tg[r * kBA + row] = d[c];
+            }
+          }
+        }
+        tmem_store16(tb + kBB + c0, d2);
         tmem_store_wait();
         tc_fence_before();
-        mbar_arrive(bar(bars.p_full[wg]));
+        warp_arrive(bar(bars.p_full[t & 1]));
       }
       if (REL && nt > 0) {
         asm volatile("bar.sync 1, 256;" ::: "memory");  // the near ds of both groups are in the table
-        if (wg == (nt & 1) && ok) {
-          // The score columns of the buffer: this group was their last reader.
+        if (ok) {
+          // Over the score columns of the buffer of tile nt, whose last readers were these warps.
           const int jb = own + off - a.window;
-          for (int q0 = 0; q0 < a.nrel && ok; q0 += 16) {
+          for (int q0 = wg * 16; q0 < a.nrel; q0 += 32) {
             float d[16];
 #pragma unroll
             for (int y = 0; y < 16; ++y) {
               const int r = q0 + y, j = jb + r;
-              d[y] = r < a.nrel && j >= 0 && j < n ? tg[r * kBA + row] * gs : 0.f;
+              d[y] = r < a.nrel && j >= 0 && j < n ? tg[r * kBA + row] : 0.f;
             }
             uint32_t u[8];
 #pragma unroll
             for (int y = 0; y < 8; ++y) u[y] = pack2<T>(d[2 * y], d[2 * y + 1]);
-            tmem_store8(tS + wg * 2 * kBB + lanes + q0 / 2, u);
+            tmem_store8(tS + (nt & 1) * 2 * kBB + lanes + q0 / 2, u);
           }
           tmem_store_wait();
           tc_fence_before();
-          if (ok) mbar_arrive(bar(bars.p_full[wg]));
+          warp_arrive(bar(bars.p_full[nt & 1]));
         }
       }
     }
@@ -453,7 +532,18 @@ cudaError_t launch(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
   const bool ovec = attn_rows_aligned(a.dq, a.sdq, a.D, 2) && attn_rows_aligned(a.dk, a.sdk, a.D, 2) &&
                     attn_rows_aligned(a.dv, a.sdv, a.D, 2);
   const int nk = cdiv(a.Tk, kBA), nq = cdiv(a.Tq, kBA);
-  attn_bwd_tc<T, DP, REL><<<dim3(nk + nq, a.H, a.B), kThreads, smem, st>>>(a, ws, nk, vec, ovec);
+  BwdMaps m = {};
+  if (vec) {
+    m.a_on = map_rows(&m.qa, a.q, a.ty, a.sq, a.B, a.H, a.Tq, a.D, kBA) &&
+             map_rows(&m.ga, a.dout, a.ty, a.sdo, a.B, a.H, a.Tq, a.D, kBA) &&
+             map_rows(&m.ka, a.k, a.ty, a.sk, a.B, a.Hkv, a.Tk, a.D, kBA) &&
+             map_rows(&m.va, a.v, a.ty, a.sv, a.B, a.Hkv, a.Tk, a.D, kBA);
+    m.b_on = map_rows(&m.qb, a.q, a.ty, a.sq, a.B, a.H, a.Tq, a.D, kBB) &&
+             map_rows(&m.gb, a.dout, a.ty, a.sdo, a.B, a.H, a.Tq, a.D, kBB) &&
+             map_rows(&m.kb, a.k, a.ty, a.sk, a.B, a.Hkv, a.Tk, a.D, kBB) &&
+             map_rows(&m.vb, a.v, a.ty, a.sv, a.B, a.Hkv, a.Tk, a.D, kBB);
+  }
+  attn_bwd_tc<T, DP, REL><<<dim3(nk + nq, a.H, a.B), kThreads, smem, st>>>(a, ws, m, nk, vec, ovec);
   return cudaGetLastError();
 }
 

@@ -49,8 +49,17 @@ struct FwdBars {
   uint64_t q_full, k_full[2], k_free[2], v_full[2], v_free[2], s_full, s_free, p_full, o_full, pv_done;
 };
 
+// Full tiles come by TMA (`on`), the rest (tails, whose rows behind a length
+// must read as zeros) by cp.async.
+struct FwdMaps {
+  RowsMap q, k, v;
+  bool q_on, kv_on;
+};
+
 template <typename T, int DP, bool REL>
-__global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, const bool vec, const bool ovec) {
+__global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_constant__ AttnArgs a,
+                                                              const __grid_constant__ FwdMaps maps, const bool vec,
+                                                              const bool ovec) {
   using C = FwdCfg<DP>;
   constexpr int ST = C::ST;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -73,16 +82,16 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
 
   if (threadIdx.x == 0) {
     s_abort = 0;
-    mbar_init(bar(bars.q_full), kLoaders);
+    mbar_init(bar(bars.q_full), 2);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(bar(bars.k_full[s]), kLoaders);
-      mbar_init(bar(bars.v_full[s]), kLoaders);
+      mbar_init(bar(bars.k_full[s]), 2);
+      mbar_init(bar(bars.v_full[s]), 2);
       mbar_init(bar(bars.k_free[s]), 1);
       mbar_init(bar(bars.v_free[s]), 1);
     }
     mbar_init(bar(bars.s_full), 1);
-    mbar_init(bar(bars.p_full), kBM);
-    mbar_init(bar(bars.s_free), kBM);
+    mbar_init(bar(bars.p_full), 4);
+    mbar_init(bar(bars.s_free), 4);
     mbar_init(bar(bars.o_full), 1);
     mbar_init(bar(bars.pv_done), 1);
     fence_async_smem();
@@ -99,6 +108,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
     if (nt > 0 && warp == 4) {
       if (lane == 0) {
         constexpr uint32_t id_s = idesc_attn<T>(kBN, false), id_o = idesc_attn<T>(DP, true);
+        const uint64_t dQ = sdesc<64>(sQ), dK = sdesc<64>(sK), mV = desc_mn(sV, C::chunk);
         bool ok = mbar_wait_fast(bar(bars.q_full), 0, abort);
         int kt = 0, vt = 0, pp = 0, sf = 0;
         auto scores = [&](uint32_t id) {  // S = q . (tile kt)^T
@@ -106,11 +116,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
           ok = ok && mbar_wait_fast(bar(bars.k_full[s]), (kt / ST) & 1, abort);
           if (!ok) return;
           tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < DP / 16; ++c) {
-            const uint32_t o = (c >> 2) * C::chunk + (c & 3) * 32;
-            mma_bf16(tS, sdesc<64>(sQ + o), sdesc<64>(sK + s * C::tile + o), id, c > 0);
-          }
+          mma_rows<DP>(tS, dQ, C::chunk, dK + s * (C::tile >> 4), C::chunk, id);
           mma_commit(bar(bars.k_free[s]));
           mma_commit(bar(bars.s_full));
           ++kt;
@@ -120,15 +126,18 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
           ++sf;
           tc_fence_after();
         };
-        auto values = [&](int rows, uint32_t acc) {  // O += P . (tile vt)
+        auto values = [&](auto rows, bool first) {  // O (+)= P . (tile vt)
           const int s = vt % ST;
           ok = ok && mbar_wait_fast(bar(bars.v_full[s]), (vt / ST) & 1, abort);
           ok = ok && mbar_wait_fast(bar(bars.p_full), pp & 1, abort);
           ++pp;
           if (!ok) return;
           tc_fence_after();
-          for (int c = 0; c < rows / 16; ++c)
-            mma_ts(tO, tP + c * 8, desc_mn(sV + s * C::tile + c * 2048, C::chunk), id_o, acc | (c > 0));
+          const uint64_t m = mV + s * (C::tile >> 4);
+          if (first) mma_ts_first(tO, tP, m, id_o);
+          else mma_ts_acc(tO, tP, m, id_o);
+#pragma unroll
+          for (int c = 1; c < rows / 16; ++c) mma_ts_acc(tO, tP + c * 8, m + c * (2048 >> 4), id_o);
           mma_commit(bar(bars.v_free[s]));
           if (C::own_p) mma_commit(bar(bars.pv_done));
           ++vt;
@@ -145,11 +154,11 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
           } else {
             scores(id_s);
           }
-          values(kBN, t > 0);
+          values(std::integral_constant<int, kBN>(), t == 0);
         }
         mma_commit(bar(bars.o_full));
         if (REL && ok) {
-          values(nrp, 1);
+          values(nrp, false);
           mma_commit(bar(bars.o_full));
         }
         if (!ok) raise_err(&g_gave_up, abort, 1);
@@ -159,7 +168,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
       __syncwarp();
     } else if (nt > 0 && warp < 7) {
       const int tid = threadIdx.x - 5 * 32;
-      const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + (int64_t)i0 * a.sq.t;
+      const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h;
       const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
       const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
       Handover ho;
@@ -171,8 +180,25 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
         if (n >= ST) ok = ho.wait_free(bar(is_k ? bars.k_free[s] : bars.v_free[s]), (n / ST - 1) & 1, abort);
         return ok ? (is_k ? sK : sV) + s * C::tile : 0;
       };
-      load_tile<T, DP, kBM>(sQ, C::chunk, q, a.sq.t, ql - i0, D, vec, tid);
-      ho.next(bar(bars.q_full));
+      // One tile: by TMA from the first loader warp, or by both warps' copies.
+      auto fetch = [&](uint32_t dst, uint32_t full, bool on, const RowsMap& m, int head, const T* p, int64_t stride,
+                       int row, int valid) {
+        if (on && row + kBM <= valid) {
+          ho.flush();
+          if (warp == 5) {
+            if (lane == 0) {
+              mbar_expect_tx(full, C::tile);
+              tma_tile<DP>(dst, C::chunk, m, full, row, head, b);
+            }
+          } else {
+            warp_arrive(full);
+          }
+        } else {
+          load_tile<T, DP, kBM>(dst, C::chunk, p + (int64_t)row * stride, stride, valid - row, D, vec, tid);
+          ho.next(full);
+        }
+      };
+      fetch(sQ, bar(bars.q_full), maps.q_on, maps.q, h, q, a.sq.t, i0, ql);
       if (REL) {
         load_tile<T, DP, 32>(sK, C::chunk, static_cast<const T*>(a.relk), D, a.nrel, D, vec, tid);
         ho.next(bar(bars.k_full[kt++]));
@@ -180,12 +206,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
       for (int t = 0; t < nt && ok; ++t) {
         uint32_t dst = stage(true, kt);
         if (!dst) break;
-        load_tile<T, DP, kBN>(dst, C::chunk, k + (int64_t)t * kBN * a.sk.t, a.sk.t, kl - t * kBN, D, vec, tid);
-        ho.next(bar(bars.k_full[kt++ % ST]));
+        fetch(dst, bar(bars.k_full[kt++ % ST]), maps.kv_on, maps.k, hk, k, a.sk.t, t * kBN, kl);
         dst = stage(false, vt);
         if (!dst) break;
-        load_tile<T, DP, kBN>(dst, C::chunk, v + (int64_t)t * kBN * a.sv.t, a.sv.t, kl - t * kBN, D, vec, tid);
-        ho.next(bar(bars.v_full[vt++ % ST]));
+        fetch(dst, bar(bars.v_full[vt++ % ST]), maps.kv_on, maps.v, hk, v, a.sv.t, t * kBN, kl);
       }
       if (REL && ok) {
         const uint32_t dst = stage(false, vt);
@@ -220,7 +244,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
               if (r0 + r < a.nrel) tab[(r0 + r) * kBM + row] = v[r];
           }
         tc_fence_before();
-        mbar_arrive(bar(bars.s_free));
+        warp_arrive(bar(bars.s_free));
       }
       for (int t = 0; t < nt && ok; ++t) {
         ok = warp_wait(bar(bars.s_full), sp++ & 1, abort);
@@ -232,7 +256,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
         tmem_load64(tS + lanes + 64, s + 64);
         if (C::own_p) {
           tc_fence_before();
-          mbar_arrive(bar(bars.s_free));
+          warp_arrive(bar(bars.s_free));
         }
         if (REL) {
           // Offsets of the warp's rows in this tile: j - pos + w for its first and last row.
@@ -308,7 +332,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
         tmem_store32(tP + lanes + 32, p + 32);
         tmem_store_wait();
         tc_fence_before();
-        mbar_arrive(bar(bars.p_full));
+        warp_arrive(bar(bars.p_full));
       }
       ok = ok && warp_wait(bar(bars.o_full), 0, abort);
       if (REL && ok) {
@@ -329,7 +353,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const AttnArgs a, 
         }
         tmem_store_wait();
         tc_fence_before();
-        mbar_arrive(bar(bars.p_full));
+        warp_arrive(bar(bars.p_full));
         ok = warp_wait(bar(bars.o_full), 1, abort);
       }
       if (!ok) raise_err(&g_gave_up, abort, 1);
@@ -375,7 +399,13 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
                    attn_rows_aligned(a.v, a.sv, a.D, 2) && reinterpret_cast<uintptr_t>(a.relk) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(a.relv) % 16 == 0;
   const bool ovec = attn_rows_aligned(a.o, a.so, a.D, 2);
-  attn_fwd_tc<T, DP, REL><<<dim3(cdiv(a.Tq, kBM), a.H, a.B), kFwdThreads, smem, st>>>(a, vec, ovec);
+  FwdMaps m = {};
+  if (vec) {
+    m.q_on = map_rows(&m.q, a.q, a.ty, a.sq, a.B, a.H, a.Tq, a.D, kBM);
+    m.kv_on = map_rows(&m.k, a.k, a.ty, a.sk, a.B, a.Hkv, a.Tk, a.D, kBN) &&
+              map_rows(&m.v, a.v, a.ty, a.sv, a.B, a.Hkv, a.Tk, a.D, kBN);
+  }
+  attn_fwd_tc<T, DP, REL><<<dim3(cdiv(a.Tq, kBM), a.H, a.B), kFwdThreads, smem, st>>>(a, m, vec, ovec);
   return cudaGetLastError();
 }
 
