@@ -267,6 +267,15 @@ struct Handover {
   }
 };
 
+// One lane of the warp, the same at every use.  The issuing warp runs its loop
+// with all lanes and only the MMAs under this predicate, so that descriptors
+// stay in uniform registers.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // A bounded wait of a whole warp, with one answer for all its lanes (the TMEM
 // accesses after it need the warp together).
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
   const uint32_t sA0 = base, sA1 = sA0 + C::tileA, sB = sA1 + C::tileA, sR = sB + ST * C::stage;
   float* tables = reinterpret_cast<float*>(smem_raw + (base - raw) + 2 * C::tileA + ST * C::stage + C::relk);
   const uint32_t sTab = smem_u32(tables);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int b = blockIdx.z, D = a.D, g = a.H / a.Hkv;
   const bool keys = (int)blockIdx.x < nk;
   if (keys && (int)blockIdx.y >= a.Hkv) return;
@@ -155,59 +155,60 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
 
   if (warp >= 8) {
     if (nt > 0 && warp == 8) {
-      if (lane == 0) {
-        constexpr uint32_t id_s = idesc_attn<T>(kBB, false), id_a = idesc_attn<T>(DP, true);
-        const uint64_t dA0 = sdesc<64>(sA0), dA1 = sdesc<64>(sA1), dB = sdesc<64>(sB), mB = desc_mn(sB, C::chunkB);
-        bool ok = mbar_wait_fast(bar(bars.a_full), 0, abort);
-        int fs = 0, fr = 0, us = 0;  // stage and round to fill from next, stage in use
-        auto scores = [&](int t) {
-          const int s = fs;
-          ok = ok && mbar_wait_fast(bar(bars.b_full[s]), fr & 1, abort);
-          if (!ok) return;
-          if (++fs == ST) fs = 0, ++fr;
-          tc_fence_after();
-          const uint32_t d = tS + (t & 1) * 2 * kBB;
-          const uint64_t b0 = dB + s * (C::stage >> 4);
+      constexpr uint32_t id_s = idesc_attn<T>(kBB, false), id_a = idesc_attn<T>(DP, true);
+      const bool lead = elect_lane();
+      const uint64_t dA0 = sdesc<64>(sA0), dA1 = sdesc<64>(sA1), dB = sdesc<64>(sB), mB = desc_mn(sB, C::chunkB);
+      int fs = 0, fr = 0, us = 0;  // stage and round to fill from next, stage in use
+      bool ok = warp_wait(bar(bars.a_full), 0, abort);
+      auto scores = [&](int t) {
+        ok = ok && warp_wait(bar(bars.b_full[fs]), fr & 1, abort);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t d = tS + (t & 1) * 2 * kBB, done = bar(bars.s_full[t & 1]);
+        const uint64_t b0 = dB + fs * (C::stage >> 4);
+        if (++fs == ST) fs = 0, ++fr;
+        if (lead) {
           mma_rows<DP>(d, dA0, C::chunkA, b0, C::chunkB, id_s);
           mma_rows<DP>(d + kBB, dA1, C::chunkA, b0 + (C::tileB >> 4), C::chunkB, id_s);
-          mma_commit(bar(bars.s_full[t & 1]));
-        };
-        scores(0);
-        for (int t = 0; t < nt && ok; ++t) {
-          if (t + 1 < nt) scores(t + 1);
-          const int s = us;
-          if (++us == ST) us = 0;
-          ok = ok && mbar_wait_fast(bar(bars.p_full[t & 1]), (t >> 1) & 1, abort);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t p = tS + (t & 1) * 2 * kBB;
-          const uint64_t m0 = mB + s * (C::stage >> 4), m1 = m0 + (C::tileB >> 4);
-          // Each group's 32 operand columns lie over the first half of its own scores.
-          auto accumulate = [&](uint32_t acc, uint32_t op, uint64_t m) {
-            if (t == 0) mma_ts_first(acc, op, m, id_a);
-            else mma_ts_acc(acc, op, m, id_a);
+          mma_commit(done);
+        }
+        __syncwarp();
+      };
+      scores(0);
+      for (int t = 0; t < nt && ok; ++t) {
+        if (t + 1 < nt) scores(t + 1);
+        ok = ok && warp_wait(bar(bars.p_full[t & 1]), (t >> 1) & 1, abort);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t p = tS + (t & 1) * 2 * kBB, done = bar(bars.b_free[us]);
+        const uint64_t m0 = mB + us * (C::stage >> 4), m1 = m0 + (C::tileB >> 4);
+        if (++us == ST) us = 0;
+        // Each group's 32 operand columns lie over the first half of its own scores.
+        auto accumulate = [&](uint32_t acc, uint32_t op, uint64_t m) {
+          if (t == 0) mma_ts_first(acc, op, m, id_a);
+          else mma_ts_acc(acc, op, m, id_a);
 #pragma unroll
-            for (int c = 1; c < kBB / 16; ++c)
-              mma_ts_acc(acc, op + (c >> 1) * kHalfB + (c & 1) * 8, m + c * (2048 >> 4), id_a);
-          };
+          for (int c = 1; c < kBB / 16; ++c)
+            mma_ts_acc(acc, op + (c >> 1) * kHalfB + (c & 1) * 8, m + c * (2048 >> 4), id_a);
+        };
+        if (lead) {
           if (keys) accumulate(tAcc0, p, m1);
           accumulate(tAcc1, p + kBB, m0);
-          mma_commit(bar(bars.b_free[s]));
+          mma_commit(done);
         }
-        if (REL && !keys && ok) {
-          // dq += (near ds) relk; the operand comes over the buffer of tile nt, in its order.
-          ok = mbar_wait_fast(bar(bars.r_full), 0, abort) &&
-               mbar_wait_fast(bar(bars.p_full[nt & 1]), (nt >> 1) & 1, abort);
-          tc_fence_after();
-          if (ok)
-            for (int c = 0; c < (a.nrel + 15) / 16; ++c)
-              mma_ts_acc(tAcc1, tS + (nt & 1) * 2 * kBB + c * 8, desc_mn(sR + c * 2048, C::chunkR), id_a);
-        }
-        mma_commit(bar(bars.acc_full));
-        if (!ok) raise_err(&g_gave_up, abort, 1);
-        mbar_wait_fast(bar(bars.acc_full), 0, abort);  // nothing in flight when memory is given back
+        __syncwarp();
       }
-      __syncwarp();
+      if (REL && !keys && ok) {
+        // dq += (near ds) relk; the operand comes over the buffer of tile nt, in its order.
+        ok = warp_wait(bar(bars.r_full), 0, abort) && warp_wait(bar(bars.p_full[nt & 1]), (nt >> 1) & 1, abort);
+        tc_fence_after();
+        if (ok && lead)
+          for (int c = 0; c < (a.nrel + 15) / 16; ++c)
+            mma_ts_acc(tAcc1, tS + (nt & 1) * 2 * kBB + c * 8, desc_mn(sR + c * 2048, C::chunkR), id_a);
+      }
+      if (lead) mma_commit(bar(bars.acc_full));
+      if (!ok) raise_err(&g_gave_up, abort, 1);
+      warp_wait(bar(bars.acc_full), 0, abort);  // nothing in flight when memory is given back
     } else if (nt > 0 && warp < 11) {
       const int tid = threadIdx.x - 9 * 32;
       Handover ho;

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
   const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t sQ = base, sK = sQ + C::tile, sV = sK + ST * C::tile;
   float* tab = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + C::smem);  // [nrel][128]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // Long rows of a causal mask first, so that the last blocks are short ones.
   const int i0 = (int)(gridDim.x - 1 - blockIdx.x) * kBM, h = blockIdx.y, b = blockIdx.z;
   const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk), off = kl - ql;
@@ -106,66 +106,75 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
   if (warp >= 4) {
     reg_dec<kRestRegs>();
     if (nt > 0 && warp == 4) {
-      if (lane == 0) {
-        constexpr uint32_t id_s = idesc_attn<T>(kBN, false), id_o = idesc_attn<T>(DP, true);
-        const uint64_t dQ = sdesc<64>(sQ), dK = sdesc<64>(sK), mV = desc_mn(sV, C::chunk);
-        bool ok = mbar_wait_fast(bar(bars.q_full), 0, abort);
-        int kt = 0, vt = 0, pp = 0, sf = 0;
-        auto scores = [&](uint32_t id) {  // S = q . (tile kt)^T
-          const int s = kt % ST;
-          ok = ok && mbar_wait_fast(bar(bars.k_full[s]), (kt / ST) & 1, abort);
-          if (!ok) return;
-          tc_fence_after();
-          mma_rows<DP>(tS, dQ, C::chunk, dK + s * (C::tile >> 4), C::chunk, id);
-          mma_commit(bar(bars.k_free[s]));
-          mma_commit(bar(bars.s_full));
-          ++kt;
-        };
-        auto scores_read = [&] {  // the softmax warps hold S in registers
-          ok = ok && mbar_wait_fast(bar(bars.s_free), sf & 1, abort);
-          ++sf;
-          tc_fence_after();
-        };
-        auto values = [&](auto rows, bool first) {  // O (+)= P . (tile vt)
-          const int s = vt % ST;
-          ok = ok && mbar_wait_fast(bar(bars.v_full[s]), (vt / ST) & 1, abort);
-          ok = ok && mbar_wait_fast(bar(bars.p_full), pp & 1, abort);
-          ++pp;
-          if (!ok) return;
-          tc_fence_after();
-          const uint64_t m = mV + s * (C::tile >> 4);
+      constexpr uint32_t id_s = idesc_attn<T>(kBN, false), id_o = idesc_attn<T>(DP, true);
+      const bool lead = elect_lane();
+      const uint64_t dQ = sdesc<64>(sQ), dK = sdesc<64>(sK), mV = desc_mn(sV, C::chunk);
+      bool ok = warp_wait(bar(bars.q_full), 0, abort);
+      int kt = 0, vt = 0, pp = 0, sf = 0;
+      auto scores = [&](uint32_t id) {  // S = q . (tile kt)^T
+        const int s = kt % ST;
+        ok = ok && warp_wait(bar(bars.k_full[s]), (kt / ST) & 1, abort);
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t d = dK + s * (C::tile >> 4);
+        const uint32_t kf = bar(bars.k_free[s]), sfull = bar(bars.s_full);
+        if (lead) {
+          mma_rows<DP>(tS, dQ, C::chunk, d, C::chunk, id);
+          mma_commit(kf);
+          mma_commit(sfull);
+        }
+        __syncwarp();
+        ++kt;
+      };
+      auto scores_read = [&] {  // the softmax warps hold S in registers
+        ok = ok && warp_wait(bar(bars.s_free), sf & 1, abort);
+        ++sf;
+        tc_fence_after();
+      };
+      auto values = [&](auto rows, bool first) {  // O (+)= P . (tile vt)
+        const int s = vt % ST;
+        ok = ok && warp_wait(bar(bars.v_full[s]), (vt / ST) & 1, abort);
+        ok = ok && warp_wait(bar(bars.p_full), pp & 1, abort);
+        ++pp;
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t m = mV + s * (C::tile >> 4);
+        const uint32_t vf = bar(bars.v_free[s]), done = bar(bars.pv_done);
+        if (lead) {
           if (first) mma_ts_first(tO, tP, m, id_o);
           else mma_ts_acc(tO, tP, m, id_o);
 #pragma unroll
           for (int c = 1; c < rows / 16; ++c) mma_ts_acc(tO, tP + c * 8, m + c * (2048 >> 4), id_o);
-          mma_commit(bar(bars.v_free[s]));
-          if (C::own_p) mma_commit(bar(bars.pv_done));
-          ++vt;
-        };
-        if (REL) {
-          scores(idesc_attn<T>(nrp, false));
-          scores_read();
+          mma_commit(vf);
+          if (C::own_p) mma_commit(done);
         }
-        if (C::own_p) scores(id_s);
-        for (int t = 0; t < nt && ok; ++t) {
-          if (C::own_p) {
-            scores_read();
-            if (t + 1 < nt) scores(id_s);
-          } else {
-            scores(id_s);
-          }
-          values(std::integral_constant<int, kBN>(), t == 0);
-        }
-        mma_commit(bar(bars.o_full));
-        if (REL && ok) {
-          values(nrp, false);
-          mma_commit(bar(bars.o_full));
-        }
-        if (!ok) raise_err(&g_gave_up, abort, 1);
-        // Nothing of this block is in flight when its memory is given back.
-        mbar_wait_fast(bar(bars.o_full), REL && ok ? 1 : 0, abort);
+        __syncwarp();
+        ++vt;
+      };
+      if (REL) {
+        scores(idesc_attn<T>(nrp, false));
+        scores_read();
       }
-      __syncwarp();
+      if (C::own_p) scores(id_s);
+      for (int t = 0; t < nt && ok; ++t) {
+        if (C::own_p) {
+          scores_read();
+          if (t + 1 < nt) scores(id_s);
+        } else {
+          scores(id_s);
+        }
+        values(std::integral_constant<int, kBN>(), t == 0);
+      }
+      if (lead) mma_commit(bar(bars.o_full));
+      int fin = 0;
+      if (REL && ok) {
+        values(nrp, false);
+        if (lead) mma_commit(bar(bars.o_full));
+        fin = 1;
+      }
+      if (!ok) raise_err(&g_gave_up, abort, 1);
+      // Nothing of this block is in flight when its memory is given back.
+      warp_wait(bar(bars.o_full), fin, abort);
     } else if (nt > 0 && warp < 7) {
       const int tid = threadIdx.x - 5 * 32;
       const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h;
