@@ -4,16 +4,19 @@
 
 namespace gsv {
 
-constexpr int kRelRows = 64;  // query rows of one head whose relative gradients one block sums
-inline int64_t rel_blocks(const AttnArgs& a) { return (int64_t)a.B * a.H * cdiv(a.Tq, kRelRows); }
-
+// Query rows of one head whose relative gradients are one partial sum: the
+// query tile of the tensor-core kernel, or a block of the fp32 one.
+constexpr int kRelRows = 64, kRelRowsTensor = 128;
+inline int64_t rel_blocks(const AttnArgs& a) {
+  return (int64_t)a.B * a.H * cdiv(a.Tq, a.ty == Ty::F32 ? kRelRows : kRelRowsTensor);
+}
 constexpr float kHalfShift = 15.f;  // fp16 probabilities are carried as 2^15 p
 
 // Backward workspace, all fp32: per query row (b, h, i) ndelta = -do . o and
 // nlse2 = -lse log2(e), plus kHalfShift for fp16 (-inf for a row without keys,
 // so that every exp2 of it is 0); for fp16 the norms |do_i| and |v_j| + max
 // |relv|; per row and offset the products q . relk_r, do . relv_r (read by the
-// score tiles) and the near values of p and ds (written by the dq tiles);
+// score tiles); fp32: the near values of p and ds (written by the dq tiles);
 // partial sums of the relative gradients.
 struct BwdWs {
   float *ndelta, *nlse2, *ndo, *nv, *qrel, *grel, *pband, *sband, *part;
@@ -38,8 +41,10 @@ inline BwdWs carve_bwd(const AttnArgs& a) {
   if (a.nrel) {
     w.qrel = take(rows * a.nrel);
     w.grel = take(rows * a.nrel);
-    w.pband = take(rows * a.nrel);
-    w.sband = take(rows * a.nrel);
+    if (a.ty == Ty::F32) {
+      w.pband = take(rows * a.nrel);
+      w.sband = take(rows * a.nrel);
+    }
     w.part = take((size_t)rel_blocks(a) * 2 * a.nrel * a.D);
   }
   w.bytes = at;
@@ -52,7 +57,7 @@ cudaError_t attn_bwd_tensor(const AttnArgs& a, const BwdWs& ws, cudaStream_t st)
 cudaError_t attn_bwd_cores(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
 // ndelta, nlse2, the norms and the relative products of every row.
 cudaError_t attn_bwd_rows(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
-// drelk, drelv from the near values.
+// drelk, drelv from the near values (fp32) or the query tiles' partial sums.
 cudaError_t attn_bwd_rel(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
 
 }  // namespace gsv

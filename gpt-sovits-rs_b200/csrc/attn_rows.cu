@@ -23,17 +23,20 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Channels d0 .. d0 + 7 of a row, zeros from D on.
+// Channels d0 .. d0 + 7 of a row, zeros from D on.  With `vec` (whole aligned
+// vectors) a lane past the row's end takes the last vector and drops it, so
+// that the load stands under no branch and several rows' loads overlap.
 template <typename T>
 __device__ __forceinline__ void load8(const T* row, int d0, int D, bool vec, float* f) {
-  if (vec && d0 < D) {
+  if (vec) {
     constexpr int V = 16 / sizeof(T);
+    const T* p = row + min(d0, D - 8);
 #pragma unroll
     for (int k = 0; k < 8; k += V) {
-      const uint4 u = *reinterpret_cast<const uint4*>(row + d0 + k);
+      const uint4 u = *reinterpret_cast<const uint4*>(p + k);
       const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[k + i] = to_f(e[i]);
+      for (int i = 0; i < V; ++i) f[k + i] = d0 < D ? to_f(e[i]) : 0.f;
     }
   } else {
 #pragma unroll
@@ -58,11 +61,13 @@ __device__ __forceinline__ float dot8(const float* a, const float* b) {
 // the rounding of ds itself, take delta = sum_j p_ij dp_ij instead (fp32
 // inputs have no such rounding).
 template <typename T, int G>
-__global__ void __launch_bounds__(kRowThreads) bwd_rows_kernel(const AttnArgs a, const BwdWs ws, const bool vec) {
+__global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_constant__ AttnArgs a,
+                                                               const __grid_constant__ BwdWs ws, const int nq,
+                                                               const bool vec) {
   extern __shared__ float sm[];  // relk, relv as [nrel][8 G]
   constexpr bool F16 = std::is_same<T, __half>::value, kExact = std::is_same<T, float>::value;
   constexpr int L = 8 * G, R = kRowThreads / G;
-  const int D = a.D, lane = threadIdx.x % G, grp = threadIdx.x / G, d0 = lane * 8;
+  const int D = a.D, lane = threadIdx.x % G, d0 = lane * 8, h = blockIdx.y, b = blockIdx.z;
   float* srk = sm;
   float* srv = srk + a.nrel * L;
   for (int e = threadIdx.x; e < a.nrel * L; e += kRowThreads) {
@@ -70,92 +75,78 @@ __global__ void __launch_bounds__(kRowThreads) bwd_rows_kernel(const AttnArgs a,
     srk[e] = d < D ? to_f(static_cast<const T*>(a.relk)[r * D + d]) : 0.f;
     srv[e] = d < D ? to_f(static_cast<const T*>(a.relv)[r * D + d]) : 0.f;
   }
-  __syncthreads();
-  if (F16) {
+  if (a.nrel) __syncthreads();
+  const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk);
+  if (F16 && (int)blockIdx.x >= nq) {  // the key rows' norms
+    if (h >= a.Hkv) return;
+    const int j = ((int)blockIdx.x - nq) * R + threadIdx.x / G;
     float ev = 0.f;  // largest |relv|^2
     if ((threadIdx.x & 31) < a.nrel)
       for (int d = 0; d < L; ++d) ev = fmaf(srv[(threadIdx.x & 31) * L + d], srv[(threadIdx.x & 31) * L + d], ev);
     ev = sqrtf(warp_max(ev));
-    const int64_t keys = (int64_t)a.B * a.Hkv * a.Tk, steps = (keys + R - 1) / R;
-    for (int64_t x = blockIdx.x; x < steps; x += gridDim.x) {
-      const int64_t row = x * R + grp;
-      const int64_t bh = row / max(a.Tk, 1);
-      const int j = (int)(row - bh * a.Tk), b = (int)(bh / a.Hkv), h = (int)(bh - (int64_t)b * a.Hkv);
-      float s = 0.f;
-      const bool in = row < keys && j < clamp_len(a.klen, b, a.Tk);
-      if (in) {
-        float v[8];
-        load8(static_cast<const T*>(a.v) + b * a.sv.b + h * a.sv.h + j * a.sv.t, d0, D, vec, v);
-        s = dot8(v, v);
-      }
-      s = group_sum<G>(s);
-      if (in && lane == 0) ws.nv[row] = sqrtf(s) + ev;
+    float v[8] = {};
+    if (j < kl) load8(static_cast<const T*>(a.v) + b * a.sv.b + h * a.sv.h + j * a.sv.t, d0, D, vec, v);
+    const float s = group_sum<G>(dot8(v, v));
+    if (j < kl && lane == 0) ws.nv[((int64_t)b * a.Hkv + h) * a.Tk + j] = sqrtf(s) + ev;
+    return;
+  }
+  const int i = (int)blockIdx.x * R + threadIdx.x / G;
+  const bool in = i < a.Tq;
+  const int64_t row = ((int64_t)b * a.H + h) * a.Tq + i;
+  const int n = in ? allowed_keys(i, ql, kl, a.causal) : 0;
+  const float sl2 = a.scale * kLog2e;
+  float g[8] = {}, q[8] = {}, o[8] = {};
+  if (n > 0) {
+    load8(static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + i * a.sdo.t, d0, D, vec, g);
+    load8(static_cast<const T*>(a.o) + b * a.so.b + h * a.so.h + i * a.so.t, d0, D, vec, o);
+    if (a.nrel || (!kExact && n <= kFewKeys))
+      load8(static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + i * a.sq.t, d0, D, vec, q);
+  }
+  float s = group_sum<G>(dot8(g, o));
+  const float lse2 = n > 0 ? a.lse[row] * kLog2e : INFINITY;
+  for (int r = 0; r < a.nrel; ++r) {
+    const float u = group_sum<G>(dot8(q, srk + r * L + d0)), w = group_sum<G>(dot8(g, srv + r * L + d0));
+    if (in && lane == r % G) {
+      ws.qrel[row * a.nrel + r] = u;
+      ws.grel[row * a.nrel + r] = w;
     }
   }
-  const int64_t rows = (int64_t)a.B * a.H * a.Tq, steps = (rows + R - 1) / R;
-  const float sl2 = a.scale * kLog2e;
-  for (int64_t x = blockIdx.x; x < steps; x += gridDim.x) {
-    const int64_t row = x * R + grp;
-    const int64_t bh = row / a.Tq;
-    const int i = (int)(row - bh * a.Tq), b = (int)(bh / a.H), h = (int)(bh - (int64_t)b * a.H);
-    const bool in = row < rows;
-    const int ql = in ? clamp_len(a.qlen, b, a.Tq) : 0, kl = in ? clamp_len(a.klen, b, a.Tk) : 0;
-    const int n = in ? allowed_keys(i, ql, kl, a.causal) : 0;
-    float g[8] = {}, q[8] = {}, o[8] = {};
-    if (n > 0) {
-      load8(static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + i * a.sdo.t, d0, D, vec, g);
-      load8(static_cast<const T*>(a.o) + b * a.so.b + h * a.so.h + i * a.so.t, d0, D, vec, o);
-      if (a.nrel || !kExact) load8(static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + i * a.sq.t, d0, D, vec, q);
-    }
-    float s = group_sum<G>(dot8(g, o));
-    const float lse2 = n > 0 ? a.lse[row] * kLog2e : INFINITY;
-    for (int r = 0; r < a.nrel; ++r) {
-      const float u = group_sum<G>(dot8(q, srk + r * L + d0)), w = group_sum<G>(dot8(g, srv + r * L + d0));
-      if (in && lane == r % G) {
-        ws.qrel[row * a.nrel + r] = u;
-        ws.grel[row * a.nrel + r] = w;
-      }
-    }
-    if (!kExact) {
-      const bool few = n > 0 && n <= kFewKeys;
-      if (__any_sync(0xffffffffu, few)) {
-        const int hk = h / (a.H / a.Hkv);
-        const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
-        const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
-        float t = 0.f;
-        const int most = (int)warp_max(few ? (float)n : 0.f);
-#pragma unroll 4
-        for (int j = 0; j < most; ++j) {
-          const bool use = few && j < n;
-          float kk[8], vv[8];
-          load8(k + (use ? j : 0) * a.sk.t, use ? d0 : D, D, vec, kk);
-          load8(v + (use ? j : 0) * a.sv.t, use ? d0 : D, D, vec, vv);
-          const unsigned r = (unsigned)(j - (i + kl - ql) + a.window);
-          if (use && r < (unsigned)a.nrel)
+  const bool few = !kExact && n > 0 && n <= kFewKeys;
+  if (!kExact && __any_sync(0xffffffffu, few)) {
+    const int hk = h / (a.H / a.Hkv), most = (int)warp_max(few ? (float)n : 0.f);
+    const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
+    const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
+    float t = 0.f;
+#pragma unroll 2
+    for (int j = 0; j < most; ++j) {
+      const bool use = few && j < n;
+      float kk[8], vv[8];
+      load8(k + (use ? j : 0) * a.sk.t, d0, D, vec, kk);
+      load8(v + (use ? j : 0) * a.sv.t, d0, D, vec, vv);
+      const unsigned r = (unsigned)(j - (i + kl - ql) + a.window);
+      if (use && r < (unsigned)a.nrel)
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-              kk[y] += srk[r * L + d0 + y];
-              vv[y] += srv[r * L + d0 + y];
-            }
-          const float sc = group_sum<G>(dot8(q, kk)), dp = group_sum<G>(dot8(g, vv));
-          if (use) t = fmaf(exp2f(fmaf(sc, sl2, -lse2)), dp, t);
+        for (int y = 0; y < 8; ++y) {
+          kk[y] += srk[r * L + d0 + y];
+          vv[y] += srv[r * L + d0 + y];
         }
-        if (few) s = t;
-      }
+      const float sc = group_sum<G>(dot8(q, kk)), dp = group_sum<G>(dot8(g, vv));
+      if (use) t = fmaf(exp2f(fmaf(sc, sl2, -lse2)), dp, t);
     }
-    const float gg = F16 ? sqrtf(group_sum<G>(dot8(g, g))) : 0.f;
-    if (in && lane == 0) {
-      ws.ndelta[row] = n > 0 ? -s : 0.f;
-      ws.nlse2[row] = (F16 ? kHalfShift : 0.f) - lse2;
-      if (F16) ws.ndo[row] = n > 0 ? gg : 0.f;
-    }
+    if (few) s = t;
+  }
+  const float gg = F16 ? sqrtf(group_sum<G>(dot8(g, g))) : 0.f;
+  if (in && lane == 0) {
+    ws.ndelta[row] = n > 0 ? -s : 0.f;
+    ws.nlse2[row] = (F16 ? kHalfShift : 0.f) - lse2;
+    if (F16) ws.ndo[row] = n > 0 ? gg : 0.f;
   }
 }
 
-// Partial sums over kRelRows query rows of one head: thread (d, half) holds
-// channel d of every offset over one half of the rows.  Fixed row order, so
+// fp32: partial sums over kRelRows query rows of one head: thread (d, half)
+// holds channel d of every offset over one half of the rows.  Fixed row order, so
 // the result does not depend on scheduling.
-template <typename T, int NR>
+template <int NR>
 __global__ void __launch_bounds__(2 * kAttnMaxD) bwd_rel_kernel(const AttnArgs a, const BwdWs ws) {
   __shared__ float sp[kRelRows][NR], ss[kRelRows][NR];
   __shared__ float red[2 * NR][kAttnMaxD];
@@ -172,13 +163,13 @@ __global__ void __launch_bounds__(2 * kAttnMaxD) bwd_rel_kernel(const AttnArgs a
   __syncthreads();
   const int d = threadIdx.x % kAttnMaxD, half = threadIdx.x / kAttnMaxD;
   float ak[NR] = {}, av[NR] = {};
-  const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + d;
-  const T* g = static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + d;
+  const float* q = static_cast<const float*>(a.q) + b * a.sq.b + h * a.sq.h + d;
+  const float* g = static_cast<const float*>(a.dout) + b * a.sdo.b + h * a.sdo.h + d;
   const int y1 = min(half * (kRelRows / 2) + kRelRows / 2, ql - i0);
 #pragma unroll 4
   for (int y = half * (kRelRows / 2); y < y1; ++y) {
-    const float qv = d < D ? to_f(q[(int64_t)(i0 + y) * a.sq.t]) : 0.f;
-    const float gv = d < D ? to_f(g[(int64_t)(i0 + y) * a.sdo.t]) : 0.f;
+    const float qv = d < D ? q[(int64_t)(i0 + y) * a.sq.t] : 0.f;
+    const float gv = d < D ? g[(int64_t)(i0 + y) * a.sdo.t] : 0.f;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
       ak[r] = fmaf(ss[y][r], qv, ak[r]);
@@ -222,14 +213,14 @@ __global__ void __launch_bounds__(512) bwd_rel_sum_kernel(const AttnArgs a, cons
 
 template <typename T, int G>
 cudaError_t rows_g(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
-  const int64_t rows = std::max((int64_t)a.B * a.H * a.Tq, (int64_t)a.B * a.Hkv * a.Tk), R = kRowThreads / G;
-  const int grid = (int)std::min<int64_t>((rows + R - 1) / R, 148 * 4);
+  constexpr int R = kRowThreads / G;
+  const int nq = cdiv(a.Tq, R), nk = a.ty == Ty::F16 ? cdiv(a.Tk, R) : 0;
   const size_t smem = sizeof(float) * 2 * a.nrel * 8 * G;
   const int el = sizeof(T);
   const bool vec = attn_rows_aligned(a.q, a.sq, a.D, el) && attn_rows_aligned(a.o, a.so, a.D, el) &&
                    attn_rows_aligned(a.dout, a.sdo, a.D, el) && attn_rows_aligned(a.k, a.sk, a.D, el) &&
                    attn_rows_aligned(a.v, a.sv, a.D, el) && a.D % 8 == 0;
-  bwd_rows_kernel<T, G><<<grid, kRowThreads, smem, st>>>(a, ws, vec);
+  bwd_rows_kernel<T, G><<<dim3(nq + nk, a.H, a.B), kRowThreads, smem, st>>>(a, ws, nq, vec);
   return cudaGetLastError();
 }
 
@@ -242,9 +233,9 @@ cudaError_t rows_t(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
 template <typename T>
 cudaError_t rel_t(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
   const int64_t blocks = rel_blocks(a);
-  if (blocks > 0) {
-    if (a.nrel <= 9) bwd_rel_kernel<T, 9><<<(unsigned)blocks, 2 * kAttnMaxD, 0, st>>>(a, ws);
-    else bwd_rel_kernel<T, 2 * kAttnMaxWindow + 1><<<(unsigned)blocks, 2 * kAttnMaxD, 0, st>>>(a, ws);
+  if (std::is_same<T, float>::value && blocks > 0) {
+    if (a.nrel <= 9) bwd_rel_kernel<9><<<(unsigned)blocks, 2 * kAttnMaxD, 0, st>>>(a, ws);
+    else bwd_rel_kernel<2 * kAttnMaxWindow + 1><<<(unsigned)blocks, 2 * kAttnMaxD, 0, st>>>(a, ws);
   }
   bwd_rel_sum_kernel<T><<<cdiv(2 * a.nrel * a.D, 32), 512, 0, st>>>(a, ws, blocks);
   return cudaGetLastError();

@@ -9,6 +9,9 @@
 //             operands of dv += P^T do and dk += dS^T q.
 //   queries:  q, do stay, k and v stream.  S = q k^T, dP = do v^T, and
 //             dq += dS k.
+//             With a window, the near columns of P and dS become one more
+//             operand each: dq += (near dS) relk, and the tile's share of
+//             drelk = (near dS)^T q and drelv = (near P)^T do.
 // That is 7 products for 5, the price of giving every gradient element one
 // owner: no atomics, no fp32 copy of dq in memory, and bits that repeat.
 //
@@ -44,8 +47,9 @@ struct BwdCfg {
   static constexpr uint32_t rel = REL ? 2 * kBB * 32 * 4 : 0;  // its relative products (up to 32 offsets)
   static constexpr uint32_t stage = 2 * tileB;
   static constexpr uint32_t relk = REL ? NC * chunkR : 0;
-  // keys: tables of ST stages; queries: two [32][128] tables.  The larger one.
-  static constexpr uint32_t tables_k = ST * (rows + rel), tables_q = REL ? 2 * 32 * kBA * 4 : 0;
+  static constexpr uint32_t bandT = 2 * 32 * 128;  // 32 offsets x 128 rows in 16 bits, two chunks of 64 rows
+  // keys: tables of ST stages; queries: two [32][128] tables and the two operands made of them.  The larger one.
+  static constexpr uint32_t tables_k = ST * (rows + rel), tables_q = REL ? 2 * 32 * kBA * 4 + 2 * bandT : 0;
   static constexpr uint32_t tables = tables_k > tables_q ? tables_k : tables_q;
   static constexpr uint32_t smem = 2 * tileA + ST * stage + relk + tables;
 };
@@ -153,6 +157,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
   // TMEM columns: two buffers of (S, dP), then the accumulators.
   const uint32_t tS = s_tmem, tAcc0 = tS + 4 * kBB, tAcc1 = tAcc0 + DP;
 
+  const uint32_t tRel = tS + ((nt + 1) & 1) * 2 * kBB;  // drelk, drelv: the scores of tile nt - 1
+
   if (warp >= 8) {
     if (nt > 0 && warp == 8) {
       constexpr uint32_t id_s = idesc_attn<T>(kBB, false), id_a = idesc_attn<T>(DP, true);
@@ -202,9 +208,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         // dq += (near ds) relk; the operand comes over the buffer of tile nt, in its order.
         ok = warp_wait(bar(bars.r_full), 0, abort) && warp_wait(bar(bars.p_full[nt & 1]), (nt >> 1) & 1, abort);
         tc_fence_after();
-        if (ok && lead)
-          for (int c = 0; c < (a.nrel + 15) / 16; ++c)
+        if (ok && lead) {
+          const int nrp = (a.nrel + 15) / 16 * 16;
+          for (int c = 0; c < nrp / 16; ++c)
             mma_ts_acc(tAcc1, tS + (nt & 1) * 2 * kBB + c * 8, desc_mn(sR + c * 2048, C::chunkR), id_a);
+          // Rows of the result: 128 channels (those past the tile's are not read); columns: offsets.
+          const uint32_t id_r = idesc_attn<T>(nrp, false) | (1u << 15), band = sTab + 2 * 32 * kBA * 4;
+          for (int x = 0; x < 2; ++x)
+            for (int c = 0; c < kBA / 16; ++c) {
+              const uint64_t m = desc_mn((x ? sA1 : sA0) + c * 2048, C::chunkA);
+              const uint64_t d = sdesc<64>(band + x * C::bandT + (c >> 2) * (C::bandT / 2) + (c & 3) * 32);
+              if (c == 0) mma_bf16_first(tRel + x * 32, m, d, id_r);
+              else mma_bf16_acc(tRel + x * 32, m, d, id_r);
+            }
+        }
       }
       if (lead) mma_commit(bar(bars.acc_full));
       if (!ok) raise_err(&g_gave_up, abort, 1);
@@ -388,8 +405,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       const int64_t qrow = row_h0 + own;
       const float nlse2 = n > 0 ? ws.nlse2[qrow] : -INFINITY, ndelta = n > 0 ? ws.ndelta[qrow] : 0.f;
       const F2 nl(nlse2, nlse2), nd(ndelta, ndelta);
-      float* tq = tables;               // q . relk by offset, [nrel][128]
-      float* tg = tables + 32 * kBA;    // do . relv, then the near ds as carried
+      float* tq = tables;               // q . relk by offset, [nrel][128]; then the near p as carried
+      float* tg = tables + 32 * kBA;    // do . relv; then the near ds as carried
       if (REL && nt > 0) {
         for (int r = wg; r < a.nrel; r += 2) {
           tq[r * kBA + row] = n > 0 ? ws.qrel[qrow * a.nrel + r] : 0.f;
@@ -439,13 +456,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
           d2[c / 2] = pack2<T>(d[c], d[c + 1]);
         }
         if (near) {
-          const float up = exp2f(-kShift), ud = 1.f / gs;
 #pragma unroll
           for (int c = 0; c < kHalfB; ++c) {
             const unsigned r = (unsigned)(d0 + c);
-            if (r < (unsigned)a.nrel && c < lim) {
-              ws.pband[qrow * a.nrel + r] = s[c] * up;
-              ws.sband[qrow * a.nrel + r] = d[c] * ud;
+            if (r < (unsigned)a.nrel) {
+              tq[r * kBA + row] = s[c];
               tg[r * kBA + row] = d[c];
             }
           }
@@ -472,6 +487,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
             for (int y = 0; y < 8; ++y) u[y] = pack2<T>(d[2 * y], d[2 * y + 1]);
             tmem_store8(tS + (nt & 1) * 2 * kBB + lanes + q0 / 2, u);
           }
+          // Group 0: ds by offset and row, group 1: p, as operands over the rows.
+          const float* from = wg == 0 ? tg : tq;
+          const uint32_t to = sTab + 2 * 32 * kBA * 4 + wg * C::bandT + (row >> 6) * (C::bandT / 2) + (row & 7) * 2;
+          for (int r = 0; r < a.nrel; ++r) {
+            const int j = jb + r;
+            const float v = j >= 0 && j < n ? from[r * kBA + row] : 0.f;
+            const uint16_t bits = (uint16_t)pack2<T>(v, 0.f);
+            asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + r * 128 + ((((row & 63) >> 3) ^ (r & 7)) << 4)), "h"(bits)
+                         : "memory");
+          }
+          fence_async_smem();
           tmem_store_wait();
           tc_fence_before();
           warp_arrive(bar(bars.p_full[nt & 1]));
@@ -509,6 +535,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
 #pragma unroll
             for (int y = 0; y < 32; ++y) o[y] = 0.f;
           if (own < a.Tq) store_row32<T>(out, c, D, ovec, o, inv);
+        }
+        if (REL) {
+          // Lane = channel; group 0: drelk, group 1: drelv.
+          const int64_t tile = ((int64_t)b * a.H + blockIdx.y) * ((int)gridDim.x - nk) + r0 / kBA;
+          float* part = ws.part + (tile * 2 + wg) * a.nrel * D + row;
+          const float f = wg == 0 ? inv : exp2f(-kShift);
+          for (int q0 = 0; q0 < a.nrel; q0 += 16) {
+            float v[16] = {};
+            if (nt > 0) tmem_load16(tRel + wg * 32 + lanes + q0, v);
+#pragma unroll
+            for (int y = 0; y < 16; ++y)
+              if (q0 + y < a.nrel && row < D) part[(int64_t)(q0 + y) * D] = v[y] * f;
+          }
         }
       }
     }
