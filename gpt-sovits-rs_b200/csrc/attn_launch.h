@@ -12,16 +12,31 @@ inline int64_t rel_blocks(const AttnArgs& a) {
 }
 constexpr float kHalfShift = 15.f;  // fp16 probabilities are carried as 2^15 p
 
-// Backward workspace, all fp32: per query row (b, h, i) ndelta = -do . o and
-// nlse2 = -lse log2(e), plus kHalfShift for fp16 (-inf for a row without keys,
-// so that every exp2 of it is 0); for fp16 the norms |do_i| and |v_j| + max
-// |relv|; per row and offset the products q . relk_r, do . relv_r (read by the
-// score tiles); fp32: the near values of p and ds (written by the dq tiles);
-// partial sums of the relative gradients.
+// Backward workspace, all fp32.  Query rows of a head are grouped in blocks of
+// kRowBlock, the last one filled up (their number even), so that a block's
+// values are one aligned run that a bulk copy can move:
+//   rows  [b][h][block][2][kRowBlock]: nlse2 = -lse log2(e), plus kHalfShift
+//         for fp16, and ndelta = -do . o; -inf and 0 for a row without keys or
+//         past Tq, so that every exp2 of it is 0
+//   rel   [b][h][block][2][kRowBlock][nrel]: q . relk_r and do . relv_r
+// fp16: the norms |do_i| [b][h][Tq] and |v_j| + max |relv| [b][hk][Tk].  fp32
+// with a window: the near values of p and ds [b][h][Tq][nrel], written by the
+// dq tiles.  part: partial sums of the relative gradients.
+constexpr int kRowBlock = 64;
 struct BwdWs {
-  float *ndelta, *nlse2, *ndo, *nv, *qrel, *grel, *pband, *sband, *part;
+  float *rows, *rel, *ndo, *nv, *pband, *sband, *part;
+  int blocks;  // row blocks of a head
   size_t bytes;
 };
+
+// nlse2 of row i of head bh (ndelta kRowBlock later), and its run of q . relk_r
+// (do . relv_r kRowBlock nrel later).
+__host__ __device__ inline float* row_at(const BwdWs& w, int64_t bh, int i) {
+  return w.rows + ((bh * w.blocks + i / kRowBlock) * 2) * kRowBlock + i % kRowBlock;
+}
+__host__ __device__ inline float* rel_at(const BwdWs& w, int64_t bh, int i, int nrel) {
+  return w.rel + (((bh * w.blocks + i / kRowBlock) * 2) * kRowBlock + i % kRowBlock) * nrel;
+}
 
 inline BwdWs carve_bwd(const AttnArgs& a) {
   BwdWs w{};
@@ -32,15 +47,15 @@ inline BwdWs carve_bwd(const AttnArgs& a) {
     return p;
   };
   const size_t rows = (size_t)a.B * a.H * a.Tq;
-  w.ndelta = take(rows);
-  w.nlse2 = take(rows);
+  w.blocks = cdiv(a.Tq, 2 * kRowBlock) * 2;
+  const size_t padded = (size_t)a.B * a.H * w.blocks * kRowBlock;
+  w.rows = take(2 * padded);
   if (a.ty == Ty::F16) {
     w.ndo = take(rows);
     w.nv = take((size_t)a.B * a.Hkv * a.Tk);
   }
   if (a.nrel) {
-    w.qrel = take(rows * a.nrel);
-    w.grel = take(rows * a.nrel);
+    w.rel = take(2 * padded * a.nrel);
     if (a.ty == Ty::F32) {
       w.pband = take(rows * a.nrel);
       w.sband = take(rows * a.nrel);
@@ -55,7 +70,7 @@ cudaError_t attn_fwd_tensor(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_fwd_cores(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_bwd_tensor(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
 cudaError_t attn_bwd_cores(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
-// ndelta, nlse2, the norms and the relative products of every row.
+// The rows, rel, ndo and nv parts of the workspace.
 cudaError_t attn_bwd_rows(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);
 // drelk, drelv from the near values (fp32) or the query tiles' partial sums.
 cudaError_t attn_bwd_rel(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);

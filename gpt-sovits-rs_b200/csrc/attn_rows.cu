@@ -91,9 +91,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_c
     return;
   }
   const int i = (int)blockIdx.x * R + threadIdx.x / G;
-  const bool in = i < a.Tq;
-  const int64_t row = ((int64_t)b * a.H + h) * a.Tq + i;
-  const int n = in ? allowed_keys(i, ql, kl, a.causal) : 0;
+  const int64_t bh = (int64_t)b * a.H + h, row = bh * a.Tq + i;
+  const int n = i < a.Tq ? allowed_keys(i, ql, kl, a.causal) : 0;
   const float sl2 = a.scale * kLog2e;
   float g[8] = {}, q[8] = {}, o[8] = {};
   if (n > 0) {
@@ -104,42 +103,50 @@ __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_c
   }
   float s = group_sum<G>(dot8(g, o));
   const float lse2 = n > 0 ? a.lse[row] * kLog2e : INFINITY;
+  float* rel = rel_at(ws, bh, i, a.nrel);
+#pragma unroll 3
   for (int r = 0; r < a.nrel; ++r) {
     const float u = group_sum<G>(dot8(q, srk + r * L + d0)), w = group_sum<G>(dot8(g, srv + r * L + d0));
-    if (in && lane == r % G) {
-      ws.qrel[row * a.nrel + r] = u;
-      ws.grel[row * a.nrel + r] = w;
+    if (lane == r % G) {
+      rel[r] = u;
+      rel[kRowBlock * a.nrel + r] = w;
     }
   }
   const bool few = !kExact && n > 0 && n <= kFewKeys;
   if (!kExact && __any_sync(0xffffffffu, few)) {
-    const int hk = h / (a.H / a.Hkv), most = (int)warp_max(few ? (float)n : 0.f);
+    // The warp takes its groups' rows in turn, one key per lane.
+    const int hk = h / (a.H / a.Hkv), wl = threadIdx.x & 31;
     const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
     const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
-    float t = 0.f;
+    for (int from = 0; from < 32; from += G) {
+      if (!__shfl_sync(0xffffffffu, few, from)) continue;
+      const int nr = __shfl_sync(0xffffffffu, n, from), ir = __shfl_sync(0xffffffffu, i, from), j = min(wl, nr - 1);
+      const float lr = __shfl_sync(0xffffffffu, lse2, from);
+      const unsigned r = (unsigned)(j - (ir + kl - ql) + a.window);
+      const bool near = r < (unsigned)a.nrel;
+      float sc = 0.f, dp = 0.f;
 #pragma unroll 2
-    for (int j = 0; j < most; ++j) {
-      const bool use = few && j < n;
-      float kk[8], vv[8];
-      load8(k + (use ? j : 0) * a.sk.t, d0, D, vec, kk);
-      load8(v + (use ? j : 0) * a.sv.t, d0, D, vec, vv);
-      const unsigned r = (unsigned)(j - (i + kl - ql) + a.window);
-      if (use && r < (unsigned)a.nrel)
+      for (int c = 0; c < D; c += 8) {
+        float kk[8], vv[8];
+        load8(k + j * a.sk.t, c, D, vec, kk);
+        load8(v + j * a.sv.t, c, D, vec, vv);
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
-          kk[y] += srk[r * L + d0 + y];
-          vv[y] += srv[r * L + d0 + y];
+          const float kr = near ? kk[y] + srk[r * L + c + y] : kk[y], vr = near ? vv[y] + srv[r * L + c + y] : vv[y];
+          sc = fmaf(__shfl_sync(0xffffffffu, q[y], from + c / 8), kr, sc);
+          dp = fmaf(__shfl_sync(0xffffffffu, g[y], from + c / 8), vr, dp);
         }
-      const float sc = group_sum<G>(dot8(q, kk)), dp = group_sum<G>(dot8(g, vv));
-      if (use) t = fmaf(exp2f(fmaf(sc, sl2, -lse2)), dp, t);
+      }
+      const float t = group_sum<32>(wl < nr ? exp2f(fmaf(sc, sl2, -lr)) * dp : 0.f);
+      if (threadIdx.x % 32 / G == from / G) s = t;
     }
-    if (few) s = t;
   }
   const float gg = F16 ? sqrtf(group_sum<G>(dot8(g, g))) : 0.f;
-  if (in && lane == 0) {
-    ws.ndelta[row] = n > 0 ? -s : 0.f;
-    ws.nlse2[row] = (F16 ? kHalfShift : 0.f) - lse2;
-    if (F16) ws.ndo[row] = n > 0 ? gg : 0.f;
+  if (lane == 0) {
+    float* rw = row_at(ws, bh, i);
+    rw[0] = (F16 ? kHalfShift : 0.f) - lse2;
+    rw[kRowBlock] = n > 0 ? -s : 0.f;
+    if (F16 && i < a.Tq) ws.ndo[row] = n > 0 ? gg : 0.f;
   }
 }
 
@@ -214,7 +221,7 @@ __global__ void __launch_bounds__(512) bwd_rel_sum_kernel(const AttnArgs a, cons
 template <typename T, int G>
 cudaError_t rows_g(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
   constexpr int R = kRowThreads / G;
-  const int nq = cdiv(a.Tq, R), nk = a.ty == Ty::F16 ? cdiv(a.Tk, R) : 0;
+  const int nq = ws.blocks * kRowBlock / R, nk = a.ty == Ty::F16 ? cdiv(a.Tk, R) : 0;
   const size_t smem = sizeof(float) * 2 * a.nrel * 8 * G;
   const int el = sizeof(T);
   const bool vec = attn_rows_aligned(a.q, a.sq, a.D, el) && attn_rows_aligned(a.o, a.so, a.D, el) &&

@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const AttnArgs a, cons
     const int first = j0 >= kl ? ql : (a.causal ? max(0, j0 - off) / kBT * kBT : 0);
     for (int hh = 0; hh < g; ++hh) {
       const int h = hk * g + hh;
-      const int64_t row = ((int64_t)b * a.H + h) * a.Tq;
+      const int64_t bh = (int64_t)b * a.H + h;
       for (int i0 = first; i0 < ql; i0 += kBT) {
         __syncthreads();
         load_rows<T, DP>(s2, static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t,
@@ -250,7 +250,9 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const AttnArgs a, cons
         for (int c = 0; c < 4; ++c) {
           const int i = i0 + tx + 16 * c;
           const int n = allowed_keys(i, ql, kl, a.causal);
-          const float nlse2 = n > 0 ? ws.nlse2[row + i] : 0.f, ndelta = n > 0 ? ws.ndelta[row + i] : 0.f;
+          const float* rw = row_at(ws, bh, i);
+          const float nlse2 = n > 0 ? rw[0] : 0.f, ndelta = n > 0 ? rw[kRowBlock] : 0.f;
+          const float* qr = rel_at(ws, bh, i, a.nrel);
           float p4[4], s4[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -258,8 +260,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const AttnArgs a, cons
             const unsigned r = (unsigned)(j - (i + off) + a.window);
             const bool ok = j < n;
             if (ok && r < (unsigned)a.nrel) {
-              s[x][c] += ws.qrel[(row + i) * a.nrel + r];
-              dp[x][c] += ws.grel[(row + i) * a.nrel + r];
+              s[x][c] += qr[r];
+              dp[x][c] += qr[kRowBlock * a.nrel + r];
             }
             p4[x] = ok ? exp2f(fmaf(s[x][c], sl2, nlse2)) : 0.f;
             s4[x] = ok ? p4[x] * (dp[x][c] + ndelta) : 0.f;
@@ -289,7 +291,7 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const AttnArgs a, cons
   }
   const int h = blockIdx.y, hk = h / g;
   const int i0 = (blockIdx.x - nk) * kBT;
-  const int64_t row = ((int64_t)b * a.H + h) * a.Tq;
+  const int64_t bh = (int64_t)b * a.H + h, row = bh * a.Tq;
   load_rows<T, DP>(s0, static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t, ql - i0,
                    D, vec);
   load_rows<T, DP>(s1, static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t,
@@ -300,8 +302,9 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const AttnArgs a, cons
   for (int x = 0; x < 4; ++x) {
     const int i = i0 + 4 * ty + x;
     n[x] = allowed_keys(i, ql, kl, a.causal);
-    nlse2[x] = n[x] > 0 ? ws.nlse2[row + i] : 0.f;
-    ndelta[x] = n[x] > 0 ? ws.ndelta[row + i] : 0.f;
+    const float* rw = row_at(ws, bh, i);
+    nlse2[x] = n[x] > 0 ? rw[0] : 0.f;
+    ndelta[x] = n[x] > 0 ? rw[kRowBlock] : 0.f;
   }
   const int last = min(i0 + kBT, ql) - 1;
   const int kend = last < i0 ? 0 : allowed_keys(last, ql, kl, a.causal);
@@ -325,8 +328,9 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const AttnArgs a, cons
         const unsigned r = (unsigned)(j - (i + off) + a.window);
         const bool ok = j < n[x], near = ok && r < (unsigned)a.nrel;
         if (near) {
-          s[x][c] += ws.qrel[(row + i) * a.nrel + r];
-          dp[x][c] += ws.grel[(row + i) * a.nrel + r];
+          const float* qr = rel_at(ws, bh, i, a.nrel);
+          s[x][c] += qr[r];
+          dp[x][c] += qr[kRowBlock * a.nrel + r];
         }
         const float p = ok ? exp2f(fmaf(s[x][c], sl2, nlse2[x])) : 0.f;
         s4[x] = ok ? p * (dp[x][c] + ndelta[x]) : 0.f;

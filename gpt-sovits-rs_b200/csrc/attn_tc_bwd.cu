@@ -44,11 +44,11 @@ struct BwdCfg {
   static constexpr uint32_t tileA = NC * chunkA, tileB = NC * chunkB;
   static constexpr int ST = NC == 2 && REL ? 3 : 4;
   static constexpr uint32_t rows = 2 * kBB * 4;  // nlse2 and ndelta of a streamed query tile
-  static constexpr uint32_t rel = REL ? 2 * kBB * 32 * 4 : 0;  // its relative products (up to 32 offsets)
+  static constexpr uint32_t rel = REL ? 2 * kBB * 32 * 4 : 0;  // its relative products (up to 31 offsets)
   static constexpr uint32_t stage = 2 * tileB;
   static constexpr uint32_t relk = REL ? NC * chunkR : 0;
   static constexpr uint32_t bandT = 2 * 32 * 128;  // 32 offsets x 128 rows in 16 bits, two chunks of 64 rows
-  // keys: tables of ST stages; queries: two [32][128] tables and the two operands made of them.  The larger one.
+  // keys: tables of ST stages; queries: the relative products of 128 rows and two operands.  The larger one.
   static constexpr uint32_t tables_k = ST * (rows + rel), tables_q = REL ? 2 * 32 * kBA * 4 + 2 * bandT : 0;
   static constexpr uint32_t tables = tables_k > tables_q ? tables_k : tables_q;
   static constexpr uint32_t smem = 2 * tileA + ST * stage + relk + tables;
@@ -58,8 +58,11 @@ struct BwdBars {
   uint64_t a_full, r_full, b_full[4], b_free[4], s_full[2], p_full[2], acc_full;
 };
 
-__device__ __forceinline__ void cp_async4(uint32_t dst, const float* src, bool in) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+// A run of the workspace (16-byte aligned, a multiple of 16 bytes).
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const float* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
 
 // Tensor maps of the resident (128-row boxes) and the streamed tiles (64-row
@@ -94,6 +97,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
   if (keys && (int)blockIdx.y >= a.Hkv) return;
   const int hk = keys ? blockIdx.y : blockIdx.y / g;
   const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk), off = kl - ql;
+  static_assert(kBB == kRowBlock && kBA == 2 * kRowBlock, "a tile's row values are whole runs of the workspace");
   // First row of the resident tiles; streamed tiles of each head, and their number in all.
   const int r0 = keys ? blockIdx.x * kBA : (int)(gridDim.x - 1 - blockIdx.x) * kBA;
   int first = 0, per = 0, heads = 1;
@@ -106,16 +110,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
     per = last < r0 ? 0 : cdiv(allowed_keys(last, ql, kl, a.causal), kBB);
   }
   const int nt = per * heads;
-  const int64_t row_h0 = ((int64_t)b * a.H + (keys ? hk * g : blockIdx.y)) * a.Tq;  // query row 0 of the first head
+  const int64_t bh0 = (int64_t)b * a.H + (keys ? hk * g : blockIdx.y);  // first head
   volatile int* abort = &s_abort;
   auto bar = [&](const uint64_t& m) { return smem_u32(&m); };
 
   if (threadIdx.x == 0) {
     s_abort = 0;
-    mbar_init(bar(bars.a_full), 2);
+    mbar_init(bar(bars.a_full), 3);  // the announcement and the two loader warps
     mbar_init(bar(bars.r_full), 2);
     for (int s = 0; s < ST; ++s) {
-      mbar_init(bar(bars.b_full[s]), 2);
+      mbar_init(bar(bars.b_full[s]), 3);
       mbar_init(bar(bars.b_free[s]), 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -129,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
   float gs = 1.f;  // the power of two that dS is carried with
   if (kHalf && nt > 0) {
     float nd = 0.f, nv = 0.f;
-    for (int64_t x = threadIdx.x; x < (int64_t)heads * a.Tq; x += kThreads) nd = fmaxf(nd, ws.ndo[row_h0 + x]);
+    for (int64_t x = threadIdx.x; x < (int64_t)heads * a.Tq; x += kThreads) nd = fmaxf(nd, ws.ndo[bh0 * a.Tq + x]);
     for (int x = threadIdx.x; x < kl; x += kThreads) nv = fmaxf(nv, ws.nv[((int64_t)b * a.Hkv + hk) * a.Tk + x]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -234,21 +238,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
       const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
       const T* dout = static_cast<const T*>(a.dout) + b * a.sdo.b;
-      const bool tma_warp = warp == 9;
-      // A pair of full tiles: the first loader warp's lane 0 issues it.
-      auto pair = [&](uint32_t d0, uint32_t d1, uint32_t chunk, uint32_t bytes, const RowsMap& m0, const RowsMap& m1,
-                      uint32_t full, int row, int h) {
-        if (lane == 0) {
-          mbar_expect_tx(full, bytes);
-          tma_tile<DP>(d0, chunk, m0, full, row, h, b);
-          tma_tile<DP>(d1, chunk, m1, full, row, h, b);
-        }
-      };
+      // Per barrier: the first warp's lane 0 announces and issues what moves by bulk copies (full tiles,
+      // row values); tails are copied by both warps, whose second arrival, or both, come when that is done.
+      const bool first_warp = warp == 9;
       const bool full_a = maps.a_on && r0 + kBA <= (keys ? kl : ql);
       const uint32_t a_full = bar(bars.a_full);
-      if (full_a && tma_warp)
-        pair(sA0, sA1, C::chunkA, 2 * C::tileA, keys ? maps.ka : maps.qa, keys ? maps.va : maps.ga, a_full, r0,
-             keys ? hk : (int)blockIdx.y);
+      if (first_warp && lane == 0) {
+        const uint32_t rel_bytes = REL && !keys ? 2u * 2 * kBB * a.nrel * 4 : 0;
+        mbar_expect_tx(a_full, (full_a ? 2 * C::tileA : 0) + rel_bytes);
+        if (full_a) {
+          const int h = keys ? hk : (int)blockIdx.y;
+          tma_tile<DP>(sA0, C::chunkA, keys ? maps.ka : maps.qa, a_full, r0, h, b);
+          tma_tile<DP>(sA1, C::chunkA, keys ? maps.va : maps.ga, a_full, r0, h, b);
+        }
+        if (REL && !keys) bulk_copy(sTab, rel_at(ws, bh0, r0, a.nrel), rel_bytes, a_full);
+      }
       if (!full_a) {
         if (keys) {
           load_tile<T, DP, kBA>(sA0, C::chunkA, k + (int64_t)r0 * a.sk.t, a.sk.t, kl - r0, D, vec, tid);
@@ -259,8 +263,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
           load_tile<T, DP, kBA>(sA1, C::chunkA, dout + h * a.sdo.h + (int64_t)r0 * a.sdo.t, a.sdo.t, ql - r0, D, vec,
                                 tid);
         }
+        ho.next(a_full);
+      } else {
+        warp_arrive(a_full);
       }
-      if (!full_a || !tma_warp) ho.next(a_full);
       if (REL && !keys) {  // needed last: a barrier of its own
         load_tile<T, DP, 32>(sR, C::chunkR, static_cast<const T*>(a.relk), D, a.nrel, D, vec, tid);
         ho.next(bar(bars.r_full));
@@ -273,44 +279,32 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         if (!ok) break;
         const int h = keys ? hk * g + hh : hk;
         const bool whole = maps.b_on && i0 + kBB <= (keys ? ql : kl);
-        if (whole) {
-          if (tma_warp)
-            pair(b0, b1, C::chunkB, 2 * C::tileB, keys ? maps.qb : maps.kb, keys ? maps.gb : maps.vb, full, i0, h);
-        } else if (keys) {
-          load_tile<T, DP, kBB>(b0, C::chunkB, q + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t, ql - i0, D, vec, tid);
-          load_tile<T, DP, kBB>(b1, C::chunkB, dout + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t, ql - i0, D, vec,
-                                tid);
-        } else {
-          load_tile<T, DP, kBB>(b0, C::chunkB, k + (int64_t)i0 * a.sk.t, a.sk.t, kl - i0, D, vec, tid);
-          load_tile<T, DP, kBB>(b1, C::chunkB, v + (int64_t)i0 * a.sv.t, a.sv.t, kl - i0, D, vec, tid);
-        }
-        if (keys && !tma_warp) {
-          const int64_t row = row_h0 + (int64_t)hh * a.Tq + i0;
+        if (first_warp && lane == 0) {
+          // Offsets of this pair of tiles: from r0 - (i0 + 63 + off) to r0 + 127 - (i0 + off).
+          const bool near = REL && keys && r0 - (i0 + kBB - 1 + off) <= a.window &&
+                            r0 + kBA - 1 - (i0 + off) >= -a.window;
+          const uint32_t rel_bytes = near ? 2u * kBB * a.nrel * 4 : 0;
+          mbar_expect_tx(full, (whole ? 2 * C::tileB : 0) + (keys ? C::rows : 0) + rel_bytes);
+          if (whole) {
+            tma_tile<DP>(b0, C::chunkB, keys ? maps.qb : maps.kb, full, i0, h, b);
+            tma_tile<DP>(b1, C::chunkB, keys ? maps.gb : maps.vb, full, i0, h, b);
+          }
           const uint32_t tab = sTab + s * (C::rows + C::rel);
-#pragma unroll
-          for (int e = lane; e < 2 * kBB; e += 32) {
-            const int c = e & (kBB - 1);
-            const bool in = i0 + c < a.Tq;
-            cp_async4(tab + e * 4, (e < kBB ? ws.nlse2 : ws.ndelta) + (in ? row + c : 0), in);
-          }
-          if (REL) {
-            // Offsets of this pair of tiles: from r0 - (i0 + 63 + off) to r0 + 127 - (i0 + off).
-            const int lo = r0 - (i0 + kBB - 1 + off), hi = r0 + kBA - 1 - (i0 + off);
-            if (lo <= a.window && hi >= -a.window)
-              for (int e = lane; e < kBB * a.nrel; e += 32) {
-                const bool in = i0 + e / a.nrel < a.Tq;
-                const int64_t at = in ? row * a.nrel + e : 0;
-                cp_async4(tab + C::rows + e * 4, ws.qrel + at, in);
-                cp_async4(tab + C::rows + (kBB * 32 + e) * 4, ws.grel + at, in);
-              }
-          }
+          if (keys) bulk_copy(tab, row_at(ws, bh0 + hh, i0), C::rows, full);
+          if (near) bulk_copy(tab + C::rows, rel_at(ws, bh0 + hh, i0, a.nrel), rel_bytes, full);
         }
-        if (whole && tma_warp) {
-          ho.flush();
-        } else if (whole && !keys) {
+        if (whole) {
           ho.flush();
           warp_arrive(full);
         } else {
+          if (keys) {
+            load_tile<T, DP, kBB>(b0, C::chunkB, q + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t, ql - i0, D, vec, tid);
+            load_tile<T, DP, kBB>(b1, C::chunkB, dout + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t, ql - i0, D, vec,
+                                  tid);
+          } else {
+            load_tile<T, DP, kBB>(b0, C::chunkB, k + (int64_t)i0 * a.sk.t, a.sk.t, kl - i0, D, vec, tid);
+            load_tile<T, DP, kBB>(b1, C::chunkB, v + (int64_t)i0 * a.sv.t, a.sv.t, kl - i0, D, vec, tid);
+          }
           ho.next(full);
         }
         if (++s == ST) {
@@ -336,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       int x = first, st = 0, round = 0;  // streamed tile within its head; its stage
       for (int t = 0; t < nt; ++t) {
         ok = warp_wait(bar(bars.s_full[t & 1]), (t >> 1) & 1, abort);
-        // The tables of the stage: written by the loaders, who signalled b_full before the MMAs began.
+        // The row values of the stage came with its tiles.
         ok = ok && warp_wait(bar(bars.b_full[st]), round & 1, abort);
         if (!ok) break;
         tc_fence_after();
@@ -352,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         tmem_load32(tb + kBB + c0, dp);
         if (REL) {
           const float* qrel = tab + 2 * kBB + c0 * a.nrel;
-          const float* grel = qrel + kBB * 32;
+          const float* grel = qrel + kBB * a.nrel;
           const int d0 = own - (i0 + off) + a.window;  // offset index of column 0; falls by one per column
           if (__any_sync(0xffffffffu, d0 >= 0 && d0 - (kHalfB - 1) < a.nrel)) {
 #pragma unroll
@@ -402,19 +396,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       }
     } else {
       const int n = allowed_keys(own, ql, kl, a.causal);
-      const int64_t qrow = row_h0 + own;
-      const float nlse2 = n > 0 ? ws.nlse2[qrow] : -INFINITY, ndelta = n > 0 ? ws.ndelta[qrow] : 0.f;
+      const float* rw = row_at(ws, bh0, own);
+      const float nlse2 = n > 0 ? rw[0] : -INFINITY, ndelta = n > 0 ? rw[kRowBlock] : 0.f;
       const F2 nl(nlse2, nlse2), nd(ndelta, ndelta);
-      float* tq = tables;               // q . relk by offset, [nrel][128]; then the near p as carried
-      float* tg = tables + 32 * kBA;    // do . relv; then the near ds as carried
-      if (REL && nt > 0) {
-        for (int r = wg; r < a.nrel; r += 2) {
-          tq[r * kBA + row] = n > 0 ? ws.qrel[qrow * a.nrel + r] : 0.f;
-          tg[r * kBA + row] = n > 0 ? ws.grel[qrow * a.nrel + r] : 0.f;
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-      }
-      for (int t = 0; t < nt; ++t) {
+      // This row's q . relk, then the near p as carried; do . relv, then the near ds as carried
+      // (an odd pitch of nrel: no bank conflicts between rows).
+      float* tq = tables + ((row / kBB) * 2 * kBB + row % kBB) * a.nrel;
+      float* tg = tq + kBB * a.nrel;
+      if (REL && nt > 0) ok = warp_wait(bar(bars.a_full), 0, abort);
+      for (int t = 0; t < nt && ok; ++t) {
         ok = warp_wait(bar(bars.s_full[t & 1]), (t >> 1) & 1, abort);
         if (!ok) break;
         tc_fence_after();
@@ -430,8 +420,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
           for (int c = 0; c < kHalfB; ++c) {
             const unsigned r = (unsigned)(d0 + c);
             if (r < (unsigned)a.nrel) {
-              s[c] += tq[r * kBA + row];
-              dp[c] += tg[r * kBA + row];
+              s[c] += tq[r];
+              dp[c] += tg[r];
             }
           }
         }
@@ -460,8 +450,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
           for (int c = 0; c < kHalfB; ++c) {
             const unsigned r = (unsigned)(d0 + c);
             if (r < (unsigned)a.nrel) {
-              tq[r * kBA + row] = s[c];
-              tg[r * kBA + row] = d[c];
+              tq[r] = s[c];
+              tg[r] = d[c];
             }
           }
         }
@@ -480,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
 #pragma unroll
             for (int y = 0; y < 16; ++y) {
               const int r = q0 + y, j = jb + r;
-              d[y] = r < a.nrel && j >= 0 && j < n ? tg[r * kBA + row] : 0.f;
+              d[y] = r < a.nrel && j >= 0 && j < n ? tg[r] : 0.f;
             }
             uint32_t u[8];
 #pragma unroll
@@ -492,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
           const uint32_t to = sTab + 2 * 32 * kBA * 4 + wg * C::bandT + (row >> 6) * (C::bandT / 2) + (row & 7) * 2;
           for (int r = 0; r < a.nrel; ++r) {
             const int j = jb + r;
-            const float v = j >= 0 && j < n ? from[r * kBA + row] : 0.f;
+            const float v = j >= 0 && j < n ? from[r] : 0.f;
             const uint16_t bits = (uint16_t)pack2<T>(v, 0.f);
             asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + r * 128 + ((((row & 63) >> 3) ^ (r & 7)) << 4)), "h"(bits)
                          : "memory");
