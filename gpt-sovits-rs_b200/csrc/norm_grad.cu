@@ -7,13 +7,15 @@
 // stays in registers between its load and its store; mean and variance are
 // two sums over those registers (no cancellation, no second read).
 //
-// [B][T][C]: R threads of a block (a power of two, 32 .. 256) share one frame
-// and hold up to E channels each as 16-byte vectors; a frame's sums go through
-// shuffles and, for R > 32, shared memory.  Rows that do not start on 16-byte
-// boundaries take single elements instead (V = 1), lanes side by side.
-// [B][C][T]: a block takes 32 frames, one per lane, and its 16 warps up to E
-// channels each; more than 16 E channels are split over a cluster whose blocks
-// exchange the frame sums through distributed shared memory.
+// [B][T][C]: R threads (a power of two, 32 .. 256) share one frame and hold up
+// to E channels each.  Blocks are persistent; every group of R threads has a
+// ring of frames in shared memory that one lane fills by bulk copies, so that
+// the loads of the next frames are in flight whatever the registers do.  Rows
+// that are not whole aligned 16-byte vectors (V = 1) are loaded directly.
+// [B][C][T]: a block takes 32 frames; a lane holds V of them (4 where rows are
+// aligned for vectors of 4, else 1) for up to 16 / V channels per warp and
+// lane.  More than 256 channels are split over a cluster whose blocks exchange
+// the frame sums through distributed shared memory.
 //
 // The backward's blocks walk many frames and keep dgamma / dbeta of their
 // channels in fp32 registers, written once per block as partial sums that a
@@ -23,7 +25,7 @@
 
 #include <algorithm>
 
-#include "attn_common.cuh"
+#include "attn_tc.cuh"
 #include "norm_grad.h"
 
 namespace cg = cooperative_groups;
@@ -31,19 +33,21 @@ namespace cg = cooperative_groups;
 namespace gsv {
 namespace {
 
+__device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out
+
 constexpr int kRowThreads = 256;
 constexpr int kTimeWarps = 16;
-constexpr int kTimeE = 16;  // channels per thread, largest: 256 channels per block
-
-template <typename T, int V>
-struct Vec {
-  T v[V];
-};
+constexpr int kTimeC = 256;  // channels of one block
 
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(const T* p, float* f) {
   if constexpr (V == 1) {
     f[0] = to_f(*p);
+  } else if constexpr (V * sizeof(T) == 8) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = to_f(e[i]);
   } else {
     const uint4 u = *reinterpret_cast<const uint4*>(p);
     const T* e = reinterpret_cast<const T*>(&u);
@@ -56,435 +60,529 @@ template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float* f) {
   if constexpr (V == 1) {
     *p = from_f<T>(f[0]);
+  } else if constexpr (V * sizeof(T) == 8) {
+    uint2 u;
+    u.x = pack2<T>(f[0], f[1]);
+    u.y = pack2<T>(f[2], f[3]);
+    *reinterpret_cast<uint2*>(p) = u;
+  } else if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
   } else {
     uint4 u;
-    T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-    for (int i = 0; i < V; ++i) e[i] = from_f<T>(f[i]);
+    u.x = pack2<T>(f[0], f[1]);
+    u.y = pack2<T>(f[2], f[3]);
+    u.z = pack2<T>(f[4], f[5]);
+    u.w = pack2<T>(f[6], f[7]);
     *reinterpret_cast<uint4*>(p) = u;
   }
 }
 
-// Sum of NS values over the R threads of a frame group; every thread gets it.
-// All threads of the block call it together.
+// Sums of NS values over the R threads of a group; every thread gets them.  The
+// buffer alternates between two halves, so one barrier per use is enough.
 template <int R, int NS>
-__device__ __forceinline__ void group_sum(float* v, float* s_red) {
+__device__ __forceinline__ void group_sum(float* v, float* s_red, int& flip) {
 #pragma unroll
   for (int n = 0; n < NS; ++n)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
   if constexpr (R > 32) {
-    const int w = threadIdx.x >> 5, g = threadIdx.x / R, nw = R / 32;
-    __syncthreads();  // the previous use has been read
+    constexpr int W = R / 32;
+    const int grp = threadIdx.x / R, w = threadIdx.x % R / 32;
+    float* buf = s_red + (flip * (kRowThreads / 32) + grp * W) * NS;
+    flip ^= 1;
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
-      for (int n = 0; n < NS; ++n) s_red[w * NS + n] = v[n];
-    __syncthreads();
+      for (int n = 0; n < NS; ++n) buf[w * NS + n] = v[n];
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(R) : "memory");
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
       v[n] = 0.f;
-      for (int k = 0; k < nw; ++k) v[n] += s_red[(g * nw + k) * NS + n];
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[n] += buf[k * NS + n];
     }
+  } else {
+    __syncwarp();
   }
 }
 
-template <typename T, int V, int E, int R>
-__global__ void __launch_bounds__(kRowThreads) norm_fwd_rows(const NormArgs a) {
-  constexpr int N = E / V, G = kRowThreads / R;
-  __shared__ float s_red[8];
+__device__ __forceinline__ void bulk_row(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+constexpr int kMaxStages = 8;
+
+template <typename T, int V, int E, int R, bool BWD>
+__global__ void __launch_bounds__(kRowThreads, BWD && E > 16 ? 1 : 2) norm_rows(const __grid_constant__ NormArgs a, const int stages) {
+  constexpr int N = E / V, G = kRowThreads / R, K = BWD ? 3 : 2;
+  constexpr bool kRing = V > 1;
+  extern __shared__ __align__(16) uint8_t s_ring[];  // [G][stages][K][C] of T
+  __shared__ float s_red[2 * (kRowThreads / 32) * 2];
+  __shared__ __align__(8) uint64_t s_bar[G][kMaxStages];
+  __shared__ int s_abort;
   const int tid = threadIdx.x % R, grp = threadIdx.x / R, C = a.C;
-  const int64_t frames = (int64_t)a.B * a.T;
-  const int64_t f = (int64_t)blockIdx.x * G + grp;
-  const bool in = f < frames;
-  const int b = in ? (int)(f / a.T) : 0, t = in ? (int)(f - (int64_t)b * a.T) : 0;
-  const bool ok = in && (!a.len || t < a.len[b]);
-  const T* x = static_cast<const T*>(a.x.p) + b * a.x.b + t * a.x.o;
-  const T* y = static_cast<const T*>(a.y.p) + b * a.y.b + t * a.y.o;
-  float s[E] = {}, u[E] = {};
-  if (ok) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int c = (tid + k * R) * V;
-      if (c < C) load_vec<T, V>(x + c, s + k * V);
+  const uint32_t row_bytes = (uint32_t)C * sizeof(T);
+  const int frames = a.B * a.T, step = gridDim.x * G;
+  int flip = 0;
+  if (kRing) {
+    if (tid == 0)
+      for (int s = 0; s < stages; ++s) mbar_init(smem_u32(&s_bar[grp][s]), 1);
+    if (threadIdx.x == 0) {
+      s_abort = 0;
+      fence_async_smem();
     }
-    if (a.y.p) {
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int c = (tid + k * R) * V;
-        if (c < C) load_vec<T, V>(y + c, u + k * V);
-      }
-    }
+    __syncthreads();
   }
-  float sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    s[e] += u[e];
-    sum += s[e];
-  }
-  group_sum<R, 1>(&sum, s_red);
-  const float mean = sum / (float)C;
-  float sq = 0.f;
+  float ga[E], be[E];  // backward: be accumulates dbeta, dg dgamma
+  float dg[BWD ? E : 1] = {};
 #pragma unroll
   for (int k = 0; k < N; ++k)
-    if ((tid + k * R) * V < C)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = s[k * V + i] - mean;
-        sq = fmaf(d, d, sq);
-      }
-  group_sum<R, 1>(&sq, s_red);
-  const float rstd = rsqrtf(sq / (float)C + a.eps);
-  if (!in) return;
-  if (tid == 0) {
-    a.mean[f] = ok ? mean : 0.f;
-    a.rstd[f] = ok ? rstd : 0.f;
-  }
-  T* out = static_cast<T*>(const_cast<void*>(a.out.p)) + b * a.out.b + t * a.out.o;
+    for (int i = 0; i < V; ++i) {
+      const int c = (tid + k * R) * V + i;
+      ga[k * V + i] = c < C ? a.gamma[c] : 0.f;
+      be[k * V + i] = !BWD && c < C ? a.beta[c] : 0.f;
+    }
+  auto valid = [&](int f, int& b, int& t) {
+    b = f / a.T;
+    t = f - b * a.T;
+    return f < frames && (!a.len || t < a.len[b]);
+  };
+  const T* X = static_cast<const T*>(a.x.p);
+  const T* Y = static_cast<const T*>(a.y.p);
+  const T* D = static_cast<const T*>(a.dout.p);
+  const uint8_t* ring = s_ring + (size_t)grp * stages * K * row_bytes;
+  auto fetch = [&](int f, int s) {  // one lane: frame f's rows into stage s
+    int b, t;
+    if (!valid(f, b, t)) return;
+    const uint32_t bar = smem_u32(&s_bar[grp][s]), dst = smem_u32(ring + (size_t)s * K * row_bytes);
+    mbar_expect_tx(bar, row_bytes * (1 + (Y ? 1 : 0) + (BWD ? 1 : 0)));
+    bulk_row(dst, X + b * a.x.b + t * a.x.o, row_bytes, bar);
+    if (Y) bulk_row(dst + row_bytes, Y + b * a.y.b + t * a.y.o, row_bytes, bar);
+    if (BWD) bulk_row(dst + 2 * row_bytes, D + b * a.dout.b + t * a.dout.o, row_bytes, bar);
+  };
+  const int f0 = blockIdx.x * G + grp;
+  if (kRing && tid == 0)
+    for (int s = 0; s < stages; ++s)
+      if (f0 + (int64_t)s * step < frames) fetch(f0 + s * step, s);
+  int s = 0;
+  uint32_t phases = 0;
+  // The statistics of the next frame are on their way while this one is worked on.
+  float mean_next = BWD && f0 < frames ? a.mean[f0] : 0.f, rstd_next = BWD && f0 < frames ? a.rstd[f0] : 0.f;
+  for (int64_t ff = f0; ff < frames; ff += step) {
+    const int f = (int)ff;
+    int b, t;
+    const bool ok = valid(f, b, t);
+    float v[E], g[BWD ? E : 1];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int c = (tid + k * R) * V;
-    if (c >= C) continue;
-    float o[V];
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = ok ? fmaf((s[k * V + i] - mean) * rstd, a.gamma[c + i], a.beta[c + i]) : 0.f;
-    store_vec<T, V>(out + c, o);
-  }
-}
-
-template <typename T, int V, int E, int R>
-__global__ void __launch_bounds__(kRowThreads) norm_bwd_rows(const NormArgs a) {
-  constexpr int N = E / V, G = kRowThreads / R;
-  extern __shared__ float s_part[];  // [2][C] when several groups share the block's partial sums
-  __shared__ float s_red[16];
-  const int tid = threadIdx.x % R, grp = threadIdx.x / R, C = a.C;
-  const int64_t frames = (int64_t)a.B * a.T;
-  float dg[E] = {}, db[E] = {}, ga[E] = {};
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int c = (tid + k * R) * V;
-    if (c < C)
-#pragma unroll
-      for (int i = 0; i < V; ++i) ga[k * V + i] = a.gamma[c + i];
-  }
-  // Every thread of the block runs the same number of steps (block barriers inside).
-  for (int64_t f0 = (int64_t)blockIdx.x * G; f0 < frames; f0 += (int64_t)gridDim.x * G) {
-    const int64_t f = f0 + grp;
-    const bool in = f < frames;
-    const int b = in ? (int)(f / a.T) : 0, t = in ? (int)(f - (int64_t)b * a.T) : 0;
-    const bool ok = in && (!a.len || t < a.len[b]);
-    float xh[E] = {}, g[E] = {}, sums[2] = {0.f, 0.f};
-    float rstd = 0.f;
+    for (int e = 0; e < (BWD ? E : 1); ++e) g[e] = 0.f;
+    const float mean = mean_next;
+    float rstd = ok ? rstd_next : 0.f;
+    if (BWD && ff + step < frames) {
+      mean_next = a.mean[f + step];
+      rstd_next = a.rstd[f + step];
+    }
     if (ok) {
-      const T* x = static_cast<const T*>(a.x.p) + b * a.x.b + t * a.x.o;
-      const T* y = static_cast<const T*>(a.y.p) + b * a.y.b + t * a.y.o;
-      const T* go = static_cast<const T*>(a.dout.p) + b * a.dout.b + t * a.dout.o;
-      float u[E] = {};
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int c = (tid + k * R) * V;
-        if (c < C) {
-          load_vec<T, V>(x + c, xh + k * V);
-          load_vec<T, V>(go + c, g + k * V);
-          if (a.y.p) load_vec<T, V>(y + c, u + k * V);
+      if (kRing) {
+        if (!warp_wait(smem_u32(&s_bar[grp][s]), phases >> s & 1, &s_abort)) {
+          // The group cannot go on together: leave the kernel's results undefined, but end it.
+          raise_err(&g_gave_up, &s_abort, 1);
         }
-      }
-      const float mean = a.mean[f];
-      rstd = a.rstd[f];
+        phases ^= 1u << s;
+        const T* sx = reinterpret_cast<const T*>(ring + (size_t)s * K * row_bytes);
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        if ((tid + k * R) * V >= C) continue;
+        for (int k = 0; k < N; ++k) {
+          const int c = (tid + k * R) * V;
+          if (c < C) {
+            load_vec<T, V>(sx + c, v + k * V);
+            if (Y) {
+              float u[V];
+              load_vec<T, V>(sx + C + c, u);
 #pragma unroll
-        for (int e = k * V; e < (k + 1) * V; ++e) {
-          xh[e] = (xh[e] + u[e] - mean) * rstd;
-          dg[e] = fmaf(g[e], xh[e], dg[e]);
-          db[e] += g[e];
-          g[e] *= ga[e];
-          sums[0] += g[e];
-          sums[1] = fmaf(g[e], xh[e], sums[1]);
+              for (int i = 0; i < V; ++i) v[k * V + i] += u[i];
+            }
+            if (BWD) load_vec<T, V>(sx + 2 * C + c, g + k * V);
+          }
+        }
+      } else {
+        float u[E];
+        // Clamped addresses: no load stands under a branch, so all are in flight together.
+        const T* x = X + b * a.x.b + t * a.x.o;
+        const T* y = Y ? Y + b * a.y.b + t * a.y.o : x;
+        const T* d = BWD ? D + b * a.dout.b + t * a.dout.o : x;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int c = min(tid + e * R, C - 1);
+          v[e] = to_f(x[c]);
+          u[e] = to_f(y[c]);
+          if (BWD) g[e] = to_f(d[c]);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const bool in = tid + e * R < C;
+          v[e] = in ? (Y ? v[e] + u[e] : v[e]) : 0.f;
+          if (BWD) g[e] = in ? g[e] : 0.f;
         }
       }
     }
-    group_sum<R, 2>(sums, s_red);
-    const float m0 = sums[0] / (float)C, m1 = sums[1] / (float)C;
-    if (!in) continue;
-    T* dx = static_cast<T*>(const_cast<void*>(a.dx.p)) + b * a.dx.b + t * a.dx.o;
+    float sums[2] = {0.f, 0.f};
+    if (!BWD) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) sums[0] += v[e];
+      group_sum<R, 1>(sums, s_red, flip);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if ((tid + k * R) * V < C)
+#pragma unroll
+          for (int e = k * V; e < (k + 1) * V; ++e) {
+            v[e] = (v[e] - mean) * rstd;
+            dg[e] = fmaf(g[e], v[e], dg[e]);
+            be[e] += g[e];
+            g[e] *= ga[e];
+            sums[0] += g[e];
+            sums[1] = fmaf(g[e], v[e], sums[1]);
+          }
+      group_sum<R, 2>(sums, s_red, flip);
+    }
+    // Every thread of the group has read the stage: it takes the frame `stages` steps on.
+    if (kRing) {
+      if (tid == 0 && ff + (int64_t)stages * step < frames) fetch(f + stages * step, s);
+      if (++s == stages) s = 0;
+    }
+    const float m0 = sums[0] / (float)C;
+    T* out = static_cast<T*>(const_cast<void*>(BWD ? a.dx.p : a.out.p)) + b * (BWD ? a.dx.b : a.out.b) +
+             t * (BWD ? a.dx.o : a.out.o);
+    if (!BWD) {
+      float sq = 0.f;
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if ((tid + k * R) * V < C)
+#pragma unroll
+          for (int e = k * V; e < (k + 1) * V; ++e) sq = fmaf(v[e] - m0, v[e] - m0, sq);
+      group_sum<R, 1>(&sq, s_red, flip);
+      rstd = rsqrtf(sq / (float)C + a.eps);
+      if (tid == 0) {
+        a.mean[f] = ok ? m0 : 0.f;
+        a.rstd[f] = ok ? rstd : 0.f;
+      }
+    }
+    const float m1 = sums[1] / (float)C;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int c = (tid + k * R) * V;
       if (c >= C) continue;
       float o[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = rstd * (g[k * V + i] - m0 - xh[k * V + i] * m1);
-      store_vec<T, V>(dx + c, o);
+      for (int i = 0; i < V; ++i) {
+        const int e = k * V + i;
+        o[i] = BWD ? rstd * (g[BWD ? e : 0] - m0 - v[e] * m1) : ok ? fmaf((v[e] - m0) * rstd, ga[e], be[e]) : 0.f;
+      }
+      store_vec<T, V>(out + c, o);
     }
   }
-  float* part = a.part + (int64_t)blockIdx.x * 2 * C;
-  // The groups add their sums in turn, so the order is fixed.
-  for (int w = 0; w < G; ++w) {
-    if (grp == w) {
+  if (BWD) {
+    // The groups add their sums in turn over the ring's memory, so the order is fixed.
+    float* s_part = reinterpret_cast<float*>(s_ring);
+    float* part = a.part + (int64_t)blockIdx.x * 2 * C;
+    __syncthreads();
+    for (int w = 0; w < G; ++w) {
+      if (grp == w) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int c = (tid + k * R) * V;
-        if (c >= C) continue;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (w > 0) {
-            dg[k * V + i] += s_part[c + i];
-            db[k * V + i] += s_part[C + c + i];
-          }
-          if (w < G - 1) {
-            s_part[c + i] = dg[k * V + i];
-            s_part[C + c + i] = db[k * V + i];
-          } else {
-            part[c + i] = dg[k * V + i];
-            part[C + c + i] = db[k * V + i];
-          }
+        for (int e = 0; e < E; ++e) {
+          const int c = (tid + e / V * R) * V + e % V;
+          if (c >= C) continue;
+          const float x = dg[BWD ? e : 0] + (w > 0 ? s_part[c] : 0.f), y = be[e] + (w > 0 ? s_part[C + c] : 0.f);
+          float* to = w < G - 1 ? s_part : part;
+          to[c] = x;
+          to[C + c] = y;
         }
       }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 
-// Sums of NS values per frame (lane) over the block's warps and the cluster.
-template <int NS>
-__device__ __forceinline__ void frame_sum(float* v, float (*s_w)[NS][32], float (*s_b)[32], cg::cluster_group& cl,
-                                          int cs) {
+// Sums of NS values for each of a lane's V frames over the block's warps and
+// the cluster (lanes that share frames have been added before).
+template <int NS, int V>
+__device__ __forceinline__ void frame_sum(float (*v)[V], float (*s_w)[NS][32], float (*s_b)[32],
+                                          cg::cluster_group& cl, int cs) {
+  constexpr int F = 32 / V;  // lanes per row of frames
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
 #pragma unroll
-  for (int n = 0; n < NS; ++n) s_w[w][n][lane] = v[n];
-  __syncthreads();
-  if (cs == 1) {
+  for (int n = 0; n < NS; ++n)
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      v[n] = 0.f;
+    for (int i = 0; i < V; ++i) {
 #pragma unroll
-      for (int k = 0; k < kTimeWarps; ++k) v[n] += s_w[k][n][lane];
+      for (int o = F; o < 32; o <<= 1) v[n][i] += __shfl_xor_sync(0xffffffffu, v[n][i], o);
+      if (lane < F) s_w[w][n][lane * V + i] = v[n][i];
     }
-    __syncthreads();
-    return;
-  }
+  __syncthreads();
   if (w < NS) {
     float t = 0.f;
 #pragma unroll
     for (int k = 0; k < kTimeWarps; ++k) t += s_w[k][w][lane];
     s_b[w][lane] = t;
   }
-  cl.sync();
+  if (cs == 1) __syncthreads();
+  else cl.sync();
 #pragma unroll
-  for (int n = 0; n < NS; ++n) {
-    v[n] = 0.f;
-    for (int k = 0; k < cs; ++k) v[n] += *cl.map_shared_rank(&s_b[n][lane], k);
+  for (int n = 0; n < NS; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[n][i] = 0.f;
+  for (int k = 0; k < cs; ++k) {
+    const float* from = cs == 1 ? &s_b[0][0] : cl.map_shared_rank(&s_b[0][0], k);
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[n][i] += from[n * 32 + (lane % F) * V + i];
   }
-  cl.sync();  // the sums have been read by every block
+  if (cs > 1) cl.sync();  // the sums have been read by every block
 }
 
-// blockIdx.x = (tile, cluster rank); a tile is 32 frames of one utterance.
-template <typename T, int E>
-__global__ void __launch_bounds__(kTimeWarps * 32) norm_fwd_time(const NormArgs a, const int cs) {
-  __shared__ float s_w[kTimeWarps][1][32];
-  __shared__ float s_b[1][32];
-  cg::cluster_group cl = cg::this_cluster();
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, C = a.C;
-  const int tiles = cdiv(a.T, 32), tile = blockIdx.x / cs, rank = blockIdx.x - tile * cs;
-  const int b = tile / tiles, t = (tile - b * tiles) * 32 + lane;
-  const bool in = t < a.T, ok = in && (!a.len || t < a.len[b]);
-  const int c0 = rank * kTimeWarps * E + w;
-  const T* x = static_cast<const T*>(a.x.p) + b * a.x.b + t;
-  const T* y = static_cast<const T*>(a.y.p) + b * a.y.b + t;
-  float s[E] = {}, u[E] = {};
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int c = c0 + e * kTimeWarps;
-    if (ok && c < C) {
-      s[e] = to_f(x[c * a.x.o]);
-      if (a.y.p) u[e] = to_f(y[c * a.y.o]);
-    }
-  }
-  float sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    s[e] += u[e];
-    sum += s[e];
-  }
-  frame_sum<1>(&sum, s_w, s_b, cl, cs);
-  const float mean = sum / (float)C;
-  float sq = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (c0 + e * kTimeWarps < C) sq = fmaf(s[e] - mean, s[e] - mean, sq);
-  frame_sum<1>(&sq, s_w, s_b, cl, cs);
-  const float rstd = rsqrtf(sq / (float)C + a.eps);
-  if (!in) return;
-  if (w == 0 && rank == 0) {
-    a.mean[(int64_t)b * a.T + t] = ok ? mean : 0.f;
-    a.rstd[(int64_t)b * a.T + t] = ok ? rstd : 0.f;
-  }
-  T* out = static_cast<T*>(const_cast<void*>(a.out.p)) + b * a.out.b + t;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int c = c0 + e * kTimeWarps;
-    if (c < C) out[c * a.out.o] = from_f<T>(ok ? fmaf((s[e] - mean) * rstd, a.gamma[c], a.beta[c]) : 0.f);
-  }
-}
-
-template <typename T, int E>
-__global__ void __launch_bounds__(kTimeWarps * 32) norm_bwd_time(const NormArgs a, const int cs) {
-  __shared__ float s_w[kTimeWarps][2][32];
-  __shared__ float s_b[2][32];
+// Blocks of a team (a cluster of cs) walk tiles of 32 frames of one utterance;
+// a team's block r holds channels r * kTimeC and up.
+template <typename T, int V, int E, bool BWD>
+__global__ void __launch_bounds__(kTimeWarps * 32, V == 1 && E > 4 ? 1 : 2) norm_time(const __grid_constant__ NormArgs a, const int cs) {
+  constexpr int F = 32 / V, NS = BWD ? 2 : 1;
+  __shared__ float s_w[kTimeWarps][NS][32];
+  __shared__ float s_b[2][NS][32];
   cg::cluster_group cl = cg::this_cluster();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, C = a.C;
   const int per_b = cdiv(a.T, 32), tiles = per_b * a.B, team = blockIdx.x / cs, rank = blockIdx.x - team * cs;
   const int teams = gridDim.x / cs;
-  const int c0 = rank * kTimeWarps * E + w;
-  float dg[E] = {}, db[E] = {};
+  // A warp's load covers V channels side by side (lanes / F) of 32 frames.
+  const int c0 = rank * kTimeC + w * V + lane / F, fl = (lane % F) * V;
+  constexpr int kStep = kTimeWarps * V;
+  float ga[E], be[E], dg[BWD ? E : 1] = {};
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int c = c0 + e * kStep;
+    ga[e] = c < C ? a.gamma[c] : 0.f;
+    be[e] = !BWD && c < C ? a.beta[c] : 0.f;
+  }
+  const int nc = c0 < C ? min(E, (C - c0 + kStep - 1) / kStep) : 0;  // this lane's channels
   for (int tile = team; tile < tiles; tile += teams) {
-    const int b = tile / per_b, t = (tile - b * per_b) * 32 + lane;
-    const bool in = t < a.T, ok = in && (!a.len || t < a.len[b]);
-    const T* x = static_cast<const T*>(a.x.p) + b * a.x.b + t;
-    const T* y = static_cast<const T*>(a.y.p) + b * a.y.b + t;
-    const T* go = static_cast<const T*>(a.dout.p) + b * a.dout.b + t;
-    float xh[E] = {}, g[E] = {}, sums[2] = {0.f, 0.f}, mean = 0.f, rstd = 0.f;
-    if (ok) {
-      mean = a.mean[(int64_t)b * a.T + t];
-      rstd = a.rstd[(int64_t)b * a.T + t];
+    const int b = tile / per_b, t = (tile - b * per_b) * 32 + fl;
+    const int n = a.len ? a.len[b] : a.T;
+    const bool in = t < a.T, some = in && t < n;
+    float v[E][V], g[BWD ? E : 1][V], u[E][V];
+    const T* x = static_cast<const T*>(a.x.p) + b * a.x.b + t + c0 * a.x.o;
+    const T* y = static_cast<const T*>(a.y.p) + b * a.y.b + t + c0 * a.y.o;
+    const T* d = static_cast<const T*>(a.dout.p) + b * a.dout.b + t + c0 * a.dout.o;
+    float mean[V], rstd[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) mean[i] = rstd[i] = 0.f;
+    if (BWD && some) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        mean[i] = a.mean[(int64_t)b * a.T + t + i];
+        rstd[i] = a.rstd[(int64_t)b * a.T + t + i];
+      }
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = c0 + e * kTimeWarps;
-      if (ok && c < C) {
-        xh[e] = to_f(x[c * a.x.o]);
-        g[e] = to_f(go[c * a.dout.o]);
-      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[e][i] = u[e][i] = 0.f;
+      if (some && e < nc) load_vec<T, V>(x + e * (kStep * a.x.o), v[e]);
     }
     if (a.y.p) {
 #pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (some && e < nc) load_vec<T, V>(y + e * (kStep * a.y.o), u[e]);
+    }
+    if (BWD) {
+#pragma unroll
       for (int e = 0; e < E; ++e) {
-        const int c = c0 + e * kTimeWarps;
-        if (ok && c < C) xh[e] += to_f(y[c * a.y.o]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[BWD ? e : 0][i] = 0.f;
+        if (some && e < nc) load_vec<T, V>(d + e * (kStep * a.dout.o), g[BWD ? e : 0]);
       }
     }
+    float sums[NS][V] = {};
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const bool ok = t + i < n;  // a frame behind the length may hold anything
+        v[e][i] = ok ? v[e][i] + u[e][i] : 0.f;
+        if (BWD) {
+          const int z = BWD ? e : 0;
+          v[e][i] = e < nc ? (v[e][i] - mean[i]) * rstd[i] : 0.f;
+          const float q = ok ? g[z][i] : 0.f;
+          dg[z] = fmaf(q, v[e][i], dg[z]);
+          be[e] += q;
+          g[z][i] = q * ga[e];
+          sums[0][i] += g[z][i];
+          sums[NS - 1][i] = fmaf(g[z][i], v[e][i], sums[NS - 1][i]);
+        } else {
+          sums[0][i] += v[e][i];
+        }
+      }
+    frame_sum<NS, V>(sums, s_w, s_b[0], cl, cs);
+    const float ic = 1.f / (float)C;
+    if (!BWD) {
+      float sq[1][V] = {};
+#pragma unroll
+      for (int i = 0; i < V; ++i) mean[i] = sums[0][i] * ic;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < nc)
+#pragma unroll
+          for (int i = 0; i < V; ++i) sq[0][i] = fmaf(v[e][i] - mean[i], v[e][i] - mean[i], sq[0][i]);
+      frame_sum<1, V>(sq, reinterpret_cast<float(*)[1][32]>(&s_w[0][0][0]), s_b[1], cl, cs);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const bool ok = t + i < n;
+        rstd[i] = ok ? rsqrtf(sq[0][i] * ic + a.eps) : 0.f;
+        mean[i] = ok ? mean[i] : 0.f;
+      }
+      if (w == 0 && rank == 0 && lane < F && in)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          a.mean[(int64_t)b * a.T + t + i] = mean[i];
+          a.rstd[(int64_t)b * a.T + t + i] = rstd[i];
+        }
+    }
+    if (in) {
+      const int64_t so = BWD ? a.dx.o : a.out.o;
+      T* out = static_cast<T*>(const_cast<void*>(BWD ? a.dx.p : a.out.p)) + b * (BWD ? a.dx.b : a.out.b) + t + c0 * so;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (e >= nc) continue;
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          o[i] = BWD ? rstd[i] * (g[BWD ? e : 0][i] - sums[0][i] * ic - v[e][i] * (sums[NS - 1][i] * ic))
+                     : t + i < n ? fmaf((v[e][i] - mean[i]) * rstd[i], ga[e], be[e]) : 0.f;
+        store_vec<T, V>(out + e * (kStep * so), o);
+      }
+    }
+    __syncthreads();  // the sums' buffers are free for the next tile
+  }
+  if (BWD) {
+    float* part = a.part + (int64_t)team * 2 * C;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = c0 + e * kTimeWarps;
-      if (c >= C) continue;
-      xh[e] = (xh[e] - mean) * rstd;
-      dg[e] = fmaf(g[e], xh[e], dg[e]);
-      db[e] += g[e];
-      g[e] *= a.gamma[c];
-      sums[0] += g[e];
-      sums[1] = fmaf(g[e], xh[e], sums[1]);
-    }
-    frame_sum<2>(sums, s_w, s_b, cl, cs);
-    const float m0 = sums[0] / (float)C, m1 = sums[1] / (float)C;
-    T* dx = static_cast<T*>(const_cast<void*>(a.dx.p)) + b * a.dx.b + t;
-    if (in) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int c = c0 + e * kTimeWarps;
-        if (c < C) dx[c * a.dx.o] = from_f<T>(rstd * (g[e] - m0 - xh[e] * m1));
+      for (int o = 1; o < F; o <<= 1) {
+        dg[BWD ? e : 0] += __shfl_xor_sync(0xffffffffu, dg[BWD ? e : 0], o);
+        be[e] += __shfl_xor_sync(0xffffffffu, be[e], o);
       }
-    }
-  }
-  float* part = a.part + (int64_t)team * 2 * C;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int c = c0 + e * kTimeWarps;
-    if (c >= C) continue;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      dg[e] += __shfl_xor_sync(0xffffffffu, dg[e], o);
-      db[e] += __shfl_xor_sync(0xffffffffu, db[e], o);
-    }
-    if (lane == 0) {
-      part[c] = dg[e];
-      part[C + c] = db[e];
+      if (lane % F == 0 && e < nc) {
+        part[c0 + e * kStep] = dg[BWD ? e : 0];
+        part[C + c0 + e * kStep] = be[e];
+      }
     }
   }
 }
 
 // dgamma, dbeta = the partial sums added in block order: 32 columns per block,
-// 8 runs of blocks side by side, then the 8 runs in turn.
-__global__ void __launch_bounds__(256) norm_part_sum(const float* part, int blocks, int C, float* dgamma,
+// 16 runs of blocks side by side, then the runs in turn.
+__global__ void __launch_bounds__(512) norm_part_sum(const float* part, int blocks, int C, float* dgamma,
                                                      float* dbeta) {
-  __shared__ float s[8][32];
+  __shared__ float s[16][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int e = blockIdx.x * 32 + lane, n = 2 * C;
   float v = 0.f;
-  if (e < n)
-    for (int k = w; k < blocks; k += 8) v += part[(int64_t)k * n + e];
+  if (e < n) {
+#pragma unroll 8
+    for (int k = w; k < blocks; k += 16) v += part[(int64_t)k * n + e];
+  }
   s[w][lane] = v;
   __syncthreads();
   if (w == 0 && e < n) {
-    for (int k = 1; k < 8; ++k) v += s[k][lane];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) v += s[k][lane];
     if (e < C) dgamma[e] = v;
     else dbeta[e - C] = v;
   }
 }
 
-// Threads of a block that share a frame, and channels per thread: as few
-// threads as hold the frame with 16 channels each, 256 threads with 32 beyond.
+// Threads that share a frame, and channels per thread.  The forward holds 32
+// channels a thread (one warp per frame up to 1024), the backward 16, since it
+// also holds gamma and two sums for each.
 struct RowShape {
   int R, E;
 };
-RowShape row_shape(int C) {
+RowShape row_shape(int C, bool bwd) {
   if (C <= 256) return {32, 8};
   if (C <= 512) return {32, 16};
-  if (C <= 1024) return {64, 16};
-  if (C <= 2048) return {128, 16};
-  if (C <= 4096) return {256, 16};
-  return {256, 32};
+  if (!bwd) return C <= 1024 ? RowShape{32, 32} : C <= 2048 ? RowShape{64, 32} : C <= 4096 ? RowShape{128, 32} : RowShape{256, 32};
+  return C <= 1024 ? RowShape{64, 16} : C <= 2048 ? RowShape{128, 16} : C <= 4096 ? RowShape{256, 16} : RowShape{256, 32};
 }
 
-int row_bwd_blocks(const NormArgs& a) {
-  const RowShape s = row_shape(a.C);
-  const int64_t n = ((int64_t)a.B * a.T + kRowThreads / s.R - 1) / (kRowThreads / s.R);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(n, 148 * 4));  // one block writes the zeros of no frames
+// Two blocks per SM, fewer when the frames do not fill them.
+int row_blocks(const NormArgs& a, bool bwd) {
+  const int G = kRowThreads / row_shape(a.C, bwd).R;
+  return std::max(1, std::min(cdiv(a.B * a.T, G), 148 * 2));
 }
 
 int time_cluster(int C) {
   int cs = 1;
-  while (cs * kTimeWarps * kTimeE < C) cs *= 2;
+  while (cs * kTimeC < C) cs *= 2;
   return cs;
 }
 
-int time_bwd_teams(const NormArgs& a) {
-  const int cs = time_cluster(a.C);
-  return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)a.B * cdiv(a.T, 32), 148 * 2 / cs));
+bool aligned(const NormTensor& t, int n, int V, int elem) {
+  return !t.p || (reinterpret_cast<uintptr_t>(t.p) % (V * elem) == 0 && t.b % V == 0 && t.o % V == 0 && n % V == 0);
+}
+bool aligned(const NormArgs& a, bool bwd, int n, int V, int elem) {
+  return aligned(a.x, n, V, elem) && aligned(a.y, n, V, elem) &&
+         (bwd ? aligned(a.dout, n, V, elem) && aligned(a.dx, n, V, elem) : aligned(a.out, n, V, elem));
 }
 
-bool vec_ok(const NormTensor& t, int C, int V, int elem) {
-  return !t.p || (reinterpret_cast<uintptr_t>(t.p) % 16 == 0 && t.b % V == 0 && t.o % V == 0 && C % V == 0 &&
-                  16 / elem == V);
+// Frames per lane of the [B][C][T] kernels.
+int time_vec(const NormArgs& a, bool bwd) { return aligned(a, bwd, a.T, 4, a.ty == Ty::F32 ? 4 : 2) ? 4 : 1; }
+
+// Two blocks per SM, one where a lane's single frames leave many channels to it.
+int time_teams(const NormArgs& a, bool bwd) {
+  const int per_sm = time_vec(a, bwd) == 1 && a.C > 4 * kTimeWarps ? 1 : 2;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)a.B * cdiv(a.T, 32), 148 * per_sm / time_cluster(a.C)));
 }
 
-template <typename T, int V, int E, int R>
-cudaError_t rows_launch(const NormArgs& a, bool bwd, cudaStream_t st) {
+template <typename T, int V, int E, int R, bool BWD>
+cudaError_t rows_launch(const NormArgs& a, cudaStream_t st) {
   constexpr int G = kRowThreads / R;
-  if (!bwd) {
-    const int64_t n = ((int64_t)a.B * a.T + G - 1) / G;
-    norm_fwd_rows<T, V, E, R><<<(unsigned)n, kRowThreads, 0, st>>>(a);
-  } else {
-    const size_t smem = G > 1 ? 2 * (size_t)a.C * sizeof(float) : 0;
-    norm_bwd_rows<T, V, E, R><<<row_bwd_blocks(a), kRowThreads, smem, st>>>(a);
+  const size_t stage = (size_t)G * (BWD ? 3 : 2) * a.C * sizeof(T), sums = BWD ? 2 * (size_t)a.C * sizeof(float) : 0;
+  // Two blocks share an SM's shared memory where two stages of each fit.
+  int stages = 0;
+  if (V > 1) {
+    stages = (int)std::min<size_t>(kMaxStages, 96 * 1024 / stage);
+    if (stages < 2) stages = (int)(200 * 1024 / stage);
   }
+  const size_t smem = std::max(stages * stage, sums);
+  int regs;
+  const cudaError_t e = kernel_setup(norm_rows<T, V, E, R, BWD>, smem, &regs);
+  if (e != cudaSuccess) return e;
+  norm_rows<T, V, E, R, BWD><<<row_blocks(a, BWD), kRowThreads, smem, st>>>(a, stages);
   return cudaGetLastError();
 }
 
-template <typename T, int V>
-cudaError_t rows_shape(const NormArgs& a, bool bwd, cudaStream_t st) {
-  const RowShape s = row_shape(a.C);
-  if (s.R == 32) return s.E == 8 ? rows_launch<T, V, 8, 32>(a, bwd, st) : rows_launch<T, V, 16, 32>(a, bwd, st);
-  if (s.R == 64) return rows_launch<T, V, 16, 64>(a, bwd, st);
-  if (s.R == 128) return rows_launch<T, V, 16, 128>(a, bwd, st);
-  return s.E == 16 ? rows_launch<T, V, 16, 256>(a, bwd, st) : rows_launch<T, V, 32, 256>(a, bwd, st);
+template <typename T, int V, bool BWD>
+cudaError_t rows_shape(const NormArgs& a, cudaStream_t st) {
+  const RowShape s = row_shape(a.C, BWD);
+  if (s.R == 32 && s.E == 8) return rows_launch<T, V, 8, 32, BWD>(a, st);
+  if (s.R == 32 && s.E == 16) return rows_launch<T, V, 16, 32, BWD>(a, st);
+  if constexpr (BWD) {
+    if (s.R == 64) return rows_launch<T, V, 16, 64, true>(a, st);
+    if (s.R == 128) return rows_launch<T, V, 16, 128, true>(a, st);
+    return s.E == 16 ? rows_launch<T, V, 16, 256, true>(a, st) : rows_launch<T, V, 32, 256, true>(a, st);
+  } else {
+    if (s.R == 32) return rows_launch<T, V, 32, 32, false>(a, st);
+    if (s.R == 64) return rows_launch<T, V, 32, 64, false>(a, st);
+    return s.R == 128 ? rows_launch<T, V, 32, 128, false>(a, st) : rows_launch<T, V, 32, 256, false>(a, st);
+  }
 }
 
-template <typename T, int E>
-cudaError_t time_launch(const NormArgs& a, bool bwd, int cs, cudaStream_t st) {
-  const int64_t tiles = (int64_t)a.B * cdiv(a.T, 32);
+template <typename T, int V, int E, bool BWD>
+cudaError_t time_launch(const NormArgs& a, int cs, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((bwd ? time_bwd_teams(a) : tiles) * cs));
+  cfg.gridDim = dim3((unsigned)(time_teams(a, BWD) * cs));
   cfg.blockDim = dim3(kTimeWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -493,48 +591,55 @@ cudaError_t time_launch(const NormArgs& a, bool bwd, int cs, cudaStream_t st) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return bwd ? cudaLaunchKernelEx(&cfg, norm_bwd_time<T, E>, a, cs) : cudaLaunchKernelEx(&cfg, norm_fwd_time<T, E>, a, cs);
+  return cudaLaunchKernelEx(&cfg, norm_time<T, V, E, BWD>, a, cs);
 }
 
-template <typename T>
-cudaError_t run_t(const NormArgs& a, bool bwd, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  if (a.rows) {
-    const bool vec = vec_ok(a.x, a.C, V, sizeof(T)) && vec_ok(a.y, a.C, V, sizeof(T)) &&
-                     (bwd ? vec_ok(a.dout, a.C, V, sizeof(T)) && vec_ok(a.dx, a.C, V, sizeof(T))
-                          : vec_ok(a.out, a.C, V, sizeof(T)));
-    return vec ? rows_shape<T, V>(a, bwd, st) : rows_shape<T, 1>(a, bwd, st);
+// E * V channels and frames per lane: as many channels as a block of 16 warps
+// needs for min(C, 256).
+template <typename T, bool BWD>
+cudaError_t time_shape(const NormArgs& a, cudaStream_t st) {
+  const int cs = time_cluster(a.C), per = cdiv(std::min(a.C, kTimeC), kTimeWarps);
+  if (time_vec(a, BWD) == 4) {
+    if (per > 12) return time_launch<T, 4, 4, BWD>(a, cs, st);
+    if (per > 8) return time_launch<T, 4, 3, BWD>(a, cs, st);
+    return per > 4 ? time_launch<T, 4, 2, BWD>(a, cs, st) : time_launch<T, 4, 1, BWD>(a, cs, st);
   }
-  const int cs = time_cluster(a.C), e = cdiv(cdiv(a.C, cs), kTimeWarps);
-  // With several blocks per frame each takes its full 256 channels.
-  if (cs > 1 || e > 12) return time_launch<T, 16>(a, bwd, cs, st);
-  if (e > 8) return time_launch<T, 12>(a, bwd, cs, st);
-  return e > 4 ? time_launch<T, 8>(a, bwd, cs, st) : time_launch<T, 4>(a, bwd, cs, st);
+  if (per > 12) return time_launch<T, 1, 16, BWD>(a, cs, st);
+  return per > 4 ? time_launch<T, 1, 12, BWD>(a, cs, st) : time_launch<T, 1, 4, BWD>(a, cs, st);
 }
 
-cudaError_t run(const NormArgs& a, bool bwd, cudaStream_t st) {
+template <typename T, bool BWD>
+cudaError_t run_t(const NormArgs& a, cudaStream_t st) {
+  if (!a.rows) return time_shape<T, BWD>(a, st);
+  constexpr int V = 16 / sizeof(T);
+  return aligned(a, BWD, a.C, V, sizeof(T)) ? rows_shape<T, V, BWD>(a, st) : rows_shape<T, 1, BWD>(a, st);
+}
+
+template <bool BWD>
+cudaError_t run(const NormArgs& a, cudaStream_t st) {
   switch (a.ty) {
-    case Ty::F32: return run_t<float>(a, bwd, st);
-    case Ty::F16: return run_t<__half>(a, bwd, st);
-    default: return run_t<__nv_bfloat16>(a, bwd, st);
+    case Ty::F32: return run_t<float, BWD>(a, st);
+    case Ty::F16: return run_t<__half, BWD>(a, st);
+    default: return run_t<__nv_bfloat16, BWD>(a, st);
   }
 }
 
 }  // namespace
 
 size_t norm_bwd_workspace(const NormArgs& a) {
-  const int n = a.rows ? row_bwd_blocks(a) : time_bwd_teams(a);
-  return (size_t)n * 2 * a.C * sizeof(float);
+  return (size_t)(a.rows ? row_blocks(a, true) : time_teams(a, true)) * 2 * a.C * sizeof(float);
 }
 
-cudaError_t norm_forward(const NormArgs& a, cudaStream_t st) { return a.T ? run(a, false, st) : cudaSuccess; }
+cudaError_t norm_forward(const NormArgs& a, cudaStream_t st) { return a.T ? run<false>(a, st) : cudaSuccess; }
 
 cudaError_t norm_backward(const NormArgs& a, cudaStream_t st) {
-  const cudaError_t e = run(a, true, st);
+  const cudaError_t e = run<true>(a, st);
   if (e != cudaSuccess) return e;
-  const int n = a.rows ? row_bwd_blocks(a) : time_bwd_teams(a);
-  norm_part_sum<<<cdiv(2 * a.C, 32), 256, 0, st>>>(a.part, n, a.C, a.dgamma, a.dbeta);
+  const int n = a.rows ? row_blocks(a, true) : time_teams(a, true);
+  norm_part_sum<<<cdiv(2 * a.C, 32), 512, 0, st>>>(a.part, n, a.C, a.dgamma, a.dbeta);
   return cudaGetLastError();
 }
+
+cudaError_t norm_gave_up(int* out, cudaStream_t st) { return take_gave_up(g_gave_up, out, st); }
 
 }  // namespace gsv

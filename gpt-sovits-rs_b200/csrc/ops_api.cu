@@ -251,11 +251,12 @@ int gsvdec_attention_backward(const gsvdec_attention* a, int device, void* strea
 int gsvdec_ops_status(int device, void* stream) {
   gsv::OnDevice dev(device);
   if (dev.rc != GSV_OK) return dev.rc;
-  int fwd = 0, bwd = 0;
+  int fwd = 0, bwd = 0, norm = 0;
   cudaError_t e = gsv::attn_fwd_gave_up(&fwd, static_cast<cudaStream_t>(stream));
   if (e == cudaSuccess) e = gsv::attn_bwd_gave_up(&bwd, static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) e = gsv::norm_gave_up(&norm, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return gsv::finish(e, "operator status");
-  return fwd || bwd ? gsv::set_err(GSV_E_TIMEOUT, "a bounded device wait of an attention call on device %d gave up", device)
+  return fwd || bwd || norm ? gsv::set_err(GSV_E_TIMEOUT, "a bounded device wait of an operator on device %d gave up", device)
                  : GSV_OK;
 }
 

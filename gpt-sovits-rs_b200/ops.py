@@ -202,8 +202,8 @@ def attention_backward(do, q, k, v, o, lse, *, scale: Optional[float] = None, ca
 
 def ops_status(device=None) -> None:
     """Waits for the current stream of ``device`` (default: the current one) and
-    raises GsvDecError(GSV_E_TIMEOUT) if a bounded device wait of an attention
-    call there gave up (gsvdec_ops_status)."""
+    raises GsvDecError(GSV_E_TIMEOUT) if a bounded device wait of an operator
+    there gave up (gsvdec_ops_status)."""
     import torch
     index = torch.cuda.current_device() if device is None else torch.device(device).index
     _check(_lib().gsvdec_ops_status(index, torch.cuda.current_stream(index).cuda_stream))

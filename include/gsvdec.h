@@ -443,7 +443,7 @@ int gsvdec_attention_forward(const gsvdec_attention* a, int device, void* stream
 int gsvdec_attention_backward(const gsvdec_attention* a, int device, void* stream);
 
 /* Waits for `stream`, then reports whether a bounded device wait of an
- * attention call on `device` gave up since the last such call (GSV_E_TIMEOUT;
+ * attention or norm call on `device` gave up since the last such call (GSV_E_TIMEOUT;
  * the results of the call concerned are undefined). */
 int gsvdec_ops_status(int device, void* stream);
 
