@@ -539,9 +539,10 @@ bool aligned(const NormArgs& a, bool bwd, int n, int V, int elem) {
 // Frames per lane of the [B][C][T] kernels.
 int time_vec(const NormArgs& a, bool bwd) { return aligned(a, bwd, a.T, 4, a.ty == Ty::F32 ? 4 : 2) ? 4 : 1; }
 
-// Two blocks per SM, one where a lane's single frames leave many channels to it.
-int time_teams(const NormArgs& a, bool bwd) {
-  const int per_sm = time_vec(a, bwd) == 1 && a.C > 4 * kTimeWarps ? 1 : 2;
+int time_per_sm(const NormArgs& a, bool bwd) {  // one block where a lane's single frames leave it many channels
+  return time_vec(a, bwd) == 1 && a.C > 4 * kTimeWarps ? 1 : 2;
+}
+int time_teams(const NormArgs& a, int per_sm) {
   return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)a.B * cdiv(a.T, 32), 148 * per_sm / time_cluster(a.C)));
 }
 
@@ -582,7 +583,7 @@ cudaError_t rows_shape(const NormArgs& a, cudaStream_t st) {
 template <typename T, int V, int E, bool BWD>
 cudaError_t time_launch(const NormArgs& a, int cs, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(time_teams(a, BWD) * cs));
+  cfg.gridDim = dim3((unsigned)(time_teams(a, time_per_sm(a, BWD)) * cs));
   cfg.blockDim = dim3(kTimeWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -626,8 +627,9 @@ cudaError_t run(const NormArgs& a, cudaStream_t st) {
 
 }  // namespace
 
+// The largest of the kernels the alignment may choose.
 size_t norm_bwd_workspace(const NormArgs& a) {
-  return (size_t)(a.rows ? row_blocks(a, true) : time_teams(a, true)) * 2 * a.C * sizeof(float);
+  return (size_t)(a.rows ? row_blocks(a, true) : time_teams(a, 2)) * 2 * a.C * sizeof(float);
 }
 
 cudaError_t norm_forward(const NormArgs& a, cudaStream_t st) { return a.T ? run<false>(a, st) : cudaSuccess; }
@@ -635,7 +637,7 @@ cudaError_t norm_forward(const NormArgs& a, cudaStream_t st) { return a.T ? run<
 cudaError_t norm_backward(const NormArgs& a, cudaStream_t st) {
   const cudaError_t e = run<true>(a, st);
   if (e != cudaSuccess) return e;
-  const int n = a.rows ? row_blocks(a, true) : time_teams(a, true);
+  const int n = a.rows ? row_blocks(a, true) : time_teams(a, time_per_sm(a, true));
   norm_part_sum<<<cdiv(2 * a.C, 32), 512, 0, st>>>(a.part, n, a.C, a.dgamma, a.dbeta);
   return cudaGetLastError();
 }

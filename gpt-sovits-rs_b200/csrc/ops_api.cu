@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "../../include/gsvdec.h"
@@ -15,23 +16,33 @@ int set_err(int code, const char* fmt, ...);  // gsvdec_api.cu
 
 namespace {
 
+// GSV_OK when `device` is a device the kernels run on; looked up once each.
+int device_ok(int device) {
+  constexpr int kMax = 64;
+  static std::atomic<int> known[kMax];  // 0 not looked up, 1 fine, else 2 + 16 major + minor
+  int n = 0;
+  if (device < 0 || device >= kMax || known[device].load(std::memory_order_acquire) == 0) {
+    if (cudaGetDeviceCount(&n) != cudaSuccess || device < 0 || device >= n || device >= kMax) {
+      cudaGetLastError();
+      return set_err(GSV_E_INVALID_ARG, "device %d is not one of the %d CUDA devices", device, n);
+    }
+    int major = 0, minor = 0;
+    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
+    cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device);
+    known[device].store(major == 10 && minor == 0 ? 1 : 2 + 16 * major + minor, std::memory_order_release);
+  }
+  const int k = known[device].load(std::memory_order_acquire);
+  if (k == 1) return GSV_OK;
+  return set_err(GSV_E_UNSUPPORTED, "device %d is sm_%d%d; the kernels are built for sm_100a", device, (k - 2) / 16,
+                 (k - 2) % 16);
+}
+
 // The caller's current device is put back when the call returns.
 struct OnDevice {
   int prev = -1;
-  int rc = GSV_OK;
-  explicit OnDevice(int device) {
-    int n = 0, major = 0, minor = 0;
-    if (cudaGetDeviceCount(&n) != cudaSuccess || device < 0 || device >= n) {
-      cudaGetLastError();
-      rc = set_err(GSV_E_INVALID_ARG, "device %d is not one of the %d CUDA devices", device, n);
-      return;
-    }
-    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
-    cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device);
-    if (major != 10 || minor != 0) {
-      rc = set_err(GSV_E_UNSUPPORTED, "device %d is sm_%d%d; the kernels are built for sm_100a", device, major, minor);
-      return;
-    }
+  int rc;
+  explicit OnDevice(int device) : rc(device_ok(device)) {
+    if (rc != GSV_OK) return;
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
     if (prev != device) {
       const cudaError_t e = cudaSetDevice(device);
@@ -59,6 +70,8 @@ bool spread(const int64_t* stride, const int* n, int axes, int64_t width) {
   int order[3] = {0, 1, 2};
   std::sort(order, order + axes, [&](int x, int y) { return stride[x] < stride[y]; });
   int64_t span = width;
+  for (int i = 0; i < axes; ++i)
+    if (n[i] == 0) return true;
   for (int i = 0; i < axes; ++i) {
     const int x = order[i];
     if (n[x] <= 1) continue;

@@ -9,7 +9,9 @@ forward calls return what their backward needs.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+import struct
 from typing import Optional
 
 _I64x3 = ctypes.c_int64 * 3
@@ -38,113 +40,136 @@ class _Norm(ctypes.Structure):
 
 LAYOUTS = {"bct": 0, "btc": 1}
 
+# The two argument structures, packed in one go (setting ctypes fields one by
+# one costs more than the smallest call's kernel).
+_ATTENTION = struct.Struct("@9if" + "2q3q9q2qq3qq" + "q3q3q9q2q" + "qQ")
+_NORM = struct.Struct("@5if" + "qqq2q2qqqqqq2q" + "qq2q2qqq" + "qQ")
+assert _ATTENTION.size == ctypes.sizeof(_Attention) and _NORM.size == ctypes.sizeof(_Norm)
+_Z3 = (0, 0, 0)
+
 
 def declare(lib) -> None:
     """Argument types of the operators' C functions."""
-    at, nt, sz = ctypes.POINTER(_Attention), ctypes.POINTER(_Norm), ctypes.POINTER(ctypes.c_size_t)
-    lib.gsvdec_attention_workspace.argtypes = [at, ctypes.c_int, sz]
-    lib.gsvdec_attention_forward.argtypes = [at, ctypes.c_int, _vp]
-    lib.gsvdec_attention_backward.argtypes = [at, ctypes.c_int, _vp]
+    sz = ctypes.POINTER(ctypes.c_size_t)
+    lib.gsvdec_attention_workspace.argtypes = [_vp, ctypes.c_int, sz]
+    lib.gsvdec_attention_forward.argtypes = [_vp, ctypes.c_int, _vp]
+    lib.gsvdec_attention_backward.argtypes = [_vp, ctypes.c_int, _vp]
     lib.gsvdec_ops_status.argtypes = [ctypes.c_int, _vp]
-    lib.gsvdec_norm_workspace.argtypes = [nt, sz]
-    lib.gsvdec_norm_forward.argtypes = [nt, ctypes.c_int, _vp]
-    lib.gsvdec_norm_backward.argtypes = [nt, ctypes.c_int, _vp]
+    lib.gsvdec_norm_workspace.argtypes = [_vp, sz]
+    lib.gsvdec_norm_forward.argtypes = [_vp, ctypes.c_int, _vp]
+    lib.gsvdec_norm_backward.argtypes = [_vp, ctypes.c_int, _vp]
 
 
-def _lib():
-    from . import library
-    return library()
+class _Calls:
+    """torch and the library's functions, looked up once."""
+
+    def __init__(self):
+        import torch
+        from . import _check, library
+        self.lib = lib = library()
+        self.check = _check
+        self.codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
+        self.empty, self.empty_strided = torch.empty, torch.empty_strided
+        self.attention_forward, self.attention_backward = lib.gsvdec_attention_forward, lib.gsvdec_attention_backward
+        self.norm_forward, self.norm_backward = lib.gsvdec_norm_forward, lib.gsvdec_norm_backward
+        # The current stream's handle without building a torch Stream object, where torch offers that.
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _check(rc: int) -> None:
-    if rc:
-        from . import _check as check
-        check(rc)
+_calls = None
 
 
-def _dtype(t) -> int:
-    import torch
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(t.dtype)
+def _get() -> _Calls:
+    global _calls
+    if _calls is None:
+        _calls = _Calls()
+    return _calls
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(backward, dtype, B, H, Hkv, Tq, Tk, D, window, causal) -> int:
+    a = _Attention()
+    a.dtype, a.B, a.H, a.Hkv, a.Tq, a.Tk, a.D, a.window, a.causal = dtype, B, H, Hkv, Tq, Tk, D, window, causal
+    a.scale = 1.0
+    n, c = ctypes.c_size_t(), _get()
+    c.check(c.lib.gsvdec_attention_workspace(ctypes.byref(a), backward, ctypes.byref(n)))
+    return n.value
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_workspace(dtype, layout, B, C, T) -> int:
+    a = _Norm()
+    a.dtype, a.layout, a.B, a.C, a.T = dtype, layout, B, C, T
+    n, c = ctypes.c_size_t(), _get()
+    c.check(c.lib.gsvdec_norm_workspace(ctypes.byref(a), ctypes.byref(n)))
+    return n.value
+
+
+def _need(name, t, shape, dtype, index, contiguous=False) -> int:
+    """Checks one tensor and returns its address."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
+    if t.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{index}")
+    if contiguous:
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    elif t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel():
+        raise ValueError(f"{name}: the last axis must be contiguous")
+    return t.data_ptr()
+
+
+def _first(name, t, ndim) -> int:
+    if not t.is_cuda or t.dim() != ndim:
+        raise ValueError(f"{name} must be a CUDA tensor with {ndim} axes")
+    return t.get_device()
+
+
+def _code(c, t) -> int:
+    code = c.codes.get(t.dtype)
     if code is None:
         raise ValueError(f"dtype must be float32, float16 or bfloat16, not {t.dtype}")
     return code
 
 
-def _take(name, t, shape, dtype, device, contiguous=False):
-    """Checks one tensor and returns its address (None stays None)."""
-    if t is None:
-        return None
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {list(shape)}, not {list(t.shape)}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not on {device}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    if not contiguous and t.shape[-1] > 1 and t.stride(-1) != 1 and t.numel():
-        raise ValueError(f"{name}: the last axis must be contiguous")
-    return t.data_ptr()
-
-
-def _run(call, a, device) -> None:
-    import torch
-    _check(call(ctypes.byref(a), device.index, torch.cuda.current_stream(device).cuda_stream))
-
-
-def _cuda(name, t, ndim):
-    if not t.is_cuda or t.dim() != ndim:
-        raise ValueError(f"{name} must be a CUDA tensor with {ndim} axes")
-    return t.device
-
-
-def _attention_args(q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v):
-    import torch
-    dev = _cuda("q", q, 4)
+def _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v):
+    """The checked inputs: (leading fields, addresses and strides up to rel_v, device index)."""
+    index = _first("q", q, 4)
+    code, t = _code(c, q), q.dtype
+    qs = q.shape
+    B, H, Tq, D = qs
     if k.dim() != 4:
         raise ValueError("k must have 4 axes")
-    B, H, Tq, D = q.shape
-    Hkv, Tk = k.shape[1], k.shape[2]
-    a = _Attention()
-    a.dtype = _dtype(q)
-    a.B, a.H, a.Hkv, a.Tq, a.Tk, a.D = B, H, Hkv, Tq, Tk, D
-    a.causal = 1 if causal else 0
-    a.scale = 1.0 / math.sqrt(D) if scale is None else scale
-    a.q = _take("q", q, (B, H, Tq, D), q.dtype, dev)
-    a.k = _take("k", k, (B, Hkv, Tk, D), q.dtype, dev)
-    a.v = _take("v", v, (B, Hkv, Tk, D), q.dtype, dev)
-    a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    a.q_lengths = _take("q_lengths", q_lengths, (B,), torch.int32, dev, True)
-    a.k_lengths = _take("k_lengths", k_lengths, (B,), torch.int32, dev, True)
-    if (rel_k is None) != (rel_v is None):
-        raise ValueError("rel_k and rel_v come together")
-    a.window = -1
-    if rel_k is not None:
-        n = rel_k.shape[0]
-        if rel_k.dim() != 2 or n % 2 == 0:
+    ks = k.shape
+    Hkv, Tk = ks[1], ks[2]
+    if ks[0] != B or ks[3] != D:
+        raise ValueError(f"k must be [{B}, heads, T, {D}], not {list(ks)}")
+    pq, pk, pv = _need("q", q, qs, t, index), _need("k", k, ks, t, index), _need("v", v, ks, t, index)
+    ql = 0 if q_lengths is None else _need("q_lengths", q_lengths, (B,), c.i32, index, True)
+    kl = 0 if k_lengths is None else _need("k_lengths", k_lengths, (B,), c.i32, index, True)
+    window, rk, rv = -1, 0, 0
+    if rel_k is not None or rel_v is not None:
+        if rel_k is None or rel_v is None:
+            raise ValueError("rel_k and rel_v come together")
+        if rel_k.dim() != 2 or rel_k.shape[0] % 2 == 0:
             raise ValueError("rel_k must be [2 w + 1, D]")
-        a.window = n // 2
-        a.rel_k = _take("rel_k", rel_k, (n, D), q.dtype, dev, True)
-        a.rel_v = _take("rel_v", rel_v, (n, D), q.dtype, dev, True)
-    return a, dev
+        n = rel_k.shape[0]
+        window = n // 2
+        rk, rv = _need("rel_k", rel_k, (n, D), t, index, True), _need("rel_v", rel_v, (n, D), t, index, True)
+    lead = (code, B, H, Hkv, Tq, Tk, D, window, 1 if causal else 0)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    return lead, (scale, ql, kl, pq, pk, pv, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], rk, rv), index
 
 
-def _workspace(a, backward, dev):
-    import torch
-    n = ctypes.c_size_t()
-    _check(_lib().gsvdec_attention_workspace(ctypes.byref(a), backward, ctypes.byref(n)))
-    ws = None
-    if n.value:
-        ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
-    return ws
-
-
-def _like(t):
-    """A new tensor of t's shape in [B, T, heads, D] memory order."""
-    import torch
-    B, H, T, D = t.shape
-    return torch.empty((B, T, H, D), dtype=t.dtype, device=t.device).transpose(1, 2)
+def _heads_last(c, t, B, H, T, D, like):
+    """A new [B, H, T, D] tensor in [B, T, H, D] memory order, and its strides."""
+    s = (T * H * D, D, H * D)
+    return c.empty_strided((B, H, T, D), (*s, 1), dtype=t, device=like.device), s
 
 
 def attention(q, k, v, *, scale: Optional[float] = None, causal: bool = False, q_lengths=None, k_lengths=None,
@@ -154,22 +179,26 @@ def attention(q, k, v, *, scale: Optional[float] = None, causal: bool = False, q
 
     q [B, H, Tq, D], k and v [B, Hkv, Tk, D] in fp32, fp16 or bf16 with any
     strides but a contiguous last axis; H a multiple of Hkv (query head h reads
-    key head h / (H / Hkv)).  ``q_lengths`` / ``k_lengths`` [B] int32: valid
-    rows.  The sequences are aligned at their ends: query i of utterance b
-    stands at key position i + k_len - q_len, which ``causal`` and the offsets
-    of ``rel_k`` / ``rel_v`` [2 w + 1, D] (learned relative keys and values,
-    offsets -w .. w) count from.  Rows without an allowed key give o = 0 and
-    lse = -inf.  o [B, H, Tq, D] has [B, Tq, H, D] memory order; lse
-    [B, H, Tq] fp32 is the log-sum-exp of each row's scores.
+    key head h / (H / Hkv)); D up to 128.  ``q_lengths`` / ``k_lengths`` [B]
+    int32: valid rows.  The sequences are aligned at their ends: query i of
+    utterance b stands at key position i + k_len - q_len, which ``causal`` and
+    the offsets of ``rel_k`` / ``rel_v`` [2 w + 1, D] (learned relative keys and
+    values, offsets -w .. w, w up to 15) count from.  Rows without an allowed
+    key give o = 0 and lse = -inf.  o [B, H, Tq, D] has [B, Tq, H, D] memory
+    order; lse [B, H, Tq] fp32 is the log-sum-exp of each row's scores.
     """
-    import torch
-    a, dev = _attention_args(q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
-    o = _like(q)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev)
-    a.o, a.lse = o.data_ptr(), lse.data_ptr()
-    a.o_stride[:] = o.stride()[:3]
-    ws = _workspace(a, 0, dev)  # noqa: F841  (alive until the call has queued its kernels)
-    _run(_lib().gsvdec_attention_forward, a, dev)
+    c = _get()
+    lead, given, index = _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
+    code, B, H, _, Tq, _, D = lead[:7]
+    o, so = _heads_last(c, q.dtype, B, H, Tq, D, q)
+    lse = c.empty((B, H, Tq), dtype=c.f32, device=q.device)
+    n = _attention_workspace(0, *lead)
+    ws = c.empty(n, dtype=c.u8, device=q.device) if n else None
+    a = _ATTENTION.pack(*lead, *given, o.data_ptr(), *so, lse.data_ptr(), 0, *_Z3, 0, 0, 0, *_Z3, *_Z3, *_Z3, 0, 0,
+                        ws.data_ptr() if n else 0, n)
+    rc = c.attention_forward(a, index, c.stream(index))
+    if rc:
+        c.check(rc)
     return o, lse
 
 
@@ -182,21 +211,28 @@ def attention_backward(do, q, k, v, o, lse, *, scale: Optional[float] = None, ca
     gradient has its input's type (gradients of shared key heads and of the
     relative rows are summed in fp32 and rounded once) and is bit-reproducible.
     """
-    import torch
-    a, dev = _attention_args(q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
-    a.d_o = _take("do", do, tuple(q.shape), q.dtype, dev)
-    a.o = _take("o", o, tuple(q.shape), q.dtype, dev)
-    a.lse = _take("lse", lse, tuple(q.shape[:3]), torch.float32, dev, True)
-    a.d_o_stride[:], a.o_stride[:] = do.stride()[:3], o.stride()[:3]
-    dq, dk, dv = _like(q), _like(k), _like(k)
-    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-    a.dq_stride[:], a.dk_stride[:], a.dv_stride[:] = dq.stride()[:3], dk.stride()[:3], dv.stride()[:3]
+    c = _get()
+    lead, given, index = _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
+    code, B, H, Hkv, Tq, Tk, D, window = lead[:8]
+    t, qs = q.dtype, q.shape
+    pdo, po = _need("do", do, qs, t, index), _need("o", o, qs, t, index)
+    pl = _need("lse", lse, qs[:3], c.f32, index, True)
+    dq, sq = _heads_last(c, t, B, H, Tq, D, q)
+    dk, sk = _heads_last(c, t, B, Hkv, Tk, D, q)
+    dv, _ = _heads_last(c, t, B, Hkv, Tk, D, q)
     drk = drv = None
-    if rel_k is not None:
-        drk, drv = torch.empty_like(rel_k), torch.empty_like(rel_v)
-        a.drel_k, a.drel_v = drk.data_ptr(), drv.data_ptr()
-    ws = _workspace(a, 1, dev)  # noqa: F841
-    _run(_lib().gsvdec_attention_backward, a, dev)
+    prk = prv = 0
+    if window >= 0:
+        drk, drv = c.empty((2 * window + 1, D), dtype=t, device=q.device), c.empty((2 * window + 1, D), dtype=t,
+                                                                                 device=q.device)
+        prk, prv = drk.data_ptr(), drv.data_ptr()
+    n = _attention_workspace(1, *lead)
+    ws = c.empty(n, dtype=c.u8, device=q.device)
+    a = _ATTENTION.pack(*lead, *given, po, *o.stride()[:3], pl, pdo, *do.stride()[:3], dq.data_ptr(), dk.data_ptr(),
+                        dv.data_ptr(), *sq, *sk, *sk, prk, prv, ws.data_ptr(), n)
+    rc = c.attention_backward(a, index, c.stream(index))
+    if rc:
+        c.check(rc)
     return dq, dk, dv, drk, drv
 
 
@@ -205,29 +241,24 @@ def ops_status(device=None) -> None:
     raises GsvDecError(GSV_E_TIMEOUT) if a bounded device wait of an operator
     there gave up (gsvdec_ops_status)."""
     import torch
-    index = torch.cuda.current_device() if device is None else torch.device(device).index
-    _check(_lib().gsvdec_ops_status(index, torch.cuda.current_stream(index).cuda_stream))
+    index = None if device is None else torch.device(device).index
+    if index is None:
+        index = torch.cuda.current_device()
+    c = _get()
+    c.check(c.lib.gsvdec_ops_status(index, c.stream(index)))
 
 
-def _norm_args(x, y, gamma, beta, lengths, layout, eps):
-    import torch
-    dev = _cuda("x", x, 3)
-    if layout not in LAYOUTS:
+def _norm_in(c, x, y, lengths, layout):
+    index = _first("x", x, 3)
+    code, t, xs = _code(c, x), x.dtype, x.shape
+    lay = LAYOUTS.get(layout)
+    if lay is None:
         raise ValueError(f"layout must be one of {sorted(LAYOUTS)}")
-    a = _Norm()
-    a.dtype, a.layout = _dtype(x), LAYOUTS[layout]
-    a.B = x.shape[0]
-    a.C, a.T = (x.shape[1], x.shape[2]) if layout == "bct" else (x.shape[2], x.shape[1])
-    a.eps = eps
-    a.x = _take("x", x, tuple(x.shape), x.dtype, dev)
-    a.y = _take("y", y, tuple(x.shape), x.dtype, dev)
-    a.x_stride[:] = x.stride()[:2]
-    if y is not None:
-        a.y_stride[:] = y.stride()[:2]
-    a.gamma = _take("gamma", gamma, (a.C,), torch.float32, dev, True)
-    a.beta = _take("beta", beta, (a.C,), torch.float32, dev, True)
-    a.lengths = _take("lengths", lengths, (a.B,), torch.int32, dev, True)
-    return a, dev
+    B, C, T = xs if lay == 0 else (xs[0], xs[2], xs[1])
+    px = _need("x", x, xs, t, index)
+    py, sy = (0, (0, 0)) if y is None else (_need("y", y, xs, t, index), y.stride()[:2])
+    ln = 0 if lengths is None else _need("lengths", lengths, (B,), c.i32, index, True)
+    return (code, lay, B, C, T), (ln, px, py, *x.stride()[:2], *sy), index
 
 
 def add_norm(x, y, gamma, beta, *, lengths=None, layout: str = "bct", eps: float = 1e-5):
@@ -235,18 +266,22 @@ def add_norm(x, y, gamma, beta, *, lengths=None, layout: str = "bct", eps: float
     EncoderLayer::forward, src/models/sovits_encp.rs:102); returns (out, mean,
     rstd).
 
-    x, y (or None) [B, C, T] (layout "bct") or [B, T, C] ("btc") in fp32, fp16
-    or bf16; gamma, beta [C] fp32; lengths [B] int32.  mean and rstd [B, T]
-    fp32 are what :func:`add_norm_backward` needs.  Frames t >= lengths[b] give
-    out = mean = rstd = 0.
+    x, y (or None) [B, C, T] (layout "bct", C up to 2048) or [B, T, C] ("btc",
+    C up to 8192) in fp32, fp16 or bf16; gamma, beta [C] fp32; lengths [B]
+    int32.  mean and rstd [B, T] fp32 are what :func:`add_norm_backward` needs.
+    Frames t >= lengths[b] give out = mean = rstd = 0.
     """
-    import torch
-    a, dev = _norm_args(x, y, gamma, beta, lengths, layout, eps)
-    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    mean, rstd = torch.empty((2, a.B, a.T), dtype=torch.float32, device=dev).unbind(0)
-    a.out, a.mean, a.rstd = out.data_ptr(), mean.data_ptr(), rstd.data_ptr()
-    a.out_stride[:] = out.stride()[:2]
-    _run(_lib().gsvdec_norm_forward, a, dev)
+    c = _get()
+    lead, given, index = _norm_in(c, x, y, lengths, layout)
+    B, C, T = lead[2:]
+    pg, pb = _need("gamma", gamma, (C,), c.f32, index, True), _need("beta", beta, (C,), c.f32, index, True)
+    out = c.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean, rstd = c.empty((B, T), dtype=c.f32, device=x.device), c.empty((B, T), dtype=c.f32, device=x.device)
+    a = _NORM.pack(*lead, eps, *given, pg, pb, mean.data_ptr(), rstd.data_ptr(), out.data_ptr(), *out.stride()[:2], 0, 0,
+                   0, 0, 0, 0, 0, 0, 0, 0)
+    rc = c.norm_forward(a, index, c.stream(index))
+    if rc:
+        c.check(rc)
     return out, mean, rstd
 
 
@@ -254,19 +289,19 @@ def add_norm_backward(d_out, x, y, gamma, mean, rstd, *, lengths=None, layout: s
     """Gradients (dx, dgamma, dbeta) of :func:`add_norm`; dx is the gradient of
     x and of y.  mean and rstd are add_norm's.  dgamma and dbeta are fp32 sums
     over the frames in a fixed order."""
-    import torch
-    a, dev = _norm_args(x, y, gamma, None, lengths, layout, 0.0)
-    a.d_out = _take("d_out", d_out, tuple(x.shape), x.dtype, dev)
-    a.d_out_stride[:] = d_out.stride()[:2]
-    a.mean = _take("mean", mean, (a.B, a.T), torch.float32, dev, True)
-    a.rstd = _take("rstd", rstd, (a.B, a.T), torch.float32, dev, True)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dgamma, dbeta = torch.empty((2, a.C), dtype=torch.float32, device=dev).unbind(0)
-    a.dx, a.dgamma, a.dbeta = dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr()
-    a.dx_stride[:] = dx.stride()[:2]
-    n = ctypes.c_size_t()
-    _check(_lib().gsvdec_norm_workspace(ctypes.byref(a), ctypes.byref(n)))
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), n.value
-    _run(_lib().gsvdec_norm_backward, a, dev)
+    c = _get()
+    lead, given, index = _norm_in(c, x, y, lengths, layout)
+    B, C, T = lead[2:]
+    pg = _need("gamma", gamma, (C,), c.f32, index, True)
+    pd = _need("d_out", d_out, x.shape, x.dtype, index)
+    pm, pr = _need("mean", mean, (B, T), c.f32, index, True), _need("rstd", rstd, (B, T), c.f32, index, True)
+    dx = c.empty(x.shape, dtype=x.dtype, device=x.device)
+    dgamma, dbeta = c.empty(C, dtype=c.f32, device=x.device), c.empty(C, dtype=c.f32, device=x.device)
+    n = _norm_workspace(*lead)
+    ws = c.empty(n, dtype=c.u8, device=x.device)
+    a = _NORM.pack(*lead, 0.0, *given, pg, 0, pm, pr, 0, 0, 0, pd, dx.data_ptr(), *d_out.stride()[:2],
+                   *dx.stride()[:2], dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), n)
+    rc = c.norm_backward(a, index, c.stream(index))
+    if rc:
+        c.check(rc)
     return dx, dgamma, dbeta

@@ -434,8 +434,8 @@ typedef struct gsvdec_attention {
   size_t workspace_bytes;
 } gsvdec_attention;
 
-/* Workspace of a forward (backward = 0) or backward call; only the sizes,
- * dtype, window, causal and strides of *a are read.  May be 0 bytes. */
+/* Workspace of a forward (backward = 0) or backward call; it depends on the
+ * sizes, dtype, window and causal of *a alone.  May be 0 bytes. */
 int gsvdec_attention_workspace(const gsvdec_attention* a, int backward, size_t* bytes);
 int gsvdec_attention_forward(const gsvdec_attention* a, int device, void* stream);
 /* Every gradient element is summed by one thread in a fixed order: equal
@@ -476,6 +476,7 @@ typedef struct gsvdec_norm {
   void* workspace;          /* gsvdec_norm_workspace bytes, 16-byte aligned */
   size_t workspace_bytes;
 } gsvdec_norm;
+/* Workspace of a backward call; it depends on the sizes and dtype alone. */
 int gsvdec_norm_workspace(const gsvdec_norm* a, size_t* bytes);
 int gsvdec_norm_forward(const gsvdec_norm* a, int device, void* stream);
 int gsvdec_norm_backward(const gsvdec_norm* a, int device, void* stream);
