@@ -1,0 +1,275 @@
+// attn_few.cu -- attention forward for few queries per key head (a decoding
+// step), all types, fp32 arithmetic (formulas in attn.h).
+//
+// With at most kFewRows rows (queries times query heads per key head) the call
+// is bound by reading k and v once.  Each row of k and v is read by G lanes, 8
+// channels each, as 16-byte vectors, and serves all rows of its key head from
+// registers.  Every group of G lanes walks its own keys, 64 bytes of k and of v
+// per lane at a time, with
+// its own running maximum and sum, so nothing is exchanged until the end; then
+// groups, warps and the blocks of a cluster (which split the keys) are joined
+// in a fixed order, the last through distributed shared memory: one launch and
+// no workspace.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "attn_common.cuh"
+#include "attn_launch.h"
+
+namespace cg = cooperative_groups;
+
+namespace gsv {
+namespace {
+
+constexpr int kFewWarps = 8;
+constexpr int kFewSplits = 8;  // largest portable cluster
+
+// Eight channels as they lie in memory, turned into fp32 where they are used.
+template <typename T>
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+  // Channels d0 .. d0 + 7 of a row, zeros from D on.
+  __device__ __forceinline__ void load(const T* row, int d0, int D, bool vec) {
+    if (vec) {
+      const T* p = row + min(d0, D - 8);
+#pragma unroll
+      for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
+        u[k] = reinterpret_cast<const uint4*>(p)[k];
+        if (d0 >= D) u[k] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    } else {
+      T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = d0 + i < D ? row[d0 + i] : from_f<T>(0.f);
+      memcpy(u, e, sizeof e);
+    }
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    T e[8];
+    memcpy(e, u, sizeof e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f(e[i]);
+  }
+};
+
+// exp2(x - m) with -inf - -inf = -inf.
+__device__ __forceinline__ float ex2_from(float x, float m) { return x == -INFINITY ? 0.f : exp2f(x - m); }
+
+template <typename T, int G, int R>
+__global__ void __launch_bounds__(kFewWarps * 32, R == 8 ? 1 : 2) attn_fwd_few(const __grid_constant__ AttnArgs a, const int cs,
+                                                               const bool vec) {
+  constexpr int KG = 32 / G, U = sizeof(T) == 4 ? 2 : 4, DP = 8 * G;  // key groups per warp, keys per step
+  __shared__ float s_acc[kFewWarps][R][DP];
+  __shared__ float s_m[kFewWarps][R], s_l[kFewWarps][R];
+  __shared__ float b_acc[R][DP], b_m[R], b_l[R];  // the block's, read by the cluster
+  cg::cluster_group cl = cg::this_cluster();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, gl = lane % G, d0 = gl * 8;
+  const int rank = blockIdx.x % cs, hk = blockIdx.y, b = blockIdx.z, D = a.D, g = a.H / a.Hkv;
+  const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk), off = kl - ql;
+  const int rows = a.Tq * g;
+  const float sl2 = a.scale * kLog2e;
+  const T* relk = static_cast<const T*>(a.relk);
+  const T* relv = static_cast<const T*>(a.relv);
+  float q[R][8], acc[R][8] = {}, m[R], l[R] = {};
+  int n[R], most = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    const int i = r / g, h = hk * g + r % g;
+    n[r] = r < rows ? allowed_keys(i, ql, kl, a.causal) : 0;
+    most = max(most, n[r]);
+#pragma unroll
+    for (int y = 0; y < 8; ++y) q[r][y] = 0.f;
+    if (n[r] > 0) {
+      Raw8<T> x;
+      x.load(static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + i * a.sq.t, d0, D, vec);
+      x.get(q[r]);
+    }
+  }
+  const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
+  const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
+  // The cluster's groups take runs of U keys in turn.
+  const int groups = cs * kFewWarps * KG, mine = (rank * kFewWarps + w) * KG + lane / G;
+  const int steps = (most + U * groups - 1) / (U * groups);  // the same for the whole cluster
+  for (int x = 0; x < steps; ++x) {
+    const int j0 = (x * groups + mine) * U;
+    Raw8<T> kr[U], vr[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) kr[u].load(k + (int64_t)min(j0 + u, most - 1) * a.sk.t, d0, D, vec);
+#pragma unroll
+    for (int u = 0; u < U; ++u) vr[u].load(v + (int64_t)min(j0 + u, most - 1) * a.sv.t, d0, D, vec);
+    float s[R][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float kk[8];
+      kr[u].get(kk);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        s[r][u] = 0.f;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) s[r][u] = fmaf(q[r][y], kk[y], s[r][u]);
+        if (a.nrel) {
+          const unsigned o = (unsigned)(j0 + u - r / g - off + a.window);
+          if (o < (unsigned)a.nrel)
+#pragma unroll
+            for (int y = 0; y < 8; ++y)
+              if (d0 + y < D) s[r][u] = fmaf(q[r][y], to_f(relk[o * D + d0 + y]), s[r][u]);
+          __syncwarp();
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float mx = m[r], sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) s[r][u] += __shfl_xor_sync(0xffffffffu, s[r][u], o);
+        s[r][u] = j0 + u < n[r] ? s[r][u] * sl2 : -INFINITY;
+        mx = fmaxf(mx, s[r][u]);
+      }
+      const float alpha = ex2_from(m[r], mx);
+      m[r] = mx;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s[r][u] = ex2_from(s[r][u], mx);
+        sum += s[r][u];
+      }
+      l[r] = fmaf(l[r], alpha, sum);
+#pragma unroll
+      for (int y = 0; y < 8; ++y) acc[r][y] *= alpha;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float vv[8];
+      vr[u].get(vv);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (a.nrel) {
+          const unsigned o = (unsigned)(j0 + u - r / g - off + a.window);
+          if (o < (unsigned)a.nrel && j0 + u < n[r])
+#pragma unroll
+            for (int y = 0; y < 8; ++y)
+              if (d0 + y < D) acc[r][y] = fmaf(s[r][u], to_f(relv[o * D + d0 + y]), acc[r][y]);
+          __syncwarp();
+        }
+        // The last key of a run that ends early is read twice, with p = 0.
+#pragma unroll
+        for (int y = 0; y < 8; ++y) acc[r][y] = fmaf(s[r][u], vv[y], acc[r][y]);
+      }
+    }
+  }
+  // Groups of the warp, then its sums to shared memory.
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    float M = m[r];
+#pragma unroll
+    for (int o = G; o < 32; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float f = ex2_from(m[r], M);
+    l[r] *= f;
+#pragma unroll
+    for (int o = G; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+      acc[r][y] *= f;
+#pragma unroll
+      for (int o = G; o < 32; o <<= 1) acc[r][y] += __shfl_xor_sync(0xffffffffu, acc[r][y], o);
+      if (lane < G) s_acc[w][r][d0 + y] = acc[r][y];
+    }
+    if (lane == 0) {
+      s_m[w][r] = M;
+      s_l[w][r] = l[r];
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < R * DP; e += kFewWarps * 32) {
+    const int r = e / DP, d = e - r * DP;
+    float M = -INFINITY, t = 0.f, L = 0.f;
+    for (int x = 0; x < kFewWarps; ++x) M = fmaxf(M, s_m[x][r]);
+    for (int x = 0; x < kFewWarps; ++x) {
+      const float f = ex2_from(s_m[x][r], M);
+      t = fmaf(f, s_acc[x][r][d], t);
+      L = fmaf(f, s_l[x][r], L);
+    }
+    b_acc[r][d] = t;
+    if (d == 0) {
+      b_m[r] = M;
+      b_l[r] = L;
+    }
+  }
+  cl.sync();
+  for (int e = rank * kFewWarps * 32 + threadIdx.x; e < R * DP; e += cs * kFewWarps * 32) {
+    const int r = e / DP, d = e - r * DP;
+    // All remote reads under way together: a block outside the cluster counts as this one with weight 0.
+    float xm[kFewSplits], xl[kFewSplits], xa[kFewSplits], M = -INFINITY, t = 0.f, L = 0.f;
+#pragma unroll
+    for (int x = 0; x < kFewSplits; ++x) {
+      const int from = x < cs ? x : rank;
+      xm[x] = *cl.map_shared_rank(&b_m[r], from);
+      xl[x] = *cl.map_shared_rank(&b_l[r], from);
+      xa[x] = *cl.map_shared_rank(&b_acc[r][d], from);
+    }
+#pragma unroll
+    for (int x = 0; x < kFewSplits; ++x) M = fmaxf(M, xm[x]);
+#pragma unroll
+    for (int x = 0; x < kFewSplits; ++x) {
+      if (x >= cs) break;
+      const float f = ex2_from(xm[x], M);
+      t = fmaf(f, xa[x], t);
+      L = fmaf(f, xl[x], L);
+    }
+    if (r >= rows) continue;
+    const int i = r / g, h = hk * g + r % g;
+    if (d < D)
+      static_cast<T*>(a.o)[b * a.so.b + h * a.so.h + i * a.so.t + d] = from_f<T>(L == 0.f ? 0.f : t / L);
+    if (d == 0 && a.lse)
+      a.lse[((int64_t)b * a.H + h) * a.Tq + i] = L == 0.f ? -INFINITY : ((M == -INFINITY ? 0.f : M) + log2f(L)) * kLn2;
+  }
+  cl.sync();  // the block's sums have been read
+}
+
+template <typename T, int G, int R>
+cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
+  // Splits: a block per SM, each with at least one full step of its groups.
+  const int step = (sizeof(T) == 4 ? 2 : 4) * (32 / G) * kFewWarps;
+  int cs = 1;
+  while (cs < kFewSplits && (int64_t)a.B * a.Hkv * cs < 148 && cs * step < a.Tk) cs *= 2;
+  const int el = sizeof(T);
+  const bool vec = attn_rows_aligned(a.q, a.sq, a.D, el) && attn_rows_aligned(a.k, a.sk, a.D, el) &&
+                   attn_rows_aligned(a.v, a.sv, a.D, el) && a.D % 8 == 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cs, a.Hkv, a.B);
+  cfg.blockDim = dim3(kFewWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_fwd_few<T, G, R>, a, cs, vec);
+}
+
+template <typename T, int G>
+cudaError_t rows(const AttnArgs& a, cudaStream_t st) {
+  const int n = a.Tq * (a.H / a.Hkv);
+  if (n <= 1) return launch<T, G, 1>(a, st);
+  if (n <= 2) return launch<T, G, 2>(a, st);
+  return n <= 4 ? launch<T, G, 4>(a, st) : launch<T, G, 8>(a, st);
+}
+
+template <typename T>
+cudaError_t width(const AttnArgs& a, cudaStream_t st) {
+  if (a.D <= 32) return rows<T, 4>(a, st);
+  return a.D <= 64 ? rows<T, 8>(a, st) : rows<T, 16>(a, st);
+}
+
+}  // namespace
+
+cudaError_t attn_fwd_few_rows(const AttnArgs& a, cudaStream_t st) {
+  if (a.ty == Ty::F32) return width<float>(a, st);
+  return a.ty == Ty::F16 ? width<__half>(a, st) : width<__nv_bfloat16>(a, st);
+}
+
+}  // namespace gsv

@@ -66,6 +66,8 @@ inline BwdWs carve_bwd(const AttnArgs& a) {
   return w;
 }
 
+constexpr int kFewRows = 8;  // most rows per key head of attn_fwd_few_rows
+cudaError_t attn_fwd_few_rows(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_fwd_tensor(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_fwd_cores(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_bwd_tensor(const AttnArgs& a, const BwdWs& ws, cudaStream_t st);

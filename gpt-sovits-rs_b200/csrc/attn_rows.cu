@@ -265,6 +265,8 @@ size_t attn_bwd_workspace(const AttnArgs& a) { return carve_bwd(a).bytes; }
 
 cudaError_t attn_forward(const AttnArgs& a, cudaStream_t st) {
   if (!a.Tq) return cudaSuccess;
+  // A tile kernel would fill 64 or 128 rows for these.
+  if ((int64_t)a.Tq * (a.H / a.Hkv) <= kFewRows) return attn_fwd_few_rows(a, st);
   return a.ty == Ty::F32 ? attn_fwd_cores(a, st) : attn_fwd_tensor(a, st);
 }
 
