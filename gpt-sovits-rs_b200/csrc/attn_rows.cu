@@ -4,6 +4,7 @@
 
 #include "attn_common.cuh"
 #include "attn_launch.h"
+#include "gsv_pdl.cuh"
 
 namespace gsv {
 namespace {
@@ -203,6 +204,7 @@ __global__ void __launch_bounds__(2 * kAttnMaxD) bwd_rel_kernel(const AttnArgs a
 template <typename T>
 __global__ void __launch_bounds__(512) bwd_rel_sum_kernel(const AttnArgs a, const BwdWs ws, const int64_t blocks) {
   __shared__ float s[16][32];
+  pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int n = a.nrel * a.D, e = blockIdx.x * 32 + lane;
   float v = 0.f;
@@ -244,8 +246,8 @@ cudaError_t rel_t(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
     if (a.nrel <= 9) bwd_rel_kernel<9><<<(unsigned)blocks, 2 * kAttnMaxD, 0, st>>>(a, ws);
     else bwd_rel_kernel<2 * kAttnMaxWindow + 1><<<(unsigned)blocks, 2 * kAttnMaxD, 0, st>>>(a, ws);
   }
-  bwd_rel_sum_kernel<T><<<cdiv(2 * a.nrel * a.D, 32), 512, 0, st>>>(a, ws, blocks);
-  return cudaGetLastError();
+  const PdlScope pdl(blocks > 0);
+  return launch_k(bwd_rel_sum_kernel<T>, cdiv(2 * a.nrel * a.D, 32), 512, 0, st, a, ws, blocks);
 }
 
 }  // namespace

@@ -27,6 +27,7 @@
 // max|v|, norms taken by the row pass); both leave the fp32 sums at the end.
 #include "attn_launch.h"
 #include "attn_tc.cuh"
+#include "gsv_pdl.cuh"
 
 namespace gsv {
 namespace {
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
     fence_async_smem();
   }
   if (warp == 8) tmem_alloc(smem_u32(&s_tmem), 512);
+  pdl_wait();  // the row pass's values
   float gs = 1.f;  // the power of two that dS is carried with
   if (kHalf && nt > 0) {
     float nd = 0.f, nv = 0.f;
@@ -573,8 +575,8 @@ cudaError_t launch(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
              map_rows(&m.kb, a.k, a.ty, a.sk, a.B, a.Hkv, a.Tk, a.D, kBB) &&
              map_rows(&m.vb, a.v, a.ty, a.sv, a.B, a.Hkv, a.Tk, a.D, kBB);
   }
-  attn_bwd_tc<T, DP, REL><<<dim3(nk + nq, a.H, a.B), kThreads, smem, st>>>(a, ws, m, nk, vec, ovec);
-  return cudaGetLastError();
+  const PdlScope pdl(a.Tq > 0);  // its set-up runs beside the end of the row pass
+  return launch_k(attn_bwd_tc<T, DP, REL>, dim3(nk + nq, a.H, a.B), kThreads, smem, st, a, ws, m, nk, vec, ovec);
 }
 
 template <typename T, int DP>

@@ -26,6 +26,7 @@
 #include <algorithm>
 
 #include "attn_tc.cuh"
+#include "gsv_pdl.cuh"
 #include "norm_grad.h"
 
 namespace cg = cooperative_groups;
@@ -486,6 +487,7 @@ __global__ void __launch_bounds__(kTimeWarps * 32, V == 1 && E > 4 ? 1 : 2) norm
 __global__ void __launch_bounds__(512) norm_part_sum(const float* part, int blocks, int C, float* dgamma,
                                                      float* dbeta) {
   __shared__ float s[16][32];
+  pdl_wait();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int e = blockIdx.x * 32 + lane, n = 2 * C;
   float v = 0.f;
@@ -638,8 +640,8 @@ cudaError_t norm_backward(const NormArgs& a, cudaStream_t st) {
   const cudaError_t e = run<true>(a, st);
   if (e != cudaSuccess) return e;
   const int n = a.rows ? row_blocks(a, true) : time_teams(a, time_per_sm(a, true));
-  norm_part_sum<<<cdiv(2 * a.C, 32), 512, 0, st>>>(a.part, n, a.C, a.dgamma, a.dbeta);
-  return cudaGetLastError();
+  const PdlScope pdl(true);
+  return launch_k(norm_part_sum, cdiv(2 * a.C, 32), 512, 0, st, (const float*)a.part, n, a.C, a.dgamma, a.dbeta);
 }
 
 cudaError_t norm_gave_up(int* out, cudaStream_t st) { return take_gave_up(g_gave_up, out, st); }
