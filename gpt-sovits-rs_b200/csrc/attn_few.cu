@@ -25,34 +25,6 @@ namespace {
 constexpr int kFewWarps = 8;
 constexpr int kFewSplits = 8;  // largest portable cluster
 
-// Eight channels as they lie in memory, turned into fp32 where they are used.
-template <typename T>
-struct Raw8 {
-  uint4 u[sizeof(T) / 2];
-  // Channels d0 .. d0 + 7 of a row, zeros from D on.
-  __device__ __forceinline__ void load(const T* row, int d0, int D, bool vec) {
-    if (vec) {
-      const T* p = row + min(d0, D - 8);
-#pragma unroll
-      for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
-        u[k] = reinterpret_cast<const uint4*>(p)[k];
-        if (d0 >= D) u[k] = make_uint4(0u, 0u, 0u, 0u);
-      }
-    } else {
-      T e[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = d0 + i < D ? row[d0 + i] : from_f<T>(0.f);
-      memcpy(u, e, sizeof e);
-    }
-  }
-  __device__ __forceinline__ void get(float* f) const {
-    T e[8];
-    memcpy(e, u, sizeof e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f(e[i]);
-  }
-};
-
 // exp2(x - m) with -inf - -inf = -inf.
 __device__ __forceinline__ float ex2_from(float x, float m) { return x == -INFINITY ? 0.f : exp2f(x - m); }
 

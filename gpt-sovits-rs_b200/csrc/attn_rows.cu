@@ -24,27 +24,6 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Channels d0 .. d0 + 7 of a row, zeros from D on.  With `vec` (whole aligned
-// vectors) a lane past the row's end takes the last vector and drops it, so
-// that the load stands under no branch and several rows' loads overlap.
-template <typename T>
-__device__ __forceinline__ void load8(const T* row, int d0, int D, bool vec, float* f) {
-  if (vec) {
-    constexpr int V = 16 / sizeof(T);
-    const T* p = row + min(d0, D - 8);
-#pragma unroll
-    for (int k = 0; k < 8; k += V) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p + k);
-      const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[k + i] = d0 < D ? to_f(e[i]) : 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = d0 + i < D ? to_f(row[d0 + i]) : 0.f;
-  }
-}
-
 __device__ __forceinline__ float dot8(const float* a, const float* b) {
   float s = 0.f;
 #pragma unroll
@@ -52,7 +31,8 @@ __device__ __forceinline__ float dot8(const float* a, const float* b) {
   return s;
 }
 
-// G lanes share one row, 8 channels each.  Query rows: delta = do . o in fp32
+// G lanes share one row, 8 channels each; a group takes U rows, whose loads are
+// all under way together.  Query rows: delta = do . o in fp32
 // and the products with the relative rows; fp16 adds the norms of the rows of
 // do and v.
 //
@@ -61,93 +41,162 @@ __device__ __forceinline__ float dot8(const float* a, const float* b) {
 // term disappears; rows of up to kFewKeys keys, where it would be as large as
 // the rounding of ds itself, take delta = sum_j p_ij dp_ij instead (fp32
 // inputs have no such rounding).
-template <typename T, int G>
+template <typename T, int G, int U>
 __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_constant__ AttnArgs a,
-                                                               const __grid_constant__ BwdWs ws, const int nq,
-                                                               const bool vec) {
+                                                                  const __grid_constant__ BwdWs ws, const int nq,
+                                                                  const bool vec) {
   extern __shared__ float sm[];  // relk, relv as [nrel][8 G]
   constexpr bool F16 = std::is_same<T, __half>::value, kExact = std::is_same<T, float>::value;
   constexpr int L = 8 * G, R = kRowThreads / G;
   const int D = a.D, lane = threadIdx.x % G, d0 = lane * 8, h = blockIdx.y, b = blockIdx.z;
+  const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk);
+  const bool key_rows = F16 && (int)blockIdx.x >= nq;
+  if (key_rows && h >= a.Hkv) return;
+  // Rows of the block: i0 + u R + group.
+  const int i0 = ((int)blockIdx.x - (key_rows ? nq : 0)) * R * U + threadIdx.x / G;
+  Raw8<T> rg[U], ro[U], rq[U];
+  if (!key_rows) {
+    const T* g = static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h;
+    const T* o = static_cast<const T*>(a.o) + b * a.so.b + h * a.so.h;
+    const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * R, a.Tq - 1);  // its values are dropped where the row has no keys
+      rg[u].load(g + i * a.sdo.t, d0, D, vec);
+      ro[u].load(o + i * a.so.t, d0, D, vec);
+      if (a.nrel) rq[u].load(q + i * a.sq.t, d0, D, vec);
+    }
+  } else {
+    const T* v = static_cast<const T*>(a.v) + b * a.sv.b + h * a.sv.h;
+#pragma unroll
+    for (int u = 0; u < U; ++u) rg[u].load(v + min(i0 + u * R, a.Tk - 1) * a.sv.t, d0, D, vec);
+  }
   float* srk = sm;
   float* srv = srk + a.nrel * L;
   for (int e = threadIdx.x; e < a.nrel * L; e += kRowThreads) {
-    const int r = e / L, d = e - r * L;
-    srk[e] = d < D ? to_f(static_cast<const T*>(a.relk)[r * D + d]) : 0.f;
-    srv[e] = d < D ? to_f(static_cast<const T*>(a.relv)[r * D + d]) : 0.f;
+    const int r = e / L, d = e % L;
+    const T k = static_cast<const T*>(a.relk)[r * D + min(d, D - 1)], v = static_cast<const T*>(a.relv)[r * D + min(d, D - 1)];
+    srk[e] = d < D ? to_f(k) : 0.f;
+    srv[e] = d < D ? to_f(v) : 0.f;
   }
   if (a.nrel) __syncthreads();
-  const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk);
-  if (F16 && (int)blockIdx.x >= nq) {  // the key rows' norms
-    if (h >= a.Hkv) return;
-    const int j = ((int)blockIdx.x - nq) * R + threadIdx.x / G;
+  if (key_rows) {
     float ev = 0.f;  // largest |relv|^2
     if ((threadIdx.x & 31) < a.nrel)
       for (int d = 0; d < L; ++d) ev = fmaf(srv[(threadIdx.x & 31) * L + d], srv[(threadIdx.x & 31) * L + d], ev);
     ev = sqrtf(warp_max(ev));
-    float v[8] = {};
-    if (j < kl) load8(static_cast<const T*>(a.v) + b * a.sv.b + h * a.sv.h + j * a.sv.t, d0, D, vec, v);
-    const float s = group_sum<G>(dot8(v, v));
-    if (j < kl && lane == 0) ws.nv[((int64_t)b * a.Hkv + h) * a.Tk + j] = sqrtf(s) + ev;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = i0 + u * R;
+      float v[8];
+      rg[u].get(v);
+      const float s = group_sum<G>(dot8(v, v));
+      if (j < kl && lane == 0) ws.nv[((int64_t)b * a.Hkv + h) * a.Tk + j] = sqrtf(s) + ev;
+    }
     return;
   }
-  const int i = (int)blockIdx.x * R + threadIdx.x / G;
-  const int64_t bh = (int64_t)b * a.H + h, row = bh * a.Tq + i;
-  const int n = i < a.Tq ? allowed_keys(i, ql, kl, a.causal) : 0;
   const float sl2 = a.scale * kLog2e;
-  float g[8] = {}, q[8] = {}, o[8] = {};
-  if (n > 0) {
-    load8(static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + i * a.sdo.t, d0, D, vec, g);
-    load8(static_cast<const T*>(a.o) + b * a.so.b + h * a.so.h + i * a.so.t, d0, D, vec, o);
-    if (a.nrel || (!kExact && n <= kFewKeys))
-      load8(static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + i * a.sq.t, d0, D, vec, q);
+  const int64_t bh = (int64_t)b * a.H + h;
+  float delta[U], lse2[U], norm[U];
+  int n[U];
+  bool any_few = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = i0 + u * R;
+    n[u] = i < a.Tq ? allowed_keys(i, ql, kl, a.causal) : 0;
+    lse2[u] = a.lse[bh * a.Tq + min(i, a.Tq - 1)] * kLog2e;
+    any_few = any_few || (n[u] > 0 && n[u] <= kFewKeys);
   }
-  float s = group_sum<G>(dot8(g, o));
-  const float lse2 = n > 0 ? a.lse[row] * kLog2e : INFINITY;
-  float* rel = rel_at(ws, bh, i, a.nrel);
-#pragma unroll 3
-  for (int r = 0; r < a.nrel; ++r) {
-    const float u = group_sum<G>(dot8(q, srk + r * L + d0)), w = group_sum<G>(dot8(g, srv + r * L + d0));
-    if (lane == r % G) {
-      rel[r] = u;
-      rel[kRowBlock * a.nrel + r] = w;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float g[8], o[8];
+    rg[u].get(g);
+    ro[u].get(o);
+    delta[u] = group_sum<G>(dot8(g, o));
+    norm[u] = F16 ? sqrtf(group_sum<G>(dot8(g, g))) : 0.f;
+    if (n[u] == 0) delta[u] = norm[u] = 0.f, lse2[u] = INFINITY;
+  }
+  if (a.nrel) {
+    const int last = ws.blocks * kRowBlock;
+    float q[U][8], g[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      rq[u].get(q[u]);
+      rg[u].get(g[u]);
+    }
+#pragma unroll 1
+    for (int r = 0; r < a.nrel; ++r) {
+      float x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u] = dot8(q[u], srk + r * L + d0);
+        y[u] = dot8(g[u], srv + r * L + d0);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u] = group_sum<G>(x[u]);
+        y[u] = group_sum<G>(y[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * R;
+        if (i < last && lane == r % G) {
+          float* rel = rel_at(ws, bh, i, a.nrel) + r;
+          rel[0] = n[u] > 0 ? x[u] : 0.f;
+          rel[kRowBlock * a.nrel] = n[u] > 0 ? y[u] : 0.f;
+        }
+      }
     }
   }
-  const bool few = !kExact && n > 0 && n <= kFewKeys;
-  if (!kExact && __any_sync(0xffffffffu, few)) {
-    // The warp takes its groups' rows in turn, one key per lane.
+  if (!kExact && __any_sync(0xffffffffu, any_few)) {
+    // The warp takes its rows in turn, one key per lane; q and do come again, broadcast to the warp.
     const int hk = h / (a.H / a.Hkv), wl = threadIdx.x & 31;
     const T* k = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
     const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
-    for (int from = 0; from < 32; from += G) {
-      if (!__shfl_sync(0xffffffffu, few, from)) continue;
-      const int nr = __shfl_sync(0xffffffffu, n, from), ir = __shfl_sync(0xffffffffu, i, from), j = min(wl, nr - 1);
-      const float lr = __shfl_sync(0xffffffffu, lse2, from);
-      const unsigned r = (unsigned)(j - (ir + kl - ql) + a.window);
-      const bool near = r < (unsigned)a.nrel;
-      float sc = 0.f, dp = 0.f;
-#pragma unroll 2
-      for (int c = 0; c < D; c += 8) {
-        float kk[8], vv[8];
-        load8(k + j * a.sk.t, c, D, vec, kk);
-        load8(v + j * a.sv.t, c, D, vec, vv);
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          const float kr = near ? kk[y] + srk[r * L + c + y] : kk[y], vr = near ? vv[y] + srv[r * L + c + y] : vv[y];
-          sc = fmaf(__shfl_sync(0xffffffffu, q[y], from + c / 8), kr, sc);
-          dp = fmaf(__shfl_sync(0xffffffffu, g[y], from + c / 8), vr, dp);
+    for (int u = 0; u < U; ++u) {
+#pragma unroll 1
+      for (int from = 0; from < 32; from += G) {
+        const int nr = __shfl_sync(0xffffffffu, n[u], from);
+        if (nr == 0 || nr > kFewKeys) continue;
+        const int ir = __shfl_sync(0xffffffffu, i0 + u * R, from), j = min(wl, nr - 1);
+        const float lr = __shfl_sync(0xffffffffu, lse2[u], from);
+        const T* q = static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + ir * a.sq.t;
+        const T* g = static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + ir * a.sdo.t;
+        const unsigned r = (unsigned)(j - (ir + kl - ql) + a.window);
+        const bool near = r < (unsigned)a.nrel;
+        float sc = 0.f, dp = 0.f;
+#pragma unroll 2
+        for (int c = 0; c < D; c += 8) {
+          Raw8<T> kr, vr, qr, gr;
+          kr.load(k + j * a.sk.t, c, D, vec);
+          vr.load(v + j * a.sv.t, c, D, vec);
+          qr.load(q, c, D, vec);
+          gr.load(g, c, D, vec);
+          float kk[8], vv[8], qq[8], gg[8];
+          kr.get(kk);
+          vr.get(vv);
+          qr.get(qq);
+          gr.get(gg);
+          if (near)
+#pragma unroll
+            for (int y = 0; y < 8; ++y) kk[y] += srk[r * L + c + y], vv[y] += srv[r * L + c + y];
+          sc += dot8(qq, kk);
+          dp += dot8(gg, vv);
         }
+        const float t = group_sum<32>(wl < nr ? exp2f(fmaf(sc, sl2, -lr)) * dp : 0.f);
+        if (threadIdx.x % 32 / G == from / G) delta[u] = t;
       }
-      const float t = group_sum<32>(wl < nr ? exp2f(fmaf(sc, sl2, -lr)) * dp : 0.f);
-      if (threadIdx.x % 32 / G == from / G) s = t;
     }
   }
-  const float gg = F16 ? sqrtf(group_sum<G>(dot8(g, g))) : 0.f;
-  if (lane == 0) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = i0 + u * R;
+    if (lane != 0 || i >= ws.blocks * kRowBlock) continue;
     float* rw = row_at(ws, bh, i);
-    rw[0] = (F16 ? kHalfShift : 0.f) - lse2;
-    rw[kRowBlock] = n > 0 ? -s : 0.f;
-    if (F16 && i < a.Tq) ws.ndo[row] = n > 0 ? gg : 0.f;
+    rw[0] = (F16 ? kHalfShift : 0.f) - lse2[u];
+    rw[kRowBlock] = -delta[u];
+    if (F16 && i < a.Tq) ws.ndo[bh * a.Tq + i] = norm[u];
   }
 }
 
@@ -222,14 +271,14 @@ __global__ void __launch_bounds__(512) bwd_rel_sum_kernel(const AttnArgs a, cons
 
 template <typename T, int G>
 cudaError_t rows_g(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
-  constexpr int R = kRowThreads / G;
-  const int nq = ws.blocks * kRowBlock / R, nk = a.ty == Ty::F16 ? cdiv(a.Tk, R) : 0;
+  constexpr int U = 2, R = kRowThreads / G * U;
+  const int nq = cdiv(ws.blocks * kRowBlock, R), nk = a.ty == Ty::F16 ? cdiv(a.Tk, R) : 0;
   const size_t smem = sizeof(float) * 2 * a.nrel * 8 * G;
   const int el = sizeof(T);
   const bool vec = attn_rows_aligned(a.q, a.sq, a.D, el) && attn_rows_aligned(a.o, a.so, a.D, el) &&
                    attn_rows_aligned(a.dout, a.sdo, a.D, el) && attn_rows_aligned(a.k, a.sk, a.D, el) &&
                    attn_rows_aligned(a.v, a.sv, a.D, el) && a.D % 8 == 0;
-  bwd_rows_kernel<T, G><<<dim3(nq + nk, a.H, a.B), kRowThreads, smem, st>>>(a, ws, nq, vec);
+  bwd_rows_kernel<T, G, U><<<dim3(nq + nk, a.H, a.B), kRowThreads, smem, st>>>(a, ws, nq, vec);
   return cudaGetLastError();
 }
 

@@ -196,7 +196,7 @@ constexpr int kLoaders = 64;  // threads that load tiles (two warps)
 // reach the accumulators).  `vec`: rows are whole aligned 16-byte vectors and
 // move by cp.async; else by single elements.  A chunk's 8 (or 4) units per row
 // divide the 64 threads, so a thread keeps its unit and its swizzle and steps
-// down the rows by one constant: three instructions per copy.
+// down the rows by one constant.
 template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void load_tile(uint32_t dst, uint32_t chunk, const T* g, int64_t stride, int valid, int D,
                                           bool vec, int tid) {
@@ -208,13 +208,12 @@ __device__ __forceinline__ void load_tile(uint32_t dst, uint32_t chunk, const T*
     uint32_t a = dst + c * chunk + r0 * 128 + ((u ^ r0) & 7) * 16;
     const T* p = g + (int64_t)r0 * stride + col;
     const int64_t ps = (int64_t)step * stride;
-    if (vec && valid >= ROWS && DP == D) {
-#pragma unroll 4
-      for (int i = 0; i < ROWS / step; ++i, a += step * 128, p += ps) cp_async16(a, p, 16);
-    } else if (vec) {
-      for (int r = r0; r < ROWS; r += step, a += step * 128, p += ps) {
-        const bool in = r < valid && col < D;
-        cp_async16(a, in ? (const void*)p : (const void*)g, in ? 16 : 0);
+    if (vec) {
+      const bool in = col < D;
+#pragma unroll 8
+      for (int i = 0; i < ROWS / step; ++i, a += step * 128, p += ps) {
+        const bool use = in && r0 + i * step < valid;
+        cp_async16(a, use ? p : g, use ? 16 : 0);
       }
     } else {
       for (int r = r0; r < ROWS; r += step, a += step * 128, p += ps) {
@@ -302,13 +301,13 @@ struct RowsMap {
 
 // False when the tensor cannot be mapped; its tiles then move by cp.async.
 bool map_rows(RowsMap* m, const void* p, Ty ty, const Str3& s, int B, int heads, int T, int D, int rows) {
-  if (T < rows || s.t <= 0 || !encode_fn()) return false;
+  if (T < 1 || (s.t <= 0 && T > 1) || !encode_fn()) return false;
   m->mh = heads > 1 && s.h != 0;
   m->mb = B > 1 && s.b != 0;
   const cuuint64_t pad = ((cuuint64_t)D * 2 + 15) / 16 * 16;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)(m->mh ? heads : 1),
                               (cuuint64_t)(m->mb ? B : 1)};
-  const cuuint64_t strides[3] = {(cuuint64_t)s.t * 2, m->mh ? (cuuint64_t)s.h * 2 : pad,
+  const cuuint64_t strides[3] = {T > 1 ? (cuuint64_t)s.t * 2 : pad, m->mh ? (cuuint64_t)s.h * 2 : pad,
                                  m->mb ? (cuuint64_t)s.b * 2 : pad};
   const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, es[4] = {1, 1, 1, 1};
   return encode_fn()(&m->map, ty == Ty::F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
@@ -317,7 +316,13 @@ bool map_rows(RowsMap* m, const void* p, Ty ty, const Str3& s, int B, int heads,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// One tile of whole valid rows by TMA (one thread); its bytes count on `bar`.
+// Whether TMA gives a tile its zeros: all its rows are valid, or those that are
+// not lie past the tensor's end, where TMA fills.
+__device__ __forceinline__ bool tma_fits(int row, int rows, int valid, int T) {
+  return row + rows <= valid || valid == T;
+}
+
+// One tile by TMA (one thread); its bytes count on `bar`.
 template <int DP>
 __device__ __forceinline__ void tma_tile(uint32_t dst, uint32_t chunk, const RowsMap& m, uint32_t bar, int row, int h,
                                          int b) {
@@ -335,25 +340,38 @@ __device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// One row of 32 output channels starting at channel c.
+// How rows of an output may be written: 0 by elements, 1 by 16-byte, 2 by
+// 32-byte vectors (whole sectors per lane).
+inline int store_mode(const void* p, const Str3& s, int D) {
+  if (!attn_rows_aligned(p, s, D, 2)) return 0;
+  const bool wide = reinterpret_cast<uintptr_t>(p) % 32 == 0 && s.b % 16 == 0 && s.h % 16 == 0 && s.t % 16 == 0;
+  return wide && D % 16 == 0 ? 2 : 1;
+}
+
+// One row of 32 output channels starting at channel c, times f.
 template <typename T>
-__device__ __forceinline__ void store_row32(T* row, int c, int D, bool vec, const float* v, float f) {
+__device__ __forceinline__ void store_row32(T* row, int c, int D, int mode, const float* v, float f) {
+  if (mode) {
+    uint4 u[4];
 #pragma unroll
-  for (int k = 0; k < 32; k += 8) {
-    if (vec) {
-      if (c + k < D) {
-        uint4 u;
-        u.x = pack2<T>(v[k] * f, v[k + 1] * f);
-        u.y = pack2<T>(v[k + 2] * f, v[k + 3] * f);
-        u.z = pack2<T>(v[k + 4] * f, v[k + 5] * f);
-        u.w = pack2<T>(v[k + 6] * f, v[k + 7] * f);
-        *reinterpret_cast<uint4*>(row + c + k) = u;
-      }
+    for (int k = 0; k < 4; ++k) {
+      u[k].x = pack2<T>(v[8 * k] * f, v[8 * k + 1] * f);
+      u[k].y = pack2<T>(v[8 * k + 2] * f, v[8 * k + 3] * f);
+      u[k].z = pack2<T>(v[8 * k + 4] * f, v[8 * k + 5] * f);
+      u[k].w = pack2<T>(v[8 * k + 6] * f, v[8 * k + 7] * f);
+    }
+    if (mode == 2) {
+      if (c < D) st_global_v8(row + c, u[0], u[1]);
+      if (c + 16 < D) st_global_v8(row + c + 16, u[2], u[3]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + k + i < D) row[c + k + i] = from_f<T>(v[k + i] * f);
+      for (int k = 0; k < 4; ++k)
+        if (c + 8 * k < D) *reinterpret_cast<uint4*>(row + c + 8 * k) = u[k];
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (c + i < D) row[c + i] = from_f<T>(v[i] * f);
   }
 }
 

@@ -67,8 +67,8 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const float* src, uint32
 }
 
 // Tensor maps of the resident (128-row boxes) and the streamed tiles (64-row
-// boxes); `on`: full tiles come by TMA, the rest (tails, whose rows behind a
-// length must read as zeros) by cp.async.
+// boxes); `on`: tiles come by TMA unless they hold rows behind a length, which
+// must read as zeros: those come by cp.async.
 struct BwdMaps {
   RowsMap qa, ka, va, ga, qb, kb, vb, gb;
   bool a_on, b_on;
@@ -78,7 +78,7 @@ template <typename T, int DP, bool REL>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant__ AttnArgs a,
                                                            const __grid_constant__ BwdWs ws,
                                                            const __grid_constant__ BwdMaps maps, const int nk,
-                                                           const bool vec, const bool ovec) {
+                                                           const bool vec, const int ovec) {
   using C = BwdCfg<DP, REL>;
   constexpr int ST = C::ST;
   constexpr bool kHalf = std::is_same<T, __half>::value;
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       // Per barrier: the first warp's lane 0 announces and issues what moves by bulk copies (full tiles,
       // row values); tails are copied by both warps, whose second arrival, or both, come when that is done.
       const bool first_warp = warp == 9;
-      const bool full_a = maps.a_on && r0 + kBA <= (keys ? kl : ql);
+      const bool full_a = maps.a_on && tma_fits(r0, kBA, keys ? kl : ql, keys ? a.Tk : a.Tq);
       const uint32_t a_full = bar(bars.a_full);
       if (first_warp && lane == 0) {
         const uint32_t rel_bytes = REL && !keys ? 2u * 2 * kBB * a.nrel * 4 : 0;
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         if (round > 0) ok = ho.wait_free(bar(bars.b_free[s]), (round - 1) & 1, abort);
         if (!ok) break;
         const int h = keys ? hk * g + hh : hk;
-        const bool whole = maps.b_on && i0 + kBB <= (keys ? ql : kl);
+        const bool whole = maps.b_on && tma_fits(i0, kBB, keys ? ql : kl, keys ? a.Tq : a.Tk);
         if (first_warp && lane == 0) {
           // Offsets of this pair of tiles: from r0 - (i0 + 63 + off) to r0 + 127 - (i0 + off).
           const bool near = REL && keys && r0 - (i0 + kBB - 1 + off) <= a.window &&
@@ -561,8 +561,8 @@ cudaError_t launch(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
   const bool vec = attn_rows_aligned(a.q, a.sq, a.D, 2) && attn_rows_aligned(a.k, a.sk, a.D, 2) &&
                    attn_rows_aligned(a.v, a.sv, a.D, 2) && attn_rows_aligned(a.dout, a.sdo, a.D, 2) &&
                    reinterpret_cast<uintptr_t>(a.relk) % 16 == 0;
-  const bool ovec = attn_rows_aligned(a.dq, a.sdq, a.D, 2) && attn_rows_aligned(a.dk, a.sdk, a.D, 2) &&
-                    attn_rows_aligned(a.dv, a.sdv, a.D, 2);
+  const int ovec = std::min(store_mode(a.dq, a.sdq, a.D),
+                            std::min(store_mode(a.dk, a.sdk, a.D), store_mode(a.dv, a.sdv, a.D)));
   const int nk = cdiv(a.Tk, kBA), nq = cdiv(a.Tq, kBA);
   BwdMaps m = {};
   if (vec) {

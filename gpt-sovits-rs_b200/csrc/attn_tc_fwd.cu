@@ -49,8 +49,8 @@ struct FwdBars {
   uint64_t q_full, k_full[2], k_free[2], v_full[2], v_free[2], s_full, s_free, p_full, o_full, pv_done;
 };
 
-// Full tiles come by TMA (`on`), the rest (tails, whose rows behind a length
-// must read as zeros) by cp.async.
+// Tiles come by TMA (`on`) unless they hold rows behind a length, which must
+// read as zeros: those come by cp.async.
 struct FwdMaps {
   RowsMap q, k, v;
   bool q_on, kv_on;
@@ -59,7 +59,7 @@ struct FwdMaps {
 template <typename T, int DP, bool REL>
 __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_constant__ AttnArgs a,
                                                               const __grid_constant__ FwdMaps maps, const bool vec,
-                                                              const bool ovec) {
+                                                              const int ovec) {
   using C = FwdCfg<DP>;
   constexpr int ST = C::ST;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -191,8 +191,8 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
       };
       // One tile: by TMA from the first loader warp, or by both warps' copies.
       auto fetch = [&](uint32_t dst, uint32_t full, bool on, const RowsMap& m, int head, const T* p, int64_t stride,
-                       int row, int valid) {
-        if (on && row + kBM <= valid) {
+                       int row, int valid, int T_) {
+        if (on && tma_fits(row, kBM, valid, T_)) {
           ho.flush();
           if (warp == 5) {
             if (lane == 0) {
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
           ho.next(full);
         }
       };
-      fetch(sQ, bar(bars.q_full), maps.q_on, maps.q, h, q, a.sq.t, i0, ql);
+      fetch(sQ, bar(bars.q_full), maps.q_on, maps.q, h, q, a.sq.t, i0, ql, a.Tq);
       if (REL) {
         load_tile<T, DP, 32>(sK, C::chunk, static_cast<const T*>(a.relk), D, a.nrel, D, vec, tid);
         ho.next(bar(bars.k_full[kt++]));
@@ -215,10 +215,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
       for (int t = 0; t < nt && ok; ++t) {
         uint32_t dst = stage(true, kt);
         if (!dst) break;
-        fetch(dst, bar(bars.k_full[kt++ % ST]), maps.kv_on, maps.k, hk, k, a.sk.t, t * kBN, kl);
+        fetch(dst, bar(bars.k_full[kt++ % ST]), maps.kv_on, maps.k, hk, k, a.sk.t, t * kBN, kl, a.Tk);
         dst = stage(false, vt);
         if (!dst) break;
-        fetch(dst, bar(bars.v_full[vt++ % ST]), maps.kv_on, maps.v, hk, v, a.sv.t, t * kBN, kl);
+        fetch(dst, bar(bars.v_full[vt++ % ST]), maps.kv_on, maps.v, hk, v, a.sv.t, t * kBN, kl, a.Tk);
       }
       if (REL && ok) {
         const uint32_t dst = stage(false, vt);
@@ -407,7 +407,7 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
   const bool vec = attn_rows_aligned(a.q, a.sq, a.D, 2) && attn_rows_aligned(a.k, a.sk, a.D, 2) &&
                    attn_rows_aligned(a.v, a.sv, a.D, 2) && reinterpret_cast<uintptr_t>(a.relk) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(a.relv) % 16 == 0;
-  const bool ovec = attn_rows_aligned(a.o, a.so, a.D, 2);
+  const int ovec = store_mode(a.o, a.so, a.D);
   FwdMaps m = {};
   if (vec) {
     m.q_on = map_rows(&m.q, a.q, a.ty, a.sq, a.B, a.H, a.Tq, a.D, kBM);
