@@ -48,12 +48,14 @@ __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_c
   extern __shared__ float sm[];  // relk, relv as [nrel][8 G]
   constexpr bool F16 = std::is_same<T, __half>::value, kExact = std::is_same<T, float>::value;
   constexpr int L = 8 * G, R = kRowThreads / G;
-  const int D = a.D, lane = threadIdx.x % G, d0 = lane * 8, h = blockIdx.y, b = blockIdx.z;
+  // Heads fastest: the blocks of the first rows, which take longest (few keys), start first.
+  const int tile = blockIdx.x / (a.H * a.B), bh32 = blockIdx.x - tile * (a.H * a.B);
+  const int D = a.D, lane = threadIdx.x % G, d0 = lane * 8, b = bh32 / a.H, h = bh32 - b * a.H;
   const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk);
-  const bool key_rows = F16 && (int)blockIdx.x >= nq;
+  const bool key_rows = F16 && tile >= nq;
   if (key_rows && h >= a.Hkv) return;
   // Rows of the block: i0 + u R + group.
-  const int i0 = ((int)blockIdx.x - (key_rows ? nq : 0)) * R * U + threadIdx.x / G;
+  const int i0 = (tile - (key_rows ? nq : 0)) * R * U + threadIdx.x / G;
   Raw8<T> rg[U], ro[U], rq[U];
   if (!key_rows) {
     const T* g = static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h;
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_c
         const unsigned r = (unsigned)(j - (ir + kl - ql) + a.window);
         const bool near = r < (unsigned)a.nrel;
         float sc = 0.f, dp = 0.f;
-#pragma unroll 2
+#pragma unroll 4
         for (int c = 0; c < D; c += 8) {
           Raw8<T> kr, vr, qr, gr;
           kr.load(k + j * a.sk.t, c, D, vec);
@@ -278,7 +280,7 @@ cudaError_t rows_g(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
   const bool vec = attn_rows_aligned(a.q, a.sq, a.D, el) && attn_rows_aligned(a.o, a.so, a.D, el) &&
                    attn_rows_aligned(a.dout, a.sdo, a.D, el) && attn_rows_aligned(a.k, a.sk, a.D, el) &&
                    attn_rows_aligned(a.v, a.sv, a.D, el) && a.D % 8 == 0;
-  bwd_rows_kernel<T, G, U><<<dim3(nq + nk, a.H, a.B), kRowThreads, smem, st>>>(a, ws, nq, vec);
+  bwd_rows_kernel<T, G, U><<<(unsigned)((int64_t)(nq + nk) * a.H * a.B), kRowThreads, smem, st>>>(a, ws, nq, vec);
   return cudaGetLastError();
 }
 
