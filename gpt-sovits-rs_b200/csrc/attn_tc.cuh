@@ -151,6 +151,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // Two fp32 lanes per instruction.
 struct F2 {
   unsigned long long v;
+  F2() = default;
   __device__ __forceinline__ F2(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
   __device__ __forceinline__ void get(float& lo, float& hi) const {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));

@@ -176,16 +176,16 @@ __global__ void __launch_bounds__(kRowThreads, BWD && E > 16 ? 1 : 2) norm_rows(
     int b, t;
     const bool ok = valid(f, b, t);
     float v[E], g[BWD ? E : 1];
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = 0.f;
-#pragma unroll
-    for (int e = 0; e < (BWD ? E : 1); ++e) g[e] = 0.f;
     const float mean = mean_next;
     float rstd = ok ? rstd_next : 0.f;
     if (BWD && ff + step < frames) {
       mean_next = a.mean[f + step];
       rstd_next = a.rstd[f + step];
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < (BWD ? E : 1); ++e) g[e] = 0.f;
     if (ok) {
       if (kRing) {
         if (!warp_wait(smem_u32(&s_bar[grp][s]), phases >> s & 1, &s_abort)) {
@@ -203,7 +203,9 @@ __global__ void __launch_bounds__(kRowThreads, BWD && E > 16 ? 1 : 2) norm_rows(
               float u[V];
               load_vec<T, V>(sx + C + c, u);
 #pragma unroll
-              for (int i = 0; i < V; ++i) v[k * V + i] += u[i];
+              for (int i = 0; i < V; i += 2)
+                add2(F2(v[k * V + i], v[k * V + i + (V > 1)]), F2(u[i], u[i + (V > 1)]))
+                    .get(v[k * V + i], v[k * V + i + (V > 1)]);
             }
             if (BWD) load_vec<T, V>(sx + 2 * C + c, g + k * V);
           }
@@ -229,24 +231,39 @@ __global__ void __launch_bounds__(kRowThreads, BWD && E > 16 ? 1 : 2) norm_rows(
         }
       }
     }
+    // Channels past C hold zeros; g is zero there too, so only (v - mean) has to be kept out of sums.
     float sums[2] = {0.f, 0.f};
     if (!BWD) {
+      F2 sa(0.f, 0.f), sb(0.f, 0.f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) sums[0] += v[e];
+      for (int e = 0; e < E; e += 4) {
+        sa = add2(sa, F2(v[e], v[e + 1]));
+        sb = add2(sb, F2(v[e + 2], v[e + 3]));
+      }
+      add2(sa, sb).get(sums[0], sums[1]);
+      sums[0] += sums[1];
       group_sum<R, 1>(sums, s_red, flip);
     } else {
+      F2 s0(0.f, 0.f), s1(0.f, 0.f);
+      const F2 nm(-mean, -mean), rs(rstd, rstd);
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        if ((tid + k * R) * V < C)
-#pragma unroll
-          for (int e = k * V; e < (k + 1) * V; ++e) {
-            v[e] = (v[e] - mean) * rstd;
-            dg[e] = fmaf(g[e], v[e], dg[e]);
-            be[e] += g[e];
-            g[e] *= ga[e];
-            sums[0] += g[e];
-            sums[1] = fmaf(g[e], v[e], sums[1]);
-          }
+      for (int e = 0; e < E; e += 2) {
+        const int z = BWD ? e : 0, z1 = BWD ? e + 1 : 0;
+        const F2 xh = mul2(add2(F2(v[e], v[e + 1]), nm), rs);
+        F2 q(g[z], g[z1]);
+        fma2(q, xh, F2(dg[z], dg[z1])).get(dg[z], dg[z1]);
+        add2(F2(be[e], be[e + 1]), q).get(be[e], be[e + 1]);
+        q = mul2(q, F2(ga[e], ga[e + 1]));
+        s0 = add2(s0, q);
+        s1 = fma2(q, xh, s1);
+        xh.get(v[e], v[e + 1]);
+        q.get(g[z], g[z1]);
+      }
+      float lo, hi;
+      s0.get(lo, hi);
+      sums[0] = lo + hi;
+      s1.get(lo, hi);
+      sums[1] = lo + hi;
       group_sum<R, 2>(sums, s_red, flip);
     }
     // Every thread of the group has read the stage: it takes the frame `stages` steps on.
@@ -258,29 +275,53 @@ __global__ void __launch_bounds__(kRowThreads, BWD && E > 16 ? 1 : 2) norm_rows(
     T* out = static_cast<T*>(const_cast<void*>(BWD ? a.dx.p : a.out.p)) + b * (BWD ? a.dx.b : a.out.b) +
              t * (BWD ? a.dx.o : a.out.o);
     if (!BWD) {
-      float sq = 0.f;
+      F2 sq(0.f, 0.f);
+      const F2 nm(-m0, -m0);
 #pragma unroll
       for (int k = 0; k < N; ++k)
-        if ((tid + k * R) * V < C)
+        if ((tid + k * R) * V < C) {
+          if constexpr (V > 1) {
 #pragma unroll
-          for (int e = k * V; e < (k + 1) * V; ++e) sq = fmaf(v[e] - m0, v[e] - m0, sq);
-      group_sum<R, 1>(&sq, s_red, flip);
-      rstd = rsqrtf(sq / (float)C + a.eps);
+            for (int e = k * V; e < (k + 1) * V; e += 2) {
+              const F2 d = add2(F2(v[e], v[e + 1]), nm);
+              sq = fma2(d, d, sq);
+              d.get(v[e], v[e + 1]);
+            }
+          } else {
+            v[k] -= m0;
+            float lo, hi;
+            sq.get(lo, hi);
+            sq = F2(fmaf(v[k], v[k], lo), hi);
+          }
+        }
+      float lo, hi;
+      sq.get(lo, hi);
+      lo += hi;
+      group_sum<R, 1>(&lo, s_red, flip);
+      rstd = rsqrtf(lo / (float)C + a.eps);
       if (tid == 0) {
         a.mean[f] = ok ? m0 : 0.f;
         a.rstd[f] = ok ? rstd : 0.f;
       }
     }
     const float m1 = sums[1] / (float)C;
+    // Backward: rstd (g - m0 - v m1) with rstd = 0 on frames left out.
+    const F2 rs(rstd, rstd), n0(-m0, -m0), n1(-m1, -m1);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int c = (tid + k * R) * V;
       if (c >= C) continue;
       float o[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = k * V + i;
-        o[i] = BWD ? rstd * (g[BWD ? e : 0] - m0 - v[e] * m1) : ok ? fmaf((v[e] - m0) * rstd, ga[e], be[e]) : 0.f;
+      for (int i = 0; i < V; i += 2) {
+        const int e = k * V + i, e1 = e + (V > 1), i1 = i + (V > 1);
+        if (BWD) {
+          const int z = BWD ? e : 0, z1 = BWD ? e1 : 0;
+          mul2(fma2(F2(v[e], v[e1]), n1, add2(F2(g[z], g[z1]), n0)), rs).get(o[i], o[i1]);
+        } else {
+          fma2(mul2(F2(v[e], v[e1]), rs), F2(ga[e], ga[e1]), F2(be[e], be[e1])).get(o[i], o[i1]);
+          if (!ok) o[i] = o[i1] = 0.f;
+        }
       }
       store_vec<T, V>(out + c, o);
     }
