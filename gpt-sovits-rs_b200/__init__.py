@@ -45,7 +45,7 @@ EXPORTS = (
     "gsvdec_forward_multi", "gsvdec_plan_multi", "gsvdec_sync_status", "gsvdec_selftest_wait",
     "gsvdec_set_alloc_fail_after", "gsvdec_workspace_bytes",
     "gsvdec_attention_workspace", "gsvdec_attention_forward", "gsvdec_attention_backward", "gsvdec_ops_status",
-    "gsvdec_norm_workspace", "gsvdec_norm_forward", "gsvdec_norm_backward",
+    "gsvdec_encp_attention", "gsvdec_norm_workspace", "gsvdec_norm_forward", "gsvdec_norm_backward",
 )
 
 # EncP encoder stacks (GSV_ENCP_SSL / _TEXT / _2), by their enc_p.* names.
@@ -117,6 +117,7 @@ def library(path: Optional[Path] = None) -> ctypes.CDLL:
     lib.gsvdec_encp_info.argtypes = [vp, ctypes.POINTER(i), ctypes.POINTER(i), ctypes.POINTER(i),
                                      ctypes.POINTER(i)]
     lib.gsvdec_encp_add_norm.argtypes = [vp, i, i, i, vp, vp, vp, i, i, vp, i, vp]
+    lib.gsvdec_encp_attention.argtypes = [vp, i, i, vp, vp, i, i, vp, i, vp]
     lib.gsvdec_encp_ffn.argtypes = [vp, i, i, vp, vp, i, i, vp, i, vp]
     lib.gsvdec_encp_layer.argtypes = [vp, i, i, vp, vp, vp, i, i, vp, i, vp]
     lib.gsvdec_encp_speed_len.argtypes = [i, ctypes.c_float, ctypes.POINTER(i)]
@@ -434,6 +435,31 @@ class Decoder:
         out = np.empty_like(xa)
         _check(library().gsvdec_encp_add_norm(self._h, self._stack(stack), layer, norm, _ptr(xa), _ptr(ya),
                                               _ptr(ln), B, T, _ptr(out), MEM_HOST, None))
+        return out
+
+    def encp_attention(self, stack, layer: int, x, lengths=None) -> np.ndarray:
+        """self_attn.forward(x, x_mask) of EncoderLayer::forward
+        (src/models/sovits_encp.rs:98-101) on host arrays: x [B, C, T]; frames
+        behind their length are left out as keys and give 0."""
+        xa = _host_f32(x)
+        B, C, T = xa.shape
+        ln = self._lengths(lengths, B)
+        out = np.empty_like(xa)
+        _check(library().gsvdec_encp_attention(self._h, self._stack(stack), layer, _ptr(xa), _ptr(ln), B, T, _ptr(out),
+                                               MEM_HOST, None))
+        return out
+
+    def encp_attention_device(self, stack, layer: int, x, lengths=None, out=None, stream=None):
+        """Stream-async encp_attention on CUDA tensors (torch): x, out [B, C, T] fp32, lengths int32."""
+        import torch
+        B, C, T = x.shape
+        assert x.is_cuda and x.dtype == torch.float32 and x.is_contiguous()
+        if out is None:
+            out = torch.empty_like(x)
+        st = stream if stream is not None else torch.cuda.current_stream(x.device).cuda_stream
+        p = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())  # noqa: E731
+        _check(library().gsvdec_encp_attention(self._h, self._stack(stack), layer, p(x), p(lengths), B, T, p(out),
+                                               MEM_DEVICE, ctypes.c_void_p(st)))
         return out
 
     def encp_ffn(self, stack, layer: int, x, lengths=None) -> np.ndarray:

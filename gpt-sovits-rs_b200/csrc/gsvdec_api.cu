@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "../../include/gsvdec.h"
+#include "attn.h"
 #include "gsv_kernels.h"
 #include "gsv_pdl.cuh"
 #include "safetensors.h"
@@ -394,6 +395,11 @@ int load_flow(const gsvdec_tensor* ts, int n, const std::string& prefix, HostFlo
 struct HostEncpLayer {
   HostConv c1, c2;
   std::vector<float> g1, b1, g2, b2;
+  // The layer's self-attention, where its tensors are there and of a form that
+  // the attention kernels take (gsvdec_encp_attention).
+  HostConv q, k, v, o;
+  std::vector<float> rel_k, rel_v;  // [2 w + 1][D]
+  int D = 0;                        // 0: no attention
 };
 
 struct HostEncp {
@@ -409,6 +415,26 @@ int load_vec(const TensorMap& tm, const std::string& key, int n, std::vector<flo
   if (!t) return set_err(GSV_E_MISSING_KEY, "Key '%s' not found in state dict", key.c_str());
   if (numel(t) != n) return set_err(GSV_E_SHAPE, "%s must have %d values", key.c_str(), n);
   return to_f32(t, v);
+}
+
+// attn_layers.<i>.{conv_q, conv_k, conv_v, conv_o} (1x1) and its learned
+// relative keys and values emb_rel_{k, v} [1, 2 w + 1, D], shared by the C / D
+// heads.  Optional: a layer without them, or with others, has no attention here.
+void load_encp_attention(const TensorMap& tm, const std::string& p, int C, HostEncpLayer& L) {
+  const gsvdec_tensor *rk = tm.get(p + ".emb_rel_k"), *rv = tm.get(p + ".emb_rel_v");
+  if (!rk || !rv || rk->ndim != 3 || rv->ndim != 3) return;
+  for (int i = 0; i < 3; ++i)
+    if (rk->shape[i] != rv->shape[i]) return;
+  const int64_t n = rk->shape[1], D = rk->shape[2];
+  if (rk->shape[0] != 1 || n < 1 || n % 2 == 0 || n > 2 * kAttnMaxWindow + 1 || D < 1 || D > kAttnMaxD || C % D) return;
+  HostConv* cs[4] = {&L.q, &L.k, &L.v, &L.o};
+  const char* names[4] = {".conv_q", ".conv_k", ".conv_v", ".conv_o"};
+  for (int i = 0; i < 4; ++i) {
+    if (!tm.get(p + names[i] + ".weight") || load_plain(tm, p + names[i], *cs[i]) != GSV_OK) return;
+    if (cs[i]->d0 != C || cs[i]->d1 != C || cs[i]->K != 1) return;
+  }
+  if (to_f32(rk, L.rel_k) != GSV_OK || to_f32(rv, L.rel_v) != GSV_OK) return;
+  L.D = (int)D;
 }
 
 int load_encp(const gsvdec_tensor* ts, int n, HostEncp& e) {
@@ -434,6 +460,7 @@ int load_encp(const gsvdec_tensor* ts, int n, HostEncp& e) {
       GSV_TRY(load_vec(tm, p + ".norm_layers_1." + is + ".beta", C, L.b1));
       GSV_TRY(load_vec(tm, p + ".norm_layers_2." + is + ".gamma", C, L.g2));
       GSV_TRY(load_vec(tm, p + ".norm_layers_2." + is + ".beta", C, L.b2));
+      load_encp_attention(tm, p + ".attn_layers." + is, C, L);
       e.stacks[s].push_back(std::move(L));
     }
   }
@@ -757,12 +784,18 @@ struct gsvdec {
   struct EncpLayer {
     GemmConv ffn1, ffn2;
     size_t norm = 0;  // float offset of gamma1, beta1, gamma2, beta2 (C each) in d_encp_norm
+    // Self-attention: D channels per head (0: none), 2 window + 1 relative rows
+    // at byte offset rel (keys, then values) in d_encp_rel, mode dtype.
+    GemmConv q, k, v, o;
+    int D = 0, window = 0;
+    size_t rel = 0;
   };
   std::vector<EncpLayer> encp[3];
   GemmConv encp_proj;
   bool has_encp_proj = false;
   int encp_C = 0, encp_F = 0;
   float* d_encp_norm = nullptr;
+  void* d_encp_rel = nullptr;
   void* ews = nullptr;
   size_t ews_bytes = 0;
   // Multi-device decode (gsvdec_forward_multi): this handle's worker stream
@@ -1713,6 +1746,8 @@ int create_impl(const gsvdec_tensor* ts, int n, int mode, int device, gsvdec_t**
       for (auto& L : st) {
         all.push_back(&L.c1);
         all.push_back(&L.c2);
+        if (L.D)
+          for (HostConv* x : {&L.q, &L.k, &L.v, &L.o}) all.push_back(x);
       }
     if (he.has_proj) all.push_back(&he.proj);
     materialize_all(all);
@@ -1852,6 +1887,15 @@ int create_impl(const gsvdec_tensor* ts, int n, int mode, int device, gsvdec_t**
   }
   // The EncP chains (optional), packed into the same weight arena.
   std::vector<float> encp_norm;
+  std::vector<uint8_t> encp_rel;
+  const size_t rel_elem = h->dt == Dt::BF16 ? 2 : 4;
+  auto conv_ok = [&](const HostConv& c) {  // a 1x1 conv the mode's GEMM takes
+    if (h->dt != Dt::BF16) return true;
+    TapConv op{};
+    op.nseg = 1; op.seg[0].Cin = c.d1; op.seg[0].ntaps = 1; op.seg[0].offstep = 1;
+    op.N = op.Cout = c.d0;
+    return tapconv_tc_supported(op);
+  };
   for (int s = 0; s < 3; ++s)
     for (const HostEncpLayer& L : he.stacks[s]) {
       gsvdec::EncpLayer E;
@@ -1859,6 +1903,27 @@ int create_impl(const gsvdec_tensor* ts, int n, int mode, int device, gsvdec_t**
       E.ffn2 = pk.conv(L.c2);
       E.norm = encp_norm.size();
       for (const std::vector<float>* v : {&L.g1, &L.b1, &L.g2, &L.b2}) encp_norm.insert(encp_norm.end(), v->begin(), v->end());
+      if (L.D && conv_ok(L.q)) {
+        E.q = pk.conv(L.q);
+        E.k = pk.conv(L.k);
+        E.v = pk.conv(L.v);
+        E.o = pk.conv(L.o);
+        E.D = L.D;
+        E.window = (int)(L.rel_k.size() / L.D) / 2;
+        E.rel = encp_rel.size();
+        for (const std::vector<float>* v : {&L.rel_k, &L.rel_v}) {
+          const size_t at = encp_rel.size();
+          encp_rel.resize((at + v->size() * rel_elem + 255) / 256 * 256);
+          for (size_t i = 0; i < v->size(); ++i) {
+            if (rel_elem == 4) {
+              memcpy(encp_rel.data() + at + 4 * i, &(*v)[i], 4);
+            } else {
+              const uint16_t u = __bfloat16_as_ushort(__float2bfloat16_rn((*v)[i]));
+              memcpy(encp_rel.data() + at + 2 * i, &u, 2);
+            }
+          }
+        }
+      }
       h->encp_C = L.c1.d1;
       h->encp_F = std::max(h->encp_F, L.c1.d0);
       h->encp[s].push_back(E);
@@ -1939,6 +2004,10 @@ int create_impl(const gsvdec_tensor* ts, int n, int mode, int device, gsvdec_t**
     CUDA_TRY(cudaMemcpy(h->d_encp_norm, encp_norm.data(), sizeof(float) * encp_norm.size(),
                         cudaMemcpyHostToDevice));
   }
+  if (!encp_rel.empty()) {
+    CUDA_TRY(dev_malloc(&h->d_encp_rel, encp_rel.size()));
+    CUDA_TRY(cudaMemcpy(h->d_encp_rel, encp_rel.data(), encp_rel.size(), cudaMemcpyHostToDevice));
+  }
   CUDA_TRY(cudaHostAlloc(reinterpret_cast<void**>(&h->h_err), sizeof(int), cudaHostAllocMapped));
   *reinterpret_cast<volatile int*>(h->h_err) = 0;
   CUDA_TRY(cudaHostGetDevicePointer(reinterpret_cast<void**>(&h->d_err), h->h_err, 0));
@@ -1965,6 +2034,7 @@ void destroy_impl(gsvdec* h) {
   cudaFree(h->d_flow_cond_w);
   cudaFree(h->d_flow_cond_b);
   cudaFree(h->d_encp_norm);
+  cudaFree(h->d_encp_rel);
   cudaFree(h->ews);
   for (auto& e : h->ev)
     if (e) cudaEventDestroy(e);
@@ -2367,6 +2437,87 @@ int encp_add_norm_impl(gsvdec* h, int stack, int layer, int norm, const float* x
   return finish_host(h, st, {{out, od}}, n, mem_kind);
 }
 
+// The layer's self-attention: q, k, v projections in one grouped launch (time
+// major), the attention on their [B][T][heads][D] rows, conv_o, relayout.
+int encp_attention_impl(gsvdec* h, int stack, int layer, const float* x, const int32_t* lengths, int B, int T,
+                        float* out, int mem_kind, cudaStream_t st) {
+  GSV_TRY(encp_common(h, B, T, mem_kind));
+  if (!x || !out) return set_err(GSV_E_INVALID_ARG, "x and out must not be NULL");
+  const gsvdec::EncpLayer* L = nullptr;
+  GSV_TRY(encp_layer(h, stack, layer, &L));
+  if (!L->D)
+    return set_err(GSV_E_UNSUPPORTED, "%s.attn_layers.%d was not loaded (absent, or not 1x1 convs with relative rows)",
+                   kEncpStacks[stack], layer);
+  const int C = h->encp_C;
+  if (B > 65535 || T > (1 << 24) || (int64_t)B * T * C > (int64_t)1 << 34)
+    return set_err(GSV_E_INVALID_ARG, "request too large");
+  const size_t n = (size_t)B * C * T, eb = act_bytes(h);
+  CUDA_TRY(cudaSetDevice(h->device));
+  std::vector<char*> sc;
+  GSV_TRY(encp_scratch(h, {n * 4, n * 4, n * eb, n * eb, n * eb, n * eb, (size_t)B * 4}, sc));
+  int rc = GSV_OK;
+  const float* xd = stage_in(x, n, sc[0], mem_kind, st, &rc);
+  const int* ld = stage_in(lengths, (size_t)B, sc[6], mem_kind, st, &rc);
+  GSV_TRY(rc);
+  float* od = mem_kind == GSV_MEM_DEVICE ? out : reinterpret_cast<float*>(sc[1]);
+  begin_run(h, st);
+  const double e = (double)eb;
+  const std::string nm = std::string(kEncpStacks[stack]) + "." + std::to_string(layer);
+  CUDA_TRY(launch_transpose_in(xd, B, C, T, 0, T, nullptr, sc[2], h->dt, st));
+  GSV_TRY(after_launch(h, st, "encp.input_relayout", 1, 0, 0.0, (4.0 + e) * n));
+  {
+    TapConvGroup g{};
+    Work wk;
+    const GemmConv* cs[3] = {&L->q, &L->k, &L->v};
+    for (int i = 0; i < 3; ++i) {
+      g.op[i] = make_op(h, *cs[i], B, sc[2], T);
+      g.op[i].out_raw = sc[3 + i];
+      wk.add(*cs[i], B, T, 0, e);
+    }
+    g.n = 3;
+    GSV_TRY(run_group(h, g, st, nm + ".conv_qkv", wk));
+  }
+  const int D = L->D, H = C / D, rel = 2 * L->window + 1;
+  AttnArgs a{};
+  a.ty = h->dt == Dt::BF16 ? Ty::BF16 : Ty::F32;
+  a.B = B;
+  a.H = a.Hkv = H;
+  a.Tq = a.Tk = T;
+  a.D = D;
+  a.window = L->window;
+  a.nrel = rel;
+  a.scale = 1.0f / std::sqrt((float)D);
+  a.q = sc[3];
+  a.k = sc[4];
+  a.v = sc[5];
+  a.relk = static_cast<const char*>(h->d_encp_rel) + L->rel;
+  a.relv = static_cast<const char*>(a.relk) + ((size_t)rel * D * eb + 255) / 256 * 256;
+  a.qlen = a.klen = ld;
+  a.o = sc[2];  // the projections have read it
+  a.sq = a.sk = a.sv = a.so = Str3{(int64_t)T * C, D, C};
+  const size_t aws = attn_fwd_workspace(a);
+  if (aws) return set_err(GSV_E_UNSUPPORTED, "attention needs a workspace of %zu bytes", aws);
+  CUDA_TRY(attn_forward(a, st));
+  GSV_TRY(after_launch(h, st, nm + ".attention", 1, 0, 4.0 * B * (double)T * T * C, 4.0 * e * n));
+  {
+    TapConv op = make_op(h, L->o, B, sc[2], T);
+    op.out_raw = sc[3];
+    op.len = ld;  // frames behind the length give 0
+    Work wk;
+    wk.add(L->o, B, T, 0, e);
+    GSV_TRY(run_one(h, op, st, nm + ".conv_o", wk));
+  }
+  CUDA_TRY(launch_to_ncl(sc[3], h->dt, B, T, C, od, st));
+  GSV_TRY(after_launch(h, st, "encp.output_relayout", 1, 0, 0.0, (4.0 + e) * n));
+  GSV_TRY(finish_host(h, st, {{out, od}}, n, mem_kind));
+  if (mem_kind == GSV_MEM_HOST) {
+    int gave_up = 0;
+    CUDA_TRY(attn_fwd_gave_up(&gave_up, st));
+    if (gave_up) return set_err(GSV_E_TIMEOUT, "a bounded device wait of the attention gave up");
+  }
+  return GSV_OK;
+}
+
 // conv_1 + ReLU, conv_2 + residual, norm2 + x_mask + relayout: the FFN half of
 // EncoderLayer::forward on the time-major operand xt ([B][T][C], mode dtype).
 int ffn_tail(gsvdec* h, int stack, int layer, const gsvdec::EncpLayer* L, void* xt, void* ht, void* vt,
@@ -2543,6 +2694,8 @@ int gsvdec_create_from_file(const char* path, int mode, int device, gsvdec_t** o
     auto wanted = [](const std::string& k) {
       if (k.compare(0, 4, "dec.") == 0 || k.compare(0, 11, "flow.flows.") == 0) return true;
       if (k.compare(0, 6, "enc_p.") != 0) return false;
+      // The stacks' own layers; the cross-attention of enc_p.mrte is not among them.
+      if (k.find(".attn_layers.") != std::string::npos) return k.compare(0, 13, "enc_p.encoder") == 0;
       return k.find(".ffn_layers.") != std::string::npos || k.find(".norm_layers_") != std::string::npos ||
              k.compare(0, 11, "enc_p.proj.") == 0;
     };
@@ -2670,6 +2823,11 @@ int gsvdec_encp_add_norm(gsvdec_t* h, int stack, int layer, int norm, const floa
                          const int32_t* lengths, int B, int T, float* out, int mem_kind, void* stream) {
   return gsv::encp_add_norm_impl(h, stack, layer, norm, x, y, lengths, B, T, out, mem_kind,
                                  static_cast<cudaStream_t>(stream));
+}
+
+int gsvdec_encp_attention(gsvdec_t* h, int stack, int layer, const float* x, const int32_t* lengths, int B,
+                          int T, float* out, int mem_kind, void* stream) {
+  return gsv::encp_attention_impl(h, stack, layer, x, lengths, B, T, out, mem_kind, static_cast<cudaStream_t>(stream));
 }
 
 int gsvdec_encp_ffn(gsvdec_t* h, int stack, int layer, const float* x, const int32_t* lengths, int B,

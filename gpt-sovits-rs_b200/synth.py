@@ -146,8 +146,8 @@ def make_encp_state_dict(seed: int = 20, layers=None, hidden: int = ENCP_HIDDEN,
     src/models/sovits_encp.rs:54-96, 348-369, 752-771): per layer i of each
     stack ``ffn_layers.{i}.conv_1`` [F, C, k] and ``conv_2`` [C, F, k] with
     biases, ``norm_layers_{1,2}.{i}.{gamma, beta}`` [C]; and ``enc_p.proj``
-    [2 out, C, 1] with bias.  Attention weights are not generated (the
-    attention itself is not part of these chains)."""
+    [2 out, C, 1] with bias.  The attention's tensors come from
+    make_encp_attention_state_dict."""
     rng = np.random.default_rng(seed)
     layers = ENCP_LAYERS if layers is None else layers
     sd = {}
@@ -167,6 +167,26 @@ def make_encp_state_dict(seed: int = 20, layers=None, hidden: int = ENCP_HIDDEN,
     if with_proj:
         sd["enc_p.proj.weight"] = rng.standard_normal((2 * out_channels, C, 1), dtype=np.float32) * np.float32(C ** -0.5)
         sd["enc_p.proj.bias"] = rng.standard_normal(2 * out_channels, dtype=np.float32) * np.float32(0.5)
+    return sd
+
+
+def make_encp_attention_state_dict(seed: int = 30, layers=None, hidden: int = ENCP_HIDDEN, heads: int = 2,
+                                   window: int = 4) -> dict:
+    """The ``enc_p.<stack>.attn_layers.<i>`` tensors (float32), seeded:
+    conv_{q, k, v, o} [C, C, 1] with biases and emb_rel_{k, v}
+    [1, 2 window + 1, C / heads]."""
+    rng = np.random.default_rng(seed)
+    layers = ENCP_LAYERS if layers is None else layers
+    C, D = hidden, hidden // heads
+    sd = {}
+    for stack, n in layers.items():
+        for i in range(n):
+            p = f"enc_p.{stack}.attn_layers.{i}"
+            for c in ("conv_q", "conv_k", "conv_v", "conv_o"):
+                sd[f"{p}.{c}.weight"] = rng.standard_normal((C, C, 1), dtype=np.float32) * np.float32(C ** -0.5)
+                sd[f"{p}.{c}.bias"] = rng.standard_normal(C, dtype=np.float32) * np.float32(0.05)
+            for r in ("emb_rel_k", "emb_rel_v"):
+                sd[f"{p}.{r}"] = rng.standard_normal((1, 2 * window + 1, D), dtype=np.float32) * np.float32(D ** -0.5)
     return sd
 
 

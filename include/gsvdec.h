@@ -105,7 +105,8 @@ int gsvdec_create(const gsvdec_tensor* tensors, int n_tensors, int mode, int dev
 /* Same as gsvdec_create, reading the tensors from a safetensors file
  * (the format written by src/bin/gpt-sovits-convert.rs:282-309 and read by
  * src/utils/weights.rs:116-162).  Only the tensors the handle uses are read:
- * dec.*, flow.flows.* and the enc_p.* FFN / LayerNorm / proj tensors. */
+ * dec.*, flow.flows.* and the enc_p.* attention / FFN / LayerNorm / proj
+ * tensors. */
 int gsvdec_create_from_file(const char* safetensors_path, int mode, int device, gsvdec_t** out);
 
 int gsvdec_destroy(gsvdec_t* h);
@@ -170,7 +171,8 @@ int gsvdec_flow_decode(gsvdec_t* h, const float* z_p, const float* g, const int3
 /* ---- EncP fused elementwise chains (optional) ----------------------------
  * Present when the tensors include enc_p.* encoder layers: per layer i of a
  * stack, "<stack>.ffn_layers.<i>.conv_{1,2}.{weight,bias}" and
- * "<stack>.norm_layers_{1,2}.<i>.{gamma,beta}" (EncoderLayer::load,
+ * "<stack>.norm_layers_{1,2}.<i>.{gamma,beta}", optionally the layer's
+ * "<stack>.attn_layers.<i>.*" (EncoderLayer::load,
  * src/models/sovits_encp.rs:54-96; FeedForward::load :348-369), and
  * "enc_p.proj.{weight,bias}" (:752-771).  Stacks: */
 #define GSV_ENCP_SSL 0  /* enc_p.encoder_ssl  */
@@ -191,6 +193,17 @@ int gsvdec_encp_info(const gsvdec_t* h, int n_layers[3], int* channels, int* fil
  * :109). */
 int gsvdec_encp_add_norm(gsvdec_t* h, int stack, int layer, int norm, const float* x, const float* y,
                          const int32_t* lengths, int B, int T, float* out, int mem_kind, void* stream);
+
+/* The self-attention of EncoderLayer::forward (self_attn.forward(x, x_mask),
+ * src/models/sovits_encp.rs:98-101): conv_o(attention(conv_q(x), conv_k(x),
+ * conv_v(x))) with the layer's learned relative keys and values, scale 1 /
+ * sqrt(D).  Needs "<stack>.attn_layers.<i>.{conv_q, conv_k, conv_v,
+ * conv_o}.{weight [C, C, 1], bias}" and "emb_rel_{k, v}" [1, 2 w + 1, D]
+ * (w <= 15, D <= 128) among the handle's tensors, else GSV_E_UNSUPPORTED.
+ * With lengths, keys t >= lengths[b] are left out and frames t >= lengths[b]
+ * of out are 0.  x, out [B, C, T] fp32; out is gsvdec_encp_layer's `attn`. */
+int gsvdec_encp_attention(gsvdec_t* h, int stack, int layer, const float* x, const int32_t* lengths, int B,
+                          int T, float* out, int mem_kind, void* stream);
 
 /* The FFN half of EncoderLayer::forward (src/models/sovits_encp.rs:104-109):
  * out = norm_layers_2[layer](x + conv_2(relu(conv_1(x)))) * x_mask, convs
