@@ -70,7 +70,8 @@ class _Calls:
         self.check = _check
         self.codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
-        self.empty, self.empty_strided = torch.empty, torch.empty_strided
+        # Allocations are most of a small call's host time; these are the cheaper of torch's.
+        self.empty_strided, self.empty_like = torch.empty_strided, torch.empty_like
         self.attention_forward, self.attention_backward = lib.gsvdec_attention_forward, lib.gsvdec_attention_backward
         self.norm_forward, self.norm_backward = lib.gsvdec_norm_forward, lib.gsvdec_norm_backward
         # The current stream's handle without building a torch Stream object, where torch offers that.
@@ -166,10 +167,26 @@ def _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
     return lead, (scale, ql, kl, pq, pk, pv, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], rk, rv), index
 
 
-def _heads_last(c, t, B, H, T, D, like):
+def _rows(c, dtype, n, m, device):
+    """A new contiguous [n, m] tensor."""
+    return c.empty_strided((n, m), (m, 1), dtype=dtype, device=device)
+
+
+def _line(c, dtype, n, device):
+    return c.empty_strided((n,), (1,), dtype=dtype, device=device)
+
+
+def _same(c, x):
+    """A new contiguous tensor of x's shape and type, and its leading strides."""
+    _, m, n = x.shape
+    t = c.empty_like(x) if x.is_contiguous() else c.empty_strided(x.shape, (m * n, n, 1), dtype=x.dtype, device=x.device)
+    return t, m * n, n
+
+
+def _heads_last(c, t, B, H, T, D, device):
     """A new [B, H, T, D] tensor in [B, T, H, D] memory order, and its strides."""
     s = (T * H * D, D, H * D)
-    return c.empty_strided((B, H, T, D), (*s, 1), dtype=t, device=like.device), s
+    return c.empty_strided((B, H, T, D), (*s, 1), dtype=t, device=device), s
 
 
 def attention(q, k, v, *, scale: Optional[float] = None, causal: bool = False, q_lengths=None, k_lengths=None,
@@ -190,10 +207,11 @@ def attention(q, k, v, *, scale: Optional[float] = None, causal: bool = False, q
     c = _get()
     lead, given, index = _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
     code, B, H, _, Tq, _, D = lead[:7]
-    o, so = _heads_last(c, q.dtype, B, H, Tq, D, q)
-    lse = c.empty((B, H, Tq), dtype=c.f32, device=q.device)
+    dev = q.device
+    o, so = _heads_last(c, q.dtype, B, H, Tq, D, dev)
+    lse = c.empty_strided((B, H, Tq), (H * Tq, Tq, 1), dtype=c.f32, device=dev)
     n = _attention_workspace(0, *lead)
-    ws = c.empty(n, dtype=c.u8, device=q.device) if n else None
+    ws = _line(c, c.u8, n, dev) if n else None
     a = _ATTENTION.pack(*lead, *given, o.data_ptr(), *so, lse.data_ptr(), 0, *_Z3, 0, 0, 0, *_Z3, *_Z3, *_Z3, 0, 0,
                         ws.data_ptr() if n else 0, n)
     rc = c.attention_forward(a, index, c.stream(index))
@@ -217,17 +235,17 @@ def attention_backward(do, q, k, v, o, lse, *, scale: Optional[float] = None, ca
     t, qs = q.dtype, q.shape
     pdo, po = _need("do", do, qs, t, index), _need("o", o, qs, t, index)
     pl = _need("lse", lse, qs[:3], c.f32, index, True)
-    dq, sq = _heads_last(c, t, B, H, Tq, D, q)
-    dk, sk = _heads_last(c, t, B, Hkv, Tk, D, q)
-    dv, _ = _heads_last(c, t, B, Hkv, Tk, D, q)
+    dev = q.device
+    dq, sq = _heads_last(c, t, B, H, Tq, D, dev)
+    dk, sk = _heads_last(c, t, B, Hkv, Tk, D, dev)
+    dv, _ = _heads_last(c, t, B, Hkv, Tk, D, dev)
     drk = drv = None
     prk = prv = 0
     if window >= 0:
-        drk, drv = c.empty((2 * window + 1, D), dtype=t, device=q.device), c.empty((2 * window + 1, D), dtype=t,
-                                                                                 device=q.device)
+        drk, drv = _rows(c, t, 2 * window + 1, D, dev), _rows(c, t, 2 * window + 1, D, dev)
         prk, prv = drk.data_ptr(), drv.data_ptr()
     n = _attention_workspace(1, *lead)
-    ws = c.empty(n, dtype=c.u8, device=q.device)
+    ws = _line(c, c.u8, n, dev)
     a = _ATTENTION.pack(*lead, *given, po, *o.stride()[:3], pl, pdo, *do.stride()[:3], dq.data_ptr(), dk.data_ptr(),
                         dv.data_ptr(), *sq, *sk, *sk, prk, prv, ws.data_ptr(), n)
     rc = c.attention_backward(a, index, c.stream(index))
@@ -275,9 +293,10 @@ def add_norm(x, y, gamma, beta, *, lengths=None, layout: str = "bct", eps: float
     lead, given, index = _norm_in(c, x, y, lengths, layout)
     B, C, T = lead[2:]
     pg, pb = _need("gamma", gamma, (C,), c.f32, index, True), _need("beta", beta, (C,), c.f32, index, True)
-    out = c.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = c.empty((B, T), dtype=c.f32, device=x.device), c.empty((B, T), dtype=c.f32, device=x.device)
-    a = _NORM.pack(*lead, eps, *given, pg, pb, mean.data_ptr(), rstd.data_ptr(), out.data_ptr(), *out.stride()[:2], 0, 0,
+    dev = x.device
+    out, s0, s1 = _same(c, x)
+    mean, rstd = _rows(c, c.f32, B, T, dev), _rows(c, c.f32, B, T, dev)
+    a = _NORM.pack(*lead, eps, *given, pg, pb, mean.data_ptr(), rstd.data_ptr(), out.data_ptr(), s0, s1, 0, 0,
                    0, 0, 0, 0, 0, 0, 0, 0)
     rc = c.norm_forward(a, index, c.stream(index))
     if rc:
@@ -295,12 +314,13 @@ def add_norm_backward(d_out, x, y, gamma, mean, rstd, *, lengths=None, layout: s
     pg = _need("gamma", gamma, (C,), c.f32, index, True)
     pd = _need("d_out", d_out, x.shape, x.dtype, index)
     pm, pr = _need("mean", mean, (B, T), c.f32, index, True), _need("rstd", rstd, (B, T), c.f32, index, True)
-    dx = c.empty(x.shape, dtype=x.dtype, device=x.device)
-    dgamma, dbeta = c.empty(C, dtype=c.f32, device=x.device), c.empty(C, dtype=c.f32, device=x.device)
+    dev = x.device
+    dx, s0, s1 = _same(c, x)
+    dgamma, dbeta = _line(c, c.f32, C, dev), _line(c, c.f32, C, dev)
     n = _norm_workspace(*lead)
-    ws = c.empty(n, dtype=c.u8, device=x.device)
+    ws = _line(c, c.u8, n, dev)
     a = _NORM.pack(*lead, 0.0, *given, pg, 0, pm, pr, 0, 0, 0, pd, dx.data_ptr(), *d_out.stride()[:2],
-                   *dx.stride()[:2], dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), n)
+                   s0, s1, dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), n)
     rc = c.norm_backward(a, index, c.stream(index))
     if rc:
         c.check(rc)
