@@ -13,6 +13,18 @@
 namespace gsv {
 namespace {
 
+__device__ __forceinline__ void tmem_load8(uint32_t taddr, float* v) {
+  uint32_t r[8];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 __device__ __forceinline__ void tmem_load16(uint32_t taddr, float* v) {
   uint32_t r[16];
   asm volatile(
@@ -323,6 +335,10 @@ __device__ __forceinline__ bool tma_fits(int row, int rows, int valid, int T) {
   return row + rows <= valid || valid == T;
 }
 
+__device__ __forceinline__ void prefetch_map(const RowsMap& m) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&m.map)) : "memory");
+}
+
 // One tile by TMA (one thread); its bytes count on `bar`.
 template <int DP>
 __device__ __forceinline__ void tma_tile(uint32_t dst, uint32_t chunk, const RowsMap& m, uint32_t bar, int row, int h,
@@ -334,6 +350,30 @@ __device__ __forceinline__ void tma_tile(uint32_t dst, uint32_t chunk, const Row
         " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst + c * chunk),
         "l"(reinterpret_cast<uint64_t>(&m.map)), "r"(bar), "r"(c * 64), "r"(row), "r"(h * m.mh), "r"(b * m.mb)
         : "memory");
+}
+
+// Cluster barrier (every thread of the cluster), and a read of another block's
+// shared memory at the place of this block's `addr`.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float cluster_load(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 
 template <int N>

@@ -74,6 +74,34 @@ struct BwdMaps {
   bool a_on, b_on;
 };
 
+// Adds the relative terms to the near scores and dP of a group's 32 columns, in
+// TMEM, eight columns at a time (a rolled loop: inside the passes over all
+// columns it would make those several times their size).  Column c has offset
+// index d0 + step c; the warp's near columns are [begin, end).
+template <typename F>
+__device__ __forceinline__ void near_terms(uint32_t ts, int d0, int step, int begin, int end, int nrel, F add) {
+  begin = max(0, begin);
+  end = min(kHalfB, end);
+  if (begin >= end) return;
+#pragma unroll 1
+  for (int c8 = begin & ~7; c8 < end; c8 += 8) {
+    float x[8], y[8];
+    tmem_load8(ts + c8, x);
+    tmem_load8(ts + kBB + c8, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned r = (unsigned)(d0 + step * (c8 + e));
+      if (r < (unsigned)nrel) add(c8 + e, r, x[e], y[e]);
+    }
+    uint32_t u[8], v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(x[e]), v[e] = __float_as_uint(y[e]);
+    tmem_store8(ts + c8, u);
+    tmem_store8(ts + kBB + c8, v);
+  }
+  tmem_store_wait();
+}
+
 template <typename T, int DP, bool REL>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant__ AttnArgs a,
                                                            const __grid_constant__ BwdWs ws,
@@ -131,6 +159,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
     fence_async_smem();
   }
   if (warp == 8) tmem_alloc(smem_u32(&s_tmem), 512);
+  if (threadIdx.x == 9 * 32 && maps.a_on && maps.b_on) {
+    prefetch_map(keys ? maps.ka : maps.qa);
+    prefetch_map(keys ? maps.va : maps.ga);
+    prefetch_map(keys ? maps.qb : maps.kb);
+    prefetch_map(keys ? maps.gb : maps.vb);
+  }
   pdl_wait();  // the row pass's values
   float gs = 1.f;  // the power of two that dS is carried with
   if (kHalf && nt > 0) {
@@ -343,24 +377,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         const float* nlse2 = tab + c0;
         const float* ndelta = tab + kBB + c0;
         const uint32_t tb = tS + (t & 1) * 2 * kBB + lanes;
+        if (REL) {
+          // Offset index of column 0; it falls by one per column and grows by one per row.
+          const int d0 = own - (i0 + off) + a.window;
+          const float* qrel = tab + 2 * kBB + c0 * a.nrel;
+          near_terms(tb + c0, d0, -1, d0 - lane - a.nrel + 1, d0 - lane + 32, a.nrel, [&](int c, unsigned r, float& x, float& y) {
+            x += qrel[c * a.nrel + r];
+            y += qrel[(kBB + c) * a.nrel + r];
+          });
+        }
         float s[kHalfB], dp[kHalfB];
         tmem_load32(tb + c0, s);
         tmem_load32(tb + kBB + c0, dp);
-        if (REL) {
-          const float* qrel = tab + 2 * kBB + c0 * a.nrel;
-          const float* grel = qrel + kBB * a.nrel;
-          const int d0 = own - (i0 + off) + a.window;  // offset index of column 0; falls by one per column
-          if (__any_sync(0xffffffffu, d0 >= 0 && d0 - (kHalfB - 1) < a.nrel)) {
-#pragma unroll
-            for (int c = 0; c < kHalfB; ++c) {
-              const unsigned r = (unsigned)(d0 - c);
-              if (r < (unsigned)a.nrel) {
-                s[c] += qrel[c * a.nrel + r];
-                dp[c] += grel[c * a.nrel + r];
-              }
-            }
-          }
-        }
         float p[kHalfB];
 #pragma unroll
         for (int c = 0; c < kHalfB; c += 4) {
@@ -412,21 +440,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         tc_fence_after();
         const int j0 = t * kBB + c0, lim = n - j0;
         const int d0 = j0 - (own + off) + a.window;
-        const bool near = REL && __any_sync(0xffffffffu, d0 < a.nrel && d0 + kHalfB > 0);
         const uint32_t tb = tS + (t & 1) * 2 * kBB + lanes;
+        if (REL)  // the tables then hold the near scores and dp themselves
+          near_terms(tb + c0, d0, 1, -(d0 + lane), a.nrel + 31 - (d0 + lane), a.nrel, [&](int, unsigned r, float& x, float& y) {
+            x += tq[r];
+            y += tg[r];
+            tq[r] = x;
+            tg[r] = y;
+          });
         float s[kHalfB], dp[kHalfB];
         tmem_load32(tb + c0, s);
         tmem_load32(tb + kBB + c0, dp);
-        if (near) {
-#pragma unroll
-          for (int c = 0; c < kHalfB; ++c) {
-            const unsigned r = (unsigned)(d0 + c);
-            if (r < (unsigned)a.nrel) {
-              s[c] += tq[r];
-              dp[c] += tg[r];
-            }
-          }
-        }
         float d[kHalfB];
 #pragma unroll
         for (int c = 0; c < kHalfB; c += 2) {
@@ -447,47 +471,38 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
           mul2(u, F2(s[c], s[c + 1])).get(d[c], d[c + 1]);
           d2[c / 2] = pack2<T>(d[c], d[c + 1]);
         }
-        if (near) {
-#pragma unroll
-          for (int c = 0; c < kHalfB; ++c) {
-            const unsigned r = (unsigned)(d0 + c);
-            if (r < (unsigned)a.nrel) {
-              tq[r] = s[c];
-              tg[r] = d[c];
-            }
-          }
-        }
         tmem_store16(tb + kBB + c0, d2);
         tmem_store_wait();
         tc_fence_before();
         warp_arrive(bar(bars.p_full[t & 1]));
       }
       if (REL && nt > 0) {
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // the near ds of both groups are in the table
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the near values of both groups are in the tables
         if (ok) {
           // Over the score columns of the buffer of tile nt, whose last readers were these warps.
           const int jb = own + off - a.window;
-          for (int q0 = wg * 16; q0 < a.nrel; q0 += 32) {
+          // Their p (group 1) and ds (group 0) as operands over the rows, and ds as dq's.
+          const uint32_t to = sTab + 2 * 32 * kBA * 4 + wg * C::bandT + (row >> 6) * (C::bandT / 2) + (row & 7) * 2;
+#pragma unroll 1
+          for (int q0 = 0; q0 < a.nrel; q0 += 16) {
             float d[16];
 #pragma unroll
             for (int y = 0; y < 16; ++y) {
               const int r = q0 + y, j = jb + r;
-              d[y] = r < a.nrel && j >= 0 && j < n ? tg[r] : 0.f;
+              const bool in = r < a.nrel && j >= 0 && j < n;
+              const float p = in ? ex2(fmaf(tq[in ? r : 0], sl2, nlse2)) : 0.f;
+              const float v = wg == 1 ? p : in ? p * ((tg[in ? r : 0] + ndelta) * (kHalf ? gp : 1.f)) : 0.f;
+              d[y] = v;
+              const uint16_t bits = (uint16_t)pack2<T>(v, 0.f);
+              if (r < a.nrel)
+                asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + r * 128 + ((((row & 63) >> 3) ^ (r & 7)) << 4)),
+                             "h"(bits)
+                             : "memory");
             }
             uint32_t u[8];
 #pragma unroll
             for (int y = 0; y < 8; ++y) u[y] = pack2<T>(d[2 * y], d[2 * y + 1]);
-            tmem_store8(tS + (nt & 1) * 2 * kBB + lanes + q0 / 2, u);
-          }
-          // Group 0: ds by offset and row, group 1: p, as operands over the rows.
-          const float* from = wg == 0 ? tg : tq;
-          const uint32_t to = sTab + 2 * 32 * kBA * 4 + wg * C::bandT + (row >> 6) * (C::bandT / 2) + (row & 7) * 2;
-          for (int r = 0; r < a.nrel; ++r) {
-            const int j = jb + r;
-            const float v = j >= 0 && j < n ? from[r] : 0.f;
-            const uint16_t bits = (uint16_t)pack2<T>(v, 0.f);
-            asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + r * 128 + ((((row & 63) >> 3) ^ (r & 7)) << 4)), "h"(bits)
-                         : "memory");
+            if (wg == 0) tmem_store8(tS + (nt & 1) * 2 * kBB + lanes + q0 / 2, u);
           }
           fence_async_smem();
           tmem_store_wait();

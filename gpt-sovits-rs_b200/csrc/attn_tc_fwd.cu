@@ -23,6 +23,11 @@
 // a table of 2 w + 1 values per row; the near scores replace their table entry
 // when their tile comes by, and after the last tile their probabilities are
 // one more P operand against the relative values' tile.
+//
+// Where the query tiles alone leave SMs idle, the blocks of a cluster deal out
+// a query tile's key tiles among them and join their sums at the end, each
+// block for its share of the rows, through distributed shared memory (rank
+// order, one launch, no workspace).
 #include "attn_launch.h"
 #include "attn_tc.cuh"
 
@@ -58,24 +63,28 @@ struct FwdMaps {
 
 template <typename T, int DP, bool REL>
 __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_constant__ AttnArgs a,
-                                                              const __grid_constant__ FwdMaps maps, const bool vec,
-                                                              const int ovec) {
+                                                              const __grid_constant__ FwdMaps maps, const int cs,
+                                                              const bool vec, const int ovec) {
   using C = FwdCfg<DP>;
   constexpr int ST = C::ST;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ FwdBars bars;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
+  __shared__ float s_m[kBM], s_l[kBM];  // for the other blocks of the cluster
+  __shared__ float s_w[8][kBM / 2];
   const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t sQ = base, sK = sQ + C::tile, sV = sK + ST * C::tile;
   float* tab = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + C::smem);  // [nrel][128]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   // Long rows of a causal mask first, so that the last blocks are short ones.
-  const int i0 = (int)(gridDim.x - 1 - blockIdx.x) * kBM, h = blockIdx.y, b = blockIdx.z;
+  const int rank = blockIdx.x % cs;
+  const int i0 = (int)(gridDim.x - 1 - blockIdx.x) / cs * kBM, h = blockIdx.y, b = blockIdx.z;
   const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk), off = kl - ql;
   const int last = min(i0 + kBM, ql) - 1;
   const int kend = last < i0 ? 0 : allowed_keys(last, ql, kl, a.causal);
-  const int nt = (kend + kBN - 1) / kBN;
+  // This block's key tiles: rank, rank + cs, ...
+  const int all = (kend + kBN - 1) / kBN, nt = all > rank ? (all - rank + cs - 1) / cs : 0;
   const int hk = h / (a.H / a.Hkv), D = a.D;
   volatile int* abort = &s_abort;
   auto bar = [&](const uint64_t& m) { return smem_u32(&m); };
@@ -97,6 +106,11 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
     fence_async_smem();
   }
   if (warp == 4) tmem_alloc(smem_u32(&s_tmem), 256);
+  if (threadIdx.x == 5 * 32 && maps.kv_on) {
+    prefetch_map(maps.q);
+    prefetch_map(maps.k);
+    prefetch_map(maps.v);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -215,10 +229,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
       for (int t = 0; t < nt && ok; ++t) {
         uint32_t dst = stage(true, kt);
         if (!dst) break;
-        fetch(dst, bar(bars.k_full[kt++ % ST]), maps.kv_on, maps.k, hk, k, a.sk.t, t * kBN, kl, a.Tk);
+        fetch(dst, bar(bars.k_full[kt++ % ST]), maps.kv_on, maps.k, hk, k, a.sk.t, (rank + t * cs) * kBN, kl, a.Tk);
         dst = stage(false, vt);
         if (!dst) break;
-        fetch(dst, bar(bars.v_full[vt++ % ST]), maps.kv_on, maps.v, hk, v, a.sv.t, t * kBN, kl, a.Tk);
+        fetch(dst, bar(bars.v_full[vt++ % ST]), maps.kv_on, maps.v, hk, v, a.sv.t, (rank + t * cs) * kBN, kl, a.Tk);
       }
       if (REL && ok) {
         const uint32_t dst = stage(false, vt);
@@ -230,6 +244,10 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
       ho.flush();
       cp_wait<0>();
       if (!ok) raise_err(&g_gave_up, abort, 1);
+    }
+    if (cs > 1) {  // as the softmax warps join the cluster's sums
+      cluster_sync();
+      cluster_sync();
     }
   } else {
     reg_inc<kSoftRegs>();
@@ -259,27 +277,40 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
         ok = warp_wait(bar(bars.s_full), sp++ & 1, abort);
         if (!ok) break;
         tc_fence_after();
-        const int j0 = t * kBN;
+        const int j0 = (rank + t * cs) * kBN;
+        if (REL) {
+          // The near scores get their relative terms in TMEM, eight columns at a time (a rolled loop: the
+          // same inside the pass below would make that several times its size for a few columns).
+          // Offset index of column 0; it falls by one per row: the warp's near columns are [first, end).
+          const int d0 = j0 - (i + off) + a.window;
+          const int first = max(0, -(d0 + lane)), end = min(kBN, a.nrel + 31 - (d0 + lane));
+          if (first < end) {
+#pragma unroll 1
+            for (int c8 = first & ~7; c8 < end; c8 += 8) {
+              float x[8];
+              tmem_load8(tS + lanes + c8, x);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const unsigned r = (unsigned)(d0 + c8 + e);
+                if (r < (unsigned)a.nrel) {
+                  x[e] += tab[r * kBM + row];
+                  tab[r * kBM + row] = x[e];
+                }
+              }
+              uint32_t u[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) u[e] = __float_as_uint(x[e]);
+              tmem_store8(tS + lanes + c8, u);
+            }
+            tmem_store_wait();
+          }
+        }
         float s[kBN];
         tmem_load64(tS + lanes, s);
         tmem_load64(tS + lanes + 64, s + 64);
         if (C::own_p) {
           tc_fence_before();
           warp_arrive(bar(bars.s_free));
-        }
-        if (REL) {
-          // Offsets of the warp's rows in this tile: j - pos + w for its first and last row.
-          const int d0 = j0 - (i + off) + a.window;
-          if (__any_sync(0xffffffffu, d0 < a.nrel && d0 + kBN > 0)) {
-#pragma unroll
-            for (int c = 0; c < kBN; ++c) {
-              const unsigned r = (unsigned)(d0 + c);
-              if (r < (unsigned)a.nrel) {
-                s[c] += tab[r * kBM + row];
-                tab[r * kBM + row] = s[c];
-              }
-            }
-          }
         }
         const int lim = n - j0;
         if (__any_sync(0xffffffffu, lim < kBN)) {
@@ -353,7 +384,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
 #pragma unroll
           for (int x = 0; x < 16; ++x) {
             const int r = r0 + x, j = base_j + r;
-            pr[x] = r < a.nrel && j >= 0 && j < n ? ex2(fmaf(tab[r * kBM + row], sl2, -mu)) : 0.f;
+            pr[x] = r < a.nrel && j >= 0 && j < n && ((j / kBN) & (cs - 1)) == rank ? ex2(fmaf(tab[r * kBM + row], sl2, -mu)) : 0.f;
           }
           uint32_t u[8];
 #pragma unroll
@@ -368,26 +399,118 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
       if (!ok) raise_err(&g_gave_up, abort, 1);
       tc_fence_after();
     }
-    if (ok && i < a.Tq) {
+    T* out = static_cast<T*>(a.o) + b * a.so.b + h * a.so.h;
+    float* lse = a.lse ? a.lse + ((int64_t)b * a.H + h) * a.Tq : nullptr;
+    if (cs == 1) {
       const bool some = nt > 0 && l != 0.f;
-      T* out = static_cast<T*>(a.o) + b * a.so.b + h * a.so.h + (int64_t)i * a.so.t;
-      if (a.lse)
-        a.lse[((int64_t)b * a.H + h) * a.Tq + i] =
-            some ? ((m == -INFINITY ? 0.f : m * sl2) + log2f(l)) * kLn2 : -INFINITY;
-      if (!some) {
-        float z[32] = {};
-        for (int c = 0; c < DP; c += 32) store_row32<T>(out, c, D, ovec, z, 0.f);
-      }
-    }
-    if (nt > 0 && ok) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* out = static_cast<T*>(a.o) + b * a.so.b + h * a.so.h + (int64_t)i * a.so.t;
+      const float inv = some ? 1.f / l : 0.f;
+      if (ok && i < a.Tq && lse)
+        lse[i] = some ? ((m == -INFINITY ? 0.f : m * sl2) + log2f(l)) * kLn2 : -INFINITY;
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
         float o[32];
-        tmem_load32(tO + lanes + c, o);
-        if (i < a.Tq && l != 0.f) store_row32<T>(out, c, D, ovec, o, inv);
+        if (nt > 0 && ok) tmem_load32(tO + lanes + c, o);
+        if (!some)
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = 0.f;
+        if (ok && i < a.Tq) store_row32<T>(out + (int64_t)i * a.so.t, c, D, ovec, o, inv);
       }
+    } else {
+      // This block's sums as [row][channel] over the K and V rings, whose tiles have all been used;
+      // the 16-byte unit u of a row sits at unit u ^ (row & 7), so that neither side has bank conflicts.
+      const uint32_t sO = sK + row * DP * 4;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        if (nt > 0 && ok) tmem_load32(tO + lanes + c, o);
+#pragma unroll
+        for (int x = 0; x < 32; x += 4) {
+          const uint32_t at = sO + (((c + x) / 4) ^ (row & 7)) * 16;
+          asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(nt > 0 ? o[x] : 0.f),
+                       "f"(nt > 0 ? o[x + 1] : 0.f), "f"(nt > 0 ? o[x + 2] : 0.f), "f"(nt > 0 ? o[x + 3] : 0.f)
+                       : "memory");
+        }
+      }
+      s_m[row] = nt > 0 ? m : -INFINITY;
+      s_l[row] = nt > 0 ? l : 0.f;
+      cluster_sync();
+      // The weights of the blocks' sums in each row of this block's share.
+      const int per = kBM / cs;
+      if (row < per) {
+        const int y = rank * per + row, iy = i0 + y;
+        float w[8], v[8], M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          w[x] = x < cs ? cluster_load(cluster_addr(smem_u32(s_m + y), x)) : -INFINITY;
+          v[x] = x < cs ? cluster_load(cluster_addr(smem_u32(s_l + y), x)) : 0.f;
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) M = fmaxf(M, w[x]);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          w[x] = w[x] == -INFINITY ? 0.f : ex2((w[x] - M) * sl2);
+          L = fmaf(w[x], v[x], L);
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) s_w[x][row] = L == 0.f ? 0.f : w[x] * inv;
+        if (iy < a.Tq && lse) lse[iy] = L == 0.f ? -INFINITY : ((M == -INFINITY ? 0.f : M * sl2) + log2f(L)) * kLn2;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // 8 channels of a row per step, lanes side by side; two steps and two ranks under way together.
+      constexpr int U = DP / 8;
+      for (int e0 = row; e0 < per * U; e0 += 2 * kBM) {
+        float o[2][8] = {};
+        for (int x = 0; x < cs; x += 2) {
+          float4 v[2][2][2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int e = min(e0 + j * kBM, per * U - 1), y = rank * per + e / U, u = e % U * 2;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t from = cluster_addr(sK + y * DP * 4, x + k);
+              v[j][k][0] = cluster_load4(from + (u ^ (y & 7)) * 16);
+              v[j][k][1] = cluster_load4(from + ((u + 1) ^ (y & 7)) * 16);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int e = min(e0 + j * kBM, per * U - 1);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const float f = s_w[x + k][e / U];
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                o[j][4 * q] = fmaf(f, v[j][k][q].x, o[j][4 * q]);
+                o[j][4 * q + 1] = fmaf(f, v[j][k][q].y, o[j][4 * q + 1]);
+                o[j][4 * q + 2] = fmaf(f, v[j][k][q].z, o[j][4 * q + 2]);
+                o[j][4 * q + 3] = fmaf(f, v[j][k][q].w, o[j][4 * q + 3]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int e = e0 + j * kBM, iy = i0 + rank * per + e / U, c = e % U * 8;
+          if (e >= per * U || iy >= a.Tq) continue;
+          T* to = out + (int64_t)iy * a.so.t + c;
+          if (ovec) {
+            if (c < D) {
+              uint4 u;
+              u.x = pack2<T>(o[j][0], o[j][1]);
+              u.y = pack2<T>(o[j][2], o[j][3]);
+              u.z = pack2<T>(o[j][4], o[j][5]);
+              u.w = pack2<T>(o[j][6], o[j][7]);
+              *reinterpret_cast<uint4*>(to) = u;
+            }
+          } else {
+#pragma unroll
+            for (int y = 0; y < 8; ++y)
+              if (c + y < D) to[y] = from_f<T>(o[j][y]);
+          }
+        }
+      }
+      cluster_sync();  // the sums have been read
     }
     tc_fence_before();
   }
@@ -414,8 +537,22 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
     m.kv_on = map_rows(&m.k, a.k, a.ty, a.sk, a.B, a.Hkv, a.Tk, a.D, kBN) &&
               map_rows(&m.v, a.v, a.ty, a.sv, a.B, a.Hkv, a.Tk, a.D, kBN);
   }
-  attn_fwd_tc<T, DP, REL><<<dim3(cdiv(a.Tq, kBM), a.H, a.B), kFwdThreads, smem, st>>>(a, m, vec, ovec);
-  return cudaGetLastError();
+  // Two blocks fit an SM: split while that leaves none of them waiting for a second turn.
+  const int nq = cdiv(a.Tq, kBM), nk = cdiv(a.Tk, kBN);
+  int cs = 1;
+  while (cs < 8 && 2 * cs <= nk && (int64_t)nq * a.H * a.B * 2 * cs <= 2 * sm_count()) cs *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(nq * cs, a.H, a.B);
+  cfg.blockDim = dim3(kFwdThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cs > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, attn_fwd_tc<T, DP, REL>, a, m, cs, vec, ovec);
 }
 
 template <typename T, int DP>

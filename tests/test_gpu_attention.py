@@ -92,6 +92,23 @@ def test_ragged_with_empty_sequences(gsv, dtype, causal):
         assert torch.all(dk[b, :, m:] == 0) and torch.all(dv[b, :, m:] == 0)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("Tq,Tk,D", [(130, 1025, 96), (9, 2300, 64), (40, 1500, 128), (300, 900, 32)])
+def test_long_keys_are_split_and_joined(gsv, dtype, Tq, Tk, D):
+    # Few query tiles: the key tiles of one are dealt out to several blocks.
+    x = make(dtype, 1, 2, 1, Tq, Tk, D, w=4)
+    run_and_check(gsv, x, causal=True)
+    run_and_check(gsv, x, q_lengths=lengths(Tq - 1), k_lengths=lengths(Tk // 2))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("H,Hkv,Tq", [(1, 1, 1), (8, 1, 1), (4, 2, 2), (3, 3, 7), (2, 1, 4)])
+@pytest.mark.parametrize("D", [20, 32, 64, 128])
+def test_few_queries(gsv, dtype, H, Hkv, Tq, D):
+    x = make(dtype, 2, H, Hkv, Tq, 1000, D, w=2)
+    run_and_check(gsv, x, causal=True, k_lengths=lengths(1000, 3))
+
+
 def test_lengths_outside_the_tensor_are_clamped(gsv):
     x = make("bf16", 3, 2, 2, 50, 60, 32)
     run_and_check(gsv, x, q_lengths=lengths(-3, 50, 99), k_lengths=lengths(60, 1 << 30, -(1 << 31)))
