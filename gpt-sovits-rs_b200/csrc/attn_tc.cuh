@@ -244,6 +244,18 @@ __device__ __forceinline__ void load_tile(uint32_t dst, uint32_t chunk, const T*
   }
 }
 
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // One arrival for a warp, after what its lanes did before (32 lanes arriving on
 // one barrier are served one by one).
 __device__ __forceinline__ void warp_arrive(uint32_t bar) {
@@ -273,7 +285,8 @@ struct Handover {
     bar = full;
   }
   __device__ __forceinline__ bool wait_free(uint32_t empty, uint32_t parity, volatile int* abort) {
-    if (__all_sync(0xffffffffu, mbar_try_nohint(empty, parity))) return true;
+    // A test that returns at once: a try_wait may sleep for microseconds with a tile not handed over.
+    if (__all_sync(0xffffffffu, mbar_test(empty, parity))) return true;
     flush();
     return __all_sync(0xffffffffu, mbar_wait_fast(empty, parity, abort));
   }
