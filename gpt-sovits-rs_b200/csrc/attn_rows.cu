@@ -2,8 +2,8 @@
 // the relative keys and values, and the choice of kernels of both directions.
 #include <algorithm>
 
-#include "attn_common.cuh"
 #include "attn_launch.h"
+#include "attn_tc.cuh"
 #include "gsv_pdl.cuh"
 
 namespace gsv {
@@ -32,7 +32,10 @@ __device__ __forceinline__ float dot8(const float* a, const float* b) {
 }
 
 // G lanes share one row, 8 channels each; a group takes U rows, whose loads are
-// all under way together.  Query rows: delta = do . o in fp32
+// all under way together.  The products with the relative rows are taken from
+// shared memory by one thread per row and three offsets (a fifth of the
+// instructions of products shared by G lanes, most of which were reductions).
+// Query rows: delta = do . o in fp32
 // and the products with the relative rows; fp16 adds the norms of the rows of
 // do and v.
 //
@@ -45,9 +48,9 @@ template <typename T, int G, int U>
 __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_constant__ AttnArgs a,
                                                                   const __grid_constant__ BwdWs ws, const int nq,
                                                                   const bool vec) {
-  extern __shared__ float sm[];  // relk, relv as [nrel][8 G]
+  extern __shared__ __align__(16) float sm[];  // relk, relv as [nrel][P], then q, do as [R U][P]
   constexpr bool F16 = std::is_same<T, __half>::value, kExact = std::is_same<T, float>::value;
-  constexpr int L = 8 * G, R = kRowThreads / G;
+  constexpr int L = 8 * G, P = L + 4, R = kRowThreads / G;
   // Heads fastest: the blocks of the first rows, which take longest (few keys), start first.
   const int tile = blockIdx.x / (a.H * a.B), bh32 = blockIdx.x - tile * (a.H * a.B);
   const int D = a.D, lane = threadIdx.x % G, d0 = lane * 8, b = bh32 / a.H, h = bh32 - b * a.H;
@@ -74,18 +77,33 @@ __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_c
     for (int u = 0; u < U; ++u) rg[u].load(v + min(i0 + u * R, a.Tk - 1) * a.sv.t, d0, D, vec);
   }
   float* srk = sm;
-  float* srv = srk + a.nrel * L;
+  float* srv = srk + a.nrel * P;
+  float* srows = srv + a.nrel * P;  // q; do R U P later
   for (int e = threadIdx.x; e < a.nrel * L; e += kRowThreads) {
     const int r = e / L, d = e % L;
     const T k = static_cast<const T*>(a.relk)[r * D + min(d, D - 1)], v = static_cast<const T*>(a.relv)[r * D + min(d, D - 1)];
-    srk[e] = d < D ? to_f(k) : 0.f;
-    srv[e] = d < D ? to_f(v) : 0.f;
+    srk[r * P + d] = d < D ? to_f(k) : 0.f;
+    srv[r * P + d] = d < D ? to_f(v) : 0.f;
+  }
+  if (a.nrel && !key_rows) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float q[8], g[8];
+      rq[u].get(q);
+      rg[u].get(g);
+      float4* to = reinterpret_cast<float4*>(srows + (u * R + threadIdx.x / G) * P + d0);
+      to[0] = make_float4(q[0], q[1], q[2], q[3]);
+      to[1] = make_float4(q[4], q[5], q[6], q[7]);
+      to += R * U * P / 4;
+      to[0] = make_float4(g[0], g[1], g[2], g[3]);
+      to[1] = make_float4(g[4], g[5], g[6], g[7]);
+    }
   }
   if (a.nrel) __syncthreads();
   if (key_rows) {
     float ev = 0.f;  // largest |relv|^2
     if ((threadIdx.x & 31) < a.nrel)
-      for (int d = 0; d < L; ++d) ev = fmaf(srv[(threadIdx.x & 31) * L + d], srv[(threadIdx.x & 31) * L + d], ev);
+      for (int d = 0; d < L; ++d) ev = fmaf(srv[(threadIdx.x & 31) * P + d], srv[(threadIdx.x & 31) * P + d], ev);
     ev = sqrtf(warp_max(ev));
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -119,34 +137,44 @@ __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_c
     if (n[u] == 0) delta[u] = norm[u] = 0.f, lse2[u] = INFINITY;
   }
   if (a.nrel) {
-    const int last = ws.blocks * kRowBlock;
-    float q[U][8], g[U][8];
+    const int base = tile * R * U;
+    constexpr int O = 3;  // offsets per thread: q and do are read once for three
+    const int groups = (a.nrel + O - 1) / O;
+    for (int e = threadIdx.x; e < groups * R * U; e += kRowThreads) {
+      const int y = e % (R * U), r0 = e / (R * U) * O, i = base + y;
+      const float4* q = reinterpret_cast<const float4*>(srows + y * P);
+      const float4* g = q + R * U * P / 4;
+      const float4 *rk[O], *rv[O];
+      F2 x[O], z[O];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      rq[u].get(q[u]);
-      rg[u].get(g[u]);
-    }
-#pragma unroll 1
-    for (int r = 0; r < a.nrel; ++r) {
-      float x[U], y[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        x[u] = dot8(q[u], srk + r * L + d0);
-        y[u] = dot8(g[u], srv + r * L + d0);
+      for (int o = 0; o < O; ++o) {
+        rk[o] = reinterpret_cast<const float4*>(srk + min(r0 + o, a.nrel - 1) * P);
+        rv[o] = reinterpret_cast<const float4*>(srv + min(r0 + o, a.nrel - 1) * P);
+        x[o] = z[o] = F2(0.f, 0.f);
       }
+#pragma unroll 2
+      for (int c = 0; c < L / 4; ++c) {
+        const float4 a4 = q[c], c4 = g[c];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        x[u] = group_sum<G>(x[u]);
-        y[u] = group_sum<G>(y[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int i = i0 + u * R;
-        if (i < last && lane == r % G) {
-          float* rel = rel_at(ws, bh, i, a.nrel) + r;
-          rel[0] = n[u] > 0 ? x[u] : 0.f;
-          rel[kRowBlock * a.nrel] = n[u] > 0 ? y[u] : 0.f;
+        for (int o = 0; o < O; ++o) {
+          const float4 b4 = rk[o][c], d4 = rv[o][c];
+          x[o] = fma2(F2(a4.x, a4.y), F2(b4.x, b4.y), x[o]);
+          x[o] = fma2(F2(a4.z, a4.w), F2(b4.z, b4.w), x[o]);
+          z[o] = fma2(F2(c4.x, c4.y), F2(d4.x, d4.y), z[o]);
+          z[o] = fma2(F2(c4.z, c4.w), F2(d4.z, d4.w), z[o]);
         }
+      }
+      if (i >= ws.blocks * kRowBlock) continue;
+      const bool in = i < a.Tq && allowed_keys(i, ql, kl, a.causal) > 0;
+      float* rel = rel_at(ws, bh, i, a.nrel);
+#pragma unroll
+      for (int o = 0; o < O; ++o) {
+        if (r0 + o >= a.nrel) continue;
+        float lo, hi;
+        x[o].get(lo, hi);
+        rel[r0 + o] = in ? lo + hi : 0.f;
+        z[o].get(lo, hi);
+        rel[kRowBlock * a.nrel + r0 + o] = in ? lo + hi : 0.f;
       }
     }
   }
@@ -182,7 +210,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_c
           gr.get(gg);
           if (near)
 #pragma unroll
-            for (int y = 0; y < 8; ++y) kk[y] += srk[r * L + c + y], vv[y] += srv[r * L + c + y];
+            for (int y = 0; y < 8; ++y) kk[y] += srk[r * P + c + y], vv[y] += srv[r * P + c + y];
           sc += dot8(qq, kk);
           dp += dot8(gg, vv);
         }
@@ -275,7 +303,10 @@ template <typename T, int G>
 cudaError_t rows_g(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
   constexpr int U = 2, R = kRowThreads / G * U;
   const int nq = cdiv(ws.blocks * kRowBlock, R), nk = a.ty == Ty::F16 ? cdiv(a.Tk, R) : 0;
-  const size_t smem = sizeof(float) * 2 * a.nrel * 8 * G;
+  const size_t smem = a.nrel ? sizeof(float) * 2 * (a.nrel + R) * (8 * G + 4) : 0;
+  int regs;
+  const cudaError_t e = kernel_setup(bwd_rows_kernel<T, G, U>, smem, &regs);
+  if (e != cudaSuccess) return e;
   const int el = sizeof(T);
   const bool vec = attn_rows_aligned(a.q, a.sq, a.D, el) && attn_rows_aligned(a.o, a.so, a.D, el) &&
                    attn_rows_aligned(a.dout, a.sdo, a.D, el) && attn_rows_aligned(a.k, a.sk, a.D, el) &&
