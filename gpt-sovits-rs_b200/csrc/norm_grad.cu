@@ -349,7 +349,9 @@ __global__ void __launch_bounds__(kRowThreads, BWD && E > 16 ? 1 : 2) norm_rows(
 }
 
 // Sums of NS values for each of a lane's V frames over the block's warps and
-// the cluster (lanes that share frames have been added before).
+// the cluster (lanes that share frames are added first).  s_b must be another
+// buffer than the call's before: the one cluster barrier of each call then also
+// says that the buffer before it has been read.
 template <int NS, int V>
 __device__ __forceinline__ void frame_sum(float (*v)[V], float (*s_w)[NS][32], float (*s_b)[32],
                                           cg::cluster_group& cl, int cs) {
@@ -383,13 +385,12 @@ __device__ __forceinline__ void frame_sum(float (*v)[V], float (*s_w)[NS][32], f
 #pragma unroll
       for (int i = 0; i < V; ++i) v[n][i] += from[n * 32 + (lane % F) * V + i];
   }
-  if (cs > 1) cl.sync();  // the sums have been read by every block
 }
 
 // Blocks of a team (a cluster of cs) walk tiles of 32 frames of one utterance;
-// a team's block r holds channels r * kTimeC and up.
+// a team's block r holds the channels from r * 16 E V.
 template <typename T, int V, int E, bool BWD>
-__global__ void __launch_bounds__(kTimeWarps * 32, V == 1 && E > 4 ? 1 : 2) norm_time(const __grid_constant__ NormArgs a, const int cs) {
+__global__ void __launch_bounds__(kTimeWarps * 32, BWD && V == 1 && E > 4 ? 1 : 2) norm_time(const __grid_constant__ NormArgs a, const int cs) {
   constexpr int F = 32 / V, NS = BWD ? 2 : 1;
   __shared__ float s_w[kTimeWarps][NS][32];
   __shared__ float s_b[2][NS][32];
@@ -398,74 +399,92 @@ __global__ void __launch_bounds__(kTimeWarps * 32, V == 1 && E > 4 ? 1 : 2) norm
   const int per_b = cdiv(a.T, 32), tiles = per_b * a.B, team = blockIdx.x / cs, rank = blockIdx.x - team * cs;
   const int teams = gridDim.x / cs;
   // A warp's load covers V channels side by side (lanes / F) of 32 frames.
-  const int c0 = rank * kTimeC + w * V + lane / F, fl = (lane % F) * V;
   constexpr int kStep = kTimeWarps * V;
-  float ga[E], be[E], dg[BWD ? E : 1] = {};
+  const int c0 = rank * E * kStep + w * V + lane / F, fl = (lane % F) * V;
+  // A lane with single frames has up to 16 channels: their weights are read where they are used.
+  constexpr bool kHeld = V > 1;
+  float ga[kHeld ? E : 1], be[BWD || kHeld ? E : 1], dg[BWD ? E : 1] = {};
+  if (BWD)
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int c = c0 + e * kStep;
-    ga[e] = c < C ? a.gamma[c] : 0.f;
-    be[e] = !BWD && c < C ? a.beta[c] : 0.f;
+    for (int e = 0; e < E; ++e) be[BWD ? e : 0] = 0.f;
+  if constexpr (kHeld) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = c0 + e * kStep;
+      ga[e] = c < C ? a.gamma[c] : 0.f;
+      if (!BWD) be[e] = c < C ? a.beta[c] : 0.f;
+    }
   }
+  auto gamma = [&](int e) { return kHeld ? ga[kHeld ? e : 0] : a.gamma[min(c0 + e * kStep, C - 1)]; };
+  auto beta = [&](int e) { return kHeld ? be[BWD || kHeld ? e : 0] : a.beta[min(c0 + e * kStep, C - 1)]; };
+  int flip = 0;
   const int nc = c0 < C ? min(E, (C - c0 + kStep - 1) / kStep) : 0;  // this lane's channels
   for (int tile = team; tile < tiles; tile += teams) {
     const int b = tile / per_b, t = (tile - b * per_b) * 32 + fl;
     const int n = a.len ? a.len[b] : a.T;
-    const bool in = t < a.T, some = in && t < n;
-    float v[E][V], g[BWD ? E : 1][V], u[E][V];
-    const T* x = static_cast<const T*>(a.x.p) + b * a.x.b + t + c0 * a.x.o;
-    const T* y = static_cast<const T*>(a.y.p) + b * a.y.b + t + c0 * a.y.o;
-    const T* d = static_cast<const T*>(a.dout.p) + b * a.dout.b + t + c0 * a.dout.o;
-    float mean[V], rstd[V];
+    const bool in = t < a.T;
+    float v[E][V], g[BWD ? E : 1][V], u[E][V], mean[V], rstd[V];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[e][i] = u[e][i] = g[BWD ? e : 0][i] = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) mean[i] = rstd[i] = 0.f;
-    if (BWD && some) {
+    if (t - fl < n) {  // the tile has frames to read (the same for the whole block)
+      // With single frames a thread has up to 48 loads: clamped addresses, values dropped below, so that
+      // none stands under a branch of its own and all are under way together.
+      const bool some = in && t < n;
+      const int tc = V == 1 ? min(t, a.T - 1) : t, cc = V == 1 ? min(c0, C - 1) : c0;
+      const T* x = static_cast<const T*>(a.x.p) + b * a.x.b + tc + cc * a.x.o;
+      const T* y = static_cast<const T*>(a.y.p) + b * a.y.b + tc + cc * a.y.o;
+      const T* d = static_cast<const T*>(a.dout.p) + b * a.dout.b + tc + cc * a.dout.o;
+      const int last = max(nc - 1, 0);
+      if (BWD && (V == 1 || some)) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        mean[i] = a.mean[(int64_t)b * a.T + t + i];
-        rstd[i] = a.rstd[(int64_t)b * a.T + t + i];
+        for (int i = 0; i < V; ++i) {
+          mean[i] = a.mean[(int64_t)b * a.T + tc + i];
+          rstd[i] = a.rstd[(int64_t)b * a.T + tc + i];
+        }
       }
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[e][i] = u[e][i] = 0.f;
-      if (some && e < nc) load_vec<T, V>(x + e * (kStep * a.x.o), v[e]);
-    }
-    if (a.y.p) {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (some && e < nc) load_vec<T, V>(y + e * (kStep * a.y.o), u[e]);
-    }
-    if (BWD) {
+        if (V == 1 || (some && e < nc)) load_vec<T, V>(x + (V == 1 ? min(e, last) : e) * (kStep * a.x.o), v[e]);
+      if (a.y.p) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
+        for (int e = 0; e < E; ++e)
+          if (V == 1 || (some && e < nc)) load_vec<T, V>(y + (V == 1 ? min(e, last) : e) * (kStep * a.y.o), u[e]);
+      }
+      if (BWD) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) g[BWD ? e : 0][i] = 0.f;
-        if (some && e < nc) load_vec<T, V>(d + e * (kStep * a.dout.o), g[BWD ? e : 0]);
+        for (int e = 0; e < E; ++e)
+          if (V == 1 || (some && e < nc)) load_vec<T, V>(d + (V == 1 ? min(e, last) : e) * (kStep * a.dout.o), g[BWD ? e : 0]);
       }
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (BWD && t + i >= n) mean[i] = rstd[i] = 0.f;
     float sums[NS][V] = {};
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const bool ok = t + i < n;  // a frame behind the length may hold anything
+        const bool ok = t + i < n && t < a.T && e < nc;  // a frame behind the length may hold anything
         v[e][i] = ok ? v[e][i] + u[e][i] : 0.f;
         if (BWD) {
           const int z = BWD ? e : 0;
-          v[e][i] = e < nc ? (v[e][i] - mean[i]) * rstd[i] : 0.f;
+          v[e][i] = ok ? (v[e][i] - mean[i]) * rstd[i] : 0.f;
           const float q = ok ? g[z][i] : 0.f;
           dg[z] = fmaf(q, v[e][i], dg[z]);
-          be[e] += q;
-          g[z][i] = q * ga[e];
+          be[z] += q;
+          g[z][i] = q * gamma(e);
           sums[0][i] += g[z][i];
           sums[NS - 1][i] = fmaf(g[z][i], v[e][i], sums[NS - 1][i]);
         } else {
           sums[0][i] += v[e][i];
         }
       }
-    frame_sum<NS, V>(sums, s_w, s_b[0], cl, cs);
+    frame_sum<NS, V>(sums, s_w, s_b[flip], cl, cs);
+    flip ^= 1;
     const float ic = 1.f / (float)C;
     if (!BWD) {
       float sq[1][V] = {};
@@ -476,7 +495,9 @@ __global__ void __launch_bounds__(kTimeWarps * 32, V == 1 && E > 4 ? 1 : 2) norm
         if (e < nc)
 #pragma unroll
           for (int i = 0; i < V; ++i) sq[0][i] = fmaf(v[e][i] - mean[i], v[e][i] - mean[i], sq[0][i]);
-      frame_sum<1, V>(sq, reinterpret_cast<float(*)[1][32]>(&s_w[0][0][0]), s_b[1], cl, cs);
+      __syncthreads();  // the first sums of the block's warps have been read
+      frame_sum<1, V>(sq, reinterpret_cast<float(*)[1][32]>(&s_w[0][0][0]), s_b[flip], cl, cs);
+      flip ^= 1;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const bool ok = t + i < n;
@@ -500,12 +521,13 @@ __global__ void __launch_bounds__(kTimeWarps * 32, V == 1 && E > 4 ? 1 : 2) norm
 #pragma unroll
         for (int i = 0; i < V; ++i)
           o[i] = BWD ? rstd[i] * (g[BWD ? e : 0][i] - sums[0][i] * ic - v[e][i] * (sums[NS - 1][i] * ic))
-                     : t + i < n ? fmaf((v[e][i] - mean[i]) * rstd[i], ga[e], be[e]) : 0.f;
+                     : t + i < n ? fmaf((v[e][i] - mean[i]) * rstd[i], gamma(e), beta(e)) : 0.f;
         store_vec<T, V>(out + e * (kStep * so), o);
       }
     }
     __syncthreads();  // the sums' buffers are free for the next tile
   }
+  if (cs > 1) cl.sync();  // the last sums have been read
   if (BWD) {
     float* part = a.part + (int64_t)team * 2 * C;
 #pragma unroll
@@ -513,11 +535,11 @@ __global__ void __launch_bounds__(kTimeWarps * 32, V == 1 && E > 4 ? 1 : 2) norm
 #pragma unroll
       for (int o = 1; o < F; o <<= 1) {
         dg[BWD ? e : 0] += __shfl_xor_sync(0xffffffffu, dg[BWD ? e : 0], o);
-        be[e] += __shfl_xor_sync(0xffffffffu, be[e], o);
+        be[BWD ? e : 0] += __shfl_xor_sync(0xffffffffu, be[BWD ? e : 0], o);
       }
       if (lane % F == 0 && e < nc) {
         part[c0 + e * kStep] = dg[BWD ? e : 0];
-        part[C + c0 + e * kStep] = be[e];
+        part[C + c0 + e * kStep] = be[BWD ? e : 0];
       }
     }
   }
@@ -565,11 +587,7 @@ int row_blocks(const NormArgs& a, bool bwd) {
   return std::max(1, std::min(cdiv(a.B * a.T, G), 148 * 2));
 }
 
-int time_cluster(int C) {
-  int cs = 1;
-  while (cs * kTimeC < C) cs *= 2;
-  return cs;
-}
+int time_cluster(int C) { return cdiv(C, kTimeC); }
 
 bool aligned(const NormTensor& t, int n, int V, int elem) {
   return !t.p || (reinterpret_cast<uintptr_t>(t.p) % (V * elem) == 0 && t.b % V == 0 && t.o % V == 0 && n % V == 0);
@@ -582,8 +600,8 @@ bool aligned(const NormArgs& a, bool bwd, int n, int V, int elem) {
 // Frames per lane of the [B][C][T] kernels.
 int time_vec(const NormArgs& a, bool bwd) { return aligned(a, bwd, a.T, 4, a.ty == Ty::F32 ? 4 : 2) ? 4 : 1; }
 
-int time_per_sm(const NormArgs& a, bool bwd) {  // one block where a lane's single frames leave it many channels
-  return time_vec(a, bwd) == 1 && a.C > 4 * kTimeWarps ? 1 : 2;
+int time_per_sm(const NormArgs& a, bool bwd) {  // one block where a lane's single frames leave it many sums
+  return bwd && time_vec(a, bwd) == 1 && a.C > 4 * kTimeWarps ? 1 : 2;
 }
 int time_teams(const NormArgs& a, int per_sm) {
   return (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)a.B * cdiv(a.T, 32), 148 * per_sm / time_cluster(a.C)));
@@ -638,11 +656,11 @@ cudaError_t time_launch(const NormArgs& a, int cs, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, norm_time<T, V, E, BWD>, a, cs);
 }
 
-// E * V channels and frames per lane: as many channels as a block of 16 warps
-// needs for min(C, 256).
+// E channels of V frames per lane: as many as a block of 16 warps needs for its
+// even share of C.
 template <typename T, bool BWD>
 cudaError_t time_shape(const NormArgs& a, cudaStream_t st) {
-  const int cs = time_cluster(a.C), per = cdiv(std::min(a.C, kTimeC), kTimeWarps);
+  const int cs = time_cluster(a.C), per = cdiv(cdiv(a.C, cs), kTimeWarps);
   if (time_vec(a, BWD) == 4) {
     if (per > 12) return time_launch<T, 4, 4, BWD>(a, cs, st);
     if (per > 8) return time_launch<T, 4, 3, BWD>(a, cs, st);
