@@ -193,6 +193,19 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+// What pack2's rounding of the two values lost.
+template <typename T>
+__device__ __forceinline__ F2 lost2(uint32_t packed, F2 x) {
+  float lo, hi;
+  if constexpr (std::is_same<T, __half>::value) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&packed));
+    lo = f.x, hi = f.y;
+  } else {
+    lo = __uint_as_float(packed << 16), hi = __uint_as_float(packed & 0xffff0000u);
+  }
+  return fma2(F2(lo, hi), F2(-1.f, -1.f), x);
+}
+
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }

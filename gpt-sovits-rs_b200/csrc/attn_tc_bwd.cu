@@ -25,6 +25,14 @@
 // 2^15 only, so P is carried as 2^15 P and dS with a power of two per head,
 // the largest that no |dS| can overflow with (|dP - delta| <= 2 max|do|
 // max|v|, norms taken by the row pass); both leave the fp32 sums at the end.
+// Over many terms that rounding and the one of the result are alike, 1.41 times
+// the latter together (measured 1.41 to 1.48 from 256 terms up, and up to 1.6
+// below).  Sequences of up to kFineT therefore add what the operands' rounding
+// lost as a second operand of each product (1.0 to 1.1 times): their launches
+// wait more than they multiply, so it costs 1 to 7 % there against 14 to 18 %
+// on long ones.  The near values always take both parts.
+#include <algorithm>
+
 #include "attn_launch.h"
 #include "attn_tc.cuh"
 #include "gsv_pdl.cuh"
@@ -36,6 +44,7 @@ __device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out
 
 constexpr int kBA = 128, kBB = 64;  // rows of the resident and of the streamed tiles
 constexpr int kHalfB = kBB / 2;
+constexpr int kFineT = 256;  // longest sequences with operands of twice the precision
 constexpr int kThreads = 384;
 
 template <int DP, bool REL>
@@ -49,8 +58,8 @@ struct BwdCfg {
   static constexpr uint32_t stage = 2 * tileB;
   static constexpr uint32_t relk = REL ? NC * chunkR : 0;
   static constexpr uint32_t bandT = 2 * 32 * 128;  // 32 offsets x 128 rows in 16 bits, two chunks of 64 rows
-  // keys: tables of ST stages; queries: the relative products of 128 rows and two operands.  The larger one.
-  static constexpr uint32_t tables_k = ST * (rows + rel), tables_q = REL ? 2 * 32 * kBA * 4 + 2 * bandT : 0;
+  // keys: tables of ST stages; queries: the relative products of 128 rows.  The larger one.
+  static constexpr uint32_t tables_k = ST * (rows + rel), tables_q = REL ? 2 * 32 * kBA * 4 : 0;
   static constexpr uint32_t tables = tables_k > tables_q ? tables_k : tables_q;
   static constexpr uint32_t smem = 2 * tileA + ST * stage + relk + tables;
 };
@@ -73,6 +82,18 @@ struct BwdMaps {
   RowsMap qa, ka, va, ga, qb, kb, vb, gb;
   bool a_on, b_on;
 };
+
+// What the rounding of 32 values to an operand's 16 columns lost, as 16 more.
+template <typename T>
+__device__ __forceinline__ void store_lost(uint32_t taddr, uint32_t* packed, const float* x) {
+#pragma unroll
+  for (int c = 0; c < kHalfB; c += 2) {
+    float lo, hi;
+    lost2<T>(packed[c / 2], F2(x[c], x[c + 1])).get(lo, hi);
+    packed[c / 2] = pack2<T>(lo, hi);
+  }
+  tmem_store16(taddr, packed);
+}
 
 // Adds the relative terms to the near scores and dP of a group's 32 columns, in
 // TMEM, eight columns at a time (a rolled loop: inside the passes over all
@@ -106,7 +127,7 @@ template <typename T, int DP, bool REL>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant__ AttnArgs a,
                                                            const __grid_constant__ BwdWs ws,
                                                            const __grid_constant__ BwdMaps maps, const int nk,
-                                                           const bool vec, const int ovec) {
+                                                           const bool fine, const bool vec, const int ovec) {
   using C = BwdCfg<DP, REL>;
   constexpr int ST = C::ST;
   constexpr bool kHalf = std::is_same<T, __half>::value;
@@ -229,17 +250,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         const uint32_t p = tS + (t & 1) * 2 * kBB, done = bar(bars.b_free[us]);
         const uint64_t m0 = mB + us * (C::stage >> 4), m1 = m0 + (C::tileB >> 4);
         if (++us == ST) us = 0;
-        // Each group's 32 operand columns lie over the first half of its own scores.
-        auto accumulate = [&](uint32_t acc, uint32_t op, uint64_t m) {
-          if (t == 0) mma_ts_first(acc, op, m, id_a);
+        // Each group's 16 operand columns lie over the first half of its own scores, what their rounding
+        // lost over the second.
+        auto accumulate = [&](uint32_t acc, uint32_t op, uint64_t m, bool start) {
+          if (start) mma_ts_first(acc, op, m, id_a);
           else mma_ts_acc(acc, op, m, id_a);
 #pragma unroll
           for (int c = 1; c < kBB / 16; ++c)
             mma_ts_acc(acc, op + (c >> 1) * kHalfB + (c & 1) * 8, m + c * (2048 >> 4), id_a);
         };
         if (lead) {
-          if (keys) accumulate(tAcc0, p, m1);
-          accumulate(tAcc1, p + kBB, m0);
+          if (keys) accumulate(tAcc0, p, m1, t == 0);
+          accumulate(tAcc1, p + kBB, m0, t == 0);
+          if (fine) {
+            if (keys) accumulate(tAcc0, p + 16, m1, false);
+            accumulate(tAcc1, p + kBB + 16, m0, false);
+          }
           mma_commit(done);
         }
         __syncwarp();
@@ -250,16 +276,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         tc_fence_after();
         if (ok && lead) {
           const int nrp = (a.nrel + 15) / 16 * 16;
-          for (int c = 0; c < nrp / 16; ++c)
-            mma_ts_acc(tAcc1, tS + (nt & 1) * 2 * kBB + c * 8, desc_mn(sR + c * 2048, C::chunkR), id_a);
-          // Rows of the result: 128 channels (those past the tile's are not read); columns: offsets.
-          const uint32_t id_r = idesc_attn<T>(nrp, false) | (1u << 15), band = sTab + 2 * 32 * kBA * 4;
           for (int x = 0; x < 2; ++x)
+            for (int c = 0; c < nrp / 16; ++c)
+              mma_ts_acc(tAcc1, tS + (nt & 1) * 2 * kBB + x * 16 + c * 8, desc_mn(sR + c * 2048, C::chunkR), id_a);
+          // Rows of the result: 128 channels (those past the tile's are not read); columns: offsets.
+          const uint32_t id_r = idesc_attn<T>(nrp, false) | (1u << 15);
+          for (int x = 0; x < 4; ++x)  // ds and what its rounding lost, then p
             for (int c = 0; c < kBA / 16; ++c) {
-              const uint64_t m = desc_mn((x ? sA1 : sA0) + c * 2048, C::chunkA);
-              const uint64_t d = sdesc<64>(band + x * C::bandT + (c >> 2) * (C::bandT / 2) + (c & 3) * 32);
-              if (c == 0) mma_bf16_first(tRel + x * 32, m, d, id_r);
-              else mma_bf16_acc(tRel + x * 32, m, d, id_r);
+              const uint64_t m = desc_mn((x >> 1 ? sA1 : sA0) + c * 2048, C::chunkA);
+              const uint64_t d = sdesc<64>(sB + x * C::bandT + (c >> 2) * (C::bandT / 2) + (c & 3) * 32);
+              if (x % 2 == 0 && c == 0) mma_bf16_first(tRel + (x >> 1) * 32, m, d, id_r);
+              else mma_bf16_acc(tRel + (x >> 1) * 32, m, d, id_r);
             }
         }
       }
@@ -405,21 +432,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
             if (c < skip) p[c] = 0.f;
         }
         uint32_t p2[kHalfB / 2], d2[kHalfB / 2];
+        float d[kHalfB];
 #pragma unroll
         for (int c = 0; c < kHalfB; c += 4) {
           const float4 E = *reinterpret_cast<const float4*>(ndelta + c);
           F2 u = add2(F2(dp[c], dp[c + 1]), F2(E.x, E.y)), w = add2(F2(dp[c + 2], dp[c + 3]), F2(E.z, E.w));
           if (kHalf) u = mul2(u, gp2), w = mul2(w, gp2);
-          float d[4];
-          mul2(u, F2(p[c], p[c + 1])).get(d[0], d[1]);
-          mul2(w, F2(p[c + 2], p[c + 3])).get(d[2], d[3]);
+          mul2(u, F2(p[c], p[c + 1])).get(d[c], d[c + 1]);
+          mul2(w, F2(p[c + 2], p[c + 3])).get(d[c + 2], d[c + 3]);
           p2[c / 2] = pack2<T>(p[c], p[c + 1]);
           p2[c / 2 + 1] = pack2<T>(p[c + 2], p[c + 3]);
-          d2[c / 2] = pack2<T>(d[0], d[1]);
-          d2[c / 2 + 1] = pack2<T>(d[2], d[3]);
+          d2[c / 2] = pack2<T>(d[c], d[c + 1]);
+          d2[c / 2 + 1] = pack2<T>(d[c + 2], d[c + 3]);
         }
         tmem_store16(tb + c0, p2);
         tmem_store16(tb + kBB + c0, d2);
+        if (fine) {
+          store_lost<T>(tb + c0 + 16, p2, p);
+          store_lost<T>(tb + kBB + c0 + 16, d2, d);
+        }
         tmem_store_wait();
         tc_fence_before();
         warp_arrive(bar(bars.p_full[t & 1]));
@@ -472,6 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
           d2[c / 2] = pack2<T>(d[c], d[c + 1]);
         }
         tmem_store16(tb + kBB + c0, d2);
+        if (fine) store_lost<T>(tb + kBB + c0 + 16, d2, d);
         tmem_store_wait();
         tc_fence_before();
         warp_arrive(bar(bars.p_full[t & 1]));
@@ -481,33 +513,46 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         if (ok) {
           // Over the score columns of the buffer of tile nt, whose last readers were these warps.
           const int jb = own + off - a.window;
-          // Their p (group 1) and ds (group 0) as operands over the rows, and ds as dq's.
-          const uint32_t to = sTab + 2 * 32 * kBA * 4 + wg * C::bandT + (row >> 6) * (C::bandT / 2) + (row & 7) * 2;
+          // Their p (group 1) and ds (group 0) as operands over the rows, in the ring that the last MMAs have
+          // read, and ds as dq's; each with a second operand of what its rounding lost.
+          ok = warp_wait(bar(bars.b_free[(nt - 1) % ST]), ((nt - 1) / ST) & 1, abort);
+          const uint32_t to = sB + wg * 2 * C::bandT + (row >> 6) * (C::bandT / 2) + (row & 7) * 2;
 #pragma unroll 1
-          for (int q0 = 0; q0 < a.nrel; q0 += 16) {
+          for (int q0 = 0; q0 < a.nrel && ok; q0 += 16) {
             float d[16];
+            uint32_t hi[8], lo[8];
 #pragma unroll
             for (int y = 0; y < 16; ++y) {
               const int r = q0 + y, j = jb + r;
               const bool in = r < a.nrel && j >= 0 && j < n;
               const float p = in ? ex2(fmaf(tq[in ? r : 0], sl2, nlse2)) : 0.f;
-              const float v = wg == 1 ? p : in ? p * ((tg[in ? r : 0] + ndelta) * (kHalf ? gp : 1.f)) : 0.f;
-              d[y] = v;
-              const uint16_t bits = (uint16_t)pack2<T>(v, 0.f);
-              if (r < a.nrel)
-                asm volatile("st.shared.b16 [%0], %1;" ::"r"(to + r * 128 + ((((row & 63) >> 3) ^ (r & 7)) << 4)),
-                             "h"(bits)
-                             : "memory");
+              d[y] = wg == 1 ? p : in ? p * ((tg[in ? r : 0] + ndelta) * (kHalf ? gp : 1.f)) : 0.f;
             }
-            uint32_t u[8];
 #pragma unroll
-            for (int y = 0; y < 8; ++y) u[y] = pack2<T>(d[2 * y], d[2 * y + 1]);
-            if (wg == 0) tmem_store8(tS + (nt & 1) * 2 * kBB + lanes + q0 / 2, u);
+            for (int y = 0; y < 16; y += 2) {
+              hi[y / 2] = pack2<T>(d[y], d[y + 1]);
+              float a0, a1;
+              lost2<T>(hi[y / 2], F2(d[y], d[y + 1])).get(a0, a1);
+              lo[y / 2] = pack2<T>(a0, a1);
+            }
+#pragma unroll
+            for (int y = 0; y < 16; ++y) {
+              const int r = q0 + y;
+              if (r >= a.nrel) continue;
+              const uint32_t at = to + r * 128 + ((((row & 63) >> 3) ^ (r & 7)) << 4);
+              asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"((uint16_t)(hi[y / 2] >> (16 * (y & 1)))) : "memory");
+              asm volatile("st.shared.b16 [%0], %1;" ::"r"(at + C::bandT), "h"((uint16_t)(lo[y / 2] >> (16 * (y & 1))))
+                           : "memory");
+            }
+            if (wg == 0) {
+              tmem_store8(tS + (nt & 1) * 2 * kBB + lanes + q0 / 2, hi);
+              tmem_store8(tS + (nt & 1) * 2 * kBB + lanes + 16 + q0 / 2, lo);
+            }
           }
           fence_async_smem();
           tmem_store_wait();
           tc_fence_before();
-          warp_arrive(bar(bars.p_full[nt & 1]));
+          if (ok) warp_arrive(bar(bars.p_full[nt & 1]));
         }
       }
     }
@@ -579,6 +624,7 @@ cudaError_t launch(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
   const int ovec = std::min(store_mode(a.dq, a.sdq, a.D),
                             std::min(store_mode(a.dk, a.sdk, a.D), store_mode(a.dv, a.sdv, a.D)));
   const int nk = cdiv(a.Tk, kBA), nq = cdiv(a.Tq, kBA);
+  const bool fine = std::max(a.Tq, a.Tk) <= kFineT;
   BwdMaps m = {};
   if (vec) {
     m.a_on = map_rows(&m.qa, a.q, a.ty, a.sq, a.B, a.H, a.Tq, a.D, kBA) &&
@@ -591,7 +637,7 @@ cudaError_t launch(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
              map_rows(&m.vb, a.v, a.ty, a.sv, a.B, a.Hkv, a.Tk, a.D, kBB);
   }
   const PdlScope pdl(a.Tq > 0);  // its set-up runs beside the end of the row pass
-  return launch_k(attn_bwd_tc<T, DP, REL>, dim3(nk + nq, a.H, a.B), kThreads, smem, st, a, ws, m, nk, vec, ovec);
+  return launch_k(attn_bwd_tc<T, DP, REL>, dim3(nk + nq, a.H, a.B), kThreads, smem, st, a, ws, m, nk, fine, vec, ovec);
 }
 
 template <typename T, int DP>
