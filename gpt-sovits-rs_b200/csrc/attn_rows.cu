@@ -349,7 +349,8 @@ size_t attn_bwd_workspace(const AttnArgs& a) { return carve_bwd(a).bytes; }
 
 cudaError_t attn_forward(const AttnArgs& a, cudaStream_t st) {
   if (!a.Tq) return cudaSuccess;
-  // A tile kernel would fill 64 or 128 rows for these.
+  // A tile kernel would fill 64 or 128 rows for these: 28 us (fp16) and 144 us (fp32) against 12 for one token of
+  // 16 sequences, 16 heads of 32 over 4 key heads and up to 1531 keys.
   if ((int64_t)a.Tq * (a.H / a.Hkv) <= kFewRows) return attn_fwd_few_rows(a, st);
   return a.ty == Ty::F32 ? attn_fwd_cores(a, st) : attn_fwd_tensor(a, st);
 }

@@ -109,6 +109,14 @@ def test_few_queries(gsv, dtype, H, Hkv, Tq, D):
     run_and_check(gsv, x, causal=True, k_lengths=lengths(1000, 3))
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("H,Hkv,Tq,D,w", [(8, 1, 1, 64, 15), (2, 1, 2, 96, 4), (1, 1, 8, 128, 15), (4, 2, 1, 33, 0)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_few_queries_over_long_keys(gsv, dtype, H, Hkv, Tq, D, w, causal):
+    # The keys are split over the largest clusters; the last ones, near the queries, over several of its blocks.
+    run_and_check(gsv, make(dtype, 2, H, Hkv, Tq, 9001, D, w=w), causal=causal, k_lengths=lengths(9001, 8200))
+
+
 def test_lengths_outside_the_tensor_are_clamped(gsv):
     x = make("bf16", 3, 2, 2, 50, 60, 32)
     run_and_check(gsv, x, q_lengths=lengths(-3, 50, 99), k_lengths=lengths(60, 1 << 30, -(1 << 31)))
