@@ -44,6 +44,11 @@ __device__ __forceinline__ float dot8(const float* a, const float* b) {
 // term disappears; rows of up to kFewKeys keys, where it would be as large as
 // the rounding of ds itself, take delta = sum_j p_ij dp_ij instead (fp32
 // inputs have no such rounding).
+//
+// Reads do and o (with a window q) once: 2 x 16 heads of 64, 4096 causal rows,
+// bf16, 25 us, where the 32 rows of few keys of each head take longest; 16
+// utterances of up to 500 rows, 2 heads of 96, window 4, 12 us, one or two
+// blocks an SM that wait for memory twice and then do 18 products a row.
 template <typename T, int G, int U>
 __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_constant__ AttnArgs a,
                                                                   const __grid_constant__ BwdWs ws, const int nq,

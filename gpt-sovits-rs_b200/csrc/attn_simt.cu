@@ -17,6 +17,17 @@
 // Where the largest tile row or column would outlast an even share of the work
 // on all SMs, its tiles are dealt out to the blocks of a cluster, whose sums
 // are joined in rank order through distributed shared memory.
+//
+// The tensor cores would need three 16-bit pieces per value and six products
+// for each, and room for the pieces that a block does not have at D = 128.
+//
+// Measured on B200: backward of 4 utterances, 4 heads of 128, up to 500 queries
+// and 173 keys: 87 us and 7 for the rows, 13 TFLOP/s.  The whole tiles' seven
+// products would take 27 us on all SMs at the FMA rate; a block has 8 warps an
+// SM (its tiles fill the shared memory), too few to cover the loads of the
+// streamed tiles and the barriers around them, and the units do not divide
+// evenly.  One utterance of 37 frames, 2 heads of 96, window 4, forward: 14.6
+// us, one tile a head, all of it latency.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -353,8 +364,9 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_simt(const __grid_constant_
   cl.sync();  // the block's sums have been read
 }
 
-// x / cs in [0, nk): dk, dv of one key tile and key head; the rest: dq of one
-// query tile, once per query head (the z axis carries the batch).
+// The first units (clusters) take dk, dv of one key tile and key head each, the
+// others dq of one query tile and head: the keys' units, which take a third
+// longer a tile, all start before the queries'.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const __grid_constant__ AttnArgs a,
                                                           const __grid_constant__ BwdWs ws, const int nk, const int cs,
@@ -368,18 +380,20 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const __grid_constant_
   float* sP = s3 + tile_floats<DP>();
   float* sS = sP + kBT * kLdP;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int b = blockIdx.z, D = a.D, g = a.H / a.Hkv;
+  const int D = a.D, g = a.H / a.Hkv, nq = cdiv(a.Tq, kBT);
+  const int rank = blockIdx.x % cs, unit = blockIdx.x / cs, kunits = nk * a.Hkv * a.B;
+  const bool keys = unit < kunits;
+  // Tiles slowest, the longest ones of a causal call first.
+  const int heads = (keys ? a.Hkv : a.H) * a.B, at = keys ? unit : unit - kunits;
+  const int tile = keys ? at / heads : nq - 1 - at / heads, bhu = at % heads;
+  const int b = keys ? bhu / a.Hkv : bhu / a.H;
   const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk), off = kl - ql;
   const float sl2 = a.scale * kLog2e;
   cg::cluster_group cl = cg::this_cluster();
-  const int rank = blockIdx.x % cs, unit = blockIdx.x / cs;
   const int from = rank * (kBT / cs);  // first of the rows that this block writes
   auto one = [](int, int) { return 1.f; };
-  const bool keys = unit < nk;
   if (keys) {
-    const int hk = blockIdx.y;
-    if (hk >= a.Hkv) return;  // the whole cluster
-    const int j0 = unit * kBT;
+    const int hk = bhu - b * a.Hkv, j0 = tile * kBT;
     load_rows<T, DP>(s0, static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h + (int64_t)j0 * a.sk.t, a.sk.t,
                      kl - j0, D, vec);
     load_rows<T, DP>(s1, static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h + (int64_t)j0 * a.sv.t, a.sv.t,
@@ -457,9 +471,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const __grid_constant_
     }
     return;
   }
-  const int h = blockIdx.y, hk = h / g;
-  const int i0 = (unit - nk) * kBT;
-  const int64_t bh = (int64_t)b * a.H + h, row = bh * a.Tq;
+  const int h = bhu - b * a.H, hk = h / g, i0 = tile * kBT;
+  const int64_t bh = bhu, row = bh * a.Tq;
   load_rows<T, DP>(s0, static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t, ql - i0,
                    D, vec);
   load_rows<T, DP>(s1, static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t,
@@ -546,12 +559,23 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const __grid_constant_
   cl.sync();
 }
 
-// Blocks per tile row or column: the smallest power of two at which the longest
-// one is no more than an even share of the work on all SMs (or one tile).
-int split(int64_t longest, int64_t total, int tiles) {
-  int cs = 1;
-  while (cs < 8 && 2 * cs <= tiles && longest * 148 > total * cs) cs *= 2;
-  return cs;
+// Blocks per tile row or column (a unit): the power of two with the smallest
+// estimate of the time, the longer of the longest unit's share and an even
+// share of all work on the SMs, where each block adds `set_up` (resident tiles,
+// joining).  One utterance of 500, 2 heads of 96, window 4: 65 -> 36 us forward;
+// backward 126 -> 53, and 79 with twice as many.  The cross case above: 143 ->
+// 94, and 129 with twice as many.
+int split(int64_t longest, int64_t total, int64_t units, int set_up, int tiles) {
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int cs = 1; cs <= 8 && cs <= tiles; cs *= 2) {
+    const int64_t t = std::max(((longest + cs - 1) / cs + set_up) * 148, total + units * cs * set_up);
+    if (t < least) {
+      least = t;
+      best = cs;
+    }
+  }
+  return best;
 }
 
 template <typename... K, typename... A>
@@ -579,7 +603,8 @@ cudaError_t fwd(const AttnArgs& a, cudaStream_t st) {
   const bool vec = attn_rows_aligned(a.q, a.sq, a.D, el) && attn_rows_aligned(a.k, a.sk, a.D, el) &&
                    attn_rows_aligned(a.v, a.sv, a.D, el);
   const int nq = cdiv(a.Tq, kBT), nk = cdiv(a.Tk, kBT);
-  const int cs = split(nk, (int64_t)a.B * a.H * nq * nk, nk);
+  const int64_t units = (int64_t)a.B * a.H * nq;
+  const int cs = split(nk, units * nk, units, 2, nk);  // in tiles
   return launch_split(attn_fwd_simt<T, DP>, dim3(nq * cs, a.H, a.B), cs, smem, st, a, cs, vec);
 }
 
@@ -590,10 +615,12 @@ cudaError_t bwd(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
   const bool vec = attn_rows_aligned(a.q, a.sq, a.D, el) && attn_rows_aligned(a.k, a.sk, a.D, el) &&
                    attn_rows_aligned(a.v, a.sv, a.D, el) && attn_rows_aligned(a.dout, a.sdo, a.D, el);
   const int nk = cdiv(a.Tk, kBT), nq = cdiv(a.Tq, kBT);
-  // Four products a tile for the keys' gradients, three for the queries'.
+  // In products: four a tile for the keys' gradients, three for the queries'.
   const int g = a.H / a.Hkv;
-  const int cs = split(std::max(4 * g * nq, 3 * nk), (int64_t)7 * a.B * a.H * nq * nk, std::max(nq, nk));
-  return launch_split(attn_bwd_simt<T, DP>, dim3((nk + nq) * cs, a.H, a.B), cs, smem, st, a, ws, nk, cs, vec);
+  const int64_t units = ((int64_t)nk * a.Hkv + (int64_t)nq * a.H) * a.B;
+  const int cs = split(std::max(4 * (int64_t)g * nq, 3 * (int64_t)nk), (int64_t)7 * a.B * a.H * nq * nk, units, 4,
+                       std::max(nq, nk));
+  return launch_split(attn_bwd_simt<T, DP>, dim3((unsigned)(units * cs)), cs, smem, st, a, ws, nk, cs, vec);
 }
 
 template <typename T>

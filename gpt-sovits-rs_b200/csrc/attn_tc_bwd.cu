@@ -31,6 +31,18 @@
 // lost as a second operand of each product (1.0 to 1.1 times): their launches
 // wait more than they multiply, so it costs 1 to 7 % there against 14 to 18 %
 // on long ones.  The near values always take both parts.
+//
+// Tiles come by TMA where rows are 16-byte vectors, else by cp.async (372
+// against 670 us on the first case below).
+//
+// Measured on B200, bf16.  2 x 16 heads of 64, 4096 causal tokens: 347 us (and
+// 25 for the row pass), 495 TFLOP/s of the five products, 694 of the seven; a
+// key or query tile takes its softmax warps longer (two TMEM reads, one
+// exponential and eight further operations a score, two stores) than the MMAs,
+// which they wait for in turn.  16 utterances of up to 500 frames, 2 heads of
+// 96, window 4: 28 us (12 for the rows, 3.6 for the relative sums); a block
+// has 2 to 8 tiles there, so set-up, the first loads and the relative terms
+// are half of it.
 #include <algorithm>
 
 #include "attn_launch.h"

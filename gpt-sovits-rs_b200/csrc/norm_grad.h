@@ -1,5 +1,5 @@
 // norm_grad.h -- descriptor and launchers of the residual LayerNorm operators
-// (gsvdec_add_norm_forward / _backward; kernels in norm_grad.cu).
+// (gsvdec_norm_*; kernels in norm_grad.cu).
 //
 // Per frame, over C channels:  s = x + y,  xh = (s - mean) rstd,
 //   out = xh gamma + beta

@@ -93,6 +93,8 @@ int attn_shape(const gsvdec_attention* a, AttnArgs& o) {
   if (a->B < 1 || a->B > 65535 || a->H < 1 || a->H > 65535 || a->Hkv < 1 || a->H % a->Hkv)
     return set_err(GSV_E_INVALID_ARG, "attention: B %d, H %d, Hkv %d (1 .. 65535, H a multiple of Hkv)", a->B, a->H,
                    a->Hkv);
+  if ((int64_t)a->B * a->H > 1 << 24)  // heads times tiles is a launch's number of blocks
+    return set_err(GSV_E_INVALID_ARG, "attention: B * H = %lld (up to 2^24)", (long long)a->B * a->H);
   if (a->Tq < 0 || a->Tk < 0 || a->Tq > (1 << 24) || a->Tk > (1 << 24))
     return set_err(GSV_E_INVALID_ARG, "attention: Tq %d, Tk %d (0 .. 2^24)", a->Tq, a->Tk);
   if (a->D < 1 || a->D > kAttnMaxD)

@@ -421,7 +421,7 @@ int gsvdec_workspace_bytes(const gsvdec_t* h, int64_t* bytes);
  * arithmetic accumulates in fp32 and each output is rounded once to dtype. */
 typedef struct gsvdec_attention {
   int dtype;      /* GSV_DTYPE_* of every tensor but lse */
-  int B, H, Hkv;  /* H a multiple of Hkv */
+  int B, H, Hkv;  /* 1 .. 65535, H a multiple of Hkv, B H up to 2^24 */
   int Tq, Tk;     /* may be 0 */
   int D;          /* channels per head, 1 .. 128 */
   int window;     /* w in 0 .. 15, or -1: no relative terms */
@@ -451,7 +451,7 @@ typedef struct gsvdec_attention {
  * sizes, dtype, window and causal of *a alone.  May be 0 bytes. */
 int gsvdec_attention_workspace(const gsvdec_attention* a, int backward, size_t* bytes);
 int gsvdec_attention_forward(const gsvdec_attention* a, int device, void* stream);
-/* Every gradient element is summed by one thread in a fixed order: equal
+/* Every gradient element is summed in a fixed order, without atomics: equal
  * inputs give equal bits. */
 int gsvdec_attention_backward(const gsvdec_attention* a, int device, void* stream);
 

@@ -124,3 +124,12 @@ def test_workspace_sizes(ops):
         assert n.value >= 4 * a.B * a.H * T * 2  # 64-bit arithmetic at the largest sizes
         assert lib.gsvdec_norm_workspace(ctypes.byref(norm(o, T=min(T, 1 << 20))), ctypes.byref(n)) == 0
         assert n.value >= 2 * 16 * 4
+
+
+def test_more_heads_than_a_launch_has_blocks_are_refused(ops):
+    o, lib = ops
+    a = attention(o, B=65535, H=512, Hkv=512)
+    n = ctypes.c_size_t()
+    assert lib.gsvdec_attention_forward(ctypes.byref(a), 0, None) == -1
+    assert lib.gsvdec_attention_backward(ctypes.byref(a), 0, None) == -1
+    assert lib.gsvdec_attention_workspace(ctypes.byref(a), 1, ctypes.byref(n)) == -1
