@@ -35,12 +35,12 @@
 // Tiles come by TMA where rows are 16-byte vectors, else by cp.async (372
 // against 670 us on the first case below).
 //
-// Measured on B200, bf16.  2 x 16 heads of 64, 4096 causal tokens: 347 us (and
-// 25 for the row pass), 495 TFLOP/s of the five products, 694 of the seven; a
+// Measured on B200, bf16.  2 x 16 heads of 64, 4096 causal tokens: 330 us (and
+// 25 for the row pass), 520 TFLOP/s of the five products, 730 of the seven; a
 // key or query tile takes its softmax warps longer (two TMEM reads, one
 // exponential and eight further operations a score, two stores) than the MMAs,
 // which they wait for in turn.  16 utterances of up to 500 frames, 2 heads of
-// 96, window 4: 28 us (12 for the rows, 3.6 for the relative sums); a block
+// 96, window 4: 25 us (12 for the rows, 3.6 for the relative sums); a block
 // has 2 to 8 tiles there, so set-up, the first loads and the relative terms
 // are half of it.
 #include <algorithm>
@@ -154,14 +154,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
   float* tables = reinterpret_cast<float*>(smem_raw + (base - raw) + 2 * C::tileA + ST * C::stage + C::relk);
   const uint32_t sTab = smem_u32(tables);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int b = blockIdx.z, D = a.D, g = a.H / a.Hkv;
-  const bool keys = (int)blockIdx.x < nk;
-  if (keys && (int)blockIdx.y >= a.Hkv) return;
-  const int hk = keys ? blockIdx.y : blockIdx.y / g;
+  // The keys' blocks, which do more, come first; tiles slowest, the longest ones of a causal call first
+  // (head by head, the two cases above took 17 and 2.6 us longer).
+  const int D = a.D, g = a.H / a.Hkv, nq = cdiv(a.Tq, kBA), kblocks = nk * a.Hkv * a.B;
+  const bool keys = (int)blockIdx.x < kblocks;
+  const int unit = keys ? blockIdx.x : blockIdx.x - kblocks, hn = keys ? a.Hkv : a.H, tile = unit / (hn * a.B);
+  const int b = (unit - tile * hn * a.B) / hn, head = unit % hn, hk = keys ? head : head / g;
   const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk), off = kl - ql;
   static_assert(kBB == kRowBlock && kBA == 2 * kRowBlock, "a tile's row values are whole runs of the workspace");
   // First row of the resident tiles; streamed tiles of each head, and their number in all.
-  const int r0 = keys ? blockIdx.x * kBA : (int)(gridDim.x - 1 - blockIdx.x) * kBA;
+  const int r0 = (keys ? tile : nq - 1 - tile) * kBA;
   int first = 0, per = 0, heads = 1;
   if (keys) {
     heads = g;
@@ -172,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
     per = last < r0 ? 0 : cdiv(allowed_keys(last, ql, kl, a.causal), kBB);
   }
   const int nt = per * heads;
-  const int64_t bh0 = (int64_t)b * a.H + (keys ? hk * g : blockIdx.y);  // first head
+  const int64_t bh0 = (int64_t)b * a.H + (keys ? hk * g : head);  // first head
   volatile int* abort = &s_abort;
   auto bar = [&](const uint64_t& m) { return smem_u32(&m); };
 
@@ -322,9 +324,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         const uint32_t rel_bytes = REL && !keys ? 2u * 2 * kBB * a.nrel * 4 : 0;
         mbar_expect_tx(a_full, (full_a ? 2 * C::tileA : 0) + rel_bytes);
         if (full_a) {
-          const int h = keys ? hk : (int)blockIdx.y;
-          tma_tile<DP>(sA0, C::chunkA, keys ? maps.ka : maps.qa, a_full, r0, h, b);
-          tma_tile<DP>(sA1, C::chunkA, keys ? maps.va : maps.ga, a_full, r0, h, b);
+          tma_tile<DP>(sA0, C::chunkA, keys ? maps.ka : maps.qa, a_full, r0, head, b);
+          tma_tile<DP>(sA1, C::chunkA, keys ? maps.va : maps.ga, a_full, r0, head, b);
         }
         if (REL && !keys) bulk_copy(sTab, rel_at(ws, bh0, r0, a.nrel), rel_bytes, a_full);
       }
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
           load_tile<T, DP, kBA>(sA0, C::chunkA, k + (int64_t)r0 * a.sk.t, a.sk.t, kl - r0, D, vec, tid);
           load_tile<T, DP, kBA>(sA1, C::chunkA, v + (int64_t)r0 * a.sv.t, a.sv.t, kl - r0, D, vec, tid);
         } else {
-          const int h = blockIdx.y;
+          const int h = head;
           load_tile<T, DP, kBA>(sA0, C::chunkA, q + h * a.sq.h + (int64_t)r0 * a.sq.t, a.sq.t, ql - r0, D, vec, tid);
           load_tile<T, DP, kBA>(sA1, C::chunkA, dout + h * a.sdo.h + (int64_t)r0 * a.sdo.t, a.sdo.t, ql - r0, D, vec,
                                 tid);
@@ -590,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         }
       } else {
         const int n = allowed_keys(own, ql, kl, a.causal);
-        T* out = static_cast<T*>(a.dq) + b * a.sdq.b + blockIdx.y * a.sdq.h + (int64_t)own * a.sdq.t;
+        T* out = static_cast<T*>(a.dq) + b * a.sdq.b + head * a.sdq.h + (int64_t)own * a.sdq.t;
 #pragma unroll 1
         for (int c = wg * 32; c < DP; c += 64) {
           float o[32] = {};
@@ -602,8 +603,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         }
         if (REL) {
           // Lane = channel; group 0: drelk, group 1: drelv.
-          const int64_t tile = ((int64_t)b * a.H + blockIdx.y) * ((int)gridDim.x - nk) + r0 / kBA;
-          float* part = ws.part + (tile * 2 + wg) * a.nrel * D + row;
+          const int64_t at = ((int64_t)b * a.H + head) * nq + r0 / kBA;
+          float* part = ws.part + (at * 2 + wg) * a.nrel * D + row;
           const float f = wg == 0 ? inv : exp2f(-kShift);
           for (int q0 = 0; q0 < a.nrel; q0 += 16) {
             float v[16] = {};
@@ -649,7 +650,8 @@ cudaError_t launch(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
              map_rows(&m.vb, a.v, a.ty, a.sv, a.B, a.Hkv, a.Tk, a.D, kBB);
   }
   const PdlScope pdl(a.Tq > 0);  // its set-up runs beside the end of the row pass
-  return launch_k(attn_bwd_tc<T, DP, REL>, dim3(nk + nq, a.H, a.B), kThreads, smem, st, a, ws, m, nk, fine, vec, ovec);
+  const unsigned blocks = (unsigned)(((int64_t)nk * a.Hkv + (int64_t)nq * a.H) * a.B);
+  return launch_k(attn_bwd_tc<T, DP, REL>, blocks, kThreads, smem, st, a, ws, m, nk, fine, vec, ovec);
 }
 
 template <typename T, int DP>
