@@ -29,17 +29,18 @@
 // block for its share of the rows, through distributed shared memory (rank
 // order, one launch, no workspace).
 //
-// Tiles whose rows are 16-byte vectors come by TMA, others by cp.async: 219
-// against 247 us on the first case below.
+// Tiles whose rows are 16-byte vectors come by TMA, others by cp.async, which
+// took 13 % longer on the first case below.
 //
-// Measured on B200, bf16.  4 x 16 heads of 64, 4096 causal tokens: 219 us, 625
-// TFLOP/s, 38 % of a large matrix product's rate.  The exponentials bound it
-// (their pipe is 67 % busy: 16 a cycle and SM, one per score, where the two
-// products take 8 cycles for as many), with the hand-offs between the softmax
-// and MMA warps; a quarter of the exponentials as a polynomial took 15 us
-// longer, since issue slots run short as well.  16 utterances of up to 500
-// frames, 2 heads of 96, window 4: 14.2 us, two thirds of it launch, first
-// loads and the relative terms.
+// Measured on B200, bf16.  4 x 16 heads of 64, 4096 causal tokens: 198 us, 695
+// TFLOP/s, 42 % of a large matrix product's rate.  The exponentials bound it (16
+// a cycle and SM, one per score: 120 us of that pipe, where the two products
+// take half of it), with the hand-offs between the softmax and MMA warps; a
+// quarter of the exponentials as a polynomial took 15 us longer, since issue
+// slots run short as well.  Blocks ordered head by head instead of the longest
+// rows of all heads first: 219 us.  16 utterances of up to 500 frames, 2 heads
+// of 96, window 4: 14.9 us, two thirds of it launch, first loads and the
+// relative terms.
 #include "attn_launch.h"
 #include "attn_tc.cuh"
 
@@ -89,9 +90,9 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
   const uint32_t sQ = base, sK = sQ + C::tile, sV = sK + ST * C::tile;
   float* tab = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + C::smem);  // [nrel][128]
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  // Long rows of a causal mask first, so that the last blocks are short ones.
-  const int rank = blockIdx.x % cs;
-  const int i0 = (int)(gridDim.x - 1 - blockIdx.x) / cs * kBM, h = blockIdx.y, b = blockIdx.z;
+  // Long rows of a causal mask first, of all heads, so that the last blocks are short ones.
+  const int rank = blockIdx.x % cs, unit = blockIdx.x / cs, tile = unit / (a.H * a.B);
+  const int i0 = (cdiv(a.Tq, kBM) - 1 - tile) * kBM, bh = unit - tile * a.H * a.B, b = bh / a.H, h = bh - b * a.H;
   const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk), off = kl - ql;
   const int last = min(i0 + kBM, ql) - 1;
   const int kend = last < i0 ? 0 : allowed_keys(last, ql, kl, a.causal);
@@ -556,7 +557,7 @@ cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
   int cs = 1;
   while (cs < 8 && 2 * cs <= nk && (int64_t)nq * a.H * a.B * 2 * cs <= sm_count() * (nk / (2 * cs) >= 8 ? 2 : 1)) cs *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(nq * cs, a.H, a.B);
+  cfg.gridDim = dim3((unsigned)((int64_t)nq * a.H * a.B * cs));
   cfg.blockDim = dim3(kFwdThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
