@@ -124,6 +124,14 @@ def _need(name, t, shape, dtype, index, contiguous=False) -> int:
     return t.data_ptr()
 
 
+def _tensor(name, t, shape, dtype, index):
+    """Checks one tensor; returns its address and strides (each of torch's accessors costs as much as the checks)."""
+    s = t.stride()
+    if t.shape == shape and t.dtype is dtype and t.get_device() == index and s[-1] == 1:
+        return t.data_ptr(), s
+    return _need(name, t, shape, dtype, index), s
+
+
 def _first(name, t, ndim) -> int:
     if not t.is_cuda or t.dim() != ndim:
         raise ValueError(f"{name} must be a CUDA tensor with {ndim} axes")
@@ -138,7 +146,7 @@ def _code(c, t) -> int:
 
 
 def _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v):
-    """The checked inputs: (leading fields, addresses and strides up to rel_v, device index)."""
+    """The checked inputs: (leading fields, addresses and strides up to rel_v, device index, strides of q, k, v)."""
     index = _first("q", q, 4)
     code, t = _code(c, q), q.dtype
     qs = q.shape
@@ -149,7 +157,9 @@ def _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
     Hkv, Tk = ks[1], ks[2]
     if ks[0] != B or ks[3] != D:
         raise ValueError(f"k must be [{B}, heads, T, {D}], not {list(ks)}")
-    pq, pk, pv = _need("q", q, qs, t, index), _need("k", k, ks, t, index), _need("v", v, ks, t, index)
+    pq, sq = _tensor("q", q, qs, t, index)
+    pk, sk = _tensor("k", k, ks, t, index)
+    pv, sv = _tensor("v", v, ks, t, index)
     ql = 0 if q_lengths is None else _need("q_lengths", q_lengths, (B,), c.i32, index, True)
     kl = 0 if k_lengths is None else _need("k_lengths", k_lengths, (B,), c.i32, index, True)
     window, rk, rv = -1, 0, 0
@@ -164,7 +174,8 @@ def _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
     lead = (code, B, H, Hkv, Tq, Tk, D, window, 1 if causal else 0)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
-    return lead, (scale, ql, kl, pq, pk, pv, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], rk, rv), index
+    given = (scale, ql, kl, pq, pk, pv, sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], rk, rv)
+    return lead, given, index, (qs, ks, sq, sk, sv)
 
 
 def _rows(c, dtype, n, m, device):
@@ -183,10 +194,13 @@ def _same(c, x):
     return t, m * n, n
 
 
-def _heads_last(c, t, B, H, T, D, device):
-    """A new [B, H, T, D] tensor in [B, T, H, D] memory order, and its strides."""
-    s = (T * H * D, D, H * D)
-    return c.empty_strided((B, H, T, D), (*s, 1), dtype=t, device=device), s
+def _heads_last(c, like, strides, B, H, T, D):
+    """A new [B, H, T, D] tensor of like's type in [B, T, H, D] memory order, and its strides."""
+    row = H * D
+    s = (T * row, D, row, 1)
+    if s == strides:  # like is in that order, and empty_like keeps it
+        return c.empty_like(like), s
+    return c.empty_strided((B, H, T, D), s, dtype=like.dtype, device=like.device), s
 
 
 def attention(q, k, v, *, scale: Optional[float] = None, causal: bool = False, q_lengths=None, k_lengths=None,
@@ -205,14 +219,14 @@ def attention(q, k, v, *, scale: Optional[float] = None, causal: bool = False, q
     order; lse [B, H, Tq] fp32 is the log-sum-exp of each row's scores.
     """
     c = _get()
-    lead, given, index = _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
+    lead, given, index, (_, _, sq, _, _) = _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
     code, B, H, _, Tq, _, D = lead[:7]
     dev = q.device
-    o, so = _heads_last(c, q.dtype, B, H, Tq, D, dev)
+    o, so = _heads_last(c, q, sq, B, H, Tq, D)
     lse = c.empty_strided((B, H, Tq), (H * Tq, Tq, 1), dtype=c.f32, device=dev)
     n = _attention_workspace(0, *lead)
     ws = _line(c, c.u8, n, dev) if n else None
-    a = _ATTENTION.pack(*lead, *given, o.data_ptr(), *so, lse.data_ptr(), 0, *_Z3, 0, 0, 0, *_Z3, *_Z3, *_Z3, 0, 0,
+    a = _ATTENTION.pack(*lead, *given, o.data_ptr(), *so[:3], lse.data_ptr(), 0, *_Z3, 0, 0, 0, *_Z3, *_Z3, *_Z3, 0, 0,
                         ws.data_ptr() if n else 0, n)
     rc = c.attention_forward(a, index, c.stream(index))
     if rc:
@@ -230,24 +244,26 @@ def attention_backward(do, q, k, v, o, lse, *, scale: Optional[float] = None, ca
     relative rows are summed in fp32 and rounded once) and is bit-reproducible.
     """
     c = _get()
-    lead, given, index = _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
+    lead, given, index, (qs, _, sq, sk, sv) = _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k,
+                                                            rel_v)
     code, B, H, Hkv, Tq, Tk, D, window = lead[:8]
-    t, qs = q.dtype, q.shape
-    pdo, po = _need("do", do, qs, t, index), _need("o", o, qs, t, index)
-    pl = _need("lse", lse, qs[:3], c.f32, index, True)
+    t = q.dtype
+    pdo, sdo = _tensor("do", do, qs, t, index)
+    po, so = _tensor("o", o, qs, t, index)
+    pl = _need("lse", lse, (B, H, Tq), c.f32, index, True)
     dev = q.device
-    dq, sq = _heads_last(c, t, B, H, Tq, D, dev)
-    dk, sk = _heads_last(c, t, B, Hkv, Tk, D, dev)
-    dv, _ = _heads_last(c, t, B, Hkv, Tk, D, dev)
+    dq, sq = _heads_last(c, q, sq, B, H, Tq, D)
+    dk, sk = _heads_last(c, k, sk, B, Hkv, Tk, D)
+    dv, sv = _heads_last(c, v, sv, B, Hkv, Tk, D)
     drk = drv = None
     prk = prv = 0
     if window >= 0:
-        drk, drv = _rows(c, t, 2 * window + 1, D, dev), _rows(c, t, 2 * window + 1, D, dev)
+        drk, drv = c.empty_like(rel_k), c.empty_like(rel_v)
         prk, prv = drk.data_ptr(), drv.data_ptr()
     n = _attention_workspace(1, *lead)
     ws = _line(c, c.u8, n, dev)
-    a = _ATTENTION.pack(*lead, *given, po, *o.stride()[:3], pl, pdo, *do.stride()[:3], dq.data_ptr(), dk.data_ptr(),
-                        dv.data_ptr(), *sq, *sk, *sk, prk, prv, ws.data_ptr(), n)
+    a = _ATTENTION.pack(*lead, *given, po, *so[:3], pl, pdo, *sdo[:3], dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                        *sq[:3], *sk[:3], *sv[:3], prk, prv, ws.data_ptr(), n)
     rc = c.attention_backward(a, index, c.stream(index))
     if rc:
         c.check(rc)
@@ -273,10 +289,10 @@ def _norm_in(c, x, y, lengths, layout):
     if lay is None:
         raise ValueError(f"layout must be one of {sorted(LAYOUTS)}")
     B, C, T = xs if lay == 0 else (xs[0], xs[2], xs[1])
-    px = _need("x", x, xs, t, index)
-    py, sy = (0, (0, 0)) if y is None else (_need("y", y, xs, t, index), y.stride()[:2])
+    px, sx = _tensor("x", x, xs, t, index)
+    py, sy = (0, (0, 0)) if y is None else _tensor("y", y, xs, t, index)
     ln = 0 if lengths is None else _need("lengths", lengths, (B,), c.i32, index, True)
-    return (code, lay, B, C, T), (ln, px, py, *x.stride()[:2], *sy), index
+    return (code, lay, B, C, T), (ln, px, py, sx[0], sx[1], sy[0], sy[1]), index
 
 
 def add_norm(x, y, gamma, beta, *, lengths=None, layout: str = "bct", eps: float = 1e-5):
@@ -295,7 +311,8 @@ def add_norm(x, y, gamma, beta, *, lengths=None, layout: str = "bct", eps: float
     pg, pb = _need("gamma", gamma, (C,), c.f32, index, True), _need("beta", beta, (C,), c.f32, index, True)
     dev = x.device
     out, s0, s1 = _same(c, x)
-    mean, rstd = _rows(c, c.f32, B, T, dev), _rows(c, c.f32, B, T, dev)
+    mean = _rows(c, c.f32, B, T, dev)
+    rstd = c.empty_like(mean)
     a = _NORM.pack(*lead, eps, *given, pg, pb, mean.data_ptr(), rstd.data_ptr(), out.data_ptr(), s0, s1, 0, 0,
                    0, 0, 0, 0, 0, 0, 0, 0)
     rc = c.norm_forward(a, index, c.stream(index))
@@ -312,14 +329,14 @@ def add_norm_backward(d_out, x, y, gamma, mean, rstd, *, lengths=None, layout: s
     lead, given, index = _norm_in(c, x, y, lengths, layout)
     B, C, T = lead[2:]
     pg = _need("gamma", gamma, (C,), c.f32, index, True)
-    pd = _need("d_out", d_out, x.shape, x.dtype, index)
+    pd, sd = _tensor("d_out", d_out, x.shape, x.dtype, index)
     pm, pr = _need("mean", mean, (B, T), c.f32, index, True), _need("rstd", rstd, (B, T), c.f32, index, True)
     dev = x.device
     dx, s0, s1 = _same(c, x)
-    dgamma, dbeta = _line(c, c.f32, C, dev), _line(c, c.f32, C, dev)
+    dgamma, dbeta = c.empty_like(gamma), c.empty_like(gamma)
     n = _norm_workspace(*lead)
     ws = _line(c, c.u8, n, dev)
-    a = _NORM.pack(*lead, 0.0, *given, pg, 0, pm, pr, 0, 0, 0, pd, dx.data_ptr(), *d_out.stride()[:2],
+    a = _NORM.pack(*lead, 0.0, *given, pg, 0, pm, pr, 0, 0, 0, pd, dx.data_ptr(), sd[0], sd[1],
                    s0, s1, dgamma.data_ptr(), dbeta.data_ptr(), ws.data_ptr(), n)
     rc = c.norm_backward(a, index, c.stream(index))
     if rc:
