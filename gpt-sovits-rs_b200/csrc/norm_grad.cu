@@ -577,7 +577,9 @@ __global__ void __launch_bounds__(512) norm_part_sum(const float* part, int bloc
 
 // Threads that share a frame, and channels per thread.  The forward holds 32
 // channels a thread (one warp per frame up to 1024), the backward 16, since it
-// also holds gamma and two sums for each.
+// also holds gamma and two sums for each (bf16 [8][4096][1024] backward: 64
+// threads of 16 channels 60 us, 128 of 8 in three blocks per SM 72, 32 of 32 in
+// one block 69).
 struct RowShape {
   int R, E;
 };
