@@ -177,6 +177,16 @@ def test_nothing_to_do(gsv, dtype):
     run_and_check(gsv, x)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("Tq,Tk,ql,kl", [(0, 40, 0, 40), (40, 0, 40, 0), (40, 40, 0, 40), (40, 40, 40, 0), (1, 1, 1, 0)])
+def test_nothing_to_do_on_used_memory(gsv, dtype, Tq, Tk, ql, kl):
+    # Workspace and outputs come from memory that held NaN.
+    used = [torch.full((n,), float("nan"), device="cuda") for n in [64, 256, 1024, 4096, 16384, 65536, 1 << 20] * 6]
+    x = make(dtype, 2, 2, 1, Tq, Tk, 40, w=1)
+    del used
+    run_and_check(gsv, x, q_lengths=lengths(ql, ql), k_lengths=lengths(kl, kl))
+
+
 def test_infinite_scores_stay_in_their_row(gsv):
     x = make("bf16", 1, 1, 1, 140, 140, 64)
     x["q"][0, 0, 5] = float("inf")
