@@ -134,12 +134,11 @@ __global__ void __launch_bounds__(kRowThreads, BWD && E > 16 ? 1 : 2) norm_rows(
   const int frames = a.B * a.T, step = gridDim.x * G;
   int flip = 0;
   if (kRing) {
-    if (tid == 0)
+    if (tid == 0) {
       for (int s = 0; s < stages; ++s) mbar_init(smem_u32(&s_bar[grp][s]), 1);
-    if (threadIdx.x == 0) {
-      s_abort = 0;
-      fence_async_smem();
+      fence_async_smem();  // by the lane that wrote them: a fence orders its own thread's writes only
     }
+    if (threadIdx.x == 0) s_abort = 0;
     __syncthreads();
   }
   float ga[E], be[E];  // backward: be accumulates dbeta, dg dgamma

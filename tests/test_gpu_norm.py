@@ -211,3 +211,24 @@ def test_refusals(gsv):
         with pytest.raises(gsv.GsvDecError) as e:
             gsv.add_norm(torch.zeros(shape, device="cuda"), None, w, w, layout=layout)
         assert e.value.status == "GSV_E_INVALID_ARG"
+
+
+@pytest.mark.parametrize("dtype,layout,B,C,T", [
+    # Rings of 2 .. 8 stages that are filled several times over, with frames left out among the others.
+    ("bf16", "btc", 8, 1024, 4096), ("fp16", "btc", 5, 2048, 1700), ("fp32", "btc", 1, 8192, 3000),
+    ("fp32", "btc", 3, 4096, 1000), ("fp32", "btc", 4, 192, 12000), ("bf16", "btc", 6, 8, 9000),
+    ("fp16", "btc", 3, 515, 4000),
+    # Clusters that take several tiles each, by vectors and by single frames.
+    ("bf16", "bct", 8, 700, 1600), ("bf16", "bct", 8, 700, 1601), ("fp32", "bct", 4, 2048, 2500),
+    ("fp32", "bct", 4, 2048, 2499), ("fp16", "bct", 9, 192, 4002), ("fp32", "bct", 16, 300, 1000)])
+def test_many_frames_a_block(gsv, dtype, layout, B, C, T):
+    x = make(dtype, layout, B, C, T)
+    n = torch.tensor([T, T // 3, 0, T - 1, 1, T, 2 * T // 3, 33, T][:B], dtype=torch.int32, device="cuda") \
+        if B < 10 else torch.arange(B, dtype=torch.int32, device="cuda") * T // (B - 1)
+    if B == 1:
+        n -= 5
+    for b, m in enumerate(n.tolist()):
+        for name in ("x", "y", "d_out"):
+            (x[name][b, :, m:] if layout == "bct" else x[name][b, m:]).fill_(float("nan"))
+    run_and_check(gsv, x, layout, n)
+    gsv.ops_status()
