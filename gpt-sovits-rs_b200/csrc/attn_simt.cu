@@ -583,7 +583,8 @@ int split(int64_t longest, int64_t total, int64_t units, int set_up, int tiles) 
 
 template <typename... K, typename... A>
 cudaError_t launch_split(void (*kern)(K...), dim3 grid, int cs, size_t smem, cudaStream_t st, A... args) {
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  int regs;
+  const cudaError_t e = kernel_setup(kern, smem, &regs);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
