@@ -12,6 +12,8 @@
 #include <cstring>
 #include <mutex>
 
+#include "kernel_setup.h"
+
 namespace gsv {
 namespace {
 
@@ -339,10 +341,6 @@ int smem_per_sm() {
   return cached[dev];
 }
 
-// Launch setup of a kernel done once per (kernel, device) instead of per
-// launch: the shared-memory carveout, the register count, and the dynamic
-// shared-memory limit (raised only when a launch needs more).  Short launches
-// (the flow's) were bound by these host calls.
 // Dynamic shared memory for a launch meant to hold per_sm CTAs per SM: smem,
 // padded where needed so that per_sm + 1 CTAs (1 KB reserved each) do not fit
 // the SM's shared memory.  A persistent grid of sm_count x per_sm CTAs then
@@ -355,52 +353,6 @@ size_t pad_smem_to_occupancy(size_t smem, int per_sm, int smem_sm) {
   const size_t pad = floor_excl > 1024 ? floor_excl - 1024 : 0;
   const size_t out = std::max(smem, pad);
   return out <= 227 * 1024 ? out : smem;
-}
-
-// Slots per device and kernel signature: every instantiation of a kernel
-// template shares one signature, and the tap GEMM has a few dozen.
-constexpr int kSetupSlots = 64;
-
-template <typename K>
-cudaError_t kernel_setup(K kern, size_t smem, int* regs) {
-  struct Entry {
-    int regs = 0, smem = 0;
-    bool ready = false;
-  };
-  static std::mutex mu;
-  static Entry table[64][kSetupSlots];
-  static const void* keys[64][kSetupSlots] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  std::lock_guard<std::mutex> lock(mu);
-  Entry* en = nullptr;
-  for (int i = 0; i < kSetupSlots && !en; ++i) {
-    if (keys[dev][i] == (const void*)kern) en = &table[dev][i];
-    else if (!keys[dev][i]) {
-      keys[dev][i] = (const void*)kern;
-      en = &table[dev][i];
-    }
-  }
-  Entry scratch;
-  if (!en) en = &scratch;  // more instantiations than slots on one device: no caching
-  if (!en->ready) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                         cudaSharedmemCarveoutMaxShared);
-    if (e != cudaSuccess) return e;
-    cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, kern);
-    if (e != cudaSuccess) return e;
-    en->regs = fa.numRegs;
-    en->ready = true;
-  }
-  if ((int)smem > en->smem) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    en->smem = (int)smem;
-  }
-  *regs = en->regs;
-  return cudaSuccess;
 }
 
 }  // namespace

@@ -65,3 +65,33 @@ def test_attention_with_and_without_a_window(gsv, monkeypatch, dtype, D):
     assert together(jobs, 10000) == []
     for out, want in kept:
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_norms_of_other_widths_after_every_kernel_was_used(gsv, monkeypatch):
+    # All kernels of the [B, T, C] norm (3 types, aligned or single elements, 6 shares of a row, both directions),
+    # then pairs of widths that one of them serves.
+    shares = [(256, 24), (512, 264), (1024, 520), (2048, 1032), (4096, 2056), (8192, 4104)]
+
+    def step(x, w):
+        out, mean, rstd = gsv.add_norm(x, x, w, w, layout="btc")
+        return (out, mean, rstd) + gsv.add_norm_backward(x, x, x, w, mean, rstd, layout="btc"), x, w
+
+    pairs = []
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        for off in (1, 0):
+            for widths in shares:
+                pair = []
+                for C in widths:
+                    x, w = torch.randn(1, 9, C + off, device="cuda").to(dtype)[..., off:], torch.randn(C, device="cuda")
+                    made, kept = recorded(monkeypatch, gsv, lambda: step(x, w))
+                    # The backward's workspace was torch's to give away when the call returned.
+                    ws = torch.empty(gsv.ops._norm_workspace(*gsv.ops._norm_in(gsv.ops._get(), x, x, None, "btc")[0]),
+                                     dtype=torch.uint8, device="cuda")
+                    f, a, index = made[1]
+                    made[1] = (f, a[:-16] + ws.data_ptr().to_bytes(8, "little") + a[-8:], index)
+                    pair.append((made, kept, ws, [t.clone() for t in kept[0]]))
+                pairs.append(pair)
+    for pair in pairs:
+        assert together([p[0] for p in pair], 2000) == []
+        for _, kept, _, want in pair:
+            assert all(torch.equal(a, b) for a, b in zip(kept[0], want))
