@@ -182,7 +182,8 @@ __global__ void __launch_bounds__(kRowThreads, BWD && E > 16 ? 1 : 2) norm_rows(
     int b, t;
     const bool ok = valid(f, b, t);
     float v[E], g[BWD ? E : 1];
-    const float mean = mean_next;
+    // Statistics behind a length may hold anything, as the frames do.
+    const float mean = ok ? mean_next : 0.f;
     float rstd = ok ? rstd_next : 0.f;
     if (BWD && ff + step < frames) {
       mean_next = a.mean[f + step];

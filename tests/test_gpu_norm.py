@@ -232,3 +232,19 @@ def test_many_frames_a_block(gsv, dtype, layout, B, C, T):
             (x[name][b, :, m:] if layout == "bct" else x[name][b, m:]).fill_(float("nan"))
     run_and_check(gsv, x, layout, n)
     gsv.ops_status()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("layout", ["bct", "btc"])
+@pytest.mark.parametrize("C", [192, 515, 600])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_statistics_behind_a_length_are_not_used(gsv, dtype, layout, C, bad):
+    x = make(dtype, layout, 4, C, 77)
+    n = torch.tensor([77, 0, 1, 33], dtype=torch.int32, device="cuda")
+    kw = dict(lengths=n, layout=layout)
+    _, mean, rstd = gsv.add_norm(x["x"], x["y"], x["gamma"], x["beta"], **kw)
+    want = gsv.add_norm_backward(x["d_out"], x["x"], x["y"], x["gamma"], mean, rstd, **kw)
+    for b, m in enumerate(n.tolist()):
+        mean[b, m:] = rstd[b, m:] = bad
+    for a, b in zip(gsv.add_norm_backward(x["d_out"], x["x"], x["y"], x["gamma"], mean, rstd, **kw), want):
+        assert torch.equal(a, b)
