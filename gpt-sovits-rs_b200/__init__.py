@@ -45,7 +45,7 @@ EXPORTS = (
     "gsvdec_forward_multi", "gsvdec_plan_multi", "gsvdec_sync_status", "gsvdec_selftest_wait",
     "gsvdec_set_alloc_fail_after", "gsvdec_workspace_bytes",
     "gsvdec_attention_workspace", "gsvdec_attention_forward", "gsvdec_attention_backward", "gsvdec_ops_status",
-    "gsvdec_encp_attention", "gsvdec_norm_workspace", "gsvdec_norm_forward", "gsvdec_norm_backward",
+    "gsvdec_selftest_attention_wait", "gsvdec_encp_attention", "gsvdec_norm_workspace", "gsvdec_norm_forward", "gsvdec_norm_backward",
 )
 
 # EncP encoder stacks (GSV_ENCP_SSL / _TEXT / _2), by their enc_p.* names.
@@ -127,6 +127,7 @@ def library(path: Optional[Path] = None) -> ctypes.CDLL:
     lib.gsvdec_plan_multi.argtypes = [vp, i, i, i, vp, vp]
     lib.gsvdec_sync_status.argtypes = [vp, vp]
     lib.gsvdec_selftest_wait.argtypes = [vp, ctypes.c_int64, vp]
+    lib.gsvdec_selftest_attention_wait.argtypes = [vp, i, ctypes.c_int64, vp]
     lib.gsvdec_set_alloc_fail_after.argtypes = [i]
     lib.gsvdec_workspace_bytes.argtypes = [vp, ctypes.POINTER(ctypes.c_int64)]
     ops.declare(lib)
@@ -328,6 +329,15 @@ class Decoder:
             import torch
             stream = torch.cuda.current_stream(self.info["device"]).cuda_stream
         _check(library().gsvdec_selftest_wait(self._h, int(limit_ns), ctypes.c_void_p(stream)))
+
+    def selftest_attention_wait(self, limit_ns: int = 1_000_000, stream=None) -> None:
+        """selftest_wait as the attention of this handle's enc_p calls reports
+        it (gsvdec_selftest_attention_wait)."""
+        if stream is None:
+            import torch
+            stream = torch.cuda.current_stream(self.info["device"]).cuda_stream
+        _check(library().gsvdec_selftest_attention_wait(self._h, self.info["device"], int(limit_ns),
+                                                        ctypes.c_void_p(stream)))
 
     def workspace_bytes(self) -> int:
         """Device bytes held for per-call workspaces (not the weights)."""

@@ -24,6 +24,8 @@
 
 namespace gsv {
 
+int ops_wait_selftest(int device, unsigned long long limit_ns, cudaStream_t st);  // ops_api.cu
+
 enum class Ty { F32 = 0, F16 = 1, BF16 = 2 };  // GSV_DTYPE_*
 
 constexpr int kAttnMaxD = 128;
@@ -46,6 +48,7 @@ struct AttnArgs {
   Str3 sq, sk, sv, so, sdo, sdq, sdk, sdv;
   char* ws;
   size_t ws_bytes;
+  int* err;  // a handle's error word, for its give-ups; null: the operators' own words
 };
 
 // Every row of the tensor starts on a 16-byte boundary and holds whole
@@ -64,5 +67,8 @@ cudaError_t attn_backward(const AttnArgs& a, cudaStream_t st);
 // (backward's) kernels gave up since the last such call on this device.
 cudaError_t attn_fwd_gave_up(int* out, cudaStream_t st);
 cudaError_t attn_bwd_gave_up(int* out, cudaStream_t st);
+// One bounded wait that nothing completes, reported as the forward's kernels
+// report theirs (gsvdec_selftest_attention_wait).
+cudaError_t attn_wait_selftest(const AttnArgs& a, unsigned long long limit_ns, cudaStream_t st);
 
 }  // namespace gsv

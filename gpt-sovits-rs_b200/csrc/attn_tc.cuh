@@ -320,6 +320,14 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, mbar_wait_fast(bar, parity, abort));
 }
 
+constexpr int kAttnCode = 17;  // error code of a give-up in a handle's word
+
+// A bounded wait gave up: said in the handle's word where the call has one.
+__device__ __forceinline__ void give_up(int* handle_word, int* own_word, volatile int* abort) {
+  if (handle_word) raise_err(handle_word, abort, kAttnCode);
+  else raise_err(own_word, abort, 1);
+}
+
 // Waits for the stream, then reads and clears a give-up word.
 cudaError_t take_gave_up(int& word, int* out, cudaStream_t st) {
   void* p = nullptr;

@@ -52,7 +52,7 @@
 namespace gsv {
 namespace {
 
-__device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out
+__device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out in a call without a handle
 
 constexpr int kBA = 128, kBB = 64;  // rows of the resident and of the streamed tiles
 constexpr int kHalfB = kBB / 2;
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         }
       }
       if (lead) mma_commit(bar(bars.acc_full));
-      if (!ok) raise_err(&g_gave_up, abort, 1);
+      if (!ok) give_up(a.err, &g_gave_up, abort);
       warp_wait(bar(bars.acc_full), 0, abort);  // nothing in flight when memory is given back
     } else if (nt > 0 && warp < 11) {
       const int tid = threadIdx.x - 9 * 32;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       }
       ho.flush();
       cp_wait<0>();
-      if (!ok) raise_err(&g_gave_up, abort, 1);
+      if (!ok) give_up(a.err, &g_gave_up, abort);
     }
   } else {
     const int wg = warp >> 2, row = threadIdx.x & 127, own = r0 + row, c0 = wg * kHalfB;
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       }
     }
     if (nt > 0) ok = ok && warp_wait(bar(bars.acc_full), 0, abort);
-    if (!ok) raise_err(&g_gave_up, abort, 1);
+    if (!ok) give_up(a.err, &g_gave_up, abort);
     tc_fence_after();
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {

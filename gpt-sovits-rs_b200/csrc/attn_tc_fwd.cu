@@ -47,7 +47,7 @@
 namespace gsv {
 namespace {
 
-__device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out
+__device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out in a call without a handle
 
 constexpr int kBM = 128, kBN = 128;
 constexpr int kFwdThreads = 256;
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
         if (lead) mma_commit(bar(bars.o_full));
         fin = 1;
       }
-      if (!ok) raise_err(&g_gave_up, abort, 1);
+      if (!ok) give_up(a.err, &g_gave_up, abort);
       // Nothing of this block is in flight when its memory is given back.
       warp_wait(bar(bars.o_full), fin, abort);
     } else if (nt > 0 && warp < 7) {
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
       }
       ho.flush();
       cp_wait<0>();
-      if (!ok) raise_err(&g_gave_up, abort, 1);
+      if (!ok) give_up(a.err, &g_gave_up, abort);
     }
     if (cs > 1) {  // as the softmax warps join the cluster's sums
       cluster_sync();
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
         warp_arrive(bar(bars.p_full));
         ok = warp_wait(bar(bars.o_full), 1, abort);
       }
-      if (!ok) raise_err(&g_gave_up, abort, 1);
+      if (!ok) give_up(a.err, &g_gave_up, abort);
       tc_fence_after();
     }
     T* out = static_cast<T*>(a.o) + b * a.so.b + h * a.so.h;
@@ -534,6 +534,20 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
   }
 }
 
+// A wait that runs out with nothing else in flight in its block.
+__global__ void attn_wait_selftest_kernel(const __grid_constant__ AttnArgs a, const unsigned long long limit_ns) {
+  __shared__ __align__(8) uint64_t s_bar;
+  __shared__ int s_abort;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&s_bar), 1);
+    s_abort = 0;
+    fence_async_smem();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && !mbar_wait_fast(smem_u32(&s_bar), 0, &s_abort, limit_ns))
+    give_up(a.err, &g_gave_up, &s_abort);
+}
+
 template <typename T, int DP, bool REL>
 cudaError_t launch(const AttnArgs& a, cudaStream_t st) {
   const size_t smem = FwdCfg<DP>::smem + 1024 + (size_t)a.nrel * kBM * sizeof(float);
@@ -586,6 +600,11 @@ cudaError_t width(const AttnArgs& a, cudaStream_t st) {
 
 cudaError_t attn_fwd_tensor(const AttnArgs& a, cudaStream_t st) {
   return a.ty == Ty::F16 ? width<__half>(a, st) : width<__nv_bfloat16>(a, st);
+}
+
+cudaError_t attn_wait_selftest(const AttnArgs& a, unsigned long long limit_ns, cudaStream_t st) {
+  attn_wait_selftest_kernel<<<1, 32, 0, st>>>(a, limit_ns);
+  return cudaGetLastError();
 }
 
 cudaError_t attn_fwd_gave_up(int* out, cudaStream_t st) { return take_gave_up(g_gave_up, out, st); }

@@ -2437,6 +2437,14 @@ int encp_add_norm_impl(gsvdec* h, int stack, int layer, int norm, const float* x
   return finish_host(h, st, {{out, od}}, n, mem_kind);
 }
 
+// What every attention call of a handle has in common.
+AttnArgs handle_attention(const gsvdec* h) {
+  AttnArgs a{};
+  a.ty = h->dt == Dt::BF16 ? Ty::BF16 : Ty::F32;
+  a.err = h->d_err;
+  return a;
+}
+
 // The layer's self-attention: q, k, v projections in one grouped launch (time
 // major), the attention on their [B][T][heads][D] rows, conv_o, relayout.
 int encp_attention_impl(gsvdec* h, int stack, int layer, const float* x, const int32_t* lengths, int B, int T,
@@ -2478,8 +2486,7 @@ int encp_attention_impl(gsvdec* h, int stack, int layer, const float* x, const i
     GSV_TRY(run_group(h, g, st, nm + ".conv_qkv", wk));
   }
   const int D = L->D, H = C / D, rel = 2 * L->window + 1;
-  AttnArgs a{};
-  a.ty = h->dt == Dt::BF16 ? Ty::BF16 : Ty::F32;
+  AttnArgs a = handle_attention(h);
   a.B = B;
   a.H = a.Hkv = H;
   a.Tq = a.Tk = T;
@@ -2509,13 +2516,7 @@ int encp_attention_impl(gsvdec* h, int stack, int layer, const float* x, const i
   }
   CUDA_TRY(launch_to_ncl(sc[3], h->dt, B, T, C, od, st));
   GSV_TRY(after_launch(h, st, "encp.output_relayout", 1, 0, 0.0, (4.0 + e) * n));
-  GSV_TRY(finish_host(h, st, {{out, od}}, n, mem_kind));
-  if (mem_kind == GSV_MEM_HOST) {
-    int gave_up = 0;
-    CUDA_TRY(attn_fwd_gave_up(&gave_up, st));
-    if (gave_up) return set_err(GSV_E_TIMEOUT, "a bounded device wait of the attention gave up");
-  }
-  return GSV_OK;
+  return finish_host(h, st, {{out, od}}, n, mem_kind);
 }
 
 // conv_1 + ReLU, conv_2 + residual, norm2 + x_mask + relayout: the FFN half of
@@ -2957,6 +2958,17 @@ int gsvdec_selftest_wait(gsvdec_t* h, int64_t limit_ns, void* stream) {
   GSV_TRY(gsv::take_async_error(h));
   CUDA_TRY(cudaSetDevice(h->device));
   CUDA_TRY(gsv::launch_wait_selftest(h->d_err, (unsigned long long)limit_ns, static_cast<cudaStream_t>(stream)));
+  return GSV_OK;
+}
+
+int gsvdec_selftest_attention_wait(gsvdec_t* h, int device, int64_t limit_ns, void* stream) {
+  if (limit_ns < 1000 || limit_ns > 10000000000ll)
+    return gsv::set_err(GSV_E_INVALID_ARG, "limit_ns %lld outside [1e3, 1e10]", (long long)limit_ns);
+  if (!h) return gsv::ops_wait_selftest(device, (unsigned long long)limit_ns, static_cast<cudaStream_t>(stream));
+  GSV_TRY(gsv::take_async_error(h));
+  CUDA_TRY(cudaSetDevice(h->device));
+  CUDA_TRY(gsv::attn_wait_selftest(gsv::handle_attention(h), (unsigned long long)limit_ns,
+                                   static_cast<cudaStream_t>(stream)));
   return GSV_OK;
 }
 

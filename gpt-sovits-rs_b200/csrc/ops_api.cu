@@ -242,6 +242,14 @@ int norm_call(const gsvdec_norm* in, bool bwd, int device, void* stream) {
 }
 
 }  // namespace
+
+// gsvdec_selftest_attention_wait without a handle.
+int ops_wait_selftest(int device, unsigned long long limit_ns, cudaStream_t st) {
+  OnDevice dev(device);
+  if (dev.rc != GSV_OK) return dev.rc;
+  return finish(attn_wait_selftest(AttnArgs{}, limit_ns, st), "attention wait self-test");
+}
+
 }  // namespace gsv
 
 extern "C" {

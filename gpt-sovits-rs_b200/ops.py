@@ -270,16 +270,26 @@ def attention_backward(do, q, k, v, o, lse, *, scale: Optional[float] = None, ca
     return dq, dk, dv, drk, drv
 
 
+def _index(device) -> int:
+    import torch
+    index = None if device is None else torch.device(device).index
+    return torch.cuda.current_device() if index is None else index
+
+
 def ops_status(device=None) -> None:
     """Waits for the current stream of ``device`` (default: the current one) and
     raises GsvDecError(GSV_E_TIMEOUT) if a bounded device wait of an operator
     there gave up (gsvdec_ops_status)."""
-    import torch
-    index = None if device is None else torch.device(device).index
-    if index is None:
-        index = torch.cuda.current_device()
-    c = _get()
+    index, c = _index(device), _get()
     c.check(c.lib.gsvdec_ops_status(index, c.stream(index)))
+
+
+def selftest_wait(limit_ns: int = 1_000_000, device=None) -> None:
+    """Queue a bounded wait that nothing completes on the current stream of
+    ``device``; ops_status then reports it like an operator's give-up
+    (gsvdec_selftest_attention_wait)."""
+    index, c = _index(device), _get()
+    c.check(c.lib.gsvdec_selftest_attention_wait(None, index, int(limit_ns), c.stream(index)))
 
 
 def _norm_in(c, x, y, lengths, layout):

@@ -384,6 +384,11 @@ int gsvdec_sync_status(gsvdec_t* h, void* stream);
  * that kernel when it gives up.  No reference counterpart. */
 int gsvdec_selftest_wait(gsvdec_t* h, int64_t limit_ns, void* stream);
 
+/* The same for the attention's waits.  With a handle the give-up is reported
+ * as that of gsvdec_encp_attention's attention on this handle (`device` is not
+ * used), with h = NULL as an operator's on `device` (gsvdec_ops_status). */
+int gsvdec_selftest_attention_wait(gsvdec_t* h, int device, int64_t limit_ns, void* stream);
+
 /* Allocation-failure hook (process-wide, for tests of the callers' error
  * paths): with n >= 0 the next n device allocations of the library succeed
  * and every one after them fails with GSV_E_OOM, until the hook is reset

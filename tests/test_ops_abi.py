@@ -133,3 +133,11 @@ def test_more_heads_than_a_launch_has_blocks_are_refused(ops):
     assert lib.gsvdec_attention_forward(ctypes.byref(a), 0, None) == -1
     assert lib.gsvdec_attention_backward(ctypes.byref(a), 0, None) == -1
     assert lib.gsvdec_attention_workspace(ctypes.byref(a), 1, ctypes.byref(n)) == -1
+
+
+def test_the_attention_wait_self_test_is_checked(ops):
+    _, lib = ops
+    assert lib.gsvdec_selftest_attention_wait(None, 0, 10, None) == -1
+    assert "limit_ns" in lib.gsvdec_last_error().decode()
+    assert lib.gsvdec_selftest_attention_wait(None, 4096, 1000000, None) == -1
+    assert "4096" in lib.gsvdec_last_error().decode()
