@@ -48,7 +48,7 @@ struct AttnArgs {
   Str3 sq, sk, sv, so, sdo, sdq, sdk, sdv;
   char* ws;
   size_t ws_bytes;
-  int* err;  // a handle's error word, for its give-ups; null: the operators' own words
+  int* err;  // a handle's error word, for its give-ups; null: the operators' own counts
 };
 
 // Every row of the tensor starts on a 16-byte boundary and holds whole
@@ -63,10 +63,11 @@ size_t attn_fwd_workspace(const AttnArgs& a);
 size_t attn_bwd_workspace(const AttnArgs& a);
 cudaError_t attn_forward(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_backward(const AttnArgs& a, cudaStream_t st);
-// Waits for the stream; *out != 0 when a bounded device wait of the forward's
-// (backward's) kernels gave up since the last such call on this device.
-cudaError_t attn_fwd_gave_up(int* out, cudaStream_t st);
-cudaError_t attn_bwd_gave_up(int* out, cudaStream_t st);
+// Waits for the stream; *out: a count that has grown by at least one for every
+// call without a handle in which a bounded device wait of the forward's
+// (backward's) kernels on the current device gave up.
+cudaError_t attn_fwd_give_ups(int* out, cudaStream_t st);
+cudaError_t attn_bwd_give_ups(int* out, cudaStream_t st);
 // One bounded wait that nothing completes, reported as the forward's kernels
 // report theirs (gsvdec_selftest_attention_wait).
 cudaError_t attn_wait_selftest(const AttnArgs& a, unsigned long long limit_ns, cudaStream_t st);

@@ -322,20 +322,24 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 
 constexpr int kAttnCode = 17;  // error code of a give-up in a handle's word
 
-// A bounded wait gave up: said in the handle's word where the call has one.
-__device__ __forceinline__ void give_up(int* handle_word, int* own_word, volatile int* abort) {
-  if (handle_word) raise_err(handle_word, abort, kAttnCode);
-  else raise_err(own_word, abort, 1);
+// A bounded wait gave up: said in the handle's word where the call has one,
+// else counted.  The counts only grow, so that whoever reads one takes nothing
+// from the others.
+__device__ __forceinline__ void give_up(int* handle_word, int* count, volatile int* abort) {
+  if (handle_word) {
+    raise_err(handle_word, abort, kAttnCode);
+  } else {
+    *abort = 1;
+    atomicAdd(count, 1);
+  }
 }
 
-// Waits for the stream, then reads and clears a give-up word.
-cudaError_t take_gave_up(int& word, int* out, cudaStream_t st) {
+// Waits for the stream, then reads a count of give-ups.
+cudaError_t read_give_ups(int& count, int* out, cudaStream_t st) {
   void* p = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&p, word);
+  cudaError_t e = cudaGetSymbolAddress(&p, count);
   if (e == cudaSuccess) e = cudaMemcpyAsync(out, p, sizeof(int), cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess && *out) e = cudaMemsetAsync(p, 0, sizeof(int), st);
-  return e;
+  return e == cudaSuccess ? cudaStreamSynchronize(st) : e;
 }
 
 // A [B][heads][T][D] tensor as a 4-D tensor map whose boxes are ROWS rows of a

@@ -52,7 +52,7 @@
 namespace gsv {
 namespace {
 
-__device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out in a call without a handle
+__device__ int g_give_ups;  // bounded waits of the kernels below that ran out in calls without a handle
 
 constexpr int kBA = 128, kBB = 64;  // rows of the resident and of the streamed tiles
 constexpr int kHalfB = kBB / 2;
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         }
       }
       if (lead) mma_commit(bar(bars.acc_full));
-      if (!ok) give_up(a.err, &g_gave_up, abort);
+      if (!ok) give_up(a.err, &g_give_ups, abort);
       warp_wait(bar(bars.acc_full), 0, abort);  // nothing in flight when memory is given back
     } else if (nt > 0 && warp < 11) {
       const int tid = threadIdx.x - 9 * 32;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       }
       ho.flush();
       cp_wait<0>();
-      if (!ok) give_up(a.err, &g_gave_up, abort);
+      if (!ok) give_up(a.err, &g_give_ups, abort);
     }
   } else {
     const int wg = warp >> 2, row = threadIdx.x & 127, own = r0 + row, c0 = wg * kHalfB;
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       }
     }
     if (nt > 0) ok = ok && warp_wait(bar(bars.acc_full), 0, abort);
-    if (!ok) give_up(a.err, &g_gave_up, abort);
+    if (!ok) give_up(a.err, &g_give_ups, abort);
     tc_fence_after();
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
@@ -672,6 +672,6 @@ cudaError_t attn_bwd_tensor(const AttnArgs& a, const BwdWs& ws, cudaStream_t st)
   return a.ty == Ty::F16 ? width<__half>(a, ws, st) : width<__nv_bfloat16>(a, ws, st);
 }
 
-cudaError_t attn_bwd_gave_up(int* out, cudaStream_t st) { return take_gave_up(g_gave_up, out, st); }
+cudaError_t attn_bwd_give_ups(int* out, cudaStream_t st) { return read_give_ups(g_give_ups, out, st); }
 
 }  // namespace gsv

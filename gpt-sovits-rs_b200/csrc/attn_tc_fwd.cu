@@ -47,7 +47,7 @@
 namespace gsv {
 namespace {
 
-__device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out in a call without a handle
+__device__ int g_give_ups;  // bounded waits of the kernels below that ran out in calls without a handle
 
 constexpr int kBM = 128, kBN = 128;
 constexpr int kFwdThreads = 256;
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
         if (lead) mma_commit(bar(bars.o_full));
         fin = 1;
       }
-      if (!ok) give_up(a.err, &g_gave_up, abort);
+      if (!ok) give_up(a.err, &g_give_ups, abort);
       // Nothing of this block is in flight when its memory is given back.
       warp_wait(bar(bars.o_full), fin, abort);
     } else if (nt > 0 && warp < 7) {
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
       }
       ho.flush();
       cp_wait<0>();
-      if (!ok) give_up(a.err, &g_gave_up, abort);
+      if (!ok) give_up(a.err, &g_give_ups, abort);
     }
     if (cs > 1) {  // as the softmax warps join the cluster's sums
       cluster_sync();
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
         warp_arrive(bar(bars.p_full));
         ok = warp_wait(bar(bars.o_full), 1, abort);
       }
-      if (!ok) give_up(a.err, &g_gave_up, abort);
+      if (!ok) give_up(a.err, &g_give_ups, abort);
       tc_fence_after();
     }
     T* out = static_cast<T*>(a.o) + b * a.so.b + h * a.so.h;
@@ -545,7 +545,7 @@ __global__ void attn_wait_selftest_kernel(const __grid_constant__ AttnArgs a, co
   }
   __syncthreads();
   if (threadIdx.x == 0 && !mbar_wait_fast(smem_u32(&s_bar), 0, &s_abort, limit_ns))
-    give_up(a.err, &g_gave_up, &s_abort);
+    give_up(a.err, &g_give_ups, &s_abort);
 }
 
 template <typename T, int DP, bool REL>
@@ -607,6 +607,6 @@ cudaError_t attn_wait_selftest(const AttnArgs& a, unsigned long long limit_ns, c
   return cudaGetLastError();
 }
 
-cudaError_t attn_fwd_gave_up(int* out, cudaStream_t st) { return take_gave_up(g_gave_up, out, st); }
+cudaError_t attn_fwd_give_ups(int* out, cudaStream_t st) { return read_give_ups(g_give_ups, out, st); }
 
 }  // namespace gsv

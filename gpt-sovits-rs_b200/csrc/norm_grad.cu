@@ -41,7 +41,7 @@ namespace cg = cooperative_groups;
 namespace gsv {
 namespace {
 
-__device__ int g_gave_up;  // set when a bounded wait of a kernel below ran out
+__device__ int g_give_ups;  // bounded waits of the kernels below that ran out
 
 constexpr int kRowThreads = 256;
 constexpr int kTimeWarps = 16;
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kRowThreads, BWD && E > 16 ? 1 : 2) norm_rows(
       if (kRing) {
         if (!warp_wait(smem_u32(&s_bar[grp][s]), phases >> s & 1, &s_abort)) {
           // The group cannot go on together: leave the kernel's results undefined, but end it.
-          raise_err(&g_gave_up, &s_abort, 1);
+          give_up(nullptr, &g_give_ups, &s_abort);
         }
         phases ^= 1u << s;
         const T* sx = reinterpret_cast<const T*>(ring + (size_t)s * K * row_bytes);
@@ -712,6 +712,6 @@ cudaError_t norm_backward(const NormArgs& a, cudaStream_t st) {
   return launch_k(norm_part_sum, cdiv(2 * a.C, 32), 512, 0, st, (const float*)a.part, n, a.C, a.dgamma, a.dbeta);
 }
 
-cudaError_t norm_gave_up(int* out, cudaStream_t st) { return take_gave_up(g_gave_up, out, st); }
+cudaError_t norm_give_ups(int* out, cudaStream_t st) { return read_give_ups(g_give_ups, out, st); }
 
 }  // namespace gsv

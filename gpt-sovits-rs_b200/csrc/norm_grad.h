@@ -41,8 +41,7 @@ constexpr int kNormTimeMaxC = 2048;
 size_t norm_bwd_workspace(const NormArgs& a);
 cudaError_t norm_forward(const NormArgs& a, cudaStream_t st);
 cudaError_t norm_backward(const NormArgs& a, cudaStream_t st);
-// Waits for the stream; *out != 0 when a bounded device wait gave up since the
-// last such call on this device.
-cudaError_t norm_gave_up(int* out, cudaStream_t st);
+// As attn_fwd_give_ups (attn.h).
+cudaError_t norm_give_ups(int* out, cudaStream_t st);
 
 }  // namespace gsv

@@ -16,13 +16,14 @@ int set_err(int code, const char* fmt, ...);  // gsvdec_api.cu
 
 namespace {
 
+constexpr int kMaxDevices = 64;
+
 // GSV_OK when `device` is a device the kernels run on; looked up once each.
 int device_ok(int device) {
-  constexpr int kMax = 64;
-  static std::atomic<int> known[kMax];  // 0 not looked up, 1 fine, else 2 + 16 major + minor
+  static std::atomic<int> known[kMaxDevices];  // 0 not looked up, 1 fine, else 2 + 16 major + minor
   int n = 0;
-  if (device < 0 || device >= kMax || known[device].load(std::memory_order_acquire) == 0) {
-    if (cudaGetDeviceCount(&n) != cudaSuccess || device < 0 || device >= n || device >= kMax) {
+  if (device < 0 || device >= kMaxDevices || known[device].load(std::memory_order_acquire) == 0) {
+    if (cudaGetDeviceCount(&n) != cudaSuccess || device < 0 || device >= n || device >= kMaxDevices) {
       cudaGetLastError();
       return set_err(GSV_E_INVALID_ARG, "device %d is not one of the %d CUDA devices", device, n);
     }
@@ -274,13 +275,16 @@ int gsvdec_attention_backward(const gsvdec_attention* a, int device, void* strea
 int gsvdec_ops_status(int device, void* stream) {
   gsv::OnDevice dev(device);
   if (dev.rc != GSV_OK) return dev.rc;
-  int fwd = 0, bwd = 0, norm = 0;
-  cudaError_t e = gsv::attn_fwd_gave_up(&fwd, static_cast<cudaStream_t>(stream));
-  if (e == cudaSuccess) e = gsv::attn_bwd_gave_up(&bwd, static_cast<cudaStream_t>(stream));
-  if (e == cudaSuccess) e = gsv::norm_gave_up(&norm, static_cast<cudaStream_t>(stream));
+  // What this thread has been told of; the counts themselves belong to all threads.
+  thread_local int seen[gsv::kMaxDevices][3] = {};
+  int now[3] = {};
+  cudaError_t e = gsv::attn_fwd_give_ups(&now[0], static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) e = gsv::attn_bwd_give_ups(&now[1], static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) e = gsv::norm_give_ups(&now[2], static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return gsv::finish(e, "operator status");
-  return fwd || bwd || norm ? gsv::set_err(GSV_E_TIMEOUT, "a bounded device wait of an operator on device %d gave up", device)
-                 : GSV_OK;
+  if (std::equal(now, now + 3, seen[device])) return GSV_OK;
+  std::copy(now, now + 3, seen[device]);
+  return gsv::set_err(GSV_E_TIMEOUT, "a bounded device wait of an operator on device %d gave up", device);
 }
 
 int gsvdec_norm_workspace(const gsvdec_norm* a, size_t* bytes) {

@@ -279,7 +279,7 @@ def _index(device) -> int:
 def ops_status(device=None) -> None:
     """Waits for the current stream of ``device`` (default: the current one) and
     raises GsvDecError(GSV_E_TIMEOUT) if a bounded device wait of an operator
-    there gave up (gsvdec_ops_status)."""
+    there gave up since this thread's last call (gsvdec_ops_status)."""
     index, c = _index(device), _get()
     c.check(c.lib.gsvdec_ops_status(index, c.stream(index)))
 

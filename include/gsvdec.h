@@ -461,8 +461,10 @@ int gsvdec_attention_forward(const gsvdec_attention* a, int device, void* stream
 int gsvdec_attention_backward(const gsvdec_attention* a, int device, void* stream);
 
 /* Waits for `stream`, then reports whether a bounded device wait of an
- * attention or norm call on `device` gave up since the last such call (GSV_E_TIMEOUT;
- * the results of the call concerned are undefined). */
+ * attention or norm call on `device` gave up (GSV_E_TIMEOUT; the results of the
+ * call concerned are undefined) since this host thread's last such call for the
+ * device, or, at its first, since the library was loaded: every thread is told
+ * once, whichever thread and stream the call was made on. */
 int gsvdec_ops_status(int device, void* stream);
 
 /* out = LayerNorm over channels of x + y (norm1(x + attn(x)) of

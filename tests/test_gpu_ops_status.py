@@ -4,6 +4,8 @@ operator's by gsvdec_ops_status.  The give-ups are made by
 gsvdec_selftest_attention_wait, a wait of 1 ms with nothing else in flight."""
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -63,4 +65,25 @@ def test_the_limit_is_checked(gsv, dec):
         with pytest.raises(gsv.GsvDecError) as e:
             call(10)
         assert e.value.status == "GSV_E_INVALID_ARG"
+    gsv.ops_status()
+
+
+def test_another_thread_does_not_take_the_report(gsv):
+    gsv.ops_status()
+    gsv.ops.selftest_wait()
+    torch.cuda.synchronize()
+    seen = []
+
+    def other():
+        try:
+            gsv.ops_status()
+            seen.append("GSV_OK")
+        except gsv.GsvDecError as e:
+            seen.append(e.status)
+
+    t = threading.Thread(target=other)
+    t.start()
+    t.join()
+    assert seen == ["GSV_E_TIMEOUT"]  # a thread sees every give-up it has not been told of
+    gave_up(gsv, gsv.ops_status)
     gsv.ops_status()
