@@ -2703,6 +2703,9 @@ int gsvdec_create_from_file(const char* path, int mode, int device, gsvdec_t** o
     std::vector<gsvdec_tensor> ts;
     for (const gsv::StEntry& e : f.entries()) {
       if (!wanted(e.name)) continue;
+      // A layer's attention is optional: one in a form that is not taken is left out, not refused.
+      const bool typed = e.dtype == "F32" || e.dtype == "F16" || e.dtype == "BF16";
+      if (e.name.find(".attn_layers.") != std::string::npos && (!typed || e.shape.empty() || e.shape.size() > 4)) continue;
       gsvdec_tensor t{};
       t.name = e.name.c_str();
       if (e.dtype == "F32") t.dtype = GSV_DTYPE_F32;
