@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 
 #include "../../include/gsvdec.h"
 #include "attn.h"
@@ -79,6 +80,14 @@ bool spread(const int64_t* stride, const int* n, int axes, int64_t width) {
     if (stride[x] < span) return false;
     span += stride[x] * (n[x] - 1);
   }
+  return true;
+}
+
+// Whether every address is a multiple of the element's size (the kernels load
+// whole elements; NULL counts as aligned).
+bool elements_aligned(std::initializer_list<const void*> ps, int size) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % size) return false;
   return true;
 }
 bool forward_strides(const int64_t* s, int n) {
@@ -163,6 +172,10 @@ int attn_call(const gsvdec_attention* in, bool bwd, int device, void* stream) {
   if ((q && (!a.q || !a.o)) || (k && (!a.k || !a.v)))
     return set_err(GSV_E_INVALID_ARG, "attention: q, k, v or o is NULL");
   if (a.nrel && (!a.relk || !a.relv)) return set_err(GSV_E_INVALID_ARG, "attention: a window needs rel_k and rel_v");
+  const int el = a.ty == Ty::F32 ? 4 : 2;
+  if (!elements_aligned({a.q, a.k, a.v, a.relk, a.relv, a.o}, el) || !elements_aligned({a.lse, a.qlen, a.klen}, 4) ||
+      (bwd && !elements_aligned({a.dout, a.dq, a.dk, a.dv, a.drelk, a.drelv}, el)))
+    return set_err(GSV_E_INVALID_ARG, "attention: a tensor is not aligned to its elements");
   const int nq[3] = {a.B, a.H, a.Tq}, nk[3] = {a.B, a.Hkv, a.Tk};
   if (!bwd && !spread(in->o_stride, nq, 3, a.D))
     return set_err(GSV_E_INVALID_ARG, "attention: the rows of o overlap");
@@ -225,6 +238,11 @@ int norm_call(const gsvdec_norm* in, bool bwd, int device, void* stream) {
   const bool any = a.T > 0;
   if (!a.gamma || (any && (!a.x.p || !a.mean || !a.rstd)))
     return set_err(GSV_E_INVALID_ARG, "norm: x, gamma, mean or rstd is NULL");
+  const int el = a.ty == Ty::F32 ? 4 : 2;
+  if (!elements_aligned({a.x.p, a.y.p}, el) || !elements_aligned({a.gamma, a.mean, a.rstd, a.len}, 4) ||
+      (bwd ? !elements_aligned({a.dout.p, a.dx.p}, el) || !elements_aligned({a.dgamma, a.dbeta}, 4)
+           : !elements_aligned({a.out.p}, el) || !elements_aligned({a.beta}, 4)))
+    return set_err(GSV_E_INVALID_ARG, "norm: a tensor is not aligned to its elements");
   const int64_t* s = bwd ? in->dx_stride : in->out_stride;
   const int inner = a.rows ? a.C : a.T, n[2] = {a.B, a.rows ? a.T : a.C};
   if (any && !spread(s, n, 2, inner))

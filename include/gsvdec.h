@@ -408,7 +408,8 @@ int gsvdec_workspace_bytes(const gsvdec_t* h, int64_t* bytes);
  * call takes its tensors, a workspace and a stream, keeps nothing, allocates
  * nothing and is stream-async, so it can be captured in a CUDA graph; calls
  * overlap freely as long as their outputs and workspaces differ.  Outputs and
- * workspace must not overlap inputs or one another.
+ * workspace must not overlap inputs or one another.  Every address must be a
+ * multiple of its element's size.
  *
  * Attention, for utterance b with ql = q_lengths[b] queries and kl =
  * k_lengths[b] keys (clamped to [0, Tq] / [0, Tk]; NULL: all): the sequences

@@ -141,3 +141,45 @@ def test_the_attention_wait_self_test_is_checked(ops):
     assert "limit_ns" in lib.gsvdec_last_error().decode()
     assert lib.gsvdec_selftest_attention_wait(None, 4096, 1000000, None) == -1
     assert "4096" in lib.gsvdec_last_error().decode()
+
+
+@pytest.mark.parametrize("dtype,off", [(0, 1), (0, 2), (1, 1), (2, 1)])
+@pytest.mark.parametrize("name", ["q", "k", "v", "rel_k", "rel_v", "o", "d_o", "dq", "dk", "dv", "drel_k", "drel_v"])
+def test_tensors_that_start_inside_an_element_are_refused(ops, dtype, off, name):
+    # Device 4096: nothing is launched even where the address is not looked at.
+    o, lib = ops
+    a = attention(o, dtype=dtype, **{name: FAKE + off})
+    call = lib.gsvdec_attention_backward if name.startswith("d") else lib.gsvdec_attention_forward
+    assert call(ctypes.byref(a), 4096, None) == -1
+    assert "aligned" in lib.gsvdec_last_error().decode()
+
+
+@pytest.mark.parametrize("name", ["lse", "q_lengths", "k_lengths"])
+def test_attention_values_that_start_inside_an_element_are_refused(ops, name):
+    o, lib = ops
+    for call in (lib.gsvdec_attention_forward, lib.gsvdec_attention_backward):
+        assert call(ctypes.byref(attention(o, **{name: FAKE + 2})), 4096, None) == -1
+        assert "aligned" in lib.gsvdec_last_error().decode()
+
+
+@pytest.mark.parametrize("name,off", [("x", 1), ("y", 1), ("out", 1), ("d_out", 1), ("dx", 1), ("gamma", 2),
+                                      ("beta", 2), ("mean", 2), ("rstd", 2), ("lengths", 2), ("dgamma", 2),
+                                      ("dbeta", 2)])
+def test_norm_tensors_that_start_inside_an_element_are_refused(ops, name, off):
+    o, lib = ops
+    call = lib.gsvdec_norm_backward if name.startswith("d") else lib.gsvdec_norm_forward
+    assert call(ctypes.byref(norm(o, **{name: FAKE + off})), 4096, None) == -1
+    assert "aligned" in lib.gsvdec_last_error().decode()
+
+
+def test_aligned_arguments_reach_the_device(ops):
+    o, lib = ops
+    for dtype, off in ((0, 4), (1, 2), (2, 2)):
+        odd = {n: FAKE + off for n in ("q", "k", "v", "rel_k", "rel_v", "o", "d_o", "dq", "dk", "dv", "drel_k", "drel_v")}
+        a = attention(o, dtype=dtype, lse=FAKE + 4, q_lengths=FAKE + 4, k_lengths=FAKE + 4, **odd)
+        for call in (lib.gsvdec_attention_forward, lib.gsvdec_attention_backward):
+            assert call(ctypes.byref(a), 4096, None) == -1
+            assert "4096" in lib.gsvdec_last_error().decode()
+    for call in (lib.gsvdec_norm_forward, lib.gsvdec_norm_backward):
+        assert call(ctypes.byref(norm(o, x=FAKE + 2, d_out=FAKE + 2, gamma=FAKE + 4, mean=FAKE + 4)), 4096, None) == -1
+        assert "4096" in lib.gsvdec_last_error().decode()
