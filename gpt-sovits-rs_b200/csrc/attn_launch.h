@@ -66,6 +66,30 @@ inline BwdWs carve_bwd(const AttnArgs& a) {
   return w;
 }
 
+// The row pass: G lanes share a row, and a block of kRowThreads takes kRowTurns
+// rows per group.  Query rows of all heads come first, then (fp16, for the
+// norms of v) the key rows of all key heads.
+constexpr int kRowThreads = 256, kRowTurns = 2;
+inline int row_lanes(int D) { return D <= 32 ? 4 : D <= 64 ? 8 : 16; }
+struct RowBlocks {
+  int64_t q, k;
+};
+inline RowBlocks row_blocks(const AttnArgs& a) {
+  const int rows = kRowThreads / row_lanes(a.D) * kRowTurns, padded = cdiv(a.Tq, 2 * kRowBlock) * 2 * kRowBlock;
+  return {(int64_t)cdiv(padded, rows) * a.H * a.B, a.ty == Ty::F16 ? (int64_t)cdiv(a.Tk, rows) * a.Hkv * a.B : 0};
+}
+
+// Most blocks of a launch of the call.  Tiles are split over several blocks
+// only where there are few of them, so they do not add to it.
+inline int64_t attn_most_blocks(const AttnArgs& a, bool bwd) {
+  const int tile = a.ty == Ty::F32 ? 64 : 128;
+  const int64_t q = (int64_t)cdiv(a.Tq, tile) * a.H * a.B;
+  if (!bwd) return q;
+  const RowBlocks r = row_blocks(a);
+  const int64_t main = q + (int64_t)cdiv(a.Tk, tile) * a.Hkv * a.B;
+  return main > r.q + r.k ? main : r.q + r.k;
+}
+
 constexpr int kFewRows = 8;  // most rows per key head of attn_fwd_few_rows
 cudaError_t attn_fwd_few_rows(const AttnArgs& a, cudaStream_t st);
 cudaError_t attn_fwd_tensor(const AttnArgs& a, cudaStream_t st);

@@ -9,7 +9,6 @@
 namespace gsv {
 namespace {
 
-constexpr int kRowThreads = 256;
 constexpr int kFewKeys = 32;
 
 template <int G>
@@ -51,19 +50,19 @@ __device__ __forceinline__ float dot8(const float* a, const float* b) {
 // blocks an SM that wait for memory twice and then do 18 products a row.
 template <typename T, int G, int U>
 __global__ void __launch_bounds__(kRowThreads, 4) bwd_rows_kernel(const __grid_constant__ AttnArgs a,
-                                                                  const __grid_constant__ BwdWs ws, const int nq,
-                                                                  const bool vec) {
+                                                                  const __grid_constant__ BwdWs ws,
+                                                                  const int qblocks, const bool vec) {
   extern __shared__ __align__(16) float sm[];  // relk, relv as [nrel][P], then q, do as [R U][P]
   constexpr bool F16 = std::is_same<T, __half>::value, kExact = std::is_same<T, float>::value;
   constexpr int L = 8 * G, P = L + 4, R = kRowThreads / G;
   // Heads fastest: the blocks of the first rows, which take longest (few keys), start first.
-  const int tile = blockIdx.x / (a.H * a.B), bh32 = blockIdx.x - tile * (a.H * a.B);
-  const int D = a.D, lane = threadIdx.x % G, d0 = lane * 8, b = bh32 / a.H, h = bh32 - b * a.H;
+  const bool key_rows = F16 && (int)blockIdx.x >= qblocks;
+  const int unit = blockIdx.x - (key_rows ? qblocks : 0), hn = key_rows ? a.Hkv : a.H;
+  const int tile = unit / (hn * a.B), bh32 = unit - tile * (hn * a.B);
+  const int D = a.D, lane = threadIdx.x % G, d0 = lane * 8, b = bh32 / hn, h = bh32 - b * hn;
   const int ql = clamp_len(a.qlen, b, a.Tq), kl = clamp_len(a.klen, b, a.Tk);
-  const bool key_rows = F16 && tile >= nq;
-  if (key_rows && h >= a.Hkv) return;
   // Rows of the block: i0 + u R + group.
-  const int i0 = (tile - (key_rows ? nq : 0)) * R * U + threadIdx.x / G;
+  const int i0 = tile * R * U + threadIdx.x / G;
   Raw8<T> rg[U], ro[U], rq[U];
   if (!key_rows) {
     const T* g = static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h;
@@ -306,8 +305,8 @@ __global__ void __launch_bounds__(512) bwd_rel_sum_kernel(const AttnArgs a, cons
 
 template <typename T, int G>
 cudaError_t rows_g(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
-  constexpr int U = 2, R = kRowThreads / G * U;
-  const int nq = cdiv(ws.blocks * kRowBlock, R), nk = a.ty == Ty::F16 ? cdiv(a.Tk, R) : 0;
+  constexpr int U = kRowTurns, R = kRowThreads / G * U;
+  const RowBlocks n = row_blocks(a);
   const size_t smem = a.nrel ? sizeof(float) * 2 * (a.nrel + R) * (8 * G + 4) : 0;
   int regs;
   const cudaError_t e = kernel_setup(bwd_rows_kernel<T, G, U>, smem, &regs);
@@ -316,14 +315,14 @@ cudaError_t rows_g(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
   const bool vec = attn_rows_aligned(a.q, a.sq, a.D, el) && attn_rows_aligned(a.o, a.so, a.D, el) &&
                    attn_rows_aligned(a.dout, a.sdo, a.D, el) && attn_rows_aligned(a.k, a.sk, a.D, el) &&
                    attn_rows_aligned(a.v, a.sv, a.D, el) && a.D % 8 == 0;
-  bwd_rows_kernel<T, G, U><<<(unsigned)((int64_t)(nq + nk) * a.H * a.B), kRowThreads, smem, st>>>(a, ws, nq, vec);
+  bwd_rows_kernel<T, G, U><<<(unsigned)(n.q + n.k), kRowThreads, smem, st>>>(a, ws, (int)n.q, vec);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t rows_t(const AttnArgs& a, const BwdWs& ws, cudaStream_t st) {
-  if (a.D <= 32) return rows_g<T, 4>(a, ws, st);
-  return a.D <= 64 ? rows_g<T, 8>(a, ws, st) : rows_g<T, 16>(a, ws, st);
+  const int g = row_lanes(a.D);
+  return g == 4 ? rows_g<T, 4>(a, ws, st) : g == 8 ? rows_g<T, 8>(a, ws, st) : rows_g<T, 16>(a, ws, st);
 }
 
 template <typename T>

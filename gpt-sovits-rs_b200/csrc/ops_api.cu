@@ -8,7 +8,7 @@
 #include <initializer_list>
 
 #include "../../include/gsvdec.h"
-#include "attn.h"
+#include "attn_launch.h"
 #include "norm_grad.h"
 
 namespace gsv {
@@ -187,6 +187,9 @@ int attn_call(const gsvdec_attention* in, bool bwd, int device, void* stream) {
     if (!spread(in->dq_stride, nq, 3, a.D) || !spread(in->dk_stride, nk, 3, a.D) || !spread(in->dv_stride, nk, 3, a.D))
       return set_err(GSV_E_INVALID_ARG, "attention: the rows of dq, dk or dv overlap");
   }
+  if (attn_most_blocks(a, bwd) > INT32_MAX)
+    return set_err(GSV_E_INVALID_ARG, "attention: %lld tiles of rows are more than a launch's blocks (2^31 - 1)",
+                   (long long)attn_most_blocks(a, bwd));
   rc = workspace_ok(a.ws, a.ws_bytes, bwd ? attn_bwd_workspace(a) : attn_fwd_workspace(a), "attention");
   if (rc != GSV_OK) return rc;
   OnDevice dev(device);
