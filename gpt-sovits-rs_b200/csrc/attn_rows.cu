@@ -256,9 +256,10 @@ __global__ void __launch_bounds__(2 * kAttnMaxD) bwd_rel_kernel(const AttnArgs a
   float ak[NR] = {}, av[NR] = {};
   const float* q = static_cast<const float*>(a.q) + b * a.sq.b + h * a.sq.h + d;
   const float* g = static_cast<const float*>(a.dout) + b * a.sdo.b + h * a.sdo.h + d;
+  const int y0 = max(half * (kRelRows / 2), first_query(ql, kl, a.causal) - i0);
   const int y1 = min(half * (kRelRows / 2) + kRelRows / 2, ql - i0);
 #pragma unroll 4
-  for (int y = half * (kRelRows / 2); y < y1; ++y) {
+  for (int y = y0; y < y1; ++y) {
     const float qv = d < D ? q[(int64_t)(i0 + y) * a.sq.t] : 0.f;
     const float gv = d < D ? g[(int64_t)(i0 + y) * a.sdo.t] : 0.f;
 #pragma unroll

@@ -217,15 +217,15 @@ __device__ __forceinline__ void cp_wait() {
 
 constexpr int kLoaders = 64;  // threads that load tiles (two warps)
 
-// ROWS x DP channels of a tile, from `valid` global rows of D channels;
-// everything else is zero (rows behind a length may hold NaN, and 0 . NaN would
-// reach the accumulators).  `vec`: rows are whole aligned 16-byte vectors and
+// ROWS x DP channels of a tile, from the global rows from .. valid - 1 of D
+// channels; everything else is zero (rows left out may hold NaN, and 0 . NaN
+// would reach the accumulators).  `vec`: rows are whole aligned 16-byte vectors and
 // move by cp.async; else by single elements.  A chunk's 8 (or 4) units per row
 // divide the 64 threads, so a thread keeps its unit and its swizzle and steps
 // down the rows by one constant.
 template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void load_tile(uint32_t dst, uint32_t chunk, const T* g, int64_t stride, int valid, int D,
-                                          bool vec, int tid) {
+                                          bool vec, int tid, int from = 0) {
 #pragma unroll
   for (int c = 0; c < (DP + 63) / 64; ++c) {
     constexpr int kFull = 8;
@@ -238,13 +238,13 @@ __device__ __forceinline__ void load_tile(uint32_t dst, uint32_t chunk, const T*
       const bool in = col < D;
 #pragma unroll 8
       for (int i = 0; i < ROWS / step; ++i, a += step * 128, p += ps) {
-        const bool use = in && r0 + i * step < valid;
+        const bool use = in && r0 + i * step >= from && r0 + i * step < valid;
         cp_async16(a, use ? p : g, use ? 16 : 0);
       }
     } else {
       for (int r = r0; r < ROWS; r += step, a += step * 128, p += ps) {
         uint32_t w[4] = {0u, 0u, 0u, 0u};
-        if (r < valid) {
+        if (r >= from && r < valid) {
           const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
           for (int i = 0; i < 8; ++i)

@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
     per = last < r0 ? 0 : cdiv(allowed_keys(last, ql, kl, a.causal), kBB);
   }
   const int nt = per * heads;
+  const int qfirst = first_query(ql, kl, a.causal);
   const int64_t bh0 = (int64_t)b * a.H + (keys ? hk * g : head);  // first head
   volatile int* abort = &s_abort;
   auto bar = [&](const uint64_t& m) { return smem_u32(&m); };
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       // Per barrier: the first warp's lane 0 announces and issues what moves by bulk copies (full tiles,
       // row values); tails are copied by both warps, whose second arrival, or both, come when that is done.
       const bool first_warp = warp == 9;
-      const bool full_a = maps.a_on && tma_fits(r0, kBA, keys ? kl : ql, keys ? a.Tk : a.Tq);
+      const bool full_a = maps.a_on && tma_fits(r0, kBA, keys ? kl : ql, keys ? a.Tk : a.Tq) && (keys || r0 >= qfirst);
       const uint32_t a_full = bar(bars.a_full);
       if (first_warp && lane == 0) {
         const uint32_t rel_bytes = REL && !keys ? 2u * 2 * kBB * a.nrel * 4 : 0;
@@ -335,9 +336,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
           load_tile<T, DP, kBA>(sA1, C::chunkA, v + (int64_t)r0 * a.sv.t, a.sv.t, kl - r0, D, vec, tid);
         } else {
           const int h = head;
-          load_tile<T, DP, kBA>(sA0, C::chunkA, q + h * a.sq.h + (int64_t)r0 * a.sq.t, a.sq.t, ql - r0, D, vec, tid);
+          load_tile<T, DP, kBA>(sA0, C::chunkA, q + h * a.sq.h + (int64_t)r0 * a.sq.t, a.sq.t, ql - r0, D, vec, tid,
+                                qfirst - r0);
           load_tile<T, DP, kBA>(sA1, C::chunkA, dout + h * a.sdo.h + (int64_t)r0 * a.sdo.t, a.sdo.t, ql - r0, D, vec,
-                                tid);
+                                tid, qfirst - r0);
         }
         ho.next(a_full);
       } else {
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         if (round > 0) ok = ho.wait_free(bar(bars.b_free[s]), (round - 1) & 1, abort);
         if (!ok) break;
         const int h = keys ? hk * g + hh : hk;
-        const bool whole = maps.b_on && tma_fits(i0, kBB, keys ? ql : kl, keys ? a.Tq : a.Tk);
+        const bool whole = maps.b_on && tma_fits(i0, kBB, keys ? ql : kl, keys ? a.Tq : a.Tk) && (!keys || i0 >= qfirst);
         if (first_warp && lane == 0) {
           // Offsets of this pair of tiles: from r0 - (i0 + 63 + off) to r0 + 127 - (i0 + off).
           const bool near = REL && keys && r0 - (i0 + kBB - 1 + off) <= a.window &&
@@ -374,9 +376,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
           warp_arrive(full);
         } else {
           if (keys) {
-            load_tile<T, DP, kBB>(b0, C::chunkB, q + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t, ql - i0, D, vec, tid);
+            load_tile<T, DP, kBB>(b0, C::chunkB, q + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t, ql - i0, D, vec, tid,
+                                  qfirst - i0);
             load_tile<T, DP, kBB>(b1, C::chunkB, dout + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t, ql - i0, D, vec,
-                                  tid);
+                                  tid, qfirst - i0);
           } else {
             load_tile<T, DP, kBB>(b0, C::chunkB, k + (int64_t)i0 * a.sk.t, a.sk.t, kl - i0, D, vec, tid);
             load_tile<T, DP, kBB>(b1, C::chunkB, v + (int64_t)i0 * a.sv.t, a.sv.t, kl - i0, D, vec, tid);

@@ -282,3 +282,28 @@ def test_refusals(gsv):
         gsv.attention(big, big, big)
     with pytest.raises(gsv.GsvDecError):
         gsv.attention(q[:, :1].expand(-1, 3, -1, -1), k, v)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("Tq,Tk,ql,kl", [(200, 61, (200, 150), (61, 10)), (333, 300, (333, 300), (70, 300)),
+                                         (6, 3, (6, 5), (3, 0))])
+@pytest.mark.parametrize("w", [-1, 3])
+def test_queries_without_a_key_hold_anything(gsv, dtype, Tq, Tk, ql, kl, w):
+    # With causal the first ql - kl queries see no key: they add nothing to any gradient, whatever they hold.
+    x = make(dtype, 2, 4, 2, Tq, Tk, 64, w=w)
+    for b in range(2):
+        n = ql[b] - kl[b]
+        x["q"][b, :, :n] = x["do"][b, :, :n] = 0
+    kw = dict(causal=True, q_lengths=lengths(*ql), k_lengths=lengths(*kl))
+    want = run_and_check(gsv, x, **kw)
+    for bad in (float("nan"), float("inf")):
+        for b in range(2):
+            n = ql[b] - kl[b]
+            x["q"][b, :, :n] = bad
+            x["do"][b, :, :n] = -bad
+        kw2 = dict(kw, **{n: x[n] for n in ("rel_k", "rel_v") if n in x})
+        o, lse = gsv.attention(x["q"], x["k"], x["v"], **kw2)
+        grads = gsv.attention_backward(x["do"], x["q"], x["k"], x["v"], o, lse, **kw2)
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+        for a, b in zip(grads, want[2]):
+            assert (a is None and b is None) or torch.equal(a, b)
