@@ -173,7 +173,7 @@ def _attention_in(c, q, k, v, scale, causal, q_lengths, k_lengths, rel_k, rel_v)
         rk, rv = _need("rel_k", rel_k, (n, D), t, index, True), _need("rel_v", rel_v, (n, D), t, index, True)
     lead = (code, B, H, Hkv, Tq, Tk, D, window, 1 if causal else 0)
     if scale is None:
-        scale = 1.0 / math.sqrt(D)
+        scale = 1.0 / math.sqrt(D) if D else 1.0  # without channels: refused by the library
     given = (scale, ql, kl, pq, pk, pv, sq[0], sq[1], sq[2], sk[0], sk[1], sk[2], sv[0], sv[1], sv[2], rk, rv)
     return lead, given, index, (qs, ks, sq, sk, sv)
 

@@ -307,3 +307,11 @@ def test_queries_without_a_key_hold_anything(gsv, dtype, Tq, Tk, ql, kl, w):
         assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
         for a, b in zip(grads, want[2]):
             assert (a is None and b is None) or torch.equal(a, b)
+
+
+def test_heads_without_channels_are_refused(gsv):
+    q = torch.zeros(1, 2, 4, 0, device="cuda")
+    for kw in ({}, dict(scale=1.0)):
+        with pytest.raises(gsv.GsvDecError) as e:
+            gsv.attention(q, q, q, **kw)
+        assert e.value.status == "GSV_E_INVALID_ARG"
