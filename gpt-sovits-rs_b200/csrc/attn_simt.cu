@@ -44,12 +44,11 @@ constexpr int kBT = 64;        // rows and columns of a score tile
 constexpr int kThreads = 256;
 constexpr int kLdP = kBT + 4;  // pitch of a transposed probability tile
 
-// kBT x DP floats from the global rows first .. nvalid - 1 (D channels), zeros
+// kBT x DP floats from global rows (nvalid of them, D channels), zeros
 // elsewhere.  Addresses are clamped and values dropped afterwards, so that no
 // load stands under a branch and a thread's loads are all in flight together.
 template <typename T, int DP>
-__device__ __forceinline__ void load_rows(float* s, const T* g, int64_t stride, int nvalid, int D, bool vec,
-                                          int first = 0) {
+__device__ __forceinline__ void load_rows(float* s, const T* g, int64_t stride, int nvalid, int D, bool vec) {
   constexpr int V = DP / 4, N = kBT * V / kThreads;
   float4 o[N];
   if (nvalid > 0) {
@@ -68,7 +67,7 @@ __device__ __forceinline__ void load_rows(float* s, const T* g, int64_t stride, 
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const int i = threadIdx.x + n * kThreads, r = i / V, c = (i - r * V) * 4;
-    const bool in = r >= first && r < nvalid;
+    const bool in = r < nvalid;
     float4 v;
     v.x = in && c < D ? o[n].x : 0.f;
     v.y = in && c + 1 < D ? o[n].y : 0.f;
@@ -396,7 +395,6 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const __grid_constant_
   cg::cluster_group cl = cg::this_cluster();
   const int from = rank * (kBT / cs);  // first of the rows that this block writes
   auto one = [](int, int) { return 1.f; };
-  const int qfirst = first_query(ql, kl, a.causal);
   if (keys) {
     const int hk = bhu - b * a.Hkv, j0 = tile * kBT;
     load_rows<T, DP>(s0, static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h + (int64_t)j0 * a.sk.t, a.sk.t,
@@ -404,16 +402,17 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const __grid_constant_
     load_rows<T, DP>(s1, static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h + (int64_t)j0 * a.sv.t, a.sv.t,
                      kl - j0, D, vec);
     float dk[4][W] = {}, dv[4][W] = {};
-    const int first = j0 >= kl ? ql : (a.causal ? max(0, j0 - off) / kBT * kBT : 0);
+    // From the first query that sees the tile: those without a key (they may hold anything) stay out of its sums.
+    const int first = j0 >= kl ? ql : (a.causal ? max(0, j0 - off) : 0);
     for (int hh = 0; hh < g; ++hh) {
       const int h = hk * g + hh;
       const int64_t bh = (int64_t)b * a.H + h;
       for (int i0 = first + rank * kBT; i0 < ql; i0 += cs * kBT) {
         __syncthreads();
         load_rows<T, DP>(s2, static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t,
-                         ql - i0, D, vec, qfirst - i0);
+                         ql - i0, D, vec);
         load_rows<T, DP>(s3, static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + (int64_t)i0 * a.sdo.t,
-                         a.sdo.t, ql - i0, D, vec, qfirst - i0);
+                         a.sdo.t, ql - i0, D, vec);
         __syncthreads();
         float s[4][4] = {}, dp[4][4] = {};
         dot_tile<DP>(s0, s2, ty, tx, s);
@@ -479,9 +478,9 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt(const __grid_constant_
   const int h = bhu - b * a.H, hk = h / g, i0 = tile * kBT;
   const int64_t bh = bhu, row = bh * a.Tq;
   load_rows<T, DP>(s0, static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + (int64_t)i0 * a.sq.t, a.sq.t, ql - i0,
-                   D, vec, qfirst - i0);
+                   D, vec);
   load_rows<T, DP>(s1, static_cast<const T*>(a.dout) + b * a.sdo.b + h * a.sdo.h + (int64_t)i0 * a.sdo.t, a.sdo.t,
-                   ql - i0, D, vec, qfirst - i0);
+                   ql - i0, D, vec);
   float dq[4][W] = {}, nlse2[4], ndelta[4];
   int n[4];
 #pragma unroll
