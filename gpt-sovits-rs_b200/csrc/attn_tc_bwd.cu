@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         }
       }
       if (lead) mma_commit(bar(bars.acc_full));
-      if (!ok) give_up(a.err, &g_give_ups, abort);
+      if (!ok) *abort = 1;
       warp_wait(bar(bars.acc_full), 0, abort);  // nothing in flight when memory is given back
     } else if (nt > 0 && warp < 11) {
       const int tid = threadIdx.x - 9 * 32;
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       }
       ho.flush();
       cp_wait<0>();
-      if (!ok) give_up(a.err, &g_give_ups, abort);
+      if (!ok) *abort = 1;
     }
   } else {
     const int wg = warp >> 2, row = threadIdx.x & 127, own = r0 + row, c0 = wg * kHalfB;
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       }
     }
     if (nt > 0) ok = ok && warp_wait(bar(bars.acc_full), 0, abort);
-    if (!ok) give_up(a.err, &g_give_ups, abort);
+    if (!ok) *abort = 1;
     tc_fence_after();
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
@@ -622,6 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
     tc_fence_before();
   }
   __syncthreads();
+  if (threadIdx.x == 0 && s_abort) give_up(a.err, &g_give_ups);
   if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(s_tmem, 512);

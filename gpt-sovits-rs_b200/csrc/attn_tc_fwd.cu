@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
         if (lead) mma_commit(bar(bars.o_full));
         fin = 1;
       }
-      if (!ok) give_up(a.err, &g_give_ups, abort);
+      if (!ok) *abort = 1;
       // Nothing of this block is in flight when its memory is given back.
       warp_wait(bar(bars.o_full), fin, abort);
     } else if (nt > 0 && warp < 7) {
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
       }
       ho.flush();
       cp_wait<0>();
-      if (!ok) give_up(a.err, &g_give_ups, abort);
+      if (!ok) *abort = 1;
     }
     if (cs > 1) {  // as the softmax warps join the cluster's sums
       cluster_sync();
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
         warp_arrive(bar(bars.p_full));
         ok = warp_wait(bar(bars.o_full), 1, abort);
       }
-      if (!ok) give_up(a.err, &g_give_ups, abort);
+      if (!ok) *abort = 1;
       tc_fence_after();
     }
     T* out = static_cast<T*>(a.o) + b * a.so.b + h * a.so.h;
@@ -528,6 +528,7 @@ __global__ void __launch_bounds__(kFwdThreads, 2) attn_fwd_tc(const __grid_const
     tc_fence_before();
   }
   __syncthreads();
+  if (threadIdx.x == 0 && s_abort) give_up(a.err, &g_give_ups);
   if (warp == 4) {
     tc_fence_after();
     tmem_dealloc(s_tmem, 256);
@@ -545,7 +546,7 @@ __global__ void attn_wait_selftest_kernel(const __grid_constant__ AttnArgs a, co
   }
   __syncthreads();
   if (threadIdx.x == 0 && !mbar_wait_fast(smem_u32(&s_bar), 0, &s_abort, limit_ns))
-    give_up(a.err, &g_give_ups, &s_abort);
+    give_up(a.err, &g_give_ups);
 }
 
 template <typename T, int DP, bool REL>

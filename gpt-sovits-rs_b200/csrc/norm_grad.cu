@@ -197,7 +197,8 @@ __global__ void __launch_bounds__(kRowThreads, BWD && E > 16 ? 1 : 2) norm_rows(
       if (kRing) {
         if (!warp_wait(smem_u32(&s_bar[grp][s]), phases >> s & 1, &s_abort)) {
           // The group cannot go on together: leave the kernel's results undefined, but end it.
-          give_up(nullptr, &g_give_ups, &s_abort);
+          *const_cast<volatile int*>(&s_abort) = 1;
+          give_up(nullptr, &g_give_ups);
         }
         phases ^= 1u << s;
         const T* sx = reinterpret_cast<const T*>(ring + (size_t)s * K * row_bytes);
