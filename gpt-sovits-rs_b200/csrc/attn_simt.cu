@@ -18,16 +18,18 @@
 // on all SMs, its tiles are dealt out to the blocks of a cluster, whose sums
 // are joined in rank order through distributed shared memory.
 //
-// The tensor cores would need three 16-bit pieces per value and six products
-// for each, and room for the pieces that a block does not have at D = 128.
+// Not on the tensor cores: three 16-bit pieces per value and six products for
+// each need room that a block does not have at D = 128; two TF32 pieces and
+// three products have not been tried, nor their error measured.
 //
 // Measured on B200: backward of 4 utterances, 4 heads of 128, up to 500 queries
 // and 173 keys: 87 us and 7 for the rows, 13 TFLOP/s.  The whole tiles' seven
 // products would take 27 us on all SMs at the FMA rate; a block has 8 warps an
-// SM (its tiles fill the shared memory), too few to cover the loads of the
-// streamed tiles and the barriers around them, and the units do not divide
-// evenly.  One utterance of 37 frames, 2 heads of 96, window 4, forward: 14.6
-// us, one tile a head, all of it latency.
+// SM (its tiles fill the shared memory) and loads the streamed tiles between
+// two barriers, so that nothing covers them (FMA pipe 38 % busy, issue slots
+// 32 %, 17 to 43 % from SM to SM, since the units do not divide evenly).  One
+// utterance of 37 frames, 2 heads of 96, window 4, forward: 14.8 us, one tile a
+// head, all of it latency.
 #include <cooperative_groups.h>
 
 #include <algorithm>

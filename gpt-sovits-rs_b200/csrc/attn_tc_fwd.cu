@@ -33,11 +33,11 @@
 // took 13 % longer on the first case below.
 //
 // Measured on B200, bf16.  4 x 16 heads of 64, 4096 causal tokens: 198 us, 695
-// TFLOP/s, 42 % of a large matrix product's rate.  The exponentials bound it (16
-// a cycle and SM, one per score: 120 us of that pipe, where the two products
-// take half of it), with the hand-offs between the softmax and MMA warps; a
-// quarter of the exponentials as a polynomial took 15 us longer, since issue
-// slots run short as well.  Blocks ordered head by head instead of the longest
+// TFLOP/s, 42 % of a large matrix product's rate.  The exponentials come first (16
+// a cycle and SM, one per score: 120 us of that pipe, 64 % of its cycles), the
+// two products take half of that (31 %); neither is full, because the softmax and
+// the MMA warps wait for one another (issue slots 39 %).  A quarter of the
+// exponentials as a polynomial took 15 us longer.  Blocks ordered head by head instead of the longest
 // rows of all heads first: 219 us.  16 utterances of up to 500 frames, 2 heads
 // of 96, window 4: 14.9 us, two thirds of it launch, first loads and the
 // relative terms.

@@ -24,10 +24,12 @@
 //
 // Measured on B200, bf16 [8][4096][1024]: forward 37 us, 5.4 TB/s (83 % of a
 // copy's bandwidth; 69 us where rows are not aligned, here of 1023), backward
-// 60 us, 4.5 TB/s (80 unaligned; its ring holds three tensors, so fewer frames
-// are in flight).  fp32 [64][192][500]: forward 15.8 us, backward 20.5 with
-// ragged lengths, 4 of them the second kernel; in single frames (T = 501) 18.2
-// and 31.6.  One sentence, [1][192][37]: 5.6 us, launch and two barriers.
+// 60 us, 4.5 TB/s (80 unaligned): it waits for fixed latencies, the barrier of
+// each frame and shared memory (issue slots 56 %), hardly for HBM.  fp32
+// [8][2048][1024]: 37.7 and 50.3 us, 82 % of a copy's bandwidth both.  [B][C][T],
+// fp32 [64][192][500]: forward 15.8 us, backward 20.5 with ragged lengths, 4 of
+// them the second kernel; in single frames (T = 501) 18.2 and 31.6.  One
+// sentence, [1][192][37]: 5.6 us, launch and two barriers.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -4,7 +4,8 @@ Stand-alone operators over ``gsvdec_attention_*`` and ``gsvdec_norm_*``
 (include/gsvdec.h): no handle and no state.  Each call runs on the current
 stream of its tensors' device, takes outputs and workspace from torch's
 allocator, does not synchronise and can be captured in a CUDA graph.  The
-forward calls return what their backward needs.
+forward calls return what their backward needs; autograd does not record them
+(a torch.autograd.Function of a forward and its backward makes them trainable).
 """
 from __future__ import annotations
 

@@ -421,10 +421,18 @@ int gsvdec_workspace_bytes(const gsvdec_t* h, int64_t* bytes);
  *   s_ij = scale q_i . (k_j + rel_k[r + w]),   p = softmax over the allowed j
  *   o_i = sum_j p_ij (v_j + rel_v[r + w]),      lse_i = log sum_j exp(s_ij)
  * Query head h reads key head h / (H / Hkv).  A query without an allowed key,
- * and every i >= ql, gives o = 0, lse = -inf and dq = 0; keys j >= kl are not
- * read and give dk = dv = 0.  All tensors are [B, heads, T, D] by element
- * strides (batch, head, time); the D channels of a row are contiguous.  All
- * arithmetic accumulates in fp32 and each output is rounded once to dtype. */
+ * and every i >= ql, gives o = 0, lse = -inf and dq = 0 and adds nothing to
+ * another gradient, whatever its rows hold; keys j >= kl are not read and give
+ * dk = dv = 0.  All tensors are [B, heads, T, D] by element strides (batch,
+ * head, time); the D channels of a row are contiguous.
+ *
+ * Scores, softmax statistics and sums are fp32, and each output is rounded to
+ * dtype once.  With a 16-bit dtype the probabilities p (forward and backward)
+ * and p (dp - delta) (backward) are operands of the matrix units and rounded
+ * to 16 bits first, fp16 ones scaled to its range: errors against 64 bits are
+ * then 1.3 to 1.5 times those of the rounded outputs alone.  A forward of Tq H /
+ * Hkv <= 8 keeps p in fp32, and a backward of Tq, Tk <= 256 adds what that
+ * rounding lost as second operands. */
 typedef struct gsvdec_attention {
   int dtype;      /* GSV_DTYPE_* of every tensor but lse */
   int B, H, Hkv;  /* 1 .. 65535, H a multiple of Hkv, B H up to 2^24 */
@@ -473,8 +481,9 @@ int gsvdec_ops_status(int device, void* stream);
  * backward needs:  mean, rstd = 1 / sqrt(biased variance + eps) per frame,
  * xh = (x + y - mean) rstd, out = xh gamma + beta.  Backward, with a = d_out
  * gamma:  dx = rstd (a - mean(a) - xh mean(a xh)), the gradient of x and of y
- * alike; dgamma = sum over frames of d_out xh, dbeta = sum of d_out.  Frames
- * t >= lengths[b] give out = 0, mean = rstd = 0, dx = 0 and add nothing.
+ * alike; dgamma = sum over frames of d_out xh, dbeta = sum of d_out, in fp32
+ * and a fixed order.  Frames t >= lengths[b] give out = 0, mean = rstd = 0,
+ * dx = 0 and add nothing, whatever the inputs hold there.
  * x, y, out, d_out, dx have dtype and element strides (batch, outer axis). */
 #define GSV_LAYOUT_BCT 0 /* [B, C, T], time contiguous (the reference's); C <= 2048 */
 #define GSV_LAYOUT_BTC 1 /* [B, T, C], channels contiguous; C <= 8192 */
