@@ -178,6 +178,8 @@ def _ptr(a):
 class Decoder:
     """The Generator on one B200: ``Decoder.load(...)`` then ``forward(z, g)``."""
 
+    _encp_channels = None  # looked up at the first encp_attention call
+
     def __init__(self, handle: ctypes.c_void_p):
         self._h = handle
         info = _Info()
@@ -447,12 +449,20 @@ class Decoder:
                                               _ptr(ln), B, T, _ptr(out), MEM_HOST, None))
         return out
 
+    def _need_channels(self, C: int) -> None:
+        """x of an encp_attention call has the stacks' channels: the library takes that from the handle."""
+        if self._encp_channels is None:
+            self._encp_channels = self.encp_info["channels"]
+        if self._encp_channels and C != self._encp_channels:
+            raise ValueError(f"x must have {self._encp_channels} channels, not {C}")
+
     def encp_attention(self, stack, layer: int, x, lengths=None) -> np.ndarray:
         """self_attn.forward(x, x_mask) of EncoderLayer::forward
         (src/models/sovits_encp.rs:98-101) on host arrays: x [B, C, T]; frames
         behind their length are left out as keys and give 0."""
         xa = _host_f32(x)
         B, C, T = xa.shape
+        self._need_channels(C)
         ln = self._lengths(lengths, B)
         out = np.empty_like(xa)
         _check(library().gsvdec_encp_attention(self._h, self._stack(stack), layer, _ptr(xa), _ptr(ln), B, T, _ptr(out),
@@ -463,9 +473,15 @@ class Decoder:
         """Stream-async encp_attention on CUDA tensors (torch): x, out [B, C, T] fp32, lengths int32."""
         import torch
         B, C, T = x.shape
-        assert x.is_cuda and x.dtype == torch.float32 and x.is_contiguous()
+        self._need_channels(C)
+        index = self.info["device"]
+        ops._need("x", x, (B, C, T), torch.float32, index, True)
+        if lengths is not None:
+            ops._need("lengths", lengths, (B,), torch.int32, index, True)
         if out is None:
             out = torch.empty_like(x)
+        else:
+            ops._need("out", out, (B, C, T), torch.float32, index, True)
         st = stream if stream is not None else torch.cuda.current_stream(x.device).cuda_stream
         p = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())  # noqa: E731
         _check(library().gsvdec_encp_attention(self._h, self._stack(stack), layer, p(x), p(lengths), B, T, p(out),
