@@ -38,9 +38,11 @@ __device__ __forceinline__ int allowed_keys(int i, int ql, int kl, int causal) {
   return causal ? min(kl, max(0, i + kl - ql + 1)) : kl;
 }
 
-// The first query with an allowed key, where there is one; those before it may
-// hold anything, so the backward reads them as zeros, like rows past ql.
-__device__ __forceinline__ int first_query(int ql, int kl, int causal) { return causal ? max(0, ql - kl) : 0; }
+// The first query with an allowed key (ql: none has); those before it may hold
+// anything, so the backward reads them as zeros, like rows past ql.
+__device__ __forceinline__ int first_query(int ql, int kl, int causal) {
+  return kl == 0 ? ql : causal ? max(0, ql - kl) : 0;
+}
 
 // Eight channels as they lie in memory, turned into fp32 where they are used.
 template <typename T>

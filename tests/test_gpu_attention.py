@@ -315,3 +315,20 @@ def test_heads_without_channels_are_refused(gsv):
         with pytest.raises(gsv.GsvDecError) as e:
             gsv.attention(q, q, q, **kw)
         assert e.value.status == "GSV_E_INVALID_ARG"
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("Tq,Tk", [(70, 90), (1, 1), (200, 0)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_queries_of_an_utterance_without_keys_hold_anything(gsv, dtype, Tq, Tk, causal):
+    x = make(dtype, 3, 4, 2, Tq, Tk, 48, w=4)
+    x["q"][1] = x["do"][1] = 0
+    kw = dict(causal=causal, k_lengths=lengths(Tk, 0, Tk), rel_k=x["rel_k"], rel_v=x["rel_v"])
+    want = run_and_check(gsv, x, **{n: v for n, v in kw.items() if not n.startswith("rel")})
+    x["q"][1], x["do"][1] = float("nan"), float("inf")
+    if Tk == 0:
+        x["q"][:], x["do"][:] = float("nan"), float("nan")
+    o, lse = gsv.attention(x["q"], x["k"], x["v"], **kw)
+    assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    for a, b in zip(gsv.attention_backward(x["do"], x["q"], x["k"], x["v"], o, lse, **kw), want[2]):
+        assert torch.equal(a, b)
