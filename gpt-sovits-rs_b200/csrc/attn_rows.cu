@@ -38,11 +38,12 @@ __device__ __forceinline__ float dot8(const float* a, const float* b) {
 // and the products with the relative rows; fp16 adds the norms of the rows of
 // do and v.
 //
-// The o given here carries its rounding to 16 bits, which reaches ds through
-// delta as p_ij (2^-9 |do| |o|).  Over many keys o shrinks against v and the
-// term disappears; rows of up to kFewKeys keys, where it would be as large as
-// the rounding of ds itself, take delta = sum_j p_ij dp_ij instead (fp32
-// inputs have no such rounding).
+// The o given here carries its rounding to 16 bits and that of the forward's
+// probabilities, which reach ds through delta as p_ij |do| |o's error|.  Where
+// the probabilities spread over many keys o shrinks against v and the term
+// disappears; where a row rests on one key it stays, about as large as the
+// rounding of that ds.  Rows of up to kFewKeys keys, where that is the rule, take
+// delta = sum_j p_ij dp_ij instead (fp32 inputs have no such rounding).
 //
 // Reads do and o (with a window q) once: 2 x 16 heads of 64, 4096 causal rows,
 // bf16, 25 us, where the 32 rows of few keys of each head take longest; 16
