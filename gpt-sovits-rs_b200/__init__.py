@@ -45,7 +45,8 @@ EXPORTS = (
     "gsvdec_forward_multi", "gsvdec_plan_multi", "gsvdec_sync_status", "gsvdec_selftest_wait",
     "gsvdec_set_alloc_fail_after", "gsvdec_workspace_bytes",
     "gsvdec_attention_workspace", "gsvdec_attention_forward", "gsvdec_attention_backward", "gsvdec_ops_status",
-    "gsvdec_selftest_attention_wait", "gsvdec_encp_attention", "gsvdec_norm_workspace", "gsvdec_norm_forward", "gsvdec_norm_backward",
+    "gsvdec_selftest_attention_wait", "gsvdec_encp_attention", "gsvdec_norm_workspace", "gsvdec_norm_forward",
+    "gsvdec_norm_backward",
 )
 
 # EncP encoder stacks (GSV_ENCP_SSL / _TEXT / _2), by their enc_p.* names.

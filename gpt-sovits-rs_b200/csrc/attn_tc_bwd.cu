@@ -320,7 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
       // Per barrier: the first warp's lane 0 announces and issues what moves by bulk copies (full tiles,
       // row values); tails are copied by both warps, whose second arrival, or both, come when that is done.
       const bool first_warp = warp == 9;
-      const bool full_a = maps.a_on && tma_fits(r0, kBA, keys ? kl : ql, keys ? a.Tk : a.Tq) && (keys || r0 >= qfirst);
+      const bool full_a =
+          maps.a_on && tma_fits(r0, kBA, keys ? kl : ql, keys ? a.Tk : a.Tq) && (keys || r0 >= qfirst);
       const uint32_t a_full = bar(bars.a_full);
       if (first_warp && lane == 0) {
         const uint32_t rel_bytes = REL && !keys ? 2u * 2 * kBB * a.nrel * 4 : 0;
@@ -357,7 +358,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc(const __grid_constant
         if (round > 0) ok = ho.wait_free(bar(bars.b_free[s]), (round - 1) & 1, abort);
         if (!ok) break;
         const int h = keys ? hk * g + hh : hk;
-        const bool whole = maps.b_on && tma_fits(i0, kBB, keys ? ql : kl, keys ? a.Tq : a.Tk) && (!keys || i0 >= qfirst);
+        const bool whole =
+            maps.b_on && tma_fits(i0, kBB, keys ? ql : kl, keys ? a.Tq : a.Tk) && (!keys || i0 >= qfirst);
         if (first_warp && lane == 0) {
           // Offsets of this pair of tiles: from r0 - (i0 + 63 + off) to r0 + 127 - (i0 + off).
           const bool near = REL && keys && r0 - (i0 + kBB - 1 + off) <= a.window &&

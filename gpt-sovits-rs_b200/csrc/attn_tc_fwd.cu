@@ -37,8 +37,8 @@
 // a cycle and SM, one per score: 120 us of that pipe, 64 % of its cycles), the
 // two products take half of that (31 %); neither is full, because the softmax and
 // the MMA warps wait for one another (issue slots 39 %).  A quarter of the
-// exponentials as a polynomial took 15 us longer.  Blocks ordered head by head instead of the longest
-// rows of all heads first: 219 us.  16 utterances of up to 500 frames, 2 heads
+// exponentials as a polynomial took 15 us longer.  Blocks ordered head by head
+// instead of the longest rows of all heads first: 219 us.  16 utterances of up to 500 frames, 2 heads
 // of 96, window 4: 14.9 us, two thirds of it launch, first loads and the
 // relative terms.
 #include "attn_launch.h"

@@ -95,3 +95,40 @@ def test_norms_of_other_widths_after_every_kernel_was_used(gsv, monkeypatch):
         assert together([p[0] for p in pair], 2000) == []
         for _, kept, _, want in pair:
             assert all(torch.equal(a, b) for a, b in zip(kept[0], want))
+
+
+def test_calls_on_several_streams_at_once(gsv):
+    # Kernels that share SMs, their shared memory and TMEM: every call has the bits it has alone.
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def rows(dtype, *shape):
+        return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+    def attention(q, k, v, do, **kw):
+        o, lse = gsv.attention(q, k, v, **kw)
+        return (o, lse) + gsv.attention_backward(do, q, k, v, o, lse, **kw)[:3]
+
+    def norm(x, w):
+        out, mean, rstd = gsv.add_norm(x, x, w, w, layout="btc")
+        return (out, mean, rstd) + gsv.add_norm_backward(x, x, x, w, mean, rstd, layout="btc")
+
+    bf, half, f32 = torch.bfloat16, torch.float16, torch.float32
+    a = [rows(bf, 1, 8, n, 64) for n in (128, 4096, 4096, 128)]  # key tiles split over clusters
+    b = [rows(bf, 4, 2, 500, 96) for _ in range(4)]
+    c = [rows(half, 2, 4, 300, 32) for _ in range(4)]
+    d = [rows(f32, 2, 2, 200, 128) for _ in range(4)]
+    x, w = rows(bf, 4, 1024, 512), rows(f32, 512)
+    jobs = [lambda: attention(*a), lambda: attention(*b), lambda: attention(*c, causal=True), lambda: attention(*d),
+            lambda: norm(x, w)]
+    want = [[t.clone() for t in j()] for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        outs = []
+        for s, j in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                outs.append(j())
+        torch.cuda.synchronize()
+        for out, ref in zip(outs, want):
+            assert all(torch.equal(p, q) for p, q in zip(out, ref))
+    gsv.ops_status()
